@@ -7,7 +7,8 @@ and layer classes, the LLaMA patch the debug counters and the analysis utilities
 in ``libcarekv_hip.so`` through a C ABI (include/carekv.h).  Additions of
 this build: the batched entry points ``decode_attention`` /
 ``prefill_correction`` / ``prefill_attention``, ``CAREKVAdapter`` and
-``CarekvError``.
+``CarekvError``, and for long prompts ``rotate_heads``, ``attention_mass`` /
+``evict_rows`` and ``prefix_attention``.
 """
 from .config import (CacheConfig, apply_carekv_env_overrides, layer_budget_multiplier,
                      resolve_read_knobs, resolve_store_knobs)
@@ -20,6 +21,9 @@ from .residual import ResidualStoreManager, ResidualRouter, pack_4bit, unpack_4b
 from .attention import (CAREKVAttention, CAREKVMultiHeadAttention, apply_slot_corrections, decode_attention,
                         get_debug_stats, prefill_correction, reset_debug_stats)
 from .prefill import dequantize_rows, prefill_attention, prefill_eval, quant_dequant, quantize_rows
+from .rotary import RotaryPlan, rotary_plan, rotate_heads
+from .eviction import EvictedRows, attention_mass, evict_rows
+from .prefix import prefix_attention
 from .layer import CAREKVLayer
 from .attention import get_imp_per_layer
 from .utils import (ABLATION_VARIANTS, budget_sweep, calibrate_layer_sensitivity, compute_boundary_risk_stats,
@@ -52,4 +56,5 @@ __all__ = [
     "resolve_read_knobs", "resolve_store_knobs", "get_sketch_proj", "kivi_qdq", "kivi_codes",
     "decode_attention", "prefill_correction", "prefill_attention", "prefill_eval", "quantize_rows", "dequantize_rows",
     "quant_dequant", "CAREKVAdapter", "CarekvError", "CAREKVHFCache",
+    "RotaryPlan", "rotary_plan", "rotate_heads", "EvictedRows", "attention_mass", "evict_rows", "prefix_attention",
 ]

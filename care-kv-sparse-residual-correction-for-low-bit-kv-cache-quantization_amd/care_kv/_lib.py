@@ -58,7 +58,8 @@ class DecodeParams(C.Structure):
                 ("split_pages", C.c_int32), ("phase_events", C.c_void_p), ("k_proxy", C.c_int32),
                 ("sketch_proj", C.c_void_p), ("route_policy", C.c_int32), ("adaptive_score", C.c_int32),
                 ("rel_threshold", C.c_double), ("abs_threshold", C.c_double), ("min_keep", C.c_int32),
-                ("read_counts", C.c_void_p), ("packed_pages_used", C.c_int32), ("tail_pages_used", C.c_int32)]
+                ("read_counts", C.c_void_p), ("packed_pages_used", C.c_int32), ("tail_pages_used", C.c_int32),
+                ("lse", C.c_void_p)]
 
 
 class PrefillParams(C.Structure):
@@ -77,6 +78,35 @@ class PrefillEvalParams(C.Structure):
         [("k_corr_scale", C.c_float), ("diag_cap", C.c_int32)]
 
 
+# element types (CAREKV_F16 ..)
+DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "seq_len", "n_heads", "n_kv_heads", "head_dim", "rotary_dim", "dtype",
+                                         "interleaved", "inverse", "pos_bits")] + [("scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("pos_batch", "q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "qo_sb", "qo_sh",
+                                  "qo_st", "ko_sb", "ko_sh", "ko_st")]
+
+
+class MassParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "n_queries", "n_keys", "head_dim", "dtype",
+                                         "causal", "accumulate")] + [("sm_scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "out_sb", "out_sh")]
+
+
+class EvictParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_kv_heads", "n_keys", "row_bytes", "keep", "sink", "recent")] + \
+        [(n, C.c_int64) for n in ("mass_sb", "mass_sh", "k_sb", "k_sh", "k_st", "v_sb", "v_sh", "v_st")]
+
+
+class PrefixParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "seq_len", "prefix_len", "head_dim",
+                                         "dtype")] + [("sm_scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("q_sb", "q_sh", "q_st", "k_sh", "k_st", "v_sh", "v_st", "out_sb", "out_sh", "out_st",
+                                  "own_sb", "own_sh", "own_st")]
+
+
 # page job: int32 x 6 (seq, kv_head, page, num_valid, token_start, is_recent)
 PAGE_JOB_INTS = 6
 
@@ -86,7 +116,9 @@ EXPORTS = ["carekv_store_pages", "carekv_store_prefill", "carekv_store_workspace
            "carekv_prefill_correct_workspace_bytes", "carekv_decode_attn_static", "carekv_write_base", "carekv_append_coded_rows",
            "carekv_pack_codes", "carekv_unpack_codes", "carekv_pack_4bit", "carekv_unpack_4bit",
            "carekv_quantize_rows_f32", "carekv_dequantize_rows_f32", "carekv_kivi_codes", "carekv_read_hat_pages",
-           "carekv_prefill_eval", "carekv_last_error"]
+           "carekv_prefill_eval", "carekv_rotate_heads", "carekv_attention_mass",
+           "carekv_attention_mass_workspace_bytes", "carekv_evict_rows", "carekv_prefix_attn",
+           "carekv_prefix_attn_workspace_bytes", "carekv_last_error"]
 
 # bytes of the per-GPU static workspace of carekv_decode_attn_static
 # (CAREKV_STATIC_SCRATCH_BYTES in include/carekv.h)
@@ -170,6 +202,18 @@ def load(path: str | None = None):
         lib.carekv_read_hat_pages.argtypes = [C.POINTER(Arena), i32, i32, i32, vp, vp, vp, vp, vp]
         lib.carekv_prefill_eval.restype = C.c_int
         lib.carekv_prefill_eval.argtypes = [C.POINTER(PrefillEvalParams), vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        lib.carekv_rotate_heads.restype = C.c_int
+        lib.carekv_rotate_heads.argtypes = [C.POINTER(RotaryParams), vp, vp, vp, vp, vp, vp, vp]
+        lib.carekv_attention_mass.restype = C.c_int
+        lib.carekv_attention_mass.argtypes = [C.POINTER(MassParams), vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_attention_mass_workspace_bytes.restype = i64
+        lib.carekv_attention_mass_workspace_bytes.argtypes = [C.POINTER(MassParams), i32]
+        lib.carekv_evict_rows.restype = C.c_int
+        lib.carekv_evict_rows.argtypes = [C.POINTER(EvictParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        lib.carekv_prefix_attn.restype = C.c_int
+        lib.carekv_prefix_attn.argtypes = [C.POINTER(PrefixParams), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_prefix_attn_workspace_bytes.restype = i64
+        lib.carekv_prefix_attn_workspace_bytes.argtypes = [C.POINTER(PrefixParams)]
         _lib = lib
         return lib
 
@@ -259,3 +303,72 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def aligned_rows(x: torch.Tensor, n: int = 16) -> torch.Tensor:
+    """x with the values of a row (the last dim) next to each other and every
+    row on a multiple of n bytes: x itself, or a packed copy."""
+    e = x.element_size()
+    if not x.numel() or (x.stride(-1) == 1 and x.data_ptr() % n == 0 and
+                         all(s * e % n == 0 for s in lead_strides(x))):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def lead_strides(x: torch.Tensor):
+    """Strides of the leading dims, 0 where a dim has one entry (whatever
+    torch says there is never stepped)."""
+    return [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+
+
+def same_device(what: str, *tensors):
+    """The device of every tensor given (None: skipped), a HIP device."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        ptr(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise CarekvError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory that a and b span overlaps (the same tensor apart)."""
+    if not a.numel() or not b.numel() or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()):
+        return False
+
+    def end(t):
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def check_out(out: torch.Tensor, shape, dtype, name: str, *inputs: torch.Tensor):
+    """Refuse an output of another shape or type, one whose rows are not
+    packed or repeat, and one that overlaps an input other than being it."""
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype}; got {tuple(out.shape)} {out.dtype}")
+    if out.numel() and ((out.shape[-1] > 1 and out.stride(-1) != 1) or
+                        any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride()))):
+        raise ValueError(f"{name} needs the values of a row next to each other and no repeated rows")
+    if any(overlap(out, x) for x in inputs):
+        raise ValueError(f"{name} must be its input itself or not overlap it")
+
+
+def row_counts(x, batch: int, device, name: str) -> torch.Tensor | None:
+    """Per-sequence int32 values on the device: a device tensor of `batch`
+    integers, a host sequence of them, or one int for all; None stays None."""
+    if x is None:
+        return None
+    if torch.is_tensor(x) and x.is_cuda:
+        if x.shape != (batch,) or x.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be {batch} int32 or int64 values; got {tuple(x.shape)} {x.dtype}")
+        return x.to(torch.int32).contiguous()
+    vals = [x] * batch if isinstance(x, int) else [int(v) for v in x]
+    if len(vals) != batch:
+        raise ValueError(f"{name} must have {batch} values; got {len(vals)}")
+    t = torch.tensor(vals, dtype=torch.int32)
+    # through pinned memory, so that the host does not wait for the stream
+    return t.pin_memory().to(device, non_blocking=True) if torch.device(device).type == "cuda" else t

@@ -16,7 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -24,6 +24,7 @@ import torch
 from . import _lib
 from .cache import CAREKVCache, get_sketch_proj, to_device
 from .config import CacheConfig, ReadKnobs, any_read_budget, resolve_read_knobs
+from .prefix import prefix_attention
 
 KIND_CODE = {"both": 0, "k": 1, "v": 2}
 
@@ -249,7 +250,8 @@ def prefill_correction(cache: CAREKVCache, layer: int, q: torch.Tensor, k_hat: t
 def decode_attention(cache: CAREKVCache, layer: int, q: torch.Tensor, seqs: Optional[Sequence[int]] = None, *,
                      correction: bool = True, knobs: Optional[ReadKnobs] = None, split_pages: Optional[int] = None,
                      diag_cap: int = 0, out: Optional[torch.Tensor] = None, phase_events=None,
-                     no_alloc: bool = False, n_pages: Optional[Sequence[int]] = None, count_reads: bool = True):
+                     no_alloc: bool = False, n_pages: Optional[Sequence[int]] = None, count_reads: bool = True,
+                     return_lse: bool = False, prefix: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
     """q: (B, Hq, D) fp16 post-RoPE queries of B sequences -> (B, Hq, D) fp16.
 
     With ``diag_cap > 0`` also returns the selected candidates per query
@@ -263,7 +265,16 @@ def decode_attention(cache: CAREKVCache, layer: int, q: torch.Tensor, seqs: Opti
     ``_lib.STATIC_SCRATCH_BYTES``) instead of a buffer the cache owns; the
     library call then allocates nothing (pass ``out``).  ``n_pages``: per
     sequence, attend to its first n pages only (default: all of them).
-    ``count_reads=False`` keeps the launch out of the debug read counters."""
+    ``count_reads=False`` keeps the launch out of the debug read counters.
+
+    ``return_lse`` also returns (last) the fp32 (B, Hq) natural log-sum-exp of
+    the scores behind each output (with the exact K correction the corrected
+    scores'), -inf for a sequence without tokens.  ``prefix``: (k, v), fp16
+    (Hkv, P, D) post-RoPE rows that come before every sequence's cached ones,
+    read once for the whole batch (``prefix_attention``); the outputs are the
+    softmax over both, the routing and correction those of the cached rows."""
+    if prefix is not None and no_alloc:
+        raise ValueError("decode_attention: no_alloc does not take a prefix (its workspace is allocated)")
     cfg: CacheConfig = cache.cfg
     if q.dim() == 2:
         q = q.unsqueeze(0)
@@ -328,11 +339,17 @@ def decode_attention(cache: CAREKVCache, layer: int, q: torch.Tensor, seqs: Opti
     if out is None:
         out = torch.empty(B, Hq, D, dtype=torch.float16, device=dev)
     diag = torch.empty(B, Hq, diag_cap, dtype=torch.int32, device=dev) if diag_cap > 0 else None
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse or prefix is not None else None
+    dp.lse = None if lse is None else lse.data_ptr()
+
+    def results():
+        got = (out,) + ((diag,) if diag_cap > 0 else ()) + ((lse,) if return_lse else ())
+        return got if len(got) > 1 else out
     if no_alloc:
         _lib.check(lib.carekv_decode_attn_static(a, dp, q.data_ptr(), out.data_ptr(),
                                                  None if diag is None else diag.data_ptr(), int(diag_cap),
                                                  _lib.stream_ptr(dev)), "carekv_decode_attn_static")
-        return (out, diag) if diag_cap > 0 else out
+        return results()
     nbytes = int(lib.carekv_decode_workspace_bytes(a, dp))
     if nbytes < 0:
         raise _lib.CarekvError("carekv_decode_workspace_bytes rejected the parameters")
@@ -342,7 +359,9 @@ def decode_attention(cache: CAREKVCache, layer: int, q: torch.Tensor, seqs: Opti
                                       _lib.stream_ptr(dev)), "carekv_decode_attn")
     if _lib.check_enabled():
         _lib.check_status(ws, 0, "carekv_decode_attn")
-    return (out, diag) if diag_cap > 0 else out
+    if prefix is not None:
+        out, lse = prefix_attention(q, *prefix, own=(out, lse), out=out, return_lse=True)
+    return results()
 
 
 def apply_slot_corrections(cache: CAREKVCache, cfg: CacheConfig, router, layer_id: int, kv_head: int, page_ids,

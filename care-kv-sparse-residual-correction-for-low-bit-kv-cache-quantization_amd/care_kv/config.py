@@ -56,6 +56,9 @@ def apply_carekv_env_overrides(kwargs: dict) -> dict:
     # no reference counterpart: the packed KIVI base (CacheConfig.kivi_packed)
     _set("CAREKV_KIVI_PACKED", "kivi_packed", as_bool)
     _set("CAREKV_KIVI_TAIL_PAGES", "kivi_tail_pages", int)
+    # no reference counterpart: prompt rows kept by attention weight (CacheConfig.prefill_keep)
+    for name in ("prefill_keep", "prefill_keep_sink", "prefill_keep_recent", "prefill_keep_window"):
+        _set("CAREKV_" + name.upper(), name, int)
     ls = env.get("CAREKV_LAYER_SENSITIVITY", "")
     if ls:
         try:
@@ -137,6 +140,16 @@ class CacheConfig:
     # them every output, are the side-buffer base's.
     kivi_packed: bool = False
     kivi_tail_pages: int = 0
+    # No reference counterpart.  prefill_keep > 0: of a prompt longer than that
+    # only so many rows per kv head go to the pages, the first
+    # prefill_keep_sink, the last prefill_keep_recent and the rows that gathered
+    # the most attention weight (attention_mass / evict_rows) from the prompt's
+    # last prefill_keep_window queries (0: all of them).  The prompt's own
+    # attention sees every row.
+    prefill_keep: int = 0
+    prefill_keep_sink: int = 4
+    prefill_keep_recent: int = 32
+    prefill_keep_window: int = 0
 
     def __post_init__(self):
         if self.layer_sensitivity is None:
@@ -145,6 +158,13 @@ class CacheConfig:
             self.num_kv_heads = self.num_heads
         if self.packed_storage and not self.packed_base:
             self.packed_base = True
+        if self.prefill_keep < 0 or self.prefill_keep_sink < 0 or self.prefill_keep_recent < 0 \
+                or self.prefill_keep_window < 0:
+            raise ValueError("prefill_keep, prefill_keep_sink, prefill_keep_recent and prefill_keep_window must not "
+                             "be negative")
+        if 0 < self.prefill_keep < self.prefill_keep_sink + self.prefill_keep_recent:
+            raise ValueError(f"prefill_keep={self.prefill_keep} rows cannot hold prefill_keep_sink="
+                             f"{self.prefill_keep_sink} and prefill_keep_recent={self.prefill_keep_recent}")
         checks = (
             ("scale_dtype", {"fp16", "bf16", "fp32"}), ("scale_quant", {"none", "int8"}),
             ("store_budget_mode", {"ratio", "absolute"}),

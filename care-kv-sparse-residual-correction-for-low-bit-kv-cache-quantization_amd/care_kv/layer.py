@@ -17,6 +17,12 @@ the HIP library:
   layer.py:363-456, 792-806);
 * decode attention with the comb+ex correction is ``decode_attention``
   (``carekv_decode_attn``, layer.py:1148-1160).
+
+Without a reference counterpart: ``position_embeddings`` may be (RotaryPlan,
+positions) instead of (cos, sin) tables (``rotate_heads``), ``prefix`` =
+(k, v) puts a prefix that the whole batch shares before every sequence
+(``prefix_attention``), and cfg.prefill_keep keeps only the rows of a prompt
+that its queries attend to (``attention_mass``, ``evict_rows``).
 """
 from __future__ import annotations
 
@@ -30,6 +36,9 @@ from . import _lib
 from .attention import (debug_stats_enabled, decode_attention, decode_read_mode, get_debug_stats,  # noqa: F401
                         get_imp_per_layer, importance_probe, prefill_correction, reset_debug_stats)
 from .cache import CAREKVCache
+from .eviction import attention_mass, evict_rows
+from .prefix import prefix_attention
+from .rotary import RotaryPlan, rotate_heads
 from .config import CacheConfig, any_read_budget, resolve_read_knobs
 from .prefill import eval_knobs, prefill_attention, prefill_eval, quant_dequant
 
@@ -123,6 +132,9 @@ class CAREKVLayer(nn.Module):
         B, T, _ = hidden.shape
         Hq, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         Q, K, V = self._project(hidden)
+        if position_embeddings is not None and isinstance(position_embeddings[0], RotaryPlan):
+            Q, K = rotate_heads(Q.to(F16), K.to(F16), position_embeddings[1], position_embeddings[0])
+            return Q, K, V.to(F16).contiguous()
         cos, sin = (None, None) if position_embeddings is None else (x.to(Q.dtype) for x in position_embeddings)
         q, k, v = (x.transpose(1, 2) for x in (Q, K, V))  # the projections' own layout
         if (q.dtype == F16 and q.is_cuda and B * T > 0 and all(x.is_contiguous() for x in (q, k, v))
@@ -196,7 +208,7 @@ class CAREKVLayer(nn.Module):
         return runs
 
     def _prefill_runs(self, cache: CAREKVCache, hidden: Tensor, runs, sink_tokens: int,
-                      position_embeddings, token_start_abs: int, seqs: Sequence[int]) -> Tensor:
+                      position_embeddings, token_start_abs: int, seqs: Sequence[int], prefix=None) -> Tensor:
         """A padded batch: the sequences whose rows are all real run as one
         batch, every other sequence alone over its real rows [s, e) (RoPE
         rows sliced alike), so no pad row reaches a page or an attention
@@ -207,24 +219,29 @@ class CAREKVLayer(nn.Module):
         def pe(rows, sl):
             if position_embeddings is None:
                 return None
+            if isinstance(position_embeddings[0], RotaryPlan):
+                plan, p = position_embeddings
+                p = p if p.dim() == 2 else p.unsqueeze(0)
+                return plan, (p[rows] if p.shape[0] == B else p)[:, sl]
             return tuple((x[rows] if x.shape[0] == B else x[[0] * len(rows)])[:, sl] for x in position_embeddings)
         full = [b for b, (s, e) in enumerate(runs) if (s, e) == (0, T)]
         if full:
             out[full] = self.prefill(cache, hidden[full], sink_tokens=sink_tokens,
                                      position_embeddings=pe(full, slice(None)), token_start_abs=token_start_abs,
-                                     seqs=[seqs[b] for b in full])
+                                     seqs=[seqs[b] for b in full], prefix=prefix)
         for b, (s, e) in enumerate(runs):
             if (s, e) != (0, T) and e > s:
                 out[b, s:e] = self.prefill(cache, hidden[b:b + 1, s:e], sink_tokens=sink_tokens,
                                            position_embeddings=pe([b], slice(s, e)),
-                                           token_start_abs=token_start_abs, seqs=[seqs[b]])[0]
+                                           token_start_abs=token_start_abs, seqs=[seqs[b]], prefix=prefix)[0]
         return out
 
     # ------------------------------------------------------------ prefill
     def prefill(self, cache: CAREKVCache, hidden: Tensor, sink_tokens: int = 4,
                 attention_mask: Optional[Tensor] = None,
                 position_embeddings: Optional[Tuple[Tensor, Tensor]] = None, token_start_abs: int = 0,
-                debug_stats: Optional[Dict[str, Any]] = None, seqs: Optional[Sequence[int]] = None) -> Tensor:
+                debug_stats: Optional[Dict[str, Any]] = None, seqs: Optional[Sequence[int]] = None,
+                prefix: Optional[Tuple[Tensor, Tensor]] = None) -> Tensor:
         """layer.py:643-935 for a batch: hidden (T, model_dim) or (B, T,
         model_dim) -> the attention output through W_O, same leading shape.
 
@@ -239,7 +256,13 @@ class CAREKVLayer(nn.Module):
         rows out of its pages and its attention: those sequences run over
         their real rows alone and their pad rows return zero.  The reference
         adds the mask to one sequence's scores and still stores the pad rows
-        (layer.py:952-957); its B > 1 loop cannot broadcast a batched mask."""
+        (layer.py:952-957); its B > 1 loop cannot broadcast a batched mask.
+
+        ``prefix`` (modes ``fp`` and ``base_quant``): (k, v) fp16 (Hkv, P, D),
+        post-RoPE rows before every sequence's first token; the caller's
+        position_embeddings start behind them.  cfg.prefill_keep (every mode
+        but ``carekv_stored``, whose correction needs all pages of the prompt)
+        writes only the rows kept to the pages."""
         squeeze = hidden.dim() == 2
         if squeeze:
             hidden = hidden.unsqueeze(0)
@@ -249,13 +272,27 @@ class CAREKVLayer(nn.Module):
         seqs = list(range(B)) if seqs is None else list(seqs)
         runs = self._key_runs(attention_mask, B, T)
         if runs is not None:
-            out = self._prefill_runs(cache, hidden, runs, sink_tokens, position_embeddings, token_start_abs, seqs)
+            out = self._prefill_runs(cache, hidden, runs, sink_tokens, position_embeddings, token_start_abs, seqs,
+                                     prefix)
             return out[0] if squeeze else out
+        evict = 0 < cfg.prefill_keep < T
+        if prefix is not None and mode not in ("fp", "base_quant"):
+            raise NotImplementedError(f"a shared prefix in prefill mode {mode!r}: the correction weighs a prompt's own "
+                                      "rows alone (fp and base_quant take one)")
+        if evict and (mode == "carekv_stored" or (cache.hat and mode != "fp")):
+            raise NotImplementedError(f"prefill_keep in prefill mode {mode!r} with base_quantizer="
+                                      f"{cfg.base_quantizer!r}: the mode reads the pages of the whole prompt")
         Qh, Kh, Vh = self._heads(hidden, position_embeddings)
-        hats = cache.write_prefill(self.layer_id, Kh, Vh, token_start_abs=token_start_abs,
-                                   sink_tokens=sink_tokens, seqs=seqs)
+        hats = None
+        if not evict:
+            hats = cache.write_prefill(self.layer_id, Kh, Vh, token_start_abs=token_start_abs,
+                                       sink_tokens=sink_tokens, seqs=seqs)
+        need_lse = evict or prefix is not None
+        lse = None
+        Kat = Kh  # the keys that the prompt's attention reads
         if mode == "fp":
-            O = prefill_attention(Qh, Kh, Vh)
+            O = prefill_attention(Qh, Kh, Vh, return_lse=need_lse)
+            O, lse = O if need_lse else (O, None)
         else:
             if hats is not None:  # side-buffer base: the K_hat / V_hat the pages hold (layer.py:328-332)
                 Khat, Vhat = (hats[0].unsqueeze(0), hats[1].unsqueeze(0)) if hats[0].dim() == 3 else hats
@@ -268,8 +305,9 @@ class CAREKVLayer(nn.Module):
                                           "(token_start_abs > 0): the reference scores one prompt at a time")
             # the stored-slot correction weighs the prompt rows with the base's
             # log-sum-exp; the other modes need only O
-            O, lse = prefill_attention(Qh, Khat, Vhat, return_lse=True) if stored else \
+            O, lse = prefill_attention(Qh, Khat, Vhat, return_lse=True) if stored or need_lse else \
                 (prefill_attention(Qh, Khat, Vhat), None)
+            Kat = Khat
             if mode == "carekv_eval":  # layer.py:792-806: full in-memory residuals
                 O = prefill_eval(Qh, Kh, Vh, Khat, Vhat, O, **eval_knobs(cfg.read_budget_ratio))
             if stored:  # layer.py:808-838: the sparse correction from the stored slots
@@ -280,18 +318,28 @@ class CAREKVLayer(nn.Module):
                 for b, sq in enumerate(seqs):
                     O[b] = prefill_correction(cache, self.layer_id, Qh[b].transpose(0, 1), Khat[b], Vhat[b],
                                               lse[b], seq=sq, knobs=knobs).transpose(0, 1)
+        if evict:
+            w = min(cfg.prefill_keep_window, T) or T  # the last queries, which vote
+            mass = attention_mass(Qh[:, :, T - w:], Kat, lse=lse[:, :, T - w:])
+            kept = evict_rows(mass, Kh, Vh, keep=cfg.prefill_keep, sink=cfg.prefill_keep_sink,
+                              recent=cfg.prefill_keep_recent)
+            cache.write_prefill(self.layer_id, kept.k, kept.v, token_start_abs=token_start_abs,
+                                sink_tokens=sink_tokens, seqs=seqs)
+        if prefix is not None:
+            O = prefix_attention(Qh, *prefix, own=(O, lse), out=O)
         out = self._out(O, hidden.dtype).to(hidden.dtype)
         return out[0] if squeeze else out
 
     # ------------------------------------------------------------ decode
     def decode_step(self, cache: CAREKVCache, hidden: Tensor,
                     position_embeddings: Optional[Tuple[Tensor, Tensor]] = None,
-                    debug_stats: Optional[Dict[str, Any]] = None, seqs: Optional[Sequence[int]] = None) -> Tensor:
+                    debug_stats: Optional[Dict[str, Any]] = None, seqs: Optional[Sequence[int]] = None,
+                    prefix: Optional[Tuple[Tensor, Tensor]] = None) -> Tensor:
         """layer.py:978-1163 for a batch: hidden (1, model_dim) of one
         sequence or (B, 1, model_dim) -> same shape.  Appends the token's
         K / V (store on page fill with K_orig = K_hat, layer.py:1088-1146),
         then runs the decode attention with the correction
-        ``decode_read_mode`` resolves."""
+        ``decode_read_mode`` resolves; ``prefix`` as in ``prefill``."""
         squeeze = hidden.dim() == 2
         if squeeze:
             hidden = hidden.unsqueeze(0)
@@ -301,6 +349,6 @@ class CAREKVLayer(nn.Module):
         cache.append(self.layer_id, K[:, :, 0], V[:, :, 0], seqs=seqs)
         correction, knobs = decode_read_mode(self.cfg, self.layer_id)
         O = decode_attention(cache, self.layer_id, Q[:, :, 0], seqs=seqs, correction=correction,
-                             knobs=knobs)  # (B, Hq, D)
+                             knobs=knobs, prefix=prefix)  # (B, Hq, D)
         out = self._out(O.unsqueeze(2), hidden.dtype).to(hidden.dtype)  # (B, 1, model_dim)
         return out[0] if squeeze else out

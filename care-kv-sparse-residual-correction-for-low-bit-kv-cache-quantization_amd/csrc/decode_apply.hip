@@ -451,6 +451,11 @@ __global__ __launch_bounds__(256) void decode_combine_kernel(int Hkv, int D, int
     return f2h(o);
   };
   const uint32_t h0 = fin(O.x, nm.x), h1 = fin(O.y, nm.y), h2 = fin(O.z, nm.z), h3 = fin(O.w, nm.w);
+  if (a.lse && d == 0) {
+    // the sum behind the output: the exact K correction changes it with the scores (dn)
+    const float Lc = a.k_exact && L > 0.f ? L + dn : L;
+    a.lse[orow] = Lc > 0.f ? (M + __log2f(Lc)) * 0.69314718f : -INFINITY;
+  }
   uint16_t* op = a.out + orow * D + d;
   if (out_al8) {
     *reinterpret_cast<uint2*>(op) = make_uint2(h0 | (h1 << 16), h2 | (h3 << 16));

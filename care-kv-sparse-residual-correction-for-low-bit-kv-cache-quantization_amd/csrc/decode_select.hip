@@ -270,6 +270,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8, 8))) voi
         }
       outp[d] = f2h(L > 0.f ? O / L : 0.f);
     }
+    if (a.lse && tid == 0)
+      a.lse[(long)b * a.Hq + kvh * GQ + qq] = L > 0.f ? (M + __log2f(L)) * 0.69314718f : -INFINITY;
     if (diagp)
       for (int i = tid; i < a.diag_cap; i += kBlock) diagp[i] = -1;
     return;

@@ -342,6 +342,14 @@ typedef struct carekv_decode_params {
   int32_t packed_pages_used; /* kivi_packed arenas: host upper bounds over the */
   int32_t tail_pages_used;   /* rows of min(n_pages, n_packed) and of
                               * n_pages - n_packed (ignored otherwise)         */
+  float* lse;              /* optional device fp32 [batch][n_heads], NULL to
+                            * skip: the natural log-sum-exp of the scaled
+                            * scores behind each output (no reference
+                            * counterpart; what carekv_prefix_attn joins).  With
+                            * the exact K correction the corrected scores', with
+                            * the linear one or none the base scores'; -inf for
+                            * a row without tokens.  carekv_prefill_correct
+                            * ignores it                                      */
 } carekv_decode_params;
 
 /* q, out: fp16 [batch][n_heads][head_dim].  The first int32 of the
@@ -547,6 +555,103 @@ int64_t carekv_prefill_correct_workspace_bytes(const carekv_arena* arena, const 
  * as carekv_quantize_rows (pack = 0) writes them; group must be 32. */
 int carekv_dequantize_rows(const int8_t* codes, const uint16_t* scale, int32_t rows, int32_t D, int32_t group,
                            uint16_t* out, void* stream);
+
+/* ---------------------------------------------------------------- long prompts
+ * Operators without a reference counterpart: heads at explicit rotary
+ * positions, the weight a prompt's rows gathered and the rows kept by it, and
+ * attention over a prefix that a batch shares.  Element types: */
+#define CAREKV_F16 0
+#define CAREKV_BF16 1
+#define CAREKV_F32 2
+
+/* q [batch][n_heads][seq_len][head_dim] and k likewise with n_kv_heads (0:
+ * none), under rotary positions: of each head the first rotary_dim values, in
+ * pairs (i, i + rotary_dim / 2), interleaved != 0: (2i, 2i + 1), turned by
+ * position * freqs[i] radians and multiplied by scale; the others copied.
+ * inverse != 0 turns back (times scale: the gradient of the forward call).
+ * positions: device int32 or int64 (pos_bits), sequence b's at b * pos_batch;
+ * freqs: device fp64 [rotary_dim / 2].  Angles are reduced in 64 bits, products
+ * are fp32, rounded once.  Strides in elements, of batch / head / token; the
+ * values of a head lie next to each other.  An output may be its input (the
+ * same pointer and strides); otherwise they must not overlap. */
+typedef struct carekv_rotary_params {
+  int32_t batch, seq_len, n_heads, n_kv_heads, head_dim, rotary_dim;
+  int32_t dtype;           /* CAREKV_F16, CAREKV_BF16 or CAREKV_F32            */
+  int32_t interleaved, inverse, pos_bits;
+  float scale;
+  int64_t pos_batch;       /* elements; 0: one row of positions for all        */
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st;
+  int64_t qo_sb, qo_sh, qo_st, ko_sb, ko_sh, ko_st;
+} carekv_rotary_params;
+
+int carekv_rotate_heads(const carekv_rotary_params* params, const void* q, const void* k, const void* positions,
+                        const double* freqs, void* qo, void* ko, void* stream);
+
+/* out[b][g][j] (+)= the sum over the query heads of kv head g and the query
+ * rows i that see key j of exp(sm_scale q_i.k_j - lse_i).  q [batch][n_heads]
+ * [n_queries][head_dim], k [batch][n_kv_heads][n_keys][head_dim], fp16 or bf16,
+ * strides in elements, rows 16-byte aligned; out fp32, a (sequence, kv head)'s
+ * n_keys values next to each other.  Query row i of sequence b stands at
+ * position q_start[b] + i (NULL: length - n_queries + i) and sees the keys
+ * j < lengths[b] (NULL: n_keys), with causal only j <= its position.  lse: fp32
+ * [batch][n_heads][n_queries] contiguous (carekv_prefill_attn's), or NULL:
+ * computed here.  A row that sees nothing, or whose lse is infinite, adds
+ * nothing; keys no row sees get 0; values of masked keys and rows are never
+ * used.  accumulate != 0 adds to out.  head_dim 64 or 128.  The order of every
+ * sum is fixed. */
+typedef struct carekv_mass_params {
+  int32_t batch, n_heads, n_kv_heads, n_queries, n_keys, head_dim;
+  int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
+  int32_t causal, accumulate;
+  float sm_scale;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, out_sb, out_sh;
+} carekv_mass_params;
+
+int carekv_attention_mass(const carekv_mass_params* params, const void* q, const void* k, const float* lse,
+                          const int32_t* q_start, const int32_t* lengths, float* out, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+/* have_lse: whether lse is given; -1 on bad params. */
+int64_t carekv_attention_mass_workspace_bytes(const carekv_mass_params* params, int32_t have_lse);
+
+/* Of each (sequence, kv head)'s first lengths[b] rows (NULL: n_keys) keep the
+ * first `sink`, the last `recent` and, of the others, those of largest mass
+ * (equal: the lower index; NaN below everything) up to `keep` rows, in index
+ * order: k_out / v_out [batch][n_kv_heads][keep][row_bytes], mass_out fp32 and
+ * index int32 [batch][n_kv_heads][keep], kept int32 [batch] (NULL to skip) =
+ * min(length, keep).  Places past it hold zeros and index -1.  mass fp32 (batch
+ * and head strides in elements, a head's values next to each other); K and V
+ * rows of any element type, row_bytes each (a multiple of 4), strides in bytes,
+ * 4-byte aligned.  sink + recent <= keep. */
+typedef struct carekv_evict_params {
+  int32_t batch, n_kv_heads, n_keys, row_bytes, keep, sink, recent;
+  int64_t mass_sb, mass_sh, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+} carekv_evict_params;
+
+int carekv_evict_rows(const carekv_evict_params* params, const float* mass, const void* k, const void* v,
+                      const int32_t* lengths, void* k_out, void* v_out, float* mass_out, int32_t* index,
+                      int32_t* kept, void* stream);
+
+/* out = attention of every row of q [batch][n_heads][seq_len][head_dim] over
+ * the one prefix k, v [n_kv_heads][prefix_len][head_dim], which all rows see,
+ * joined with the row's attention over tokens of its own (own, own_lse; NULL:
+ * none) as one softmax: own like q, own_lse fp32 [batch][n_heads][seq_len]
+ * contiguous, the natural log-sum-exp behind own (finite; -inf: no tokens, the
+ * row of own is not used).  lse (optional, laid out like own_lse) receives the
+ * joint log-sum-exp.  A row that sees nothing is 0 with lse -inf.  fp16 or
+ * bf16, strides in elements, rows of q, k and v 16-byte aligned; head_dim 64
+ * or 128.  out may be own (the same pointer and strides). */
+typedef struct carekv_prefix_params {
+  int32_t batch, n_heads, n_kv_heads, seq_len, prefix_len, head_dim;
+  int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
+  float sm_scale;
+  int64_t q_sb, q_sh, q_st, k_sh, k_st, v_sh, v_st;
+  int64_t out_sb, out_sh, out_st, own_sb, own_sh, own_st;
+} carekv_prefix_params;
+
+int carekv_prefix_attn(const carekv_prefix_params* params, const void* q, const void* k, const void* v,
+                       const void* own, const float* own_lse, void* out, float* lse, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int64_t carekv_prefix_attn_workspace_bytes(const carekv_prefix_params* params);
 
 const char* carekv_last_error(void);
 
