@@ -308,31 +308,45 @@ def stream_ptr(device) -> int:
 def aligned_rows(x: torch.Tensor, n: int = 16) -> torch.Tensor:
     """x with the values of a row (the last dim) next to each other and every
     row on a multiple of n bytes: x itself, or a packed copy."""
-    e = x.element_size()
-    if not x.numel() or (x.stride(-1) == 1 and x.data_ptr() % n == 0 and
-                         all(s * e % n == 0 for s in lead_strides(x))):
+    bits, e = x.data_ptr(), x.element_size()
+    st = x.stride()
+    for s in st[:-1]:
+        bits |= s * e
+    if st[-1] == 1 and not bits % n:
+        return x
+    # (what a dim of one entry has for a stride is never stepped)
+    if not x.numel() or ((st[-1] == 1 or x.shape[-1] == 1) and x.data_ptr() % n == 0 and
+                         all(s * e % n == 0 for s, m in zip(st[:-1], x.shape) if m > 1)):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def lead_strides(x: torch.Tensor):
-    """Strides of the leading dims, 0 where a dim has one entry (whatever
-    torch says there is never stepped)."""
-    return [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1])]
-
-
-def same_device(what: str, *tensors):
+def same_device(what: str, first: torch.Tensor, *others):
     """The device of every tensor given (None: skipped), a HIP device."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        ptr(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+    dev = first.device
+    if dev.type != "cuda":
+        ptr(first)
+    for t in others:
+        if t is not None and t.device != dev:
+            ptr(t)
             raise CarekvError(f"{what}: tensors on {dev} and {t.device}")
     return dev
+
+
+# the current stream's handle of a device index, without the Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def call(dev: torch.device, what: str, fn, *args):
+    """fn(*args, stream) on dev, whatever device is current; raises on an error code."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc:
+        check(rc, what)
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -350,8 +364,9 @@ def check_out(out: torch.Tensor, shape, dtype, name: str, *inputs: torch.Tensor)
     packed or repeat, and one that overlaps an input other than being it."""
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}; got {tuple(out.shape)} {out.dtype}")
-    if out.numel() and ((out.shape[-1] > 1 and out.stride(-1) != 1) or
-                        any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride()))):
+    if not out.is_contiguous() and out.numel() and (
+            (out.shape[-1] > 1 and out.stride(-1) != 1) or
+            any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride()))):
         raise ValueError(f"{name} needs the values of a row next to each other and no repeated rows")
     if any(overlap(out, x) for x in inputs):
         raise ValueError(f"{name} must be its input itself or not overlap it")

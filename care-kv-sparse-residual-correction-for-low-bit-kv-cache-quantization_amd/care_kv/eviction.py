@@ -50,7 +50,6 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
         q, k = q.unsqueeze(0), k.unsqueeze(0)
         lse = None if lse is None else lse.unsqueeze(0)
         out = None if out is None else out.unsqueeze(0)
-    q, k = q.detach(), k.detach()
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"q must be (B, Hq, Tq, D) and k (B, Hkv, Tk, D); got {tuple(q.shape)} / {tuple(k.shape)}")
     B, Hq, Tq, D = q.shape
@@ -64,7 +63,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
     if lse is not None:
         if lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32:
             raise ValueError(f"lse must be {(B, Hq, Tq)} fp32; got {tuple(lse.shape)} {lse.dtype}")
-        lse = lse.detach().contiguous()
+        lse = lse.contiguous()
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is not None:
@@ -74,22 +73,19 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
         out = torch.empty(B, Hkv, Tk, dtype=torch.float32, device=dev)
     if B and Tk:
         q, k = _lib.aligned_rows(q), _lib.aligned_rows(k)
-        pp = _lib.MassParams(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], int(bool(causal)), int(bool(accumulate)),
-                             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *_lib.lead_strides(q),
-                             *_lib.lead_strides(k), *_lib.lead_strides(out))
+        pp = _lib.MassParams(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], bool(causal), bool(accumulate),
+                             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *q.stride()[:3],
+                             *k.stride()[:3], *out.stride()[:2])
         lib = _lib.load()
-        with torch.cuda.device(dev):
-            qs = _lib.row_counts(q_start, B, dev, "q_start")
-            ln = _lib.row_counts(lengths, B, dev, "lengths")
-            nbytes = int(lib.carekv_attention_mass_workspace_bytes(pp, int(lse is not None)))
-            if nbytes < 0:
-                _lib.check(-1, "carekv_attention_mass_workspace_bytes")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _lib.check(lib.carekv_attention_mass(pp, q.data_ptr(), k.data_ptr(),
-                                                 None if lse is None else lse.data_ptr(),
-                                                 None if qs is None else qs.data_ptr(),
-                                                 None if ln is None else ln.data_ptr(), out.data_ptr(), ws.data_ptr(),
-                                                 nbytes, _lib.stream_ptr(dev)), "carekv_attention_mass")
+        qs = _lib.row_counts(q_start, B, dev, "q_start")
+        ln = _lib.row_counts(lengths, B, dev, "lengths")
+        nbytes = lib.carekv_attention_mass_workspace_bytes(pp, lse is not None)
+        if nbytes < 0:
+            _lib.check(-1, "carekv_attention_mass_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call(dev, "carekv_attention_mass", lib.carekv_attention_mass, pp, q.data_ptr(), k.data_ptr(),
+                  None if lse is None else lse.data_ptr(), None if qs is None else qs.data_ptr(),
+                  None if ln is None else ln.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out[0] if squeeze else out
 
 
@@ -108,7 +104,6 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
     squeeze = mass.dim() == 2
     if squeeze:
         mass, k, v = mass.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
-    mass, k, v = mass.detach(), k.detach(), v.detach()
     if mass.dim() != 3 or mass.dtype != torch.float32:
         raise ValueError(f"mass must be (B, Hkv, T) fp32; got {tuple(mass.shape)} {mass.dtype}")
     B, H, T = mass.shape
@@ -131,15 +126,13 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
     index = torch.empty(B, H, n, dtype=torch.int32, device=dev)
     kept = (torch.empty if B * H * n else torch.zeros)(B, dtype=torch.int32, device=dev)
     if B * H * n:
-        mass, k, v = (_lib.aligned_rows(x, 4) for x in (mass, k, v))
-        pp = _lib.EvictParams(B, H, T, D * e, n, sink, recent, *_lib.lead_strides(mass),
-                              *(s * e for s in _lib.lead_strides(k)), *(s * e for s in _lib.lead_strides(v)))
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            ln = _lib.row_counts(lengths, B, dev, "lengths")
-            _lib.check(lib.carekv_evict_rows(pp, mass.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                             None if ln is None else ln.data_ptr(), kk.data_ptr(), vv.data_ptr(),
-                                             mm.data_ptr(), index.data_ptr(), kept.data_ptr(), _lib.stream_ptr(dev)),
-                       "carekv_evict_rows")
+        mass, k, v = _lib.aligned_rows(mass, 4), _lib.aligned_rows(k, 4), _lib.aligned_rows(v, 4)
+        sk, sv = k.stride(), v.stride()
+        pp = _lib.EvictParams(B, H, T, D * e, n, sink, recent, *mass.stride()[:2], sk[0] * e, sk[1] * e, sk[2] * e,
+                              sv[0] * e, sv[1] * e, sv[2] * e)
+        ln = _lib.row_counts(lengths, B, dev, "lengths")
+        _lib.call(dev, "carekv_evict_rows", _lib.load().carekv_evict_rows, pp, mass.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), None if ln is None else ln.data_ptr(), kk.data_ptr(), vv.data_ptr(), mm.data_ptr(),
+                  index.data_ptr(), kept.data_ptr())
     got = EvictedRows(kk, vv, mm, index, kept)
     return EvictedRows(*(x[0] for x in got[:4]), kept) if squeeze else got

@@ -35,7 +35,6 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         out = None if out is None else out.unsqueeze(2)
         if own is not None:
             o_own, l_own = o_own.unsqueeze(2), l_own.unsqueeze(2)
-    q, k, v = q.detach(), k.detach(), v.detach()
     if q.dim() != 4 or k.dim() != 3:
         raise ValueError(f"q must be (B, Hq, D) or (B, Hq, T, D) and k (Hkv, P, D); got {tuple(q.shape)} / "
                          f"{tuple(k.shape)}")
@@ -52,9 +51,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                 l_own.dtype != torch.float32:
             raise ValueError(f"own must be an output like q and its fp32 log-sum-exp {tuple(q.shape[:3])}; got "
                              f"{tuple(o_own.shape)} {o_own.dtype}, {tuple(l_own.shape)} {l_own.dtype}")
-        o_own = o_own.detach()
-        o_own = o_own if o_own.stride(-1) == 1 or not o_own.numel() else o_own.contiguous()
-        l_own = l_own.detach().contiguous()
+        o_own = o_own if o_own.stride(3) == 1 else o_own.contiguous()
+        l_own = l_own.contiguous()
     if out is not None:
         _lib.check_out(out, q.shape, q.dtype, "out", q, k, v, *(() if own is None else (o_own,)))
     dev = _lib.same_device("prefix_attention", q, k, v, o_own, l_own, out)
@@ -62,22 +60,19 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(B, Hq, T, dtype=torch.float32, device=dev) if return_lse else None
     if out.numel():
-        q, k, v = (_lib.aligned_rows(x) for x in (q, k, v))
+        q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k), _lib.aligned_rows(v)
         pp = _lib.PrefixParams(B, Hq, Hkv, T, P, D, _lib.DTYPE_CODE[q.dtype],
-                               1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *_lib.lead_strides(q),
-                               *_lib.lead_strides(k), *_lib.lead_strides(v), *_lib.lead_strides(out),
-                               *((0, 0, 0) if own is None else _lib.lead_strides(o_own)))
+                               1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *q.stride()[:3],
+                               *k.stride()[:2], *v.stride()[:2], *out.stride()[:3],
+                               *((0, 0, 0) if own is None else o_own.stride()[:3]))
         lib = _lib.load()
-        with torch.cuda.device(dev):
-            nbytes = int(lib.carekv_prefix_attn_workspace_bytes(pp))
-            if nbytes < 0:
-                _lib.check(-1, "carekv_prefix_attn_workspace_bytes")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _lib.check(lib.carekv_prefix_attn(pp, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                              None if own is None else o_own.data_ptr(),
-                                              None if own is None else l_own.data_ptr(), out.data_ptr(),
-                                              None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes,
-                                              _lib.stream_ptr(dev)), "carekv_prefix_attn")
+        nbytes = lib.carekv_prefix_attn_workspace_bytes(pp)
+        if nbytes < 0:
+            _lib.check(-1, "carekv_prefix_attn_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call(dev, "carekv_prefix_attn", lib.carekv_prefix_attn, pp, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  None if own is None else o_own.data_ptr(), None if own is None else l_own.data_ptr(), out.data_ptr(),
+                  None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     if one:
         out, lse = out.squeeze(2), None if lse is None else lse.squeeze(2)
     return (out, lse) if return_lse else out

@@ -109,7 +109,6 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         a, b = rotate_heads(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, plan, inverse=inverse,
                             out=None if out is None else (qo.unsqueeze(0), None if ko is None else ko.unsqueeze(0)))
         return a[0], None if b is None else b[0]
-    q, k = q.detach(), None if k is None else k.detach()
     if q.dim() != 4:
         raise ValueError(f"q must be (B, heads, T, D) or (heads, T, D); got {tuple(q.shape)}")
     B, Hq, T, D = q.shape
@@ -126,27 +125,29 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise ValueError(f"positions must be ({B}, {T}), (1, {T}) or ({T},); got {tuple(positions.shape)}")
     if out is not None and (len(out) != 2 or out[0] is None or (out[1] is None) != (k is None)):
         raise ValueError("out must be (q_out, k_out), k_out None only without k")
-    qo, ko = (None, None) if out is None else out
-    for x, o, nm in ((q, qo, "q_out"), (k, ko, "k_out")):
-        if o is not None:
-            _lib.check_out(o, x.shape, x.dtype, nm, x)
-    dev = _lib.same_device("rotate_heads", q, k, positions, plan.freqs, qo, ko)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=dev) if qo is None else qo
-    if k is not None:
-        ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if ko is None else ko
-    pos = pos.contiguous() if pos.stride(-1) != 1 else pos
-    q = q.contiguous() if q.stride(-1) != 1 else q
-    k = k.contiguous() if k is not None and k.stride(-1) != 1 else k
-    s = [0] * 12
-    for at, x in ((0, q), (3, k), (6, qo), (9, ko)):
-        if x is not None:
-            s[at:at + 3] = _lib.lead_strides(x)
-    pp = _lib.RotaryParams(B, T, Hq, 0 if k is None else k.shape[1], D, plan.rotary_dim, _lib.DTYPE_CODE[q.dtype],
-                           int(plan.layout == "interleaved"), int(bool(inverse)), 64 if pos.dtype == torch.int64 else 32,
-                           plan.scale, pos.stride(0) if pos.shape[0] > 1 else 0, *s)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.carekv_rotate_heads(pp, q.data_ptr(), None if k is None else k.data_ptr(), pos.data_ptr(),
-                                           plan.freqs.data_ptr(), qo.data_ptr(), None if ko is None else ko.data_ptr(),
-                                           _lib.stream_ptr(dev)), "carekv_rotate_heads")
+    if out is not None:
+        _lib.check_out(out[0], q.shape, q.dtype, "q_out", q)
+        if k is not None:
+            _lib.check_out(out[1], k.shape, k.dtype, "k_out", k)
+    dev = _lib.same_device("rotate_heads", q, k, positions, plan.freqs, *(() if out is None else out))
+    if out is None:
+        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    else:
+        qo, ko = out
+    pos = pos if pos.stride(1) == 1 or T == 1 else pos.contiguous()
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    sq, so = q.stride(), qo.stride()
+    if k is None:
+        hk, kp, kop, sk, sko = 0, None, None, (0, 0, 0), (0, 0, 0)
+    else:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        hk, kp, kop, sk, sko = k.shape[1], k.data_ptr(), ko.data_ptr(), k.stride(), ko.stride()
+    pp = _lib.RotaryParams(B, T, Hq, hk, D, plan.rotary_dim, _lib.DTYPE_CODE[q.dtype], plan.layout == "interleaved",
+                           bool(inverse), 64 if pos.dtype == torch.int64 else 32, plan.scale,
+                           pos.stride(0) if pos.shape[0] > 1 else 0, *sq[:3], *sk[:3], *so[:3], *sko[:3])
+    _lib.call(dev, "carekv_rotate_heads", _lib.load().carekv_rotate_heads, pp, q.data_ptr(), kp, pos.data_ptr(),
+              plan.freqs.data_ptr(), qo.data_ptr(), kop)
     return qo, ko

@@ -170,8 +170,9 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
   a.m_sb = p.mass_sb * 4; a.m_sh = p.mass_sh * 4;
   a.k_sb = p.k_sb; a.k_sh = p.k_sh; a.k_st = p.k_st; a.v_sb = p.v_sb; a.v_sh = p.v_sh; a.v_st = p.v_st;
   a.H = p.n_kv_heads; a.T = p.n_keys; a.keep = p.keep; a.sink = p.sink; a.recent = p.recent; a.row_bytes = p.row_bytes;
-  uintptr_t bits = (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)p.row_bytes;
-  for (int64_t x : {p.k_sb, p.k_sh, p.k_st, p.v_sb, p.v_sh, p.v_st}) bits |= (uintptr_t)x;
+  const uintptr_t bits = operand_bits(k, {{p.batch, p.k_sb}, {p.n_kv_heads, p.k_sh}, {p.n_keys, p.k_st}}) |
+                         operand_bits(v, {{p.batch, p.v_sb}, {p.n_kv_heads, p.v_sh}, {p.n_keys, p.v_st}}) |
+                         (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)p.row_bytes;
   CAREKV_REQUIRE((bits & 3) == 0, "K and V rows must be 4-byte aligned");
   const bool wide = (bits & 15) == 0;
   const int per = p.row_bytes / (wide ? 16 : 4);

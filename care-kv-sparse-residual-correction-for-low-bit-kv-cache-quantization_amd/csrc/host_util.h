@@ -4,7 +4,9 @@
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "carekv.h"
 
@@ -30,6 +32,15 @@ void set_error(const char* fmt, ...);
       return CAREKV_ELAUNCH;                                                                \
     }                                                                                       \
   } while (0)
+
+// The bits of an operand's address and of the strides (bytes) of the dims it
+// steps: those of one entry do not count, whatever the caller has there.
+inline uintptr_t operand_bits(const void* p, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+  uintptr_t bits = (uintptr_t)p;
+  for (const auto& d : dims)
+    if (d.first > 1) bits |= (uintptr_t)d.second;
+  return bits;
+}
 
 // Validate the arena against what the kernels support.  On failure the
 // message is left in last_error_buf().

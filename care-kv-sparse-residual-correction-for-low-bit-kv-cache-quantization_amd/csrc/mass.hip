@@ -5,19 +5,35 @@
 // Query row i stands at position q_start + i and sees the keys j below
 // min(length, position + 1) (not causal: below the length).
 //
-// Key-stationary: a work-group keeps 128 keys (4 waves of 32, the A operand of
-// S^T = K Q^T in registers) and walks over 32-query tiles of every head of the
-// group staged in LDS, so that a key's weights add up in one lane group's
-// registers and nothing of size queries x keys is written.  Rows are walked a
-// head at a time from the first that sees the block, or, where a head has
-// fewer rows than a tile, all heads' rows as one list.  Without lse a first
-// pass of the same walk writes each block's (maximum, sum) per row and
-// mass_join_kernel joins them; the second pass reads K again from the caches.
+// mass_kernel, key-stationary: a work-group keeps 256 keys (8 waves of 32, the
+// A operand of S^T = K Q^T in registers) and walks over 64-row tiles of q
+// staged in LDS, so that a key's weights add up in registers and nothing of
+// size queries x keys is written.  Heads are walked one after the other, each
+// from the first row that sees the block; heads of fewer than 32 rows as one
+// list.  Where the key blocks alone do not fill the GPU a walk is cut into
+// parts, whose sums mass_sum_kernel adds in order.
+//
+// stats_kernel, its mirror image for calls without lse: 256 query rows
+// stationary, key tiles walked, each lane with its own (reference, sum) per row.
+// The reference is no maximum, only a value that no logit passes by 2^64: sums
+// stay in 32-bit range, their accuracy is relative, so that it need not move
+// with every larger score.  mass_join_kernel joins the walks' parts.
+//
+// mass_few_kernel, at most 16 rows a kv head (a decode step): a work-group a
+// (sequence, kv head), the scores of all keys in LDS, K read once, one launch.
+//
+// Measured, 32 / 8 heads, D = 128, 8192 causal rows with lse (275 GFLOP of
+// products, 1.07e9 exponentials): 355-370 us, 0.75 PFLOP/s; the same with 4
+// waves of 64 keys (2 waves a SIMD, or 3) and with 32 x 32 products (374).
+// Without its exponentials it took 322 us, without products 240, without LDS
+// reads 297, without tile loads 311: no one pipe bounds it, their sum does.  A
+// window of 64 rows on 4 x 8191 keys: 28 us statistics, 31 us weights, each
+// reading K (67 MB, 13 us at the copy rate).
 //
 // Sums: a lane adds at most kFlush tiles' weights before they go to an outer
 // sum, so that a key's total over 2^15 rows keeps the accuracy of a short sum.
-// The rows' statistics are (M, w): a weight is 2^(x - M) w, with w = 1 / sum,
-// or for a given lse the part of lse log2(e) that a 32-bit M does not hold.
+// A row's statistics are (M, w): a weight is 2^(x - M) w, with w = 1 / sum, or
+// for a given lse the part of lse log2(e) that a 32-bit M does not hold.
 #include <algorithm>
 
 #include "mfma16.h"
@@ -31,106 +47,300 @@ struct MassArgs {
   const int32_t* q_start;  // [B], or null: the last Tq of the length
   const int32_t* lengths;  // [B], or null
   float* out;
-  float* part;             // [B][Hkv][rows][nkb][2] maximum (base 2), sum
-  float* stat;             // [B][Hkv][rows][2] M, w
+  float* part;             // [B][Hkv][rows][nsk][2] reference (base 2), sum
+  float* stat;             // [B][Hkv][rows][2] M, w (no lse)
+  float* opart;            // [parts][B][Hkv][Tk], parts > 1
   long q_sb, q_sh, q_st, k_sb, k_sh, k_st;  // bytes
   long o_sb, o_sh;                          // elements
-  int B, Hq, Hkv, G, Tq, Tk, nkb, causal, accumulate;
-  int nseg, seg;           // the walk: nseg lists of seg rows
+  int B, Hq, Hkv, G, Tq, Tk, causal, accumulate;
+  int nkb, psg, prow;      // mass walks: key blocks; a walk's lists and each list's rows cut into so many parts
+  int parts;               // psg * prow
+  int nqb, nsk;            // statistics: row blocks, parts of a walk
+  int nseg, seg;           // a mass walk: nseg lists of seg rows
   float sm_log2;
 };
 
-constexpr int kMassKeys = 128, kMassTile = 32, kFlush = 16;
+constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072;
 
-// Keys that row (head-local) t of sequence b sees: j < the result (0: none)
-__device__ __forceinline__ int mass_limit(const MassArgs& a, int b, int t) {
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-  if (!a.causal) return len;
-  const long pos = (a.q_start ? (long)a.q_start[b] : (long)len - a.Tq) + t;
-  return (int)max(0L, min((long)len, pos + 1));
+// A sequence's visible keys: row t sees j < min(len, qs + t + 1), not causal: j < len.
+struct MassSeq {
+  int len;
+  long qs;
+};
+__device__ __forceinline__ MassSeq mass_seq(const MassArgs& a, int b) {
+  MassSeq s;
+  s.len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  s.qs = a.q_start ? (long)a.q_start[b] : (long)s.len - a.Tq;
+  return s;
+}
+__device__ __forceinline__ int mass_limit(const MassArgs& a, const MassSeq& s, int t) {
+  return a.causal ? (int)max(0L, min((long)s.len, s.qs + t + 1)) : s.len;
 }
 
-template <typename ET, int D, bool STATS>
-__global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
+// (M, w) of a row with log-sum-exp l: l log2(e) = M + rest, M the rounded
+// product, rest what it lost.  Infinite l: weights of 0.  NaN goes on as NaN.
+__device__ __forceinline__ float2 lse_stat(float l) {
+  float2 st = make_float2(INFINITY, 0.f);
+  if (!(fabsf(l) >= 1e30f)) {
+    st.x = l * kLog2e;
+    const float rest = fmaf(l, kLog2e, -st.x) + l * 1.9259629911266174e-8f;  // log2(e) - float(log2(e))
+    st.y = __builtin_amdgcn_exp2f(-rest);
+  }
+  return st;
+}
+
+template <typename V8>
+__device__ __forceinline__ V8 load8(const char* p) {
+  V8 x;
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  __builtin_memcpy(&x, &v, 16);
+  return x;
+}
+
+template <typename ET, int D>
+__global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   using V8 = typename ET::V8;
-  constexpr int KS = D / 32, QRS = 2 * D + 16, CHR = D / 8, NCH = kMassTile * CHR / 256;
-  static_assert(NCH >= 1, "a thread stages whole chunks");
-  __shared__ __align__(16) char lds[2][kMassTile * QRS];
-  __shared__ float s_m[2][kMassTile], s_w[2][kMassTile];
-  __shared__ int s_lim[2][kMassTile];
-  __shared__ float s_red[STATS ? 4 * kMassTile * 2 : 1];
-  const int hb = blockIdx.x % (a.Hkv * a.B), kb = blockIdx.x / (a.Hkv * a.B);
+  constexpr int TT = kMassKeys / 128, QT = kMassTile, KS = D / 32, QRS = 2 * D + 16, CHR = D / 8, NCH = QT * CHR / 512;
+  __shared__ __align__(16) char lds[2][QT * QRS];
+  __shared__ float2 s_st[2][QT];
+  __shared__ int s_lim[2][QT];
+  // Sequences and heads go round the XCDs, and the blocks of one part, which walk over the same rows, run
+  // together: they meet in one L2.  The longest walks of a part first.
+  const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
+  const int kb = rest % a.nkb, pt = rest / a.nkb;
   const int b = hb / a.Hkv, hk = hb % a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int j0 = kb * kMassKeys + 32 * w;  // first key of the wave
+  const int j0 = kb * kMassKeys + 16 * TT * w;  // first key of the wave
+  const MassSeq sq = mass_seq(a, b);
   // K operands: tokens j0 + 16 tt + c16, dims 32 s + 8 g .. (keys past the end: the last one, masked below)
-  V8 kf[2][KS];
+  V8 kf[TT][KS];
 #pragma unroll
-  for (int tt = 0; tt < 2; ++tt) {
+  for (int tt = 0; tt < TT; ++tt) {
     const char* kp = a.k + b * a.k_sb + hk * a.k_sh + (long)min(j0 + 16 * tt + c16, a.Tk - 1) * a.k_st;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const uint4 v = *reinterpret_cast<const uint4*>(kp + (32 * s + 8 * g) * 2);
-      __builtin_memcpy(&kf[tt][s], &v, 16);
-    }
+    for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
   }
-  const long rows = (long)a.G * a.Tq;
-  const long hrow = (long)hb * rows;  // first row of this (sequence, kv head) in part / stat
+  const long hrow = (long)hb * a.G * a.Tq;  // first row of this (sequence, kv head) in stat / lse
   // rows of a list below t_first see nothing of the block
-  int t_first = 0;
-  if (a.causal && a.nseg > 1) {
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-    const long qs = a.q_start ? (long)a.q_start[b] : (long)len - a.Tq;
-    t_first = (int)min((long)a.seg, max(0L, (long)kb * kMassKeys - qs));
-    if ((long)kb * kMassKeys >= len) t_first = a.seg;
-  }
-  const int per = (a.seg - t_first + kMassTile - 1) / kMassTile, nt = per * a.nseg;
+  const bool listed = a.nseg > 1 || a.G == 1;  // a list is a head's rows
+  const int sg0 = a.nseg * (pt / a.prow) / a.psg, sg1 = a.nseg * (pt / a.prow + 1) / a.psg;
+  const int tiles = (a.seg + QT - 1) / QT, pr = pt % a.prow;
+  int t_first = (int)((long)tiles * pr / a.prow) * QT;
+  const int t_end = min((int)((long)tiles * (pr + 1) / a.prow) * QT, a.seg);
+  if (kb * kMassKeys >= sq.len) t_first = t_end;
+  else if (a.causal && listed) t_first = (int)min((long)t_end, max((long)t_first, (long)kb * kMassKeys - sq.qs));
+  const int nt = (t_end - t_first + QT - 1) / QT * (sg1 - sg0);
+  int sg = sg0, i0 = t_first;  // the tile loaded next
   uint32_t stg[NCH][4];
-  float n_m = 0.f, n_w = 0.f;
+  float2 n_st = make_float2(0.f, 0.f);
   int n_lim = 0;
-  // row of list position p of list sg: head sg and row p, or the rows of all heads in order
-  auto locate = [&](int j, int p, int& h, int& t) {
-    const int sg = j / per, i = t_first + (j - sg * per) * kMassTile + p;
-    if (a.nseg > 1) { h = sg; t = i; }
-    else { h = i / a.Tq; t = i - h * a.Tq; }
-    return i < a.seg;
-  };
-  auto load_tile = [&](int j) {
+  // A list's rows lie one row stride apart: a tile is a buffer resource of its rows (those behind the part's
+  // end read as zeros), a thread's offsets in it stay the same.  Other lists find their rows one by one.
+  uint32_t off[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      const int cid = threadIdx.x + 256 * k, row = cid / CHR, col = cid % CHR;
-      int h, t;
-      const bool in = locate(j, row, h, t);
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (in) v = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st + col * 16);
-      stg[k][0] = v.x; stg[k][1] = v.y; stg[k][2] = v.z; stg[k][3] = v.w;
-    }
-    if (threadIdx.x < kMassTile) {
-      int h, t;
-      const bool in = locate(j, threadIdx.x, h, t);
-      n_lim = in ? mass_limit(a, b, t) : 0;
-      if (!STATS && in) {
-        const float2 st = *reinterpret_cast<const float2*>(a.stat + 2 * (hrow + (long)h * a.Tq + t));
-        n_m = st.x; n_w = st.y;
-      } else {
-        n_m = 0.f; n_w = 0.f;
+  for (int k = 0; k < NCH; ++k)
+    off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.q_st + (threadIdx.x % CHR) * 16);
+  const char* qbase = a.q + b * a.q_sb + (long)hk * a.G * a.q_sh;
+  auto load_tile = [&]() {
+    if (listed) {
+      const __amdgpu_buffer_rsrc_t rq = make_rsrc(qbase + sg * a.q_sh + i0 * a.q_st,
+                                                  (uint32_t)((min(QT, t_end - i0) - 1) * a.q_st + 2 * D));
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(rq, off[k], 0, 0);
+        stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        const int i = i0 + (int)threadIdx.x / CHR + 512 / CHR * k, h = i / a.Tq, t = i - h * a.Tq;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (i < t_end)
+          v = *reinterpret_cast<const uint4*>(qbase + h * a.q_sh + t * a.q_st + (threadIdx.x % CHR) * 16);
+        stg[k][0] = v.x; stg[k][1] = v.y; stg[k][2] = v.z; stg[k][3] = v.w;
       }
     }
+    if (threadIdx.x < QT) {
+      const int i = i0 + threadIdx.x;
+      int h = sg, t = i;
+      if (!listed) { h = i / a.Tq; t = i - h * a.Tq; }
+      n_lim = 0;
+      n_st = make_float2(INFINITY, 0.f);
+      if (i < t_end) {
+        n_lim = mass_limit(a, sq, t);
+        const long r = hrow + (long)h * a.Tq + t;
+        n_st = a.lse ? lse_stat(a.lse[r]) : *reinterpret_cast<const float2*>(a.stat + 2 * r);
+      }
+    }
+    i0 += QT;
+    if (i0 >= t_end) { i0 = t_first; ++sg; }
   };
   auto store_tile = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int cid = threadIdx.x + 256 * k, row = cid / CHR, col = cid % CHR;
-      *reinterpret_cast<uint4*>(lds[buf] + row * QRS + col * 16) = make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
+      const int row = threadIdx.x / CHR + 512 / CHR * k;
+      *reinterpret_cast<uint4*>(lds[buf] + row * QRS + (threadIdx.x % CHR) * 16) =
+          make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
     }
-    if (threadIdx.x < kMassTile) {
-      s_lim[buf][threadIdx.x] = n_lim; s_m[buf][threadIdx.x] = n_m; s_w[buf][threadIdx.x] = n_w;
+    if (threadIdx.x < QT) { s_lim[buf][threadIdx.x] = n_lim; s_st[buf][threadIdx.x] = n_st; }
+  };
+  float acc[4 * TT], sum[4 * TT];
+#pragma unroll
+  for (int i = 0; i < 4 * TT; ++i) acc[i] = sum[i] = 0.f;
+  int ci = i0;  // first row of the tile computed next
+  if (nt > 0) {
+    load_tile();
+    store_tile(0);
+  }
+  __syncthreads();
+  int ni = i0;
+  if (nt > 1) load_tile();
+  for (int j = 0; j < nt; ++j) {
+    const int buf = j & 1;
+    // some pair of the tile and the wave's keys is masked
+    const bool edge = !listed || ci + QT > t_end || j0 + 16 * TT > sq.len ||
+                      (a.causal && sq.qs + ci + 1 < j0 + 16 * TT);
+    // the next 16 rows' products are issued before this one's exponentials: they run side by side
+    float4_t s[2][TT];
+    auto scores = [&](int qb, float4_t* x) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) x[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const V8 qf = load8<V8>(lds[buf] + (16 * qb + c16) * QRS + (32 * ks + 8 * g) * 2);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) x[tt] = ET::mfma(kf[tt][ks], qf, x[tt]);
+      }
+    };
+    scores(0, s[0]);
+    if (!edge) {
+#pragma unroll
+      for (int qb = 0; qb < QT / 16; ++qb) {
+        if (qb + 1 < QT / 16) scores(qb + 1, s[(qb + 1) & 1]);
+        const float2 st = s_st[buf][16 * qb + c16];
+#pragma unroll
+        for (int i = 0; i < 4 * TT; ++i)
+          acc[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[qb & 1][i / 4][i % 4], a.sm_log2, -st.x)), st.y, acc[i]);
+      }
+    } else {
+#pragma unroll
+      for (int qb = 0; qb < QT / 16; ++qb) {
+        if (qb + 1 < QT / 16) scores(qb + 1, s[(qb + 1) & 1]);
+        const float2 st = s_st[buf][16 * qb + c16];
+        const int lim = s_lim[buf][16 * qb + c16] - j0 - 4 * g;  // token 16 tt + i of the lane is seen below it
+#pragma unroll
+        for (int i = 0; i < 4 * TT; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[qb & 1][i / 4][i % 4], a.sm_log2, -st.x));
+          acc[i] = 16 * (i / 4) + i % 4 < lim ? fmaf(p, st.y, acc[i]) : acc[i];
+        }
+      }
+    }
+    if ((j + 1) % kFlush == 0) {
+#pragma unroll
+      for (int i = 0; i < 4 * TT; ++i) { sum[i] += acc[i]; acc[i] = 0.f; }
+    }
+    ci = ni;
+    if (j + 1 < nt) store_tile((j + 1) & 1);
+    if (j + 2 < nt) { ni = i0; load_tile(); }
+    __syncthreads();
+  }
+  // over the 16 query columns, in a fixed order
+  float* dst = a.parts > 1 ? a.opart + ((long)pt * nhb + hb) * a.Tk : a.out + b * a.o_sb + hk * a.o_sh;
+#pragma unroll
+  for (int i = 0; i < 4 * TT; ++i) {
+    float v = sum[i] + acc[i];
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
+    const int key = j0 + 16 * (i / 4) + 4 * g + i % 4;
+    if (c16 == 0 && key < a.Tk) dst[key] = a.accumulate && a.parts == 1 ? dst[key] + v : v;
+  }
+}
+
+// The parts of the walks, in order.
+__global__ __launch_bounds__(256) void mass_sum_kernel(MassArgs a) {
+  const long n = (long)a.B * a.Hkv * a.Tk, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v = 0.f;
+  for (int p = 0; p < a.parts; ++p) v += a.opart[p * n + i];
+  const long hb = i / a.Tk, b = hb / a.Hkv;
+  float* dst = a.out + b * a.o_sb + (hb - b * a.Hkv) * a.o_sh + (i - hb * a.Tk);
+  *dst = a.accumulate ? *dst + v : v;
+}
+
+template <typename ET, int D>
+__global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
+  using V8 = typename ET::V8;
+  constexpr int TT = 2, KT = kMassTile, KS = D / 32, KRS = 2 * D + 16, CHR = D / 8, NCH = KT * CHR / 512;
+  constexpr float kOver = 64.f;
+  __shared__ __align__(16) char lds[2][KT * KRS];
+  const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
+  const int sp = rest % a.nsk, qblk = a.nqb - 1 - rest / a.nsk;  // the longest walks (latest rows) first
+  const int b = hb / a.Hkv, hk = hb % a.Hkv;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int rows = a.G * a.Tq, r0 = qblk * 256 + 16 * TT * w;
+  const MassSeq sq = mass_seq(a, b);
+  V8 qf[TT][KS];
+  int lim[4 * TT], lo = 0x7fffffff;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    const int r = min(r0 + 16 * tt + c16, rows - 1), h = r / a.Tq, t = r - h * a.Tq;
+    const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[tt][s] = load8<V8>(qp + (32 * s + 8 * g) * 2);
+  }
+  // keys that the lane's rows r0 + 16 tt + 4 g + i see, and the furthest and nearest end over the work-group / wave
+  int hi = 0;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    int r = r0 + 16 * tt + 4 * g, t = r % a.Tq;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, ++r) {
+      lim[4 * tt + i] = r < rows ? mass_limit(a, sq, t) : 0;
+      t = t + 1 == a.Tq ? 0 : t + 1;
+      lo = min(lo, lim[4 * tt + i]);
+      hi = max(hi, lim[4 * tt + i]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 64));
+    hi = max(hi, __shfl_xor(hi, o, 64));
+  }
+  __shared__ int s_hi[8];
+  if (lane == 0) s_hi[w] = hi;
+  __syncthreads();
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  int end = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) end = max(end, s_hi[i]);
+  const int all = (end + KT - 1) / KT;
+  const int t0 = (int)((long)all * sp / a.nsk), nt = (int)((long)all * (sp + 1) / a.nsk) - t0;
+  uint32_t stg[NCH][4];
+  uint32_t off[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+    off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.k_st + (threadIdx.x % CHR) * 16);
+  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
+  auto load_tile = [&](int j) {  // (keys behind the sequence's end read as zeros; they are masked)
+    const int k0 = (t0 + j) * KT;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + k0 * a.k_st, (uint32_t)((min(KT, sq.len - k0) - 1) * a.k_st + 2 * D));
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(rk, off[k], 0, 0);
+      stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
     }
   };
-  float acc[8], sum[8];
+  auto store_tile = [&](int buf) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = sum[i] = 0.f;
+    for (int k = 0; k < NCH; ++k)
+      *reinterpret_cast<uint4*>(lds[buf] + (threadIdx.x / CHR + 512 / CHR * k) * KRS + (threadIdx.x % CHR) * 16) =
+          make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
+  };
+  float m[4 * TT], l[4 * TT];
+#pragma unroll
+  for (int i = 0; i < 4 * TT; ++i) { m[i] = kLowest; l[i] = 0.f; }
   if (nt > 0) {
     load_tile(0);
     store_tile(0);
@@ -138,116 +348,183 @@ __global__ __launch_bounds__(256) void mass_kernel(MassArgs a) {
   __syncthreads();
   if (nt > 1) load_tile(1);
   for (int j = 0; j < nt; ++j) {
-    const char* qb_ = lds[j & 1];
+    const int buf = j & 1, k0 = (t0 + j) * KT;
+    if (k0 < hi) {
+      const bool edge = k0 + KT > lo;
+      float4_t sb[2][TT];
+      auto scores = [&](int kb, float4_t* y) {
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      float4_t s[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
+        for (int tt = 0; tt < TT; ++tt) y[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        V8 qf;
-        *reinterpret_cast<uint4*>(&qf) = *reinterpret_cast<const uint4*>(qb_ + (16 * qb + c16) * QRS + (32 * ks + 8 * g) * 2);
-        s[0] = ET::mfma(kf[0][ks], qf, s[0]);
-        s[1] = ET::mfma(kf[1][ks], qf, s[1]);
+        for (int ks = 0; ks < KS; ++ks) {
+          const V8 kf = load8<V8>(lds[buf] + (16 * kb + c16) * KRS + (32 * ks + 8 * g) * 2);
+#pragma unroll
+          for (int tt = 0; tt < TT; ++tt) y[tt] = ET::mfma(qf[tt][ks], kf, y[tt]);
+        }
+      };
+      scores(0, sb[0]);
+#pragma unroll
+      for (int kb = 0; kb < KT / 16; ++kb) {
+        if (kb + 1 < KT / 16) scores(kb + 1, sb[(kb + 1) & 1]);
+        const float4_t* s = sb[kb & 1];
+        float x[4 * TT], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * TT; ++i) x[i] = fmaf(s[i / 4][i % 4], a.sm_log2, -m[i]);
+        if (edge) {
+          const int key = k0 + 16 * kb + c16;
+#pragma unroll
+          for (int i = 0; i < 4 * TT; ++i)
+            if (key >= lim[i]) x[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * TT; i += 2) top = fmaxf(fmaxf(top, x[i]), x[i + 1]);
+        if (__any(top > kOver)) {  // some lane's logit is past its reference by 2^64: it becomes the reference
+#pragma unroll
+          for (int i = 0; i < 4 * TT; ++i) {
+            if (x[i] > kOver) {
+              const float mn = s[i / 4][i % 4] * a.sm_log2;
+              l[i] *= __builtin_amdgcn_exp2f(m[i] - mn);
+              m[i] = mn;
+              x[i] = fmaf(s[i / 4][i % 4], a.sm_log2, -mn);  // (what the product's rounding left)
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * TT; ++i) l[i] += __builtin_amdgcn_exp2f(x[i]);
       }
-      const int col = 16 * qb + c16;
-      const int lim = s_lim[j & 1][col] - j0 - 4 * g;  // token 16 tt + i of the lane is seen below it
-      const bool edge = __any(lim < 32 - 4 * g);
-      if (STATS) {
-        float x[8], mx = kLowest;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = s[i / 4][i % 4] * a.sm_log2;
-          if (edge && 16 * (i / 4) + i % 4 >= lim) x[i] = -INFINITY;
-          mx = fmaxf(mx, x[i]);
-        }
-        mx = col_max(mx);
-        float l = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) l += __builtin_amdgcn_exp2f(x[i] - mx);
-        l = col_sum(l);
-        if (g == 0) {
-          s_red[(w * kMassTile + col) * 2] = mx;
-          s_red[(w * kMassTile + col) * 2 + 1] = l;
-        }
-      } else {
-        const float m = s_m[j & 1][col], wt = s_w[j & 1][col];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.sm_log2, -m));
-          if (!edge) acc[i] = fmaf(p, wt, acc[i]);
-          else if (16 * (i / 4) + i % 4 < lim) acc[i] = fmaf(p, wt, acc[i]);
-        }
-      }
-    }
-    if (!STATS && (j + 1) % kFlush == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) { sum[i] += acc[i]; acc[i] = 0.f; }
     }
     if (j + 1 < nt) store_tile((j + 1) & 1);
     if (j + 2 < nt) load_tile(j + 2);
     __syncthreads();
-    if (STATS) {
-      if (threadIdx.x < kMassTile) {
-        int h, t;
-        if (locate(j, threadIdx.x, h, t)) {
-          float m = kLowest, l = 0.f;
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, s_red[(i * kMassTile + threadIdx.x) * 2]);
-          for (int i = 0; i < 4; ++i)
-            l += s_red[(i * kMassTile + threadIdx.x) * 2 + 1] * __builtin_amdgcn_exp2f(s_red[(i * kMassTile + threadIdx.x) * 2] - m);
-          float* p = a.part + 2 * ((hrow + (long)h * a.Tq + t) * a.nkb + kb);
-          p[0] = m;
-          p[1] = l;
-        }
-      }
-      __syncthreads();
-    }
   }
-  if (!STATS) {
-    // over the 16 query columns, in a fixed order
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = sum[i] + acc[i];
+  for (int i = 0; i < 4 * TT; ++i) {
+    float mm = m[i];
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
-      const int key = j0 + 16 * (i / 4) + 4 * g + i % 4;
-      if (c16 == 0 && key < a.Tk) {
-        float* p = a.out + b * a.o_sb + hk * a.o_sh + key;
-        *p = a.accumulate ? *p + v : v;
-      }
+    for (int o = 1; o < 16; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+    float v = l[i] * __builtin_amdgcn_exp2f(m[i] - mm);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
+    const int r = r0 + 16 * (i / 4) + 4 * g + i % 4;
+    if (c16 == 0 && r < rows) {
+      float* p = a.part + 2 * (((long)hb * rows + r) * a.nsk + sp);
+      p[0] = mm;
+      p[1] = v;
     }
   }
 }
 
-// (M, w) of every row: from the blocks' partials, or from the given lse.  A
-// row that sees nothing, or whose lse is infinite, has (inf, 0): weights of 0.
+// (M, w) of every row from the parts of its walk.  A row that sees nothing
+// has (inf, 0): weights of 0.
 __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long per_b = (long)a.Hq * a.Tq;
-  if (i >= a.B * per_b) return;
-  const int b = (int)(i / per_b), t = (int)(i % a.Tq);
-  float m = INFINITY, w = 0.f;
-  if (a.lse) {
-    // lse log2(e) = M + rest: M the rounded product, rest what it lost (NaN goes on as NaN)
-    const float l = a.lse[i];
-    if (!(fabsf(l) >= 1e30f)) {
-      m = l * kLog2e;
-      const float rest = fmaf(l, kLog2e, -m) + l * 1.9259629911266174e-8f;  // log2(e) - float(log2(e))
-      w = __builtin_amdgcn_exp2f(-rest);
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) / 8;  // 8 lanes a row
+  const int u = threadIdx.x & 7;
+  const bool in = i < (long)a.B * a.Hq * a.Tq;
+  const float2* p = reinterpret_cast<const float2*>(a.part) + (in ? i : 0) * a.nsk;
+  float mx = kLowest, l = 0.f;
+  for (int s = u; s < a.nsk; s += 8) {
+    const float2 v = p[s];
+    const float m = fmaxf(mx, v.x);
+    l = l * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
+    mx = m;
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const float m = fmaxf(mx, __shfl_xor(mx, o, 64)), f = l * __builtin_amdgcn_exp2f(mx - m);
+    l = f + __shfl_xor(f, o, 64);
+    mx = m;
+  }
+  if (in && u == 0)
+    reinterpret_cast<float2*>(a.stat)[i] = l != 0.f ? make_float2(mx, 1.f / l) : make_float2(INFINITY, 0.f);
+}
+
+// At most 16 rows a kv head: 16 waves take 64 keys each in turn.  Lane: keys
+// 16 tt + 4 g + i, row c16.
+template <typename ET, int D>
+__global__ __launch_bounds__(1024) void mass_few_kernel(MassArgs a, int stride) {
+  using V8 = typename ET::V8;
+  constexpr int KS = D / 32, TT = 4;
+  __shared__ __align__(16) float sc[kFewLds / 4];  // [rows][stride] base-2 logits
+  __shared__ float s_m[16][16], s_l[16][16];
+  __shared__ float2 s_st[16];
+  const int hb = blockIdx.x, b = hb / a.Hkv, hk = hb % a.Hkv, rows = a.G * a.Tq;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const MassSeq sq = mass_seq(a, b);
+  const int r = min(c16, rows - 1), h = r / a.Tq, t = r - h * a.Tq;
+  const int lim = c16 < rows ? mass_limit(a, sq, t) : 0;
+  V8 qf[KS];
+  const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = load8<V8>(qp + (32 * s + 8 * g) * 2);
+  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
+  const int nt = (sq.len + 16 * TT - 1) / (16 * TT);  // tiles with keys
+  V8 kf[TT][KS];
+  auto load_keys = [&](int j) {
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      const char* kp = kbase + (long)min(16 * (TT * j + tt) + c16, sq.len - 1) * a.k_st;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
     }
-  } else {
-    // a causal row has partials of the blocks that it can see
-    const int lim = mass_limit(a, b, t), nb = (lim + kMassKeys - 1) / kMassKeys;
-    const float* p = a.part + 2 * i * a.nkb;
-    float mx = kLowest, l = 0.f;
-    for (int s = 0; s < nb; ++s) mx = fmaxf(mx, p[2 * s]);
-    for (int s = 0; s < nb; ++s) l += p[2 * s + 1] * __builtin_amdgcn_exp2f(p[2 * s] - mx);
-    if (l != 0.f) {
-      m = mx;
-      w = 1.f / l;
+  };
+  float m = kLowest, l = 0.f;
+  if (w < nt) load_keys(w);
+  for (int j = w; j < nt; j += 16) {
+    float4_t s[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) s[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) s[tt] = ET::mfma(kf[tt][ks], qf[ks], s[tt]);
+    if (j + 16 < nt) load_keys(j + 16);
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 4 * TT; ++i) {
+      const int key = 16 * (TT * j + i / 4) + 4 * g + i % 4;
+      const float x = s[i / 4][i % 4] * a.sm_log2;
+      s[i / 4][i % 4] = key < lim ? x : -INFINITY;
+      mx = fmaxf(mx, s[i / 4][i % 4]);
+    }
+    l *= __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+#pragma unroll
+    for (int i = 0; i < 4 * TT; ++i) l += __builtin_amdgcn_exp2f(s[i / 4][i % 4] - m);
+    if (c16 < rows) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<float4_t*>(sc + c16 * stride + 16 * (TT * j + tt) + 4 * g) = s[tt];
     }
   }
-  a.stat[2 * i] = m;
-  a.stat[2 * i + 1] = w;
+  const float mw = col_max(m), lw = col_sum(l * __builtin_amdgcn_exp2f(m - mw));
+  if (g == 0) { s_m[w][c16] = mw; s_l[w][c16] = lw; }
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float2 st = make_float2(INFINITY, 0.f);
+    if ((int)threadIdx.x < rows) {
+      if (a.lse) {
+        st = lse_stat(a.lse[(long)hb * rows + threadIdx.x]);
+      } else {
+        float mx = kLowest, ls = 0.f;
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s_m[i][threadIdx.x]);
+        for (int i = 0; i < 16; ++i) ls += s_l[i][threadIdx.x] * __builtin_amdgcn_exp2f(s_m[i][threadIdx.x] - mx);
+        if (ls != 0.f) st = make_float2(mx, 1.f / ls);
+      }
+    }
+    s_st[threadIdx.x] = st;
+  }
+  __syncthreads();
+  float* dst = a.out + b * a.o_sb + hk * a.o_sh;
+  for (int key = threadIdx.x; key < a.Tk; key += 1024) {
+    float v = 0.f;
+    if (key < sq.len)
+      for (int i = 0; i < rows; ++i) {
+        const float x = sc[i * stride + key];
+        const float2 st = s_st[i];
+        if (x != -INFINITY) v = fmaf(__builtin_amdgcn_exp2f(x - st.x), st.y, v);  // (masked: -inf; NaN goes on)
+      }
+    dst[key] = a.accumulate ? dst[key] + v : v;
+  }
 }
 
 namespace {
@@ -259,14 +536,43 @@ int check_mass(const carekv_mass_params* pp) {
   CAREKV_REQUIRE(p.batch >= 0 && p.n_queries >= 0 && p.n_keys >= 0, "negative counts");
   CAREKV_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0,
                  "n_heads must be a positive multiple of n_kv_heads");
+  CAREKV_REQUIRE((p.n_queries < 2 || (p.q_st >= 0 && p.q_st < (1 << 22))) &&
+                     (p.n_keys < 2 || (p.k_st >= 0 && p.k_st < (1 << 22))),
+                 "q and k row strides must be in 0 .. 2^22 elements");
   CAREKV_REQUIRE(p.n_keys < (1 << 30) && (long)p.n_queries * (p.n_heads / p.n_kv_heads) < (1L << 30),
                  "n_keys and the rows of a kv head must be below 2^30");
-  CAREKV_REQUIRE((long)p.batch * p.n_kv_heads * ((p.n_keys + 127L) / 128) < (1L << 31), "too many key blocks");
   return CAREKV_OK;
 }
+
+// How a call is cut: the kernel of few rows, or parts of the walks, 2048
+// work-groups (four rounds of the resident 512, so that the unequal causal
+// walks even out) of at least 8 tiles each.
+struct MassPlan {
+  bool few;
+  int few_stride;
+  int nkb, psg, prow, nqb, nsk;
+};
+MassPlan mass_plan(const carekv_mass_params& p) {
+  MassPlan m{};
+  const long G = p.n_heads / p.n_kv_heads, rows = G * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
+  m.few_stride = (p.n_keys + 63) / 64 * 64 + 4;
+  m.few = rows <= kFewRows && rows * m.few_stride * 4 <= kFewLds && (long)p.n_keys * p.head_dim * 2 <= (1 << 20);
+  m.nkb = (p.n_keys + kMassKeys - 1) / kMassKeys;
+  m.nqb = (int)((rows + 255) / 256);
+  const long seg = p.n_queries >= 32 ? p.n_queries : rows, nseg = p.n_queries >= 32 ? G : 1;
+  const long tiles = (seg + kMassTile - 1) / kMassTile * nseg, ktiles = ((long)p.n_keys + kMassTile - 1) / kMassTile;
+  auto cut = [&](long wgs, long walk) { return (int)std::max(1L, std::min({2048 / std::max(1L, wgs), walk / 8, 64L})); };
+  const long parts = cut(hb * m.nkb, tiles);
+  m.psg = (int)std::min(parts, nseg);
+  m.prow = (int)std::max(1L, std::min(parts / m.psg, (seg + kMassTile - 1) / kMassTile));
+  m.nsk = cut(hb * m.nqb, ktiles);
+  return m;
+}
 long mass_ws(const carekv_mass_params& p, bool have_lse) {
-  const long rows = (long)p.batch * p.n_heads * p.n_queries, nkb = (p.n_keys + kMassKeys - 1) / kMassKeys;
-  return rows * 8 * (1 + (have_lse ? 0 : nkb)) + 256;
+  const MassPlan m = mass_plan(p);
+  if (m.few) return 0;
+  const long rows = (long)p.batch * p.n_heads * p.n_queries;
+  return (have_lse ? 0 : rows * 8 * (1 + m.nsk)) + (m.psg * m.prow > 1 ? (long)m.psg * m.prow * p.batch * p.n_kv_heads * p.n_keys * 4 : 0);
 }
 }  // namespace
 
@@ -286,44 +592,55 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   if (rc != CAREKV_OK) return rc;
   const carekv_mass_params& p = *pp;
   if (p.batch == 0 || p.n_keys == 0) return CAREKV_OK;
-  CAREKV_REQUIRE(k && out && workspace && (p.n_queries == 0 || q), "null argument");
-  uintptr_t bits = (uintptr_t)q | (uintptr_t)k | (uintptr_t)workspace;
-  for (int64_t x : {p.q_sb, p.q_sh, p.q_st, p.k_sb, p.k_sh, p.k_st}) bits |= (uintptr_t)(2 * x);
+  CAREKV_REQUIRE(k && out && (workspace || mass_ws(p, lse != nullptr) == 0) && (p.n_queries == 0 || q), "null argument");
+  const uintptr_t bits = operand_bits(q, {{p.batch, 2 * p.q_sb}, {p.n_heads, 2 * p.q_sh}, {p.n_queries, 2 * p.q_st}}) |
+                         operand_bits(k, {{p.batch, 2 * p.k_sb}, {p.n_kv_heads, 2 * p.k_sh}, {p.n_keys, 2 * p.k_st}}) |
+                         (uintptr_t)workspace;
   CAREKV_REQUIRE((bits & 15) == 0, "q and k rows must be 16-byte aligned");
   if (workspace_bytes < mass_ws(p, lse != nullptr)) {
     set_error("carekv_attention_mass: workspace too small (%lld < %lld)", (long long)workspace_bytes,
               (long long)mass_ws(p, lse != nullptr));
     return CAREKV_ESPACE;
   }
+  const MassPlan m = mass_plan(p);
   MassArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.lse = lse; a.q_start = q_start; a.lengths = lengths; a.out = out;
-  a.q_sb = 2 * p.q_sb; a.q_sh = 2 * p.q_sh; a.q_st = 2 * p.q_st; a.k_sb = 2 * p.k_sb; a.k_sh = 2 * p.k_sh;
-  a.k_st = 2 * p.k_st; a.o_sb = p.out_sb; a.o_sh = p.out_sh;
+  a.q_sb = 2 * p.q_sb; a.q_sh = 2 * p.q_sh; a.q_st = p.n_queries > 1 ? 2 * p.q_st : 0; a.k_sb = 2 * p.k_sb; a.k_sh = 2 * p.k_sh;
+  a.k_st = p.n_keys > 1 ? 2 * p.k_st : 0; a.o_sb = p.out_sb; a.o_sh = p.out_sh;
   a.B = p.batch; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.Tq = p.n_queries;
-  a.Tk = p.n_keys; a.nkb = (p.n_keys + kMassKeys - 1) / kMassKeys; a.causal = p.causal != 0;
-  a.accumulate = p.accumulate != 0;
-  if (p.n_queries >= kMassTile) { a.nseg = a.G; a.seg = a.Tq; }
+  a.Tk = p.n_keys; a.causal = p.causal != 0; a.accumulate = p.accumulate != 0;
+  a.nkb = m.nkb; a.psg = m.psg; a.prow = m.prow; a.parts = m.psg * m.prow; a.nqb = m.nqb; a.nsk = m.nsk;
+  if (p.n_queries >= 32) { a.nseg = a.G; a.seg = a.Tq; }
   else { a.nseg = 1; a.seg = a.G * a.Tq; }
   a.sm_log2 = (float)((double)p.sm_scale * 1.4426950408889634074);
-  const long rows = (long)p.batch * p.n_heads * p.n_queries;
+  const long rows = (long)p.batch * p.n_heads * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
   a.stat = (float*)workspace;
-  a.part = a.stat + 2 * rows;
+  a.part = a.stat + (lse ? 0 : 2 * rows);
+  a.opart = a.part + (lse ? 0 : 2 * rows * m.nsk);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)((long)a.B * a.Hkv * a.nkb));
-  CAREKV_REQUIRE((rows + 255) / 256 < (1L << 31), "too many query rows");
+  const long wgs = hb * m.nkb * a.parts, swgs = hb * m.nqb * m.nsk, sum = (hb * p.n_keys + 255) / 256;
+  CAREKV_REQUIRE(wgs < (1L << 31) && swgs < (1L << 31) && sum < (1L << 31) && (rows + 31) / 32 < (1L << 31),
+                 "too many blocks");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
     using ET = decltype(et);
     constexpr int D = decltype(d)::value;
-    if (!lse && rows > 0) {
-      hipLaunchKernelGGL((mass_kernel<ET, D, true>), grid, dim3(256), 0, s, a);
-      CAREKV_CHECK_LAUNCH("mass (row statistics)");
+    if (m.few && rows > 0) {
+      hipLaunchKernelGGL((mass_few_kernel<ET, D>), dim3((unsigned)hb), dim3(1024), 0, s, a, m.few_stride);
+      CAREKV_CHECK_LAUNCH("mass_few");
+      return CAREKV_OK;
     }
-    if (rows > 0) {
-      hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, a);
+    if (!lse && rows > 0) {
+      hipLaunchKernelGGL((stats_kernel<ET, D>), dim3((unsigned)swgs), dim3(512), 0, s, a);
+      CAREKV_CHECK_LAUNCH("mass_stats");
+      hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, a);
       CAREKV_CHECK_LAUNCH("mass_join");
     }
-    hipLaunchKernelGGL((mass_kernel<ET, D, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mass_kernel<ET, D>), dim3((unsigned)wgs), dim3(512), 0, s, a);
     CAREKV_CHECK_LAUNCH("mass");
+    if (a.parts > 1) {
+      hipLaunchKernelGGL(mass_sum_kernel, dim3((unsigned)sum), dim3(256), 0, s, a);
+      CAREKV_CHECK_LAUNCH("mass_sum");
+    }
     return CAREKV_OK;
   });
 }

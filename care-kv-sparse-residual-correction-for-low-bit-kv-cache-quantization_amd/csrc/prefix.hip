@@ -263,7 +263,7 @@ int prefix_splits(const carekv_prefix_params& p) {
   const long wgs = (M + 127) / 128 * p.n_kv_heads, tiles = ((long)p.prefix_len + 31) / 32;
   if (tiles == 0 || wgs == 0) return 0;
   long s = std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
-  const long st = 2 * std::max(p.k_st, p.v_st);
+  const long st = p.prefix_len > 1 ? 2 * std::max(p.k_st, p.v_st) : 0;
   while (s < tiles && ((tiles + s - 1) / s + 1) * 32 * st >= (1L << 30)) ++s;
   return (int)std::min(s, tiles);
 }
@@ -277,13 +277,13 @@ int check_prefix(const carekv_prefix_params* pp) {
                  "n_heads must be a positive multiple of n_kv_heads");
   CAREKV_REQUIRE(p.prefix_len < (1 << 30), "prefix_len must be below 2^30");
   CAREKV_REQUIRE((long)p.batch * p.seq_len * p.n_heads < (1L << 30), "too many rows");
-  CAREKV_REQUIRE(p.k_st >= 0 && p.v_st >= 0 && p.k_st < (1 << 22) && p.v_st < (1 << 22),
+  CAREKV_REQUIRE(p.prefix_len < 2 || (p.k_st >= 0 && p.v_st >= 0 && p.k_st < (1 << 22) && p.v_st < (1 << 22)),
                  "K and V row strides must be in 0 .. 2^22 elements");
   return CAREKV_OK;
 }
 long prefix_ws(const carekv_prefix_params& p, int ns) {
   const long rows = (long)p.batch * p.seq_len * p.n_heads;
-  return ns * rows * (2 + p.head_dim) * 4 + 256;
+  return ns * rows * (2 + p.head_dim) * 4;
 }
 }  // namespace
 
@@ -304,9 +304,11 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   const carekv_prefix_params& p = *pp;
   const long rows = (long)p.batch * p.seq_len * p.n_heads;
   if (rows == 0) return CAREKV_OK;
-  CAREKV_REQUIRE(q && out && workspace && (p.prefix_len == 0 || (k && v)) && !own == !own_lse, "null argument");
-  uintptr_t bits = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)workspace;
-  for (int64_t x : {p.q_sb, p.q_sh, p.q_st, p.k_sh, p.k_st, p.v_sh, p.v_st}) bits |= (uintptr_t)(2 * x);
+  CAREKV_REQUIRE(q && out && (workspace || prefix_splits(p) == 0) && (p.prefix_len == 0 || (k && v)) && !own == !own_lse, "null argument");
+  const uintptr_t bits = operand_bits(q, {{p.batch, 2 * p.q_sb}, {p.n_heads, 2 * p.q_sh}, {p.seq_len, 2 * p.q_st}}) |
+                         operand_bits(k, {{p.n_kv_heads, 2 * p.k_sh}, {p.prefix_len, 2 * p.k_st}}) |
+                         operand_bits(v, {{p.n_kv_heads, 2 * p.v_sh}, {p.prefix_len, 2 * p.v_st}}) |
+                         (uintptr_t)workspace;
   CAREKV_REQUIRE((bits & 15) == 0, "q, k and v rows must be 16-byte aligned");
   const int ns = prefix_splits(p);
   if (workspace_bytes < prefix_ws(p, ns)) {

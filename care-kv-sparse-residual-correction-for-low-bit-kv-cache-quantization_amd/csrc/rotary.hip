@@ -144,16 +144,16 @@ extern "C" int carekv_rotate_heads(const carekv_rotary_params* pp, const void* q
   RotaryArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.qo = (char*)qo; a.ko = (char*)ko;
   a.pos = positions; a.freqs = freqs; a.pos_batch = p.pos_batch;
-  const int64_t strides[12] = {p.q_sb, p.q_sh, p.q_st, p.k_sb, p.k_sh, p.k_st,
-                               p.qo_sb, p.qo_sh, p.qo_st, p.ko_sb, p.ko_sh, p.ko_st};
+  a.sb[0] = p.q_sb * es; a.sh[0] = p.q_sh * es; a.st[0] = p.q_st * es;
+  a.sb[1] = p.k_sb * es; a.sh[1] = p.k_sh * es; a.st[1] = p.k_st * es;
+  a.ob[0] = p.qo_sb * es; a.oh[0] = p.qo_sh * es; a.ot[0] = p.qo_st * es;
+  a.ob[1] = p.ko_sb * es; a.oh[1] = p.ko_sh * es; a.ot[1] = p.ko_st * es;
   uintptr_t bits = 0;
-  for (int i = 0; i < 12; ++i)
-    if ((i / 3) % 2 == 0 ? p.n_heads > 0 : p.n_kv_heads > 0) bits |= (uintptr_t)(strides[i] * es);
-  if (p.n_heads > 0) bits |= (uintptr_t)q | (uintptr_t)qo;
-  if (p.n_kv_heads > 0) bits |= (uintptr_t)k | (uintptr_t)ko;
   for (int i = 0; i < 2; ++i) {
-    a.sb[i] = strides[3 * i] * es; a.sh[i] = strides[3 * i + 1] * es; a.st[i] = strides[3 * i + 2] * es;
-    a.ob[i] = strides[6 + 3 * i] * es; a.oh[i] = strides[7 + 3 * i] * es; a.ot[i] = strides[8 + 3 * i] * es;
+    const int h = i ? p.n_kv_heads : p.n_heads;
+    if (h == 0) continue;
+    bits |= operand_bits(i ? k : q, {{p.batch, a.sb[i]}, {h, a.sh[i]}, {p.seq_len, a.st[i]}});
+    bits |= operand_bits(i ? ko : qo, {{p.batch, a.ob[i]}, {h, a.oh[i]}, {p.seq_len, a.ot[i]}});
   }
   a.T = p.seq_len; a.D = p.head_dim; a.R = p.rotary_dim; a.Hq = p.n_heads; a.H = (int)heads;
   a.inverse = p.inverse != 0; a.scale = p.scale; a.rows = rows;

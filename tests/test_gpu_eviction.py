@@ -54,7 +54,8 @@ def _check_mass(got, ref, rel, n):
 SHAPES = [  # B, Hq, Hkv, D, Tq, Tk
     (1, 4, 4, 64, 1, 1), (2, 8, 1, 64, 1, 300), (3, 6, 2, 128, 1, 129), (1, 32, 4, 64, 5, 5), (2, 4, 2, 128, 31, 200),
     (1, 8, 2, 64, 32, 33), (2, 6, 3, 128, 64, 700), (1, 4, 1, 64, 257, 257), (1, 2, 2, 128, 515, 515),
-    (1, 16, 16, 128, 33, 2000), (1, 2, 1, 64, 1100, 1300),
+    (1, 16, 16, 128, 33, 2000), (1, 2, 1, 64, 1100, 1300), (1, 2, 1, 64, 1, 9000), (1, 3, 3, 128, 9, 5000),
+    (2, 2, 2, 64, 16, 64), (1, 17, 1, 128, 1, 700),
 ]
 
 

@@ -123,9 +123,10 @@ def test_c_entries_refuse_before_any_launch():
         mp = _lib.MassParams(**{**mass, **bad})
         assert lib.carekv_attention_mass(mp, p, p, None, None, None, p, p, 1 << 40, None) == -1 and err(), bad
     assert lib.carekv_attention_mass_workspace_bytes(_lib.MassParams(**{**mass, "head_dim": 32}), 0) == -1
-    mp = _lib.MassParams(**mass)
+    assert lib.carekv_attention_mass_workspace_bytes(_lib.MassParams(**mass), 0) == 0  # a decode step needs none
+    mp = _lib.MassParams(**{**mass, "n_queries": 40})
     need = lib.carekv_attention_mass_workspace_bytes(mp, 0)
-    assert need > 0 and lib.carekv_attention_mass(mp, p, p, None, None, None, p, p, need - 1, None) == -3
+    assert lib.carekv_attention_mass_workspace_bytes(mp, 1) < need and lib.carekv_attention_mass(mp, p, p, None, None, None, p, p, need - 1, None) == -3
     assert lib.carekv_attention_mass(mp, odd, p, None, None, None, p, p, need, None) == -1 and "aligned" in err()
     assert lib.carekv_attention_mass(mp, p, None, None, None, None, p, p, need, None) == -1
     ev = dict(batch=1, n_kv_heads=2, n_keys=9, row_bytes=128, keep=4, sink=1, recent=1, k_sh=1152, k_st=128, v_sh=1152,
