@@ -117,7 +117,7 @@ EXPORTS = ["carekv_store_pages", "carekv_store_prefill", "carekv_store_workspace
            "carekv_pack_codes", "carekv_unpack_codes", "carekv_pack_4bit", "carekv_unpack_4bit",
            "carekv_quantize_rows_f32", "carekv_dequantize_rows_f32", "carekv_kivi_codes", "carekv_read_hat_pages",
            "carekv_prefill_eval", "carekv_rotate_heads", "carekv_attention_mass",
-           "carekv_attention_mass_workspace_bytes", "carekv_evict_rows", "carekv_prefix_attn",
+           "carekv_attention_mass_workspace_bytes", "carekv_evict_rows", "carekv_evict_rows_workspace_bytes", "carekv_prefix_attn",
            "carekv_prefix_attn_workspace_bytes", "carekv_last_error"]
 
 # bytes of the per-GPU static workspace of carekv_decode_attn_static
@@ -209,7 +209,9 @@ def load(path: str | None = None):
         lib.carekv_attention_mass_workspace_bytes.restype = i64
         lib.carekv_attention_mass_workspace_bytes.argtypes = [C.POINTER(MassParams), i32]
         lib.carekv_evict_rows.restype = C.c_int
-        lib.carekv_evict_rows.argtypes = [C.POINTER(EvictParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        lib.carekv_evict_rows.argtypes = [C.POINTER(EvictParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_evict_rows_workspace_bytes.restype = i64
+        lib.carekv_evict_rows_workspace_bytes.argtypes = [C.POINTER(EvictParams)]
         lib.carekv_prefix_attn.restype = C.c_int
         lib.carekv_prefix_attn.argtypes = [C.POINTER(PrefixParams), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.carekv_prefix_attn_workspace_bytes.restype = i64

@@ -131,8 +131,13 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
         pp = _lib.EvictParams(B, H, T, D * e, n, sink, recent, *mass.stride()[:2], sk[0] * e, sk[1] * e, sk[2] * e,
                               sv[0] * e, sv[1] * e, sv[2] * e)
         ln = _lib.row_counts(lengths, B, dev, "lengths")
-        _lib.call(dev, "carekv_evict_rows", _lib.load().carekv_evict_rows, pp, mass.data_ptr(), k.data_ptr(),
-                  v.data_ptr(), None if ln is None else ln.data_ptr(), kk.data_ptr(), vv.data_ptr(), mm.data_ptr(),
-                  index.data_ptr(), kept.data_ptr())
+        lib = _lib.load()
+        nbytes = lib.carekv_evict_rows_workspace_bytes(pp)
+        if nbytes < 0:
+            _lib.check(-1, "carekv_evict_rows_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call(dev, "carekv_evict_rows", lib.carekv_evict_rows, pp, mass.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  None if ln is None else ln.data_ptr(), kk.data_ptr(), vv.data_ptr(), mm.data_ptr(), index.data_ptr(),
+                  kept.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     got = EvictedRows(kk, vv, mm, index, kept)
     return EvictedRows(*(x[0] for x in got[:4]), kept) if squeeze else got

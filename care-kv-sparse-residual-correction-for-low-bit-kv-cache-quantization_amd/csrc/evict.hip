@@ -3,13 +3,21 @@
 // (equal weights: the lower index), `keep` in all, in index order; their K, V
 // and weight rows gathered.
 //
-// evict_select_kernel: one work-group a row.  Weights are mapped to unsigned
-// keys of the same order (NaN to 0, below -inf); three passes of 11, 11 and 10
-// bits of histograms in LDS find the key of the last kept row and how many of
-// its equals are kept, a fourth pass counts in index order and writes the
-// indices.  evict_gather_kernel copies the rows.
+// Weights are mapped to unsigned keys of the same order (NaN to 0, below -inf);
+// three histograms of 11, 11 and 10 bits find the key of the last kept row and
+// how many of its equals are kept; a scan in index order places the kept rows.
 //
-// Bound by memory: each weight and kept row read once, each kept row written.
+// Up to 8192 rows: evict_select_kernel, one work-group a (sequence, kv head),
+// the keys in registers, everything in one launch, small results gathered there
+// too.  Longer: the rows are cut into parts of 8192 (at most 64 parts), a
+// work-group each, and every histogram is a launch (evict_part_kernel): each
+// part writes its own, the next launch adds up its row's, so that nothing is
+// cleared and no sum depends on an order.  evict_gather_kernel copies the rows.
+//
+// Bound by memory: each weight and kept row read once, each kept row written;
+// the select's launches are latency.
+#include <algorithm>
+
 #include "common.h"
 #include "host_util.h"
 
@@ -36,106 +44,113 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSel = 1024;  // threads of a select work-group
+constexpr int kSel = 1024;           // threads of a select work-group
+constexpr int kEpt = 8;              // keys a thread holds
+constexpr int kChunk = kSel * kEpt;  // rows of a part's turn
+constexpr int kBins = 2048;
+constexpr int kMaxParts = 64;
+constexpr long kFuseBytes = 65536;   // K rows of a kv head gathered by the select work-group itself
 
-__global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[2048];
-  __shared__ int part[kSel / 64], s_bin, s_need;
-  const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
-  const int n = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-  const int kept = min(n, a.keep);
-  int32_t* index = a.index + (long)blockIdx.x * a.keep;
-  if (h == 0 && tid == 0 && a.kept) a.kept[b] = kept;
-  for (int i = kept + tid; i < a.keep; i += kSel) index[i] = -1;
-  if (n <= a.keep) {
-    for (int i = tid; i < n; i += kSel) index[i] = i;
-    return;
+__device__ __forceinline__ int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ int pass_bins(int pass) { return pass == 2 ? 1024 : 2048; }
+
+// The rows of a sequence: kept for certain below lo and from hi on, `need` of
+// those between by weight; none competes where every row is kept.
+struct EvictSeq {
+  int n, kept, lo, hi, need;
+};
+__device__ __forceinline__ EvictSeq evict_seq(const EvictArgs& a, int b) {
+  EvictSeq s;
+  s.n = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  s.kept = min(s.n, a.keep);
+  if (s.n <= a.keep) {
+    s.lo = s.n; s.hi = s.n; s.need = 0;
+  } else {
+    s.lo = min(a.sink, s.n);
+    s.hi = max(s.n - a.recent, s.lo);
+    s.need = s.kept - s.lo - (s.n - s.hi);
   }
-  // rows [lo, hi) compete for `need` places (1 <= need < hi - lo unless none is left); the others are kept
-  const int lo = min(a.sink, n), hi = max(n - a.recent, lo);
-  int need = kept - lo - (n - hi);
-  uint32_t prefix = 0;  // bits found so far of the last kept row's key
-  if (need > 0) {
-    const int width[3] = {11, 11, 10};
-    int sh = 32;
-    for (int pass = 0; pass < 3; ++pass) {
-      const int nb = 1 << width[pass], top = sh;
-      sh -= width[pass];
-      for (int i = tid; i < 2048; i += kSel) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSel) {
-        const uint32_t key = weight_key(m[i]);
-        if (pass == 0 || (key >> top) == (prefix >> top)) atomicAdd(&hist[(key >> sh) & (nb - 1)], 1);
-      }
-      __syncthreads();
-      // the bin, from the top, where the count passes `need`: thread t has bins nb-1-2t, nb-2-2t
-      const int b0 = nb - 1 - 2 * tid, c0 = 2 * tid < nb ? hist[b0] : 0, c1 = 2 * tid < nb ? hist[b0 - 1] : 0;
-      int x = c0 + c1;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-      }
-      if (lane == 63) part[w] = x;
-      __syncthreads();
-      int before = x - c0 - c1;
-      for (int i = 0; i < w; ++i) before += part[i];
-      if (before < need && need <= before + c0 + c1) {
-        const bool second = need > before + c0;
-        s_bin = second ? b0 - 1 : b0;
-        s_need = need - before - (second ? c0 : 0);
-      }
-      __syncthreads();
-      prefix |= (uint32_t)s_bin << sh;
-      need = s_need;
-      __syncthreads();
-    }
-  }
-  // kept: key > prefix, or one of the first `need` equals; in index order
-  const bool any = kept - lo - (n - hi) > 0;
-  int base = 0, eq_base = 0;
-  for (int t0 = 0; t0 < n; t0 += kSel) {
-    const int i = t0 + tid;
-    bool sure = false, eq = false;
-    if (i < n) {
-      if (i < lo || i >= hi) {
-        sure = true;
-      } else if (any) {
-        const uint32_t key = weight_key(m[i]);
-        sure = key > prefix;
-        eq = key == prefix;
-      }
-    }
-    const uint64_t bs = __ballot(sure), be = __ballot(eq), below = (1ull << lane) - 1;
-    if (lane == 0) part[w] = __popcll(bs) | (__popcll(be) << 16);
-    __syncthreads();
-    int ps = 0, pe = 0, ts = 0, te = 0;
-    for (int j = 0; j < kSel / 64; ++j) {
-      const int c = part[j];
-      if (j < w) { ps += c & 0xffff; pe += c >> 16; }
-      ts += c & 0xffff;
-      te += c >> 16;
-    }
-    // equals before this thread's element, and how many of them are kept
-    const int ebefore = eq_base + pe + __popcll(be & below);
-    const int pos = base + ps + __popcll(bs & below) + min(ebefore, need) - min(eq_base, need);
-    if (sure || (eq && ebefore < need)) index[pos] = i;
-    base += ts + min(eq_base + te, need) - min(eq_base, need);
-    eq_base += te;
-    __syncthreads();
-  }
+  return s;
 }
 
-// One kept row a group of threads; V: bytes a thread moves at once.
+struct SelectScratch {
+  int part[kSel / 64], part2[kSel / 64], bin, need;
+};
+
+// Exclusive prefix over the work-group of (x, y) in thread order, and the totals.
+__device__ __forceinline__ void block_scan2(int& x, int& y, int& tx, int& ty, SelectScratch& sc) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, x0 = x, y0 = y;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(x, o, 64), v = __shfl_up(y, o, 64);
+    if (lane >= o) { x += u; y += v; }
+  }
+  if (lane == 63) { sc.part[w] = x; sc.part2[w] = y; }
+  __syncthreads();
+  int bx = 0, by = 0;
+  tx = ty = 0;
+#pragma unroll
+  for (int i = 0; i < kSel / 64; ++i) {
+    if (i < w) { bx += sc.part[i]; by += sc.part2[i]; }
+    tx += sc.part[i];
+    ty += sc.part2[i];
+  }
+  x += bx - x0;
+  y += by - y0;
+  __syncthreads();
+}
+
+// The bin, from the top, where the counts pass `need`, and what is left of
+// need in it.  Thread t holds the counts c0, c1 of bins nb-1-2t, nb-2-2t (0
+// past the bins).
+__device__ __forceinline__ void find_bin(int c0, int c1, int nb, int need, int& bin, int& left, SelectScratch& sc) {
+  int before = c0 + c1, zero = 0, t0, t1;
+  block_scan2(before, zero, t0, t1, sc);
+  if (before < need && need <= before + c0 + c1) {
+    const bool second = need > before + c0;
+    sc.bin = nb - 1 - 2 * (int)threadIdx.x - (second ? 1 : 0);
+    sc.need = need - before - (second ? c0 : 0);
+  }
+  __syncthreads();
+  bin = sc.bin;
+  left = sc.need;
+}
+
+// Places of a turn's rows: thread t has rows i0 + e, e < kEpt, with their keys.
+// base: places taken before the turn, eqb: equals of thr seen before it.
+template <typename F>
+__device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* key, int i0, int end, uint32_t thr,
+                                           int left, int& base, int& eqb, SelectScratch& sc, F&& put) {
+  int sure = 0, eq = 0;
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    const int i = i0 + e;
+    const bool in = i < end, by = in && i >= q.lo && i < q.hi;
+    sure += (in && !by) || (by && q.need > 0 && key[e] > thr) ? 1 : 0;
+    eq += by && q.need > 0 && key[e] == thr ? 1 : 0;
+  }
+  int ps = sure, pe = eq, ts, te;
+  block_scan2(ps, pe, ts, te, sc);
+  int e0 = eqb + pe, pos = base + ps + min(e0, left) - min(eqb, left);
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    const int i = i0 + e;
+    const bool in = i < end, by = in && i >= q.lo && i < q.hi;
+    bool keep = (in && !by) || (by && q.need > 0 && key[e] > thr);
+    if (by && q.need > 0 && key[e] == thr) {
+      keep = e0 < left;
+      ++e0;
+    }
+    if (keep) put(pos++, i);
+  }
+  base += ts + min(eqb + te, left) - min(eqb, left);
+  eqb += te;
+}
+
+// Row r of the (sequence, kv head) at km / vm, copied to its place by threads c of the row's `per`.
 template <typename V>
-__global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a, long n, int per) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const long r = i / per;  // (sequence, kv head, kept row)
-  const int c = (int)(i - r * per) * (int)sizeof(V);
-  const long bh = r / a.keep, b = bh / a.H, h = bh - b * a.H;
-  const int j = a.index[r];
+__device__ __forceinline__ void copy_row(const EvictArgs& a, long bh, long r, int j, int c) {
+  const long b = bh / a.H, h = bh - b * a.H;
   V x{}, y{};
   if (j >= 0) {
     x = *reinterpret_cast<const V*>(a.k + b * a.k_sb + h * a.k_sh + j * a.k_st + c);
@@ -146,13 +161,167 @@ __global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a, long n, 
   if (c == 0) a.mo[r] = j >= 0 ? *reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh + j * 4L) : 0.f;
 }
 
-}  // namespace carekv
+// V: bytes a thread moves at once, void: no gather here.
+template <typename V>
+__global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
+  constexpr bool FUSE = !std::is_void<V>::value;
+  __shared__ int hist[kBins];
+  __shared__ SelectScratch sc;
+  const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x;
+  const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
+  const EvictSeq q = evict_seq(a, b);
+  int32_t* index = a.index + (long)blockIdx.x * a.keep;
+  if (h == 0 && tid == 0 && a.kept) a.kept[b] = q.kept;
+  for (int i = q.kept + tid; i < a.keep; i += kSel) index[i] = -1;
+  uint32_t key[kEpt];
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    const int i = tid * kEpt + e;
+    key[e] = i >= q.lo && i < q.hi ? weight_key(m[i]) : 0u;
+  }
+  uint32_t thr = 0;
+  int left = q.need;
+  if (q.need > 0) {
+    for (int pass = 0; pass < 3; ++pass) {
+      const int nb = pass_bins(pass), sh = pass_shift(pass), up = pass == 0 ? 0 : pass_shift(pass - 1);
+      hist[tid] = 0;
+      hist[tid + kSel] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        const int i = tid * kEpt + e;
+        if (i >= q.lo && i < q.hi && (pass == 0 || (key[e] >> up) == (thr >> up)))
+          atomicAdd(&hist[(key[e] >> sh) & (nb - 1)], 1);
+      }
+      __syncthreads();
+      const int b0 = nb - 1 - 2 * tid;
+      int bin;
+      find_bin(b0 > 0 ? hist[b0] : 0, b0 > 0 ? hist[b0 - 1] : 0, nb, left, bin, left, sc);
+      thr |= (uint32_t)bin << sh;
+      __syncthreads();
+    }
+  }
+  int base = 0, eqb = 0;
+  place_rows(q, key, tid * kEpt, q.n, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
+  if constexpr (FUSE) {
+    __syncthreads();  // (the indices, written by this work-group, are read back by it)
+    const int per = a.row_bytes / (int)sizeof(V);
+    for (int i = tid; i < a.keep * per; i += kSel) {
+      const int r = i / per;
+      copy_row<V>(a, blockIdx.x, (long)blockIdx.x * a.keep + r, index[r], (i - r * per) * (int)sizeof(V));
+    }
+  }
+}
 
-using namespace carekv;
+// Launch `pass` of a long row: adds up the row's histograms of the launch
+// before (pass 1..3), narrows the last kept key by them, and writes its part's
+// next histogram (pass 0..2) or its rows' places (pass 3).
+//   hist  [B H][3][parts][kBins]
+//   above [B H][parts]   rows of a part known to lie above the last kept key
+//   state [B H][3][2]    after each launch: the key's bits so far, places left
+__global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass, int parts, int* hist, int* above,
+                                                          int* state) {
+  __shared__ int sh_hist[kBins];
+  __shared__ SelectScratch sc;
+  const int bh = blockIdx.x / parts, pt = blockIdx.x % parts, tid = threadIdx.x;
+  const int b = bh / a.H, h = bh % a.H;
+  const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
+  const EvictSeq q = evict_seq(a, b);
+  const int i0 = (int)((long)a.T * pt / parts), i1 = min((int)((long)a.T * (pt + 1) / parts), q.n);
+  uint32_t thr = 0;
+  int left = q.need, prev_above = 0, prev_eq = 0;
+  if (q.need > 0 && pass > 0) {
+    if (pass > 1) { thr = (uint32_t)state[6 * bh + 2 * pass - 2]; left = state[6 * bh + 2 * pass - 1]; }
+    const int nb = pass_bins(pass - 1), b0 = nb - 1 - 2 * tid;
+    const int* src = hist + ((long)bh * 3 + pass - 1) * parts * kBins;
+    int2 all = make_int2(0, 0), prev = make_int2(0, 0), mine = make_int2(0, 0);  // bins b0, b0 - 1
+    if (b0 > 0)
+      for (int p0 = 0; p0 < parts; p0 += 8) {  // eight parts' loads in flight
+        int2 c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)  // (b0 is odd)
+          c[u] = *reinterpret_cast<const int2*>(src + (long)min(p0 + u, parts - 1) * kBins + b0 - 1);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + u;
+          if (p < parts) { all.x += c[u].y; all.y += c[u].x; }
+          if (p < pt) { prev.x += c[u].y; prev.y += c[u].x; }
+          if (p == pt) mine = make_int2(c[u].y, c[u].x);
+        }
+      }
+    int bin;
+    find_bin(all.x, all.y, nb, left, bin, left, sc);
+    thr |= (uint32_t)bin << pass_shift(pass - 1);
+    // rows of the bins above it: this part's so far, and after the last pass those of the parts before
+    const int2 use = pass == 3 ? prev : mine;
+    int up = (b0 > bin ? use.x : 0) + (b0 - 1 > bin ? use.y : 0);
+    int eq = (b0 == bin ? use.x : 0) + (b0 - 1 == bin ? use.y : 0);
+    int tu, te;
+    if (pass == 3 && tid < pt) up += above[(long)bh * parts + tid];  // (what the launches before found of them)
+    block_scan2(up, eq, tu, te, sc);
+    if (pass < 3) {
+      if (tid == 0) {
+        int* dst = above + (long)bh * parts + pt;
+        *dst = (pass == 1 ? 0 : *dst) + tu;
+      }
+    } else {
+      prev_above = tu;
+      prev_eq = te;
+    }
+  }
+  if (pass < 3) {
+    if (q.need <= 0) return;
+    if (pass > 0 && pt == 0 && tid == 0) { state[6 * bh + 2 * pass] = (int)thr; state[6 * bh + 2 * pass + 1] = left; }
+    const int nb = pass_bins(pass), sh = pass_shift(pass), up = pass == 0 ? 0 : pass_shift(pass - 1);
+    sh_hist[tid] = 0;
+    sh_hist[tid + kSel] = 0;
+    __syncthreads();
+    for (int i = max(i0, q.lo) + tid; i < min(i1, q.hi); i += kSel) {
+      const uint32_t key = weight_key(m[i]);
+      if (pass == 0 || (key >> up) == (thr >> up)) atomicAdd(&sh_hist[(key >> sh) & (nb - 1)], 1);
+    }
+    __syncthreads();
+    int* dst = hist + (((long)bh * 3 + pass) * parts + pt) * kBins;
+    dst[tid] = sh_hist[tid];
+    dst[tid + kSel] = sh_hist[tid + kSel];
+    return;
+  }
+  int32_t* index = a.index + (long)bh * a.keep;
+  if (pt == 0) {
+    if (h == 0 && tid == 0 && a.kept) a.kept[b] = q.kept;
+    for (int i = q.kept + tid; i < a.keep; i += kSel) index[i] = -1;
+  }
+  // places taken by the parts before: rows kept for certain, above the last kept key, the first of its equals
+  int base = min(i0, q.lo) + max(0, min(i0, q.n) - q.hi) + prev_above + min(prev_eq, left), eqb = prev_eq;
+  for (int c0 = i0; c0 < i1; c0 += kChunk) {
+    uint32_t key[kEpt];
+#pragma unroll
+    for (int e = 0; e < kEpt; ++e) {
+      const int i = c0 + tid * kEpt + e;
+      key[e] = i >= q.lo && i < min(i1, q.hi) ? weight_key(m[i]) : 0u;
+    }
+    place_rows(q, key, c0 + tid * kEpt, i1, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
+  }
+}
 
-extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mass, const void* k, const void* v,
-                                 const int32_t* lengths, void* k_out, void* v_out, float* mass_out, int32_t* index,
-                                 int32_t* kept, void* stream) {
+// One kept row a group of threads; V: bytes a thread moves at once.
+template <typename V>
+__global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a, long n, int per) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long r = i / per;  // (sequence, kv head, kept row)
+  copy_row<V>(a, r / a.keep, r, a.index[r], (int)(i - r * per) * (int)sizeof(V));
+}
+
+namespace {
+int evict_parts(const carekv_evict_params& p) {
+  return (int)std::min((long)kMaxParts, std::max(1L, ((long)p.n_keys + kChunk - 1) / kChunk));
+}
+long evict_ws(const carekv_evict_params& p) {
+  const long parts = evict_parts(p);
+  return parts == 1 ? 0 : (long)p.batch * p.n_kv_heads * (3 * parts * kBins + parts + 6) * 4;
+}
+int check_evict(const carekv_evict_params* pp) {
   CAREKV_REQUIRE(pp, "null argument");
   const carekv_evict_params& p = *pp;
   CAREKV_REQUIRE(p.batch >= 0 && p.n_kv_heads >= 0 && p.n_keys >= 0, "negative counts");
@@ -160,10 +329,35 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
                  "keep must be positive, sink and recent not negative and at most keep together");
   CAREKV_REQUIRE(p.n_keys < (1 << 30), "n_keys must be below 2^30");
   CAREKV_REQUIRE(p.row_bytes > 0 && p.row_bytes % 4 == 0, "rows must be a multiple of 4 bytes");
+  CAREKV_REQUIRE((long)p.batch * p.n_kv_heads * evict_parts(p) < (1L << 31), "too many (sequence, kv head) rows");
+  return CAREKV_OK;
+}
+}  // namespace
+
+}  // namespace carekv
+
+using namespace carekv;
+
+extern "C" int64_t carekv_evict_rows_workspace_bytes(const carekv_evict_params* pp) {
+  if (check_evict(pp) != CAREKV_OK) return -1;
+  return evict_ws(*pp);
+}
+
+extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mass, const void* k, const void* v,
+                                 const int32_t* lengths, void* k_out, void* v_out, float* mass_out, int32_t* index,
+                                 int32_t* kept, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_evict(pp);
+  if (rc != CAREKV_OK) return rc;
+  const carekv_evict_params& p = *pp;
   const long bh = (long)p.batch * p.n_kv_heads;
   if (bh == 0) return CAREKV_OK;
-  CAREKV_REQUIRE((p.n_keys == 0 || (mass && k && v)) && k_out && v_out && mass_out && index, "null argument");
-  CAREKV_REQUIRE(bh < (1L << 31), "too many (sequence, kv head) rows");
+  const int parts = evict_parts(p);
+  CAREKV_REQUIRE((p.n_keys == 0 || (mass && k && v)) && k_out && v_out && mass_out && index && (workspace || parts == 1),
+                 "null argument");
+  if (workspace_bytes < evict_ws(p)) {
+    set_error("carekv_evict_rows: workspace too small (%lld < %lld)", (long long)workspace_bytes, (long long)evict_ws(p));
+    return CAREKV_ESPACE;
+  }
   EvictArgs a{};
   a.mass = (const char*)mass; a.k = (const char*)k; a.v = (const char*)v; a.lengths = lengths;
   a.ko = (char*)k_out; a.vo = (char*)v_out; a.mo = mass_out; a.index = index; a.kept = kept;
@@ -174,13 +368,32 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
                          operand_bits(v, {{p.batch, p.v_sb}, {p.n_kv_heads, p.v_sh}, {p.n_keys, p.v_st}}) |
                          (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)p.row_bytes;
   CAREKV_REQUIRE((bits & 3) == 0, "K and V rows must be 4-byte aligned");
+  CAREKV_REQUIRE(parts == 1 || ((uintptr_t)workspace & 7) == 0, "the workspace must be 8-byte aligned");
   const bool wide = (bits & 15) == 0;
   const int per = p.row_bytes / (wide ? 16 : 4);
   const long n = bh * p.keep * per;
   CAREKV_REQUIRE((n + 255) / 256 < (1L << 31), "too many kept rows");
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)bh), dim3(kSel), 0, s, a);
-  CAREKV_CHECK_LAUNCH("evict_select");
+  if (parts == 1) {
+    const dim3 grid((unsigned)bh), block(kSel);
+    if ((long)p.keep * p.row_bytes <= kFuseBytes) {
+      if (wide) hipLaunchKernelGGL(evict_select_kernel<uint4>, grid, block, 0, s, a);
+      else hipLaunchKernelGGL(evict_select_kernel<uint32_t>, grid, block, 0, s, a);
+      CAREKV_CHECK_LAUNCH("evict_select");
+      return CAREKV_OK;
+    }
+    hipLaunchKernelGGL(evict_select_kernel<void>, grid, block, 0, s, a);
+    CAREKV_CHECK_LAUNCH("evict_select");
+  } else {
+    int* hist = (int*)workspace;
+    int* above = hist + bh * 3 * parts * kBins;
+    int* state = above + bh * parts;
+    for (int pass = 0; pass < 4; ++pass) {
+      hipLaunchKernelGGL(evict_part_kernel, dim3((unsigned)(bh * parts)), dim3(kSel), 0, s, a, pass, parts, hist, above,
+                         state);
+      CAREKV_CHECK_LAUNCH("evict_part");
+    }
+  }
   const dim3 grid((unsigned)((n + 255) / 256));
   if (wide) hipLaunchKernelGGL(evict_gather_kernel<uint4>, grid, dim3(256), 0, s, a, n, per);
   else hipLaunchKernelGGL(evict_gather_kernel<uint32_t>, grid, dim3(256), 0, s, a, n, per);

@@ -629,7 +629,8 @@ typedef struct carekv_evict_params {
 
 int carekv_evict_rows(const carekv_evict_params* params, const float* mass, const void* k, const void* v,
                       const int32_t* lengths, void* k_out, void* v_out, float* mass_out, int32_t* index,
-                      int32_t* kept, void* stream);
+                      int32_t* kept, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t carekv_evict_rows_workspace_bytes(const carekv_evict_params* params);
 
 /* out = attention of every row of q [batch][n_heads][seq_len][head_dim] over
  * the one prefix k, v [n_kv_heads][prefix_len][head_dim], which all rows see,

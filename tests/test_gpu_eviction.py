@@ -215,7 +215,8 @@ def _check_evict(care_kv, mass, k, v, keep, sink, recent, lengths):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("B,H,T,D,keep,sink,recent", [
     (1, 1, 1, 64, 1, 0, 0), (2, 3, 50, 64, 7, 2, 3), (1, 2, 1024, 128, 128, 4, 32), (2, 2, 1025, 64, 1024, 0, 0),
-    (1, 4, 5000, 128, 1300, 4, 0), (3, 1, 333, 6, 332, 100, 232), (1, 1, 20000, 64, 5, 0, 5), (2, 2, 40, 64, 64, 4, 4)])
+    (1, 4, 5000, 128, 1300, 4, 0), (2, 1, 8193, 64, 600, 1, 5), (1, 1, 300000, 64, 9000, 4, 100), (1, 1, 600000, 2, 70, 0, 1),
+    (3, 1, 333, 6, 332, 100, 232), (1, 1, 20000, 64, 5, 0, 5), (2, 2, 40, 64, 64, 4, 4)])
 def test_evict(dtype, B, H, T, D, keep, sink, recent):
     import care_kv
     print(f"evict {dtype} B={B} H={H} T={T} D={D} keep={keep} sink={sink} recent={recent}", flush=True)
@@ -228,7 +229,7 @@ def test_evict(dtype, B, H, T, D, keep, sink, recent):
         _check_evict(care_kv, m, k, v, keep, sink, recent, None)
 
 
-@pytest.mark.parametrize("n_parts", [1, 3])
+@pytest.mark.parametrize("n_parts", [1, 3, 8])
 def test_evict_lengths_and_values(n_parts):
     """Lengths of 0, 1, below, at and above keep; weights of both signs, zeros of
     both signs, infinities and NaN; NaN rows behind a sequence are not read."""

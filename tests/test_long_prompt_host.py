@@ -132,8 +132,13 @@ def test_c_entries_refuse_before_any_launch():
     ev = dict(batch=1, n_kv_heads=2, n_keys=9, row_bytes=128, keep=4, sink=1, recent=1, k_sh=1152, k_st=128, v_sh=1152,
               v_st=128)
     for bad in (dict(keep=0), dict(sink=4), dict(recent=-1), dict(row_bytes=6), dict(k_st=130), dict(n_keys=1 << 30)):
-        assert lib.carekv_evict_rows(_lib.EvictParams(**{**ev, **bad}), p, p, p, None, p, p, p, p, p, None) == -1, bad
-    assert lib.carekv_evict_rows(_lib.EvictParams(**ev), None, p, p, None, p, p, p, p, p, None) == -1
+        assert lib.carekv_evict_rows(_lib.EvictParams(**{**ev, **bad}), p, p, p, None, p, p, p, p, p, p, 1 << 40, None) == -1, bad
+    assert lib.carekv_evict_rows(_lib.EvictParams(**ev), None, p, p, None, p, p, p, p, p, p, 1 << 40, None) == -1
+    assert lib.carekv_evict_rows_workspace_bytes(_lib.EvictParams(**ev)) == 0
+    ep = _lib.EvictParams(**{**ev, "n_keys": 20000})
+    need = lib.carekv_evict_rows_workspace_bytes(ep)
+    assert need > 0 and lib.carekv_evict_rows(ep, p, p, p, None, p, p, p, p, p, p, need - 1, None) == -3
+    assert lib.carekv_evict_rows(ep, p, p, p, None, p, p, p, p, p, None, need, None) == -1
     pre = dict(batch=2, n_heads=4, n_kv_heads=2, seq_len=1, prefix_len=9, head_dim=64, q_sb=256, q_sh=64, k_sh=576,
                k_st=64, v_sh=576, v_st=64, out_sb=256, out_sh=64)
     for bad in (dict(head_dim=96), dict(dtype=2), dict(n_heads=5), dict(prefix_len=-1), dict(k_st=1 << 22), dict(v_st=-64),
