@@ -14,6 +14,7 @@
 // full; prefix_join_kernel then joins the splits' (maximum, sum, O), kept in
 // 32 bits, and the row's own part.
 #include <algorithm>
+#include <cmath>
 
 #include "host_util.h"
 #include "mfma16.h"
@@ -33,7 +34,10 @@ struct PrefixArgs {
   long q_sb, q_sh, q_st, k_sh, k_st, v_sh, v_st, o_sb, o_sh, o_st, w_sb, w_sh, w_st;  // bytes
   long rows;             // n_kv_heads * M
   int B, Hq, Hkv, G, T, P, M, nqb, nsplit;
-  float sm_log2;
+  float sm_log2;         // |scale| log2(e), 1 where that is 0
+  uint32_t q_sign;       // sign bits of two elements where the scale is negative
+  uint32_t q_keep;       // 0 where the scale is 0 (0 times the -inf of a masked score would be NaN), else all bits
+  int al8;               // rows of out and own on 8 bytes
 };
 
 // Row r of kv head hk: sequence, query head, query token.
@@ -49,15 +53,62 @@ __device__ __forceinline__ PrefixRow prefix_row(const PrefixArgs& a, int hk, int
   return x;
 }
 
-template <typename ET, int D>
-__global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
+// The row's own part, joined with the prefix's (m, L, O unnormalised) in 32
+// bits: four dims' results, and the log-sum-exp.  A row that sees nothing (no
+// prefix, lse_own = -inf) is zero with a log-sum-exp of -inf, whatever its own
+// output holds.
+template <typename ET>
+struct PrefixOwn {
+  using E = typename ET::E;
+  float lo, m, f, fo;  // own log-sum-exp (base 2), joint maximum, factors of the prefix's and the own part
+  __device__ __forceinline__ PrefixOwn(const PrefixArgs& a, const PrefixRow& x, float mp) {
+    lo = a.own ? a.own_lse[((long)x.b * a.Hq + x.h) * a.T + x.t] * kLog2e : -INFINITY;
+    m = fmaxf(lo, mp);
+    f = __builtin_amdgcn_exp2f(mp - m);
+    fo = lo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lo - m);  // (NaN goes on as NaN)
+  }
+  // dims d .. d+3 of the row (o, l: the prefix's sums), to out
+  __device__ __forceinline__ void write(const PrefixArgs& a, const PrefixRow& x, int d, float4_t o, float l) const {
+    const float L = f * l + fo;
+    o *= f;
+    if (lo != -INFINITY) {
+      const E* p = reinterpret_cast<const E*>(a.own + x.b * a.w_sb + x.h * a.w_sh + x.t * a.w_st) + d;
+      E v[4];
+      if (a.al8) __builtin_memcpy(v, __builtin_assume_aligned(p, 8), 8);
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(fo, (float)v[i], o[i]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    E* dst = reinterpret_cast<E*>(a.out + x.b * a.o_sb + x.h * a.o_sh + x.t * a.o_st) + d;
+    E w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (E)(o[i] * inv);
+    if (a.al8) __builtin_memcpy(__builtin_assume_aligned(dst, 8), w, 8);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[i] = w[i];
+  }
+  __device__ __forceinline__ void write_lse(const PrefixArgs& a, const PrefixRow& x, float l) const {
+    const float L = f * l + fo;
+    a.lse[((long)x.b * a.Hq + x.h) * a.T + x.t] = L == 0.f ? -INFINITY : (m + __log2f(L)) * kLn2;
+  }
+};
+
+// WQ waves share the keys of a tile, each with 32 rows of its own; with WQ = 1
+// the four waves have the same 32 rows and a quarter of the tile's 128 keys
+// each, joined in LDS at the end: few rows then still use every wave.
+template <typename ET, int D, int WQ>
+__global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(PrefixArgs a) {
   using V8 = typename ET::V8;
   using E = typename ET::E;
-  constexpr int KT = 32, TT = KT / 16, NQ = 2, QW = 16 * NQ, QB = 4 * QW;
+  constexpr int WK = 4 / WQ, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
   constexpr int KRS = 2 * D + 16, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
   constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / 256;
-  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS;
-  __shared__ __align__(16) char lds[2 * BUF];
+  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WK == 1 ? 2 : 1;
+  __shared__ __align__(16) char lds[NBUF * BUF];
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
 
@@ -70,14 +121,14 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int r0 = qblk * QB + QW * w;  // first row of the wave
+  const int r0 = qblk * QB + QW * (WK == 1 ? w : 0), wk = WK == 1 ? 0 : w;  // first row, key quarter of the wave
   const int tiles = (a.P + KT - 1) / KT;
   const int tile0 = (int)((long)sp * tiles / a.nsplit), tile1 = (int)((long)(sp + 1) * tiles / a.nsplit);
   const int j0 = tile0 * KT, keys = min(tile1 * KT, a.P) - j0;  // the split's keys (at least one)
-  const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.k + hk * a.k_sh + j0 * a.k_st, (uint32_t)((keys - 1) * a.k_st + 2 * D));
-  const __amdgpu_buffer_rsrc_t rv = make_rsrc(a.v + hk * a.v_sh + j0 * a.v_st, (uint32_t)((keys - 1) * a.v_st + 2 * D));
+  const char* kbase = a.k + hk * a.k_sh + j0 * a.k_st;
+  const char* vbase = a.v + hk * a.v_sh + j0 * a.v_st;
 
-  // Q^T operands: sub-block qb, step s -> row r0 + 16 qb + c16, dims 32s + 8g ..
+  // Q^T operands: sub-block qb, step s -> row r0 + 16 qb + c16, dims 32s + 8g ..; negated for a negative scale
   V8 qf[NQ][KS];
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) {
@@ -85,28 +136,35 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
     const char* qp = a.q + x.b * a.q_sb + x.h * a.q_sh + x.t * a.q_st;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const uint4 v = *reinterpret_cast<const uint4*>(qp + (32 * s + 8 * g) * 2);
+      uint4 v = *reinterpret_cast<const uint4*>(qp + (32 * s + 8 * g) * 2);
+      v.x = (v.x ^ a.q_sign) & a.q_keep; v.y = (v.y ^ a.q_sign) & a.q_keep;
+      v.z = (v.z ^ a.q_sign) & a.q_keep; v.w = (v.w ^ a.q_sign) & a.q_keep;
       __builtin_memcpy(&qf[qb][s], &v, 16);
     }
   }
 
   uint32_t stg[NCH][4];
-  auto load_tile = [&](int j) {
+  const int srow = threadIdx.x / CHR, scol = threadIdx.x % CHR * 16;  // (chunk k: row srow + 256 / CHR k of K, then V)
+  uint32_t off[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {  // chunks k < NCH / 2 are K, the rest V
-      const int rc = (threadIdx.x + 256 * k) % (KT * CHR), row = j * KT + rc / CHR, col = rc % CHR;
-      // a row past the split reads zeros: its offset is at or past the resource's end
-      const uint32_t st = (uint32_t)(k < NCH / 2 ? a.k_st : a.v_st);
-      const uint32_t off = row < keys ? row * st + col * 16 : 0x7ffffff0u;
-      const auto v = __builtin_amdgcn_raw_buffer_load_b128(k < NCH / 2 ? rk : rv, off, 0, 0);
+  for (int k = 0; k < NCH; ++k)
+    off[k] = (uint32_t)((srow + 256 / CHR * (k % (NCH / 2))) * (k < NCH / 2 ? a.k_st : a.v_st) + scol);
+  // A tile is a buffer resource of its rows, a thread's offsets in it stay the same; rows past the split read zeros.
+  auto load_tile = [&](int j) {
+    const int last = min(KT, keys - j * KT) - 1;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + (long)j * KT * a.k_st, (uint32_t)(last * a.k_st + 2 * D));
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vbase + (long)j * KT * a.v_st, (uint32_t)(last * a.v_st + 2 * D));
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(k < NCH / 2 ? rk : rv, off[k], 0, 0);
       stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
     }
   };
   auto store_tile = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int rc = (threadIdx.x + 256 * k) % (KT * CHR), row = rc / CHR, col = rc % CHR;
-      char* dst = lds + buf * BUF + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + col * 16;
+      const int row = srow + 256 / CHR * (k % (NCH / 2));
+      char* dst = lds + buf * BUF + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + scol;
       *reinterpret_cast<uint4*>(dst) = make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
     }
   };
@@ -121,15 +179,18 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   const int nt = tile1 - tile0;
-  const float c = a.sm_log2;
+  const float c = a.sm_log2;  // (not negative)
   load_tile(0);
   store_tile(0);
   __syncthreads();
   if (nt > 1) load_tile(1);
   for (int j = 0; j < nt; ++j) {
-    const char* kb = lds + (j & 1) * BUF;
-    const char* vb = kb + KBUF;
-    if (r0 < a.M) {
+    const char* kb = lds + (NBUF == 2 ? (j & 1) * BUF : 0) + 32 * wk * KRS;
+    const char* vb = lds + (NBUF == 2 ? (j & 1) * BUF : 0) + KBUF + 32 * wk * VRS;
+    const int left = keys - j * KT - 32 * wk;  // the wave's keys from here on
+    if (r0 < a.M && (WK == 1 || left > 0)) {
+      // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
+      __builtin_amdgcn_s_setprio(1);
       float4_t s[TT][NQ];
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
@@ -143,13 +204,10 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
           for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = ET::mfma(ak, qf[qb][ks], s[tt][qb]);
         }
       }
-      // base-2 logits (a negative scale would turn a maximum of s into a minimum: scaled first)
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) s[tt][qb] *= c;
-      if ((j + 1) * KT > keys) {  // the split's last tile: key 16 tt + 4g + i
-        const int lim = keys - j * KT - 4 * g;
+      __builtin_amdgcn_s_setprio(0);
+      if (left < 32) {  // the split's last keys: key 16 tt + 4g + i
+        int lim = left - 4 * g;
+        asm volatile("" : "+v"(lim));  // (keeps the compares on this branch)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
@@ -158,29 +216,42 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
 #pragma unroll
               for (int qb = 0; qb < NQ; ++qb) s[tt][qb][i] = -INFINITY;
       }
-      V8 bp[NQ];
+      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -max)
+      float mx[NQ];
+      bool any_over = false, over[NQ];
 #pragma unroll
       for (int qb = 0; qb < NQ; ++qb) {
-        float mx = -INFINITY;
+        mx[qb] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][qb][i % 4]);
-        if (__any(mx > m_run[qb])) {  // columns that keep their maximum get a factor of exactly 1
-          const float m_new = fmaxf(m_run[qb], col_max(mx));
+        for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
+        over[qb] = mx[qb] * c > m_run[qb];
+        any_over |= over[qb];
+      }
+      if (__any(any_over)) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          if (!__any(over[qb])) continue;  // columns that keep their maximum get a factor of exactly 1
+          const float m_new = fmaxf(m_run[qb], col_max(mx[qb]) * c);
           const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
           m_run[qb] = m_new;
           l_run[qb] *= f;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
         }
+      }
+      V8 bp[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
         float ls = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(s[i / 4][qb][i % 4] - m_run[qb]);
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[i / 4][qb][i % 4], c, -m_run[qb]));
           ls += p;
           bp[qb][i] = (E)p;
         }
         l_run[qb] += ls;
       }
+      __builtin_amdgcn_s_setprio(1);
       const __attribute__((address_space(3))) char* vrow =
           (const __attribute__((address_space(3))) char*)vb + (4 * g + (c16 >> 2)) * VRS + (c16 & 3) * 8;
 #pragma unroll
@@ -194,78 +265,145 @@ __global__ __launch_bounds__(256, 3) void prefix_attn_kernel(PrefixArgs a) {
         for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
       }
     }
-    if (j + 1 < nt) store_tile((j + 1) & 1);
+    __builtin_amdgcn_s_setprio(0);
+    if (NBUF == 1) __syncthreads();
+    if (j + 1 < nt) store_tile(NBUF == 2 ? (j + 1) & 1 : 0);
     if (j + 2 < nt) load_tile(j + 2);
     __syncthreads();
   }
-  // the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
+  float lt[NQ];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) lt[qb] = col_sum(l_run[qb]);
+  if constexpr (WK > 1) {
+    // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum,
+    // 16 rows at a time in the tile's LDS, added in wave order; wave w keeps the dims of tiles w DT/4 ..
+    __shared__ float s_ml[WK][QW][2];
+    float* so = reinterpret_cast<float*>(lds);  // [WK][DT][64 lanes][4]
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb)
+      if (g == 0) { s_ml[w][16 * qb + c16][0] = m_run[qb]; s_ml[w][16 * qb + c16][1] = lt[qb]; }
+    __syncthreads();
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+      float m = kLowest, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + c16][0]);
+#pragma unroll
+      for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + c16][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + c16][0] - m);
+      const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((w * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
+      m_run[qb] = m;
+      lt[qb] = l;
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < DT / 4; ++u) {
+        const int dt = w * (DT / 4) + u;
+        float4_t v = *reinterpret_cast<const float4_t*>(so + (dt * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + ((i * DT + dt) * 64 + lane) * 4);
+        o[qb][u] = v;
+      }
+      __syncthreads();
+    }
+  }
+  // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
+  constexpr int OT = WK == 1 ? DT : DT / 4;
+  const int dt0 = WK == 1 ? 0 : w * OT;
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) {
-    const float lt = col_sum(l_run[qb]);
     const int r = r0 + 16 * qb + c16;
-    if (r < a.M) {
+    if (r >= a.M) continue;
+    const bool first = g == 0 && (WK == 1 || w == 0);
+    if (a.nsplit == 1) {
+      const PrefixRow x = prefix_row(a, hk, r);
+      const PrefixOwn<ET> own(a, x, m_run[qb]);
+#pragma unroll
+      for (int u = 0; u < OT; ++u) own.write(a, x, 16 * (dt0 + u) + 4 * g, o[qb][u], lt[qb]);
+      if (a.lse && first) own.write_lse(a, x, lt[qb]);
+    } else {
       const long pr = (long)sp * a.rows + (long)hk * a.M + r;
       float* dst = a.po + pr * D + 4 * g;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(dst + 16 * dt) = o[qb][dt];
-      if (g == 0) {
+      for (int u = 0; u < OT; ++u) *reinterpret_cast<float4_t*>(dst + 16 * (dt0 + u)) = o[qb][u];
+      if (first) {
         a.pml[2 * pr] = m_run[qb];
-        a.pml[2 * pr + 1] = lt;
+        a.pml[2 * pr + 1] = lt[qb];
       }
     }
   }
 }
 
-// Four dims of one row: the splits' partials and the row's own part joined in
-// 32 bits.  A row that sees nothing (no prefix, lse_own = -inf) is zero with a
-// log-sum-exp of -inf, whatever its own output holds.
-template <typename ET>
-__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int D) {
-  using E = typename ET::E;
-  const int D4 = D / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.rows * D4) return;
-  const long pr = i / D4;
-  const int d = (int)(i - pr * D4) * 4;
+// The splits' partials of a row, and its own part: a work-group has 256 / D
+// rows; JG groups of D / 4 threads take every JG-th split of a row, four dims a
+// thread, and are added up in LDS in group order.
+template <typename ET, int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
+  constexpr int D4 = D / 4, JG = 4, RW = 256 / (D4 * JG);
+  __shared__ float4_t s_o[256];
+  __shared__ float2 s_ml[RW][JG];
+  const int d4 = threadIdx.x % D4, grp = threadIdx.x / D4 % JG, rw = threadIdx.x / (D4 * JG);
+  const long pr = (long)blockIdx.x * RW + rw;
+  const bool in = pr < a.rows;
+  float m = kLowest, L = 0.f;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+  if (in)
+    for (int s0 = grp; s0 < a.nsplit; s0 += 4 * JG) {  // four splits' loads in flight
+      float2 ml[4];
+      float4_t v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long r = min(s0 + u * JG, a.nsplit - 1) * a.rows + pr;
+        ml[u] = *reinterpret_cast<const float2*>(a.pml + 2 * r);
+        v[u] = *reinterpret_cast<const float4_t*>(a.po + r * D + 4 * d4);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u * JG >= a.nsplit) break;
+        const float mn = fmaxf(m, ml[u].x), f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[u].x - mn);
+        o = o * f + v[u] * e;
+        L = L * f + ml[u].y * e;
+        m = mn;
+      }
+    }
+  s_o[threadIdx.x] = o;
+  if (d4 == 0) s_ml[rw][grp] = make_float2(m, L);
+  __syncthreads();
+  if (!in || grp != 0) return;
+  float mm = kLowest, LL = 0.f;
+  float4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < JG; ++i) mm = fmaxf(mm, s_ml[rw][i].x);
+#pragma unroll
+  for (int i = 0; i < JG; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_ml[rw][i].x - mm);
+    LL += s_ml[rw][i].y * f;
+    O += s_o[(rw * JG + i) * D4 + d4] * f;
+  }
   const int hk = (int)(pr / a.M);
   const PrefixRow x = prefix_row(a, hk, (int)(pr - (long)hk * a.M));
-  const long lrow = ((long)x.b * a.Hq + x.h) * a.T + x.t;
-  const float lo = a.own ? a.own_lse[lrow] * kLog2e : -INFINITY;
-  float m = lo;
-  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.pml[2 * (s * a.rows + pr)]);
-  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  float L = 0.f;
-  if (lo != -INFINITY) {  // (NaN goes on as NaN)
-    const float f = __builtin_amdgcn_exp2f(lo - m);
-    const E* p = reinterpret_cast<const E*>(a.own + x.b * a.w_sb + x.h * a.w_sh + x.t * a.w_st) + d;
-    O = make_float4(f * (float)p[0], f * (float)p[1], f * (float)p[2], f * (float)p[3]);
-    L = f;
-  }
-  for (int s = 0; s < a.nsplit; ++s) {
-    const long r = s * a.rows + pr;
-    const float f = __builtin_amdgcn_exp2f(a.pml[2 * r] - m);
-    const float4 v = *reinterpret_cast<const float4*>(a.po + r * D + d);
-    L = fmaf(f, a.pml[2 * r + 1], L);
-    O.x = fmaf(f, v.x, O.x); O.y = fmaf(f, v.y, O.y); O.z = fmaf(f, v.z, O.z); O.w = fmaf(f, v.w, O.w);
-  }
-  const bool none = L == 0.f;
-  const float inv = none ? 0.f : 1.f / L;
-  E* dst = reinterpret_cast<E*>(a.out + x.b * a.o_sb + x.h * a.o_sh + x.t * a.o_st) + d;
-  dst[0] = (E)(O.x * inv); dst[1] = (E)(O.y * inv); dst[2] = (E)(O.z * inv); dst[3] = (E)(O.w * inv);
-  if (a.lse && d == 0) a.lse[lrow] = none ? -INFINITY : (m + __log2f(L)) * kLn2;
+  const PrefixOwn<ET> own(a, x, mm);
+  own.write(a, x, 4 * d4, O, LL);
+  if (a.lse && d4 == 0) own.write_lse(a, x, LL);
 }
 
 namespace {
-// Splits of the keys: until 768 work-groups (3 a CU) are there, each of at
-// least 4 tiles, and no split's rows past 2^30 bytes (32-bit offsets).
-int prefix_splits(const carekv_prefix_params& p) {
+// How a call is cut.  At most 32 rows a kv head: the four waves of a work-group
+// split a tile's keys (wq = 1); more: they split the rows.  Key splits until
+// 768 work-groups (3 a CU) are there, each of at least 4 tiles.
+struct PrefixPlan {
+  int wq, nqb, nsplit;
+};
+PrefixPlan prefix_plan(const carekv_prefix_params& p) {
+  PrefixPlan r{};
   const long M = (long)p.batch * p.seq_len * (p.n_heads / p.n_kv_heads);
-  const long wgs = (M + 127) / 128 * p.n_kv_heads, tiles = ((long)p.prefix_len + 31) / 32;
-  if (tiles == 0 || wgs == 0) return 0;
-  long s = std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
-  const long st = p.prefix_len > 1 ? 2 * std::max(p.k_st, p.v_st) : 0;
-  while (s < tiles && ((tiles + s - 1) / s + 1) * 32 * st >= (1L << 30)) ++s;
-  return (int)std::min(s, tiles);
+  r.wq = M <= 32 ? 1 : 4;
+  r.nqb = (int)((M + 32 * r.wq - 1) / (32 * r.wq));
+  const long kt = 128 / r.wq, wgs = (long)r.nqb * p.n_kv_heads, tiles = (p.prefix_len + kt - 1) / kt;
+  if (tiles == 0 || wgs == 0) return r;
+  const long s = std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
+  r.nsplit = (int)std::min(s, tiles);
+  return r;
 }
 int check_prefix(const carekv_prefix_params* pp) {
   CAREKV_REQUIRE(pp, "null argument");
@@ -283,7 +421,7 @@ int check_prefix(const carekv_prefix_params* pp) {
 }
 long prefix_ws(const carekv_prefix_params& p, int ns) {
   const long rows = (long)p.batch * p.seq_len * p.n_heads;
-  return ns * rows * (2 + p.head_dim) * 4;
+  return ns > 1 ? ns * rows * (2 + p.head_dim) * 4 : 0;
 }
 }  // namespace
 
@@ -293,7 +431,7 @@ using namespace carekv;
 
 extern "C" int64_t carekv_prefix_attn_workspace_bytes(const carekv_prefix_params* pp) {
   if (check_prefix(pp) != CAREKV_OK) return -1;
-  return prefix_ws(*pp, prefix_splits(*pp));
+  return prefix_ws(*pp, prefix_plan(*pp).nsplit);
 }
 
 extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q, const void* k, const void* v,
@@ -304,13 +442,14 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   const carekv_prefix_params& p = *pp;
   const long rows = (long)p.batch * p.seq_len * p.n_heads;
   if (rows == 0) return CAREKV_OK;
-  CAREKV_REQUIRE(q && out && (workspace || prefix_splits(p) == 0) && (p.prefix_len == 0 || (k && v)) && !own == !own_lse, "null argument");
+  CAREKV_REQUIRE(q && out && (workspace || prefix_plan(p).nsplit < 2) && (p.prefix_len == 0 || (k && v)) && !own == !own_lse, "null argument");
   const uintptr_t bits = operand_bits(q, {{p.batch, 2 * p.q_sb}, {p.n_heads, 2 * p.q_sh}, {p.seq_len, 2 * p.q_st}}) |
                          operand_bits(k, {{p.n_kv_heads, 2 * p.k_sh}, {p.prefix_len, 2 * p.k_st}}) |
                          operand_bits(v, {{p.n_kv_heads, 2 * p.v_sh}, {p.prefix_len, 2 * p.v_st}}) |
                          (uintptr_t)workspace;
   CAREKV_REQUIRE((bits & 15) == 0, "q, k and v rows must be 16-byte aligned");
-  const int ns = prefix_splits(p);
+  const PrefixPlan plan = prefix_plan(p);
+  const int ns = plan.nsplit;
   if (workspace_bytes < prefix_ws(p, ns)) {
     set_error("carekv_prefix_attn: workspace too small (%lld < %lld)", (long long)workspace_bytes,
               (long long)prefix_ws(p, ns));
@@ -323,21 +462,33 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   a.v_sh = 2 * p.v_sh; a.v_st = 2 * p.v_st; a.o_sb = 2 * p.out_sb; a.o_sh = 2 * p.out_sh; a.o_st = 2 * p.out_st;
   a.w_sb = 2 * p.own_sb; a.w_sh = 2 * p.own_sh; a.w_st = 2 * p.own_st;
   a.B = p.batch; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.T = p.seq_len;
-  a.P = p.prefix_len; a.M = p.batch * a.G * p.seq_len; a.rows = rows; a.nqb = (a.M + 127) / 128; a.nsplit = ns;
+  a.P = p.prefix_len; a.M = p.batch * a.G * p.seq_len; a.rows = rows; a.nqb = plan.nqb; a.nsplit = ns;
   a.po = (float*)workspace;
   a.pml = a.po + ns * rows * p.head_dim;
-  a.sm_log2 = (float)((double)p.sm_scale * 1.4426950408889634074);
+  a.sm_log2 = (float)(std::fabs((double)p.sm_scale) * 1.4426950408889634074);
+  a.q_sign = p.sm_scale < 0.f ? 0x80008000u : 0u;
+  a.q_keep = a.sm_log2 == 0.f ? 0u : ~0u;
+  if (a.sm_log2 == 0.f) a.sm_log2 = 1.f;
+  uintptr_t rows8 = operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}});
+  if (own) rows8 |= operand_bits(own, {{p.batch, a.w_sb}, {p.n_heads, a.w_sh}, {p.seq_len, a.w_st}});
+  a.al8 = (rows8 & 7) == 0;
   hipStream_t s = (hipStream_t)stream;
-  const long wgs = (long)a.nqb * a.Hkv * ns, jt = rows * (p.head_dim / 4);
+  const long wgs = (long)a.nqb * a.Hkv * ns;
   CAREKV_REQUIRE(wgs < (1L << 31), "too many row blocks");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
     using ET = decltype(et);
+    constexpr int D = decltype(d)::value;
     if (ns > 0) {
-      hipLaunchKernelGGL((prefix_attn_kernel<ET, decltype(d)::value>), dim3((unsigned)wgs), dim3(256), 0, s, a);
+      const dim3 grid((unsigned)wgs), block(256);
+      if (plan.wq == 4) hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 4>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 1>), grid, block, 0, s, a);
       CAREKV_CHECK_LAUNCH("prefix_attn");
     }
-    hipLaunchKernelGGL((prefix_join_kernel<ET>), dim3((unsigned)((jt + 255) / 256)), dim3(256), 0, s, a, p.head_dim);
-    CAREKV_CHECK_LAUNCH("prefix_join");
+    if (ns != 1) {
+      constexpr int RW = 256 / D;
+      hipLaunchKernelGGL((prefix_join_kernel<ET, D>), dim3((unsigned)((rows + RW - 1) / RW)), dim3(256), 0, s, a);
+      CAREKV_CHECK_LAUNCH("prefix_join");
+    }
     return CAREKV_OK;
   });
 }
