@@ -450,26 +450,26 @@ __global__ __launch_bounds__(1024) void mass_few_kernel(MassArgs a, int stride) 
   const int hb = blockIdx.x, b = hb / a.Hkv, hk = hb % a.Hkv, rows = a.G * a.Tq;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const MassSeq sq = mass_seq(a, b);
   const int r = min(c16, rows - 1), h = r / a.Tq, t = r - h * a.Tq;
-  const int lim = c16 < rows ? mass_limit(a, sq, t) : 0;
   V8 qf[KS];
   const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = load8<V8>(qp + (32 * s + 8 * g) * 2);
   const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
-  const int nt = (sq.len + 16 * TT - 1) / (16 * TT);  // tiles with keys
   V8 kf[TT][KS];
-  auto load_keys = [&](int j) {
+  auto load_keys = [&](int j) {  // (keys behind the sequence are masked, whatever they hold)
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
-      const char* kp = kbase + (long)min(16 * (TT * j + tt) + c16, sq.len - 1) * a.k_st;
+      const char* kp = kbase + (long)min(16 * (TT * j + tt) + c16, a.Tk - 1) * a.k_st;
 #pragma unroll
       for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
     }
   };
+  load_keys(w);  // on their way before the length is known
+  const MassSeq sq = mass_seq(a, b);
+  const int lim = c16 < rows ? mass_limit(a, sq, t) : 0;
+  const int nt = (sq.len + 16 * TT - 1) / (16 * TT);  // turns with keys
   float m = kLowest, l = 0.f;
-  if (w < nt) load_keys(w);
   for (int j = w; j < nt; j += 16) {
     float4_t s[TT];
 #pragma unroll

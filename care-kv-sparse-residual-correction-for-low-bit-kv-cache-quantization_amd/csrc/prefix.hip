@@ -390,7 +390,9 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
 namespace {
 // How a call is cut.  At most 32 rows a kv head: the four waves of a work-group
 // split a tile's keys (wq = 1); more: they split the rows.  Key splits until
-// 768 work-groups (3 a CU) are there, each of at least 4 tiles.
+// 768 work-groups (3 a CU) are there, each of at least 4 tiles; up to 8 tiles
+// one split, whose launch writes the results (4 x 8 rows on 1000 keys: two
+// splits and their join 8 + 4 us).
 struct PrefixPlan {
   int wq, nqb, nsplit;
 };
@@ -401,7 +403,7 @@ PrefixPlan prefix_plan(const carekv_prefix_params& p) {
   r.nqb = (int)((M + 32 * r.wq - 1) / (32 * r.wq));
   const long kt = 128 / r.wq, wgs = (long)r.nqb * p.n_kv_heads, tiles = (p.prefix_len + kt - 1) / kt;
   if (tiles == 0 || wgs == 0) return r;
-  const long s = std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
+  const long s = tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
   r.nsplit = (int)std::min(s, tiles);
   return r;
 }
