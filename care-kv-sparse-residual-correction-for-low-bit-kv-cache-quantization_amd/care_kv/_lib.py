@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import collections
 import ctypes as C
+import operator
 import os
 import threading
 import warnings
@@ -376,16 +377,28 @@ def check_out(out: torch.Tensor, shape, dtype, name: str, *inputs: torch.Tensor)
 
 def row_counts(x, batch: int, device, name: str) -> torch.Tensor | None:
     """Per-sequence int32 values on the device: a device tensor of `batch`
-    integers, a host sequence of them, or one int for all; None stays None."""
+    integers, a host sequence of them, or one int for all; None stays None.
+    Captured code takes device tensors (or one int): a graph would copy a host
+    list again on every replay, from memory that is no longer its own."""
     if x is None:
         return None
     if torch.is_tensor(x) and x.is_cuda:
         if x.shape != (batch,) or x.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be {batch} int32 or int64 values; got {tuple(x.shape)} {x.dtype}")
-        return x.to(torch.int32).contiguous()
-    vals = [x] * batch if isinstance(x, int) else [int(v) for v in x]
+        if x.device != device:
+            raise CarekvError(f"{name}: on {x.device}, the other tensors on {device}")
+        if x.dtype == torch.int64:
+            x = x.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+        return x.contiguous()
+    if isinstance(x, int):
+        return torch.full((batch,), x, dtype=torch.int32, device=device)
+    vals = [operator.index(v) for v in (x.tolist() if torch.is_tensor(x) else x)]
     if len(vals) != batch:
         raise ValueError(f"{name} must have {batch} values; got {len(vals)}")
     t = torch.tensor(vals, dtype=torch.int32)
+    if torch.device(device).type != "cuda":
+        return t
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError(f"{name}: a captured call takes a device tensor, not host values")
     # through pinned memory, so that the host does not wait for the stream
-    return t.pin_memory().to(device, non_blocking=True) if torch.device(device).type == "cuda" else t
+    return t.pin_memory().to(device, non_blocking=True)

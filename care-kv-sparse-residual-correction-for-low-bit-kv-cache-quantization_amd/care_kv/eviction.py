@@ -37,7 +37,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
     and sees the keys below ``lengths[b]`` (default Tk) and, with ``causal``, up
     to its own position: Tq = Tk is a prompt, a few last rows are a voting
     window, Tq = 1 a decode step.  q_start and lengths: a device tensor of B
-    integers, a host sequence or (q_start) one int.  lse (B, Hq, Tq) fp32: the
+    integers, one int for all, or (not in captured code) a host sequence.  lse (B, Hq, Tq) fp32: the
     rows' log-sum-exp as ``prefill_attention(..., return_lse=True)`` gives it;
     without it an extra pass computes it.  ``accumulate`` adds to ``out``, whose
     values of a head must lie next to each other.
@@ -67,7 +67,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is not None:
-        _lib.check_out(out, (B, Hkv, Tk), torch.float32, "out", *(() if lse is None else (lse,)))
+        _lib.check_out(out, (B, Hkv, Tk), torch.float32, "out", q, k, *(() if lse is None else (lse,)))
     dev = _lib.same_device("attention_mass", q, k, lse, out)
     if out is None:
         out = torch.empty(B, Hkv, Tk, dtype=torch.float32, device=dev)
@@ -98,8 +98,8 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
     mass (B, Hkv, T) fp32; k and v (B, Hkv, T, D) of any 2- or 4-byte type and
     any strides ((Hkv, T) and (Hkv, T, D) of one sequence work alike, and give
     results without the batch dim).  ``lengths``: rows of each sequence that
-    count (default T), a device tensor of B integers or a host sequence; the
-    rows behind them are not read.  The results have min(keep, T) places;
+    count (default T), a device tensor of B integers or (not in captured code) a
+    host sequence; what the rows behind them hold is not used.  The results have min(keep, T) places;
     sequences that are shorter keep every row."""
     squeeze = mass.dim() == 2
     if squeeze:

@@ -31,6 +31,14 @@ class RotaryPlan:
     freqs: torch.Tensor  # fp64 (rotary_dim / 2,), radians per position, on the device
     scale: float         # factor on the rotated values
 
+    def __post_init__(self):
+        if self.layout not in LAYOUTS:
+            raise ValueError(f"layout={self.layout!r} not in {LAYOUTS}")
+        if self.rotary_dim < 2 or self.rotary_dim % 2 or self.freqs.dtype != torch.float64 or \
+                self.freqs.shape != (self.rotary_dim // 2,) or not self.freqs.is_contiguous():
+            raise ValueError(f"a plan needs an even rotary_dim and rotary_dim / 2 packed fp64 angles (got "
+                             f"{self.rotary_dim}, {tuple(self.freqs.shape)} {self.freqs.dtype})")
+
 
 def rotary_plan(rotary_dim: int, base: float = 10000.0, *, layout: str = "half", scaling: str = "none",
                 factor: float = 1.0, original_len: Optional[int] = None, scale: Optional[float] = None,

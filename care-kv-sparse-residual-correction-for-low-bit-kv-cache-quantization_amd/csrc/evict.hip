@@ -116,35 +116,51 @@ __device__ __forceinline__ void find_bin(int c0, int c1, int nb, int need, int& 
   left = sc.need;
 }
 
-// Places of a turn's rows: thread t has rows i0 + e, e < kEpt, with their keys.
-// base: places taken before the turn, eqb: equals of thr seen before it.
+// Row e of this thread in a turn that starts at c0: a wave's loads are consecutive rows.
+__device__ __forceinline__ int turn_row(int c0, int e) {
+  return c0 + (int)(threadIdx.x >> 6) * 64 * kEpt + 64 * e + (int)(threadIdx.x & 63);
+}
+
+// Places of a turn's rows, given their keys, in index order: those kept for
+// certain or above thr, and the first `left` of its equals.  base: places taken
+// before the turn, eqb: equals seen before it.
 template <typename F>
-__device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* key, int i0, int end, uint32_t thr,
+__device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* key, int c0, int end, uint32_t thr,
                                            int left, int& base, int& eqb, SelectScratch& sc, F&& put) {
-  int sure = 0, eq = 0;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint64_t sure[kEpt], eq[kEpt];
+  int ts = 0, te = 0;
 #pragma unroll
   for (int e = 0; e < kEpt; ++e) {
-    const int i = i0 + e;
+    const int i = turn_row(c0, e);
     const bool in = i < end, by = in && i >= q.lo && i < q.hi;
-    sure += (in && !by) || (by && q.need > 0 && key[e] > thr) ? 1 : 0;
-    eq += by && q.need > 0 && key[e] == thr ? 1 : 0;
+    sure[e] = __ballot((in && !by) || (by && q.need > 0 && key[e] > thr));
+    eq[e] = __ballot(by && q.need > 0 && key[e] == thr);
+    ts += __popcll(sure[e]);
+    te += __popcll(eq[e]);
   }
-  int ps = sure, pe = eq, ts, te;
-  block_scan2(ps, pe, ts, te, sc);
-  int e0 = eqb + pe, pos = base + ps + min(e0, left) - min(eqb, left);
+  if (lane == 0) { sc.part[w] = ts; sc.part2[w] = te; }
+  __syncthreads();
+  int s0 = base, e0 = eqb, all_s = 0, all_e = 0;
+#pragma unroll
+  for (int i = 0; i < kSel / 64; ++i) {
+    if (i < w) { s0 += sc.part[i]; e0 += sc.part2[i]; }
+    all_s += sc.part[i];
+    all_e += sc.part2[i];
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+  const int eq_in = min(eqb, left);  // kept equals that base counts already
 #pragma unroll
   for (int e = 0; e < kEpt; ++e) {
-    const int i = i0 + e;
-    const bool in = i < end, by = in && i >= q.lo && i < q.hi;
-    bool keep = (in && !by) || (by && q.need > 0 && key[e] > thr);
-    if (by && q.need > 0 && key[e] == thr) {
-      keep = e0 < left;
-      ++e0;
-    }
-    if (keep) put(pos++, i);
+    const int rank = e0 + __popcll(eq[e] & below), pos = s0 + __popcll(sure[e] & below) + min(rank, left) - eq_in;
+    const bool is_eq = (eq[e] >> lane) & 1;
+    if (((sure[e] >> lane) & 1) || (is_eq && rank < left)) put(pos, turn_row(c0, e));
+    s0 += __popcll(sure[e]);
+    e0 += __popcll(eq[e]);
   }
-  base += ts + min(eqb + te, left) - min(eqb, left);
-  eqb += te;
+  base += all_s + min(eqb + all_e, left) - eq_in;
+  eqb += all_e;
 }
 
 // Row r of the (sequence, kv head) at km / vm, copied to its place by threads c of the row's `per`.
@@ -169,16 +185,16 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   __shared__ SelectScratch sc;
   const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
+  uint32_t key[kEpt];
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    const int i = turn_row(0, e);
+    key[e] = i < a.T ? weight_key(m[i]) : 0u;
+  }
   const EvictSeq q = evict_seq(a, b);
   int32_t* index = a.index + (long)blockIdx.x * a.keep;
   if (h == 0 && tid == 0 && a.kept) a.kept[b] = q.kept;
   for (int i = q.kept + tid; i < a.keep; i += kSel) index[i] = -1;
-  uint32_t key[kEpt];
-#pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    const int i = tid * kEpt + e;
-    key[e] = i >= q.lo && i < q.hi ? weight_key(m[i]) : 0u;
-  }
   uint32_t thr = 0;
   int left = q.need;
   if (q.need > 0) {
@@ -189,7 +205,7 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < kEpt; ++e) {
-        const int i = tid * kEpt + e;
+        const int i = turn_row(0, e);
         if (i >= q.lo && i < q.hi && (pass == 0 || (key[e] >> up) == (thr >> up)))
           atomicAdd(&hist[(key[e] >> sh) & (nb - 1)], 1);
       }
@@ -202,7 +218,7 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
     }
   }
   int base = 0, eqb = 0;
-  place_rows(q, key, tid * kEpt, q.n, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
+  place_rows(q, key, 0, q.n, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
   if constexpr (FUSE) {
     __syncthreads();  // (the indices, written by this work-group, are read back by it)
     const int per = a.row_bytes / (int)sizeof(V);
@@ -226,8 +242,19 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
   const int bh = blockIdx.x / parts, pt = blockIdx.x % parts, tid = threadIdx.x;
   const int b = bh / a.H, h = bh % a.H;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
+  const int i0 = (int)((long)a.T * pt / parts), t1 = (int)((long)a.T * (pt + 1) / parts);
+  // a turn's weights; the first turn's are on their way before anything else is known
+  float x[kEpt];
+  auto load_turn = [&](int c0) {
+#pragma unroll
+    for (int e = 0; e < kEpt; ++e) {
+      const int i = turn_row(c0, e);
+      x[e] = i < t1 ? m[i] : 0.f;
+    }
+  };
+  load_turn(i0);
   const EvictSeq q = evict_seq(a, b);
-  const int i0 = (int)((long)a.T * pt / parts), i1 = min((int)((long)a.T * (pt + 1) / parts), q.n);
+  const int i1 = min(t1, q.n);
   uint32_t thr = 0;
   int left = q.need, prev_above = 0, prev_eq = 0;
   if (q.need > 0 && pass > 0) {
@@ -276,9 +303,15 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
     sh_hist[tid] = 0;
     sh_hist[tid + kSel] = 0;
     __syncthreads();
-    for (int i = max(i0, q.lo) + tid; i < min(i1, q.hi); i += kSel) {
-      const uint32_t key = weight_key(m[i]);
-      if (pass == 0 || (key >> up) == (thr >> up)) atomicAdd(&sh_hist[(key >> sh) & (nb - 1)], 1);
+    for (int c0 = i0; c0 < i1; c0 += kChunk) {
+      if (c0 > i0) load_turn(c0);
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        const int i = turn_row(c0, e);
+        const uint32_t key = weight_key(x[e]);
+        if (i >= q.lo && i < min(i1, q.hi) && (pass == 0 || (key >> up) == (thr >> up)))
+          atomicAdd(&sh_hist[(key >> sh) & (nb - 1)], 1);
+      }
     }
     __syncthreads();
     int* dst = hist + (((long)bh * 3 + pass) * parts + pt) * kBins;
@@ -294,13 +327,11 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
   // places taken by the parts before: rows kept for certain, above the last kept key, the first of its equals
   int base = min(i0, q.lo) + max(0, min(i0, q.n) - q.hi) + prev_above + min(prev_eq, left), eqb = prev_eq;
   for (int c0 = i0; c0 < i1; c0 += kChunk) {
+    if (c0 > i0) load_turn(c0);
     uint32_t key[kEpt];
 #pragma unroll
-    for (int e = 0; e < kEpt; ++e) {
-      const int i = c0 + tid * kEpt + e;
-      key[e] = i >= q.lo && i < min(i1, q.hi) ? weight_key(m[i]) : 0u;
-    }
-    place_rows(q, key, c0 + tid * kEpt, i1, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
+    for (int e = 0; e < kEpt; ++e) key[e] = weight_key(x[e]);
+    place_rows(q, key, c0, i1, thr, left, base, eqb, sc, [&](int pos, int i) { index[pos] = i; });
   }
 }
 

@@ -255,6 +255,26 @@ def test_captured_and_replayed():
                 assert torch.equal(a, b)
 
 
+def test_host_lists_are_refused_in_captured_code():
+    """A captured call takes lengths on the device (or one int); host lists raise
+    and leave the capture to go on."""
+    import care_kv
+    q, k = torch.randn(2, 4, 40, 64, device="cuda").half(), torch.randn(2, 2, 90, 64, device="cuda").half()
+    want = care_kv.attention_mass(q, k, q_start=50)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(ValueError):
+            care_kv.attention_mass(q, k, lengths=[90, 3])
+        with pytest.raises(ValueError):
+            care_kv.evict_rows(want, k, k, keep=5, lengths=[90, 3])
+        got = care_kv.attention_mass(q, k, q_start=50)
+    for _ in range(3):
+        got.zero_()
+        g.replay()
+        assert torch.equal(got, want)
+
+
 def test_two_streams_at_once():
     import care_kv
     pairs = [_ops(care_kv, s) for s in (3, 4)]

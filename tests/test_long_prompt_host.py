@@ -26,6 +26,14 @@ def test_plan_refusals(kw):
         care_kv.rotary_plan(**{"rotary_dim": 64, "device": CPU, **kw})
 
 
+@pytest.mark.parametrize("r,layout,f", [(64, "pairs", torch.zeros(32).double()), (64, "half", torch.zeros(32)),
+                                        (64, "half", torch.zeros(31).double()), (63, "half", torch.zeros(31).double()),
+                                        (64, "half", torch.zeros(64).double()[::2])])
+def test_plans_made_by_hand(r, layout, f):
+    with pytest.raises(ValueError):
+        care_kv.RotaryPlan(r, layout, f, 1.0)
+
+
 def _half(*s):
     return torch.zeros(*s, dtype=torch.float16)
 
@@ -69,8 +77,11 @@ def test_row_counts():
     assert _lib.row_counts(None, 3, CPU, "x") is None
     assert _lib.row_counts(5, 3, CPU, "x").tolist() == [5, 5, 5]
     assert _lib.row_counts([1, 2, 3], 3, CPU, "x").tolist() == [1, 2, 3]
+    assert _lib.row_counts(torch.tensor([1, 2, 3]), 3, CPU, "x").tolist() == [1, 2, 3]
     with pytest.raises(ValueError):
         _lib.row_counts([1, 2], 3, CPU, "x")
+    with pytest.raises(TypeError):
+        _lib.row_counts([1.5, 2, 3], 3, CPU, "x")
 
 
 def test_evict_refusals():
@@ -145,7 +156,8 @@ def test_c_entries_refuse_before_any_launch():
                 dict(prefix_len=1 << 30), dict(q_sh=60)):
         pp = _lib.PrefixParams(**{**pre, **bad})
         assert lib.carekv_prefix_attn(pp, p, p, p, None, None, p, None, p, 1 << 40, None) == -1 and err(), bad
-    pp = _lib.PrefixParams(**pre)
+    assert lib.carekv_prefix_attn_workspace_bytes(_lib.PrefixParams(**pre)) == 0  # one split: nothing to keep
+    pp = _lib.PrefixParams(**{**pre, "prefix_len": 4000})
     need = lib.carekv_prefix_attn_workspace_bytes(pp)
     assert need > 0 and lib.carekv_prefix_attn(pp, p, p, p, None, None, p, None, p, need - 1, None) == -3
     assert lib.carekv_prefix_attn(pp, p, p, p, p, None, p, None, p, need, None) == -1  # own without its lse
