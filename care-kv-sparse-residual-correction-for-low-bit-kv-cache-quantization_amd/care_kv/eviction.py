@@ -70,7 +70,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
         _lib.check_out(out, (B, Hkv, Tk), torch.float32, "out", q, k, *(() if lse is None else (lse,)))
     dev = _lib.same_device("attention_mass", q, k, lse, out)
     if out is None:
-        out = torch.empty(B, Hkv, Tk, dtype=torch.float32, device=dev)
+        out = q.new_empty((B, Hkv, Tk), dtype=torch.float32)
     if B and Tk:
         q, k = _lib.aligned_rows(q), _lib.aligned_rows(k)
         pp = _lib.MassParams(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], bool(causal), bool(accumulate),
@@ -82,7 +82,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
         nbytes = lib.carekv_attention_mass_workspace_bytes(pp, lse is not None)
         if nbytes < 0:
             _lib.check(-1, "carekv_attention_mass_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _lib.call(dev, "carekv_attention_mass", lib.carekv_attention_mass, pp, q.data_ptr(), k.data_ptr(),
                   None if lse is None else lse.data_ptr(), None if qs is None else qs.data_ptr(),
                   None if ln is None else ln.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
@@ -120,11 +120,11 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
     n = min(int(keep), T)
     sink = min(int(sink), n)  # (with keep > T every row stays)
     recent = min(int(recent), n - sink)
-    kk = torch.empty(B, H, n, D, dtype=k.dtype, device=dev)
-    vv = torch.empty_like(kk)
-    mm = torch.empty(B, H, n, dtype=torch.float32, device=dev)
-    index = torch.empty(B, H, n, dtype=torch.int32, device=dev)
-    kept = (torch.empty if B * H * n else torch.zeros)(B, dtype=torch.int32, device=dev)
+    kk = k.new_empty((B, H, n, D))
+    vv = k.new_empty((B, H, n, D))
+    mm = mass.new_empty((B, H, n))
+    index = mass.new_empty((B, H, n), dtype=torch.int32)
+    kept = (mass.new_empty if B * H * n else mass.new_zeros)(B, dtype=torch.int32)
     if B * H * n:
         mass, k, v = _lib.aligned_rows(mass, 4), _lib.aligned_rows(k, 4), _lib.aligned_rows(v, 4)
         sk, sv = k.stride(), v.stride()
@@ -135,7 +135,7 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
         nbytes = lib.carekv_evict_rows_workspace_bytes(pp)
         if nbytes < 0:
             _lib.check(-1, "carekv_evict_rows_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = k.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _lib.call(dev, "carekv_evict_rows", lib.carekv_evict_rows, pp, mass.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if ln is None else ln.data_ptr(), kk.data_ptr(), vv.data_ptr(), mm.data_ptr(), index.data_ptr(),
                   kept.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)

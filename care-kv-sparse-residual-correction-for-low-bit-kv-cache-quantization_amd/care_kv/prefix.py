@@ -57,8 +57,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         _lib.check_out(out, q.shape, q.dtype, "out", q, k, v, *(() if own is None else (o_own,)))
     dev = _lib.same_device("prefix_attention", q, k, v, o_own, l_own, out)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=dev) if return_lse else None
+        out = q.new_empty(q.shape)
+    lse = q.new_empty((B, Hq, T), dtype=torch.float32) if return_lse else None
     if out.numel():
         q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k), _lib.aligned_rows(v)
         pp = _lib.PrefixParams(B, Hq, Hkv, T, P, D, _lib.DTYPE_CODE[q.dtype],
@@ -69,7 +69,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         nbytes = lib.carekv_prefix_attn_workspace_bytes(pp)
         if nbytes < 0:
             _lib.check(-1, "carekv_prefix_attn_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _lib.call(dev, "carekv_prefix_attn", lib.carekv_prefix_attn, pp, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if own is None else o_own.data_ptr(), None if own is None else l_own.data_ptr(), out.data_ptr(),
                   None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)

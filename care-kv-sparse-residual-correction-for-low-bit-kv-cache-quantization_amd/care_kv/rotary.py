@@ -139,8 +139,8 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
             _lib.check_out(out[1], k.shape, k.dtype, "k_out", k)
     dev = _lib.same_device("rotate_heads", q, k, positions, plan.freqs, *(() if out is None else out))
     if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        qo = q.new_empty(q.shape)
+        ko = None if k is None else k.new_empty(k.shape)
     else:
         qo, ko = out
     pos = pos if pos.stride(1) == 1 or T == 1 else pos.contiguous()

@@ -116,6 +116,34 @@ __device__ __forceinline__ void find_bin(int c0, int c1, int nb, int need, int& 
   left = sc.need;
 }
 
+// find_bin by one wave over counts in LDS: each lane adds up a run of bins from
+// the top, then the lanes share the bins of the run that passes `need`.
+__device__ __forceinline__ void find_bin_wave(const int* hist, int nb, int need, SelectScratch& sc) {
+  const int lane = threadIdx.x & 63, per = nb / 64;  // 32 or 16 bins
+  auto scan = [&](int c) {
+    int x = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o, 64);
+      if (lane >= o) x += y;
+    }
+    return x - c;
+  };
+  int c = 0;
+  for (int i = 0; i < per; i += 4) {
+    const int4 v = *reinterpret_cast<const int4*>(hist + nb - (lane + 1) * per + i);
+    c += v.x + v.y + v.z + v.w;
+  }
+  const int before = scan(c);
+  const int run = __ffsll((unsigned long long)__ballot(before < need && need <= before + c)) - 1;
+  const int left = need - __shfl(before, run, 64);
+  const int bin = nb - 1 - run * per - lane, d = lane < per ? hist[bin] : 0, b2 = scan(d);
+  if (b2 < left && left <= b2 + d) {
+    sc.bin = bin;
+    sc.need = left - b2;
+  }
+}
+
 // Row e of this thread in a turn that starts at c0: a wave's loads are consecutive rows.
 __device__ __forceinline__ int turn_row(int c0, int e) {
   return c0 + (int)(threadIdx.x >> 6) * 64 * kEpt + 64 * e + (int)(threadIdx.x & 63);
@@ -181,10 +209,11 @@ __device__ __forceinline__ void copy_row(const EvictArgs& a, long bh, long r, in
 template <typename V>
 __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   constexpr bool FUSE = !std::is_void<V>::value;
-  __shared__ int hist[kBins];
+  __shared__ __align__(16) int hist[3][kBins];
   __shared__ SelectScratch sc;
   const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
+  for (int i = tid; i < 3 * kBins; i += kSel) hist[0][i] = 0;
   uint32_t key[kEpt];
 #pragma unroll
   for (int e = 0; e < kEpt; ++e) {
@@ -198,23 +227,20 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   uint32_t thr = 0;
   int left = q.need;
   if (q.need > 0) {
+    __syncthreads();
     for (int pass = 0; pass < 3; ++pass) {
       const int nb = pass_bins(pass), sh = pass_shift(pass), up = pass == 0 ? 0 : pass_shift(pass - 1);
-      hist[tid] = 0;
-      hist[tid + kSel] = 0;
-      __syncthreads();
 #pragma unroll
       for (int e = 0; e < kEpt; ++e) {
         const int i = turn_row(0, e);
         if (i >= q.lo && i < q.hi && (pass == 0 || (key[e] >> up) == (thr >> up)))
-          atomicAdd(&hist[(key[e] >> sh) & (nb - 1)], 1);
+          atomicAdd(&hist[pass][(key[e] >> sh) & (nb - 1)], 1);
       }
       __syncthreads();
-      const int b0 = nb - 1 - 2 * tid;
-      int bin;
-      find_bin(b0 > 0 ? hist[b0] : 0, b0 > 0 ? hist[b0 - 1] : 0, nb, left, bin, left, sc);
-      thr |= (uint32_t)bin << sh;
+      if (tid < 64) find_bin_wave(hist[pass], nb, left, sc);
       __syncthreads();
+      thr |= (uint32_t)sc.bin << sh;
+      left = sc.need;
     }
   }
   int base = 0, eqb = 0;
