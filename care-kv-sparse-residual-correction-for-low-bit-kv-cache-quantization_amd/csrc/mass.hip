@@ -10,8 +10,9 @@
 // staged in LDS, so that a key's weights add up in registers and nothing of
 // size queries x keys is written.  Heads are walked one after the other, each
 // from the first row that sees the block; heads of fewer than 32 rows as one
-// list.  Where the key blocks alone do not fill the GPU a walk is cut into
-// parts, whose sums mass_sum_kernel adds in order.
+// list.  A work-group takes a pair of blocks, early and late, whose causal walks
+// have the same length together, or an equal part of a pair's walk; the parts'
+// sums are added in order by mass_sum_kernel.
 //
 // stats_kernel, its mirror image for calls without lse: 256 query rows
 // stationary, key tiles walked, each lane with its own (reference, sum) per row.
@@ -22,13 +23,17 @@
 // mass_few_kernel, at most 16 rows a kv head (a decode step): a work-group a
 // (sequence, kv head), the scores of all keys in LDS, K read once, one launch.
 //
-// Measured, 32 / 8 heads, D = 128, 8192 causal rows with lse (275 GFLOP of
-// products, 1.07e9 exponentials): 355-370 us, 0.75 PFLOP/s; the same with 4
-// waves of 64 keys (2 waves a SIMD, or 3) and with 32 x 32 products (374).
-// Without its exponentials it took 322 us, without products 240, without LDS
-// reads 297, without tile loads 311: no one pipe bounds it, their sum does.  A
-// window of 64 rows on 4 x 8191 keys: 28 us statistics, 31 us weights, each
-// reading K (67 MB, 13 us at the copy rate).
+// Measured, D = 128, 8192 causal rows with lse: 32 / 8 heads 321 us + 5 for the
+// sum of the parts (275 GFLOP of visible products, 1.07e9 exponentials: 0.84
+// PFLOP/s), 32 / 32 heads 304; long uncut walks reach 1.0 PFLOP/s.  Bound: a
+// 16 x 16 x 32 product with the exponential and two fused multiply-adds of its
+// four scores a lane takes a SIMD 25 cycles at best (measured in registers
+// alone; the product itself 16), 180 us of the 321.  Blocks in order instead of
+// pairs, 2048 work-groups: 350; LDS rows padded by 16 bytes (9.0 cycles a read
+// against 5.6): 360; masked wave tiles not skipped: 337; 4 waves of 64 keys or
+// 32 x 32 products were slower (363 and 374 before these).  A window of 64 rows
+// on 4 x 8191 keys: 28 us statistics, 31 us weights, each reading K (67 MB, 13
+// us at the copy rate).
 //
 // Sums: a lane adds at most kFlush tiles' weights before they go to an outer
 // sum, so that a key's total over 2^15 rows keeps the accuracy of a short sum.
@@ -53,8 +58,7 @@ struct MassArgs {
   long q_sb, q_sh, q_st, k_sb, k_sh, k_st;  // bytes
   long o_sb, o_sh;                          // elements
   int B, Hq, Hkv, G, Tq, Tk, causal, accumulate;
-  int nkb, psg, prow;      // mass walks: key blocks; a walk's lists and each list's rows cut into so many parts
-  int parts;               // psg * prow
+  int nkb, parts;          // mass walks: key blocks, parts that a pair of blocks' walk is cut into
   int nqb, nsk;            // statistics: row blocks, parts of a walk
   int nseg, seg;           // a mass walk: nseg lists of seg rows
   float sm_log2;
@@ -100,55 +104,63 @@ __device__ __forceinline__ V8 load8(const char* p) {
 template <typename ET, int D>
 __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   using V8 = typename ET::V8;
-  constexpr int TT = kMassKeys / 128, QT = kMassTile, KS = D / 32, QRS = 2 * D + 16, CHR = D / 8, NCH = QT * CHR / 512;
+  constexpr int TT = kMassKeys / 128, QT = kMassTile, KS = D / 32, QRS = 2 * D + 32, CHR = D / 8, NCH = QT * CHR / 512;
   __shared__ __align__(16) char lds[2][QT * QRS];
+  static_assert(QT == 64, "a wave has a tile's rows");
   __shared__ float2 s_st[2][QT];
   __shared__ int s_lim[2][QT];
-  // Sequences and heads go round the XCDs, and the blocks of one part, which walk over the same rows, run
-  // together: they meet in one L2.  The longest walks of a part first.
+  __shared__ float s_sum[4 * TT][512];  // the outer sums: the registers they would take spill others
+  // Sequences and heads go round the XCDs, the blocks of one part run together: they meet in one L2.
   const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
-  const int kb = rest % a.nkb, pt = rest / a.nkb;
+  const int np = (a.nkb + 1) / 2, pair = rest % np, pt = rest / np;
   const int b = hb / a.Hkv, hk = hb % a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int j0 = kb * kMassKeys + 16 * TT * w;  // first key of the wave
   const MassSeq sq = mass_seq(a, b);
+  const long hrow = (long)hb * a.G * a.Tq;  // first row of this (sequence, kv head) in stat / lse
+  const bool listed = a.nseg > 1 || a.G == 1;  // a list is a head's rows
+  // rows of a list below first_row see nothing of block kb
+  auto first_row = [&](int kb) {
+    if (kb * kMassKeys >= sq.len) return a.seg;
+    return a.causal && listed ? (int)min((long)a.seg, max(0L, (long)kb * kMassKeys - sq.qs)) : 0;
+  };
+  auto tiles_of = [&](int kb) { return (a.seg - first_row(kb) + QT - 1) / QT * a.nseg; };
+  // The pair's walks, one after the other, as one: this part's tiles of it.
+  const int kb_b = a.nkb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (kb_b > pair ? tiles_of(kb_b) : 0);
+  const int lo = (int)((long)n_all * pt / a.parts), hi = (int)((long)n_all * (pt + 1) / a.parts);
+  float* dst = a.parts > 1 ? a.opart + ((long)pt * nhb + hb) * a.Tk : a.out + b * a.o_sb + hk * a.o_sh;
+  const uint32_t off0 = (uint32_t)(threadIdx.x / CHR * a.q_st + (threadIdx.x % CHR) * 16);
+  const char* qbase = a.q + b * a.q_sb + (long)hk * a.G * a.q_sh;
+#pragma unroll 1
+  for (int f = 0; f < (kb_b > pair ? 2 : 1); ++f) {
+  const int kb = f ? kb_b : pair, j0 = kb * kMassKeys + 16 * TT * w;  // the block, the wave's first key
+  const int t_first = first_row(kb), t_end = a.seg, per = max(1, (t_end - t_first + QT - 1) / QT);
+  const int at = max(lo - (f ? n_a : 0), 0), nt = min(hi, f ? n_all : n_a) - (f ? n_a : 0) - at;
+  int sg = at / per, i0 = t_first + (at - sg * per) * QT;  // the tile loaded next
   // K operands: tokens j0 + 16 tt + c16, dims 32 s + 8 g .. (keys past the end: the last one, masked below)
   V8 kf[TT][KS];
+  if (nt > 0) {
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-    const char* kp = a.k + b * a.k_sb + hk * a.k_sh + (long)min(j0 + 16 * tt + c16, a.Tk - 1) * a.k_st;
+    for (int tt = 0; tt < TT; ++tt) {
+      const char* kp = a.k + b * a.k_sb + hk * a.k_sh + (long)min(j0 + 16 * tt + c16, a.Tk - 1) * a.k_st;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
+      for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
+    }
   }
-  const long hrow = (long)hb * a.G * a.Tq;  // first row of this (sequence, kv head) in stat / lse
-  // rows of a list below t_first see nothing of the block
-  const bool listed = a.nseg > 1 || a.G == 1;  // a list is a head's rows
-  const int sg0 = a.nseg * (pt / a.prow) / a.psg, sg1 = a.nseg * (pt / a.prow + 1) / a.psg;
-  const int tiles = (a.seg + QT - 1) / QT, pr = pt % a.prow;
-  int t_first = (int)((long)tiles * pr / a.prow) * QT;
-  const int t_end = min((int)((long)tiles * (pr + 1) / a.prow) * QT, a.seg);
-  if (kb * kMassKeys >= sq.len) t_first = t_end;
-  else if (a.causal && listed) t_first = (int)min((long)t_end, max((long)t_first, (long)kb * kMassKeys - sq.qs));
-  const int nt = (t_end - t_first + QT - 1) / QT * (sg1 - sg0);
-  int sg = sg0, i0 = t_first;  // the tile loaded next
   uint32_t stg[NCH][4];
   float2 n_st = make_float2(0.f, 0.f);
-  int n_lim = 0;
-  // A list's rows lie one row stride apart: a tile is a buffer resource of its rows (those behind the part's
+  int n_lim = 0, turn = 0, sturn = 0;  // the wave of the tile loaded / stored next
+  // A list's rows lie one row stride apart: a tile is a buffer resource of its rows (those behind the list's
   // end read as zeros), a thread's offsets in it stay the same.  Other lists find their rows one by one.
-  uint32_t off[NCH];
-#pragma unroll
-  for (int k = 0; k < NCH; ++k)
-    off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.q_st + (threadIdx.x % CHR) * 16);
-  const char* qbase = a.q + b * a.q_sb + (long)hk * a.G * a.q_sh;
   auto load_tile = [&]() {
     if (listed) {
       const __amdgpu_buffer_rsrc_t rq = make_rsrc(qbase + sg * a.q_sh + i0 * a.q_st,
                                                   (uint32_t)((min(QT, t_end - i0) - 1) * a.q_st + 2 * D));
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b128(rq, off[k], 0, 0);
+        uint32_t off = off0;
+        asm volatile("" : "+v"(off));  // (added here, not kept in a register of its own)
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(rq, off + (uint32_t)(512 / CHR * k * a.q_st), 0, 0);
         stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
       }
     } else {
@@ -161,18 +173,24 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
         stg[k][0] = v.x; stg[k][1] = v.y; stg[k][2] = v.z; stg[k][3] = v.w;
       }
     }
-    if (threadIdx.x < QT) {
-      const int i = i0 + threadIdx.x;
+    // the rows' statistics, by another wave every tile, as they lie: they are turned into (M, w) when they are
+    // stored, so that no wave waits for them here
+    if (w == turn) {
+      const int i = i0 + lane;
       int h = sg, t = i;
-      if (!listed) { h = i / a.Tq; t = i - h * a.Tq; }
-      n_lim = 0;
+      if (!listed) {
+        h = i / a.Tq;
+        t = i - h * a.Tq;
+        n_lim = i < t_end ? mass_limit(a, sq, t) : 0;
+      }
+      const long r = hrow + (long)h * a.Tq + t;
       n_st = make_float2(INFINITY, 0.f);
       if (i < t_end) {
-        n_lim = mass_limit(a, sq, t);
-        const long r = hrow + (long)h * a.Tq + t;
-        n_st = a.lse ? lse_stat(a.lse[r]) : *reinterpret_cast<const float2*>(a.stat + 2 * r);
+        if (a.lse) n_st.x = a.lse[r];
+        else n_st = *reinterpret_cast<const float2*>(a.stat + 2 * r);
       }
     }
+    turn = (turn + 1) & 7;
     i0 += QT;
     if (i0 >= t_end) { i0 = t_first; ++sg; }
   };
@@ -183,11 +201,15 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
       *reinterpret_cast<uint4*>(lds[buf] + row * QRS + (threadIdx.x % CHR) * 16) =
           make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
     }
-    if (threadIdx.x < QT) { s_lim[buf][threadIdx.x] = n_lim; s_st[buf][threadIdx.x] = n_st; }
+    if (w == sturn) {
+      if (!listed) s_lim[buf][lane] = n_lim;
+      s_st[buf][lane] = a.lse ? lse_stat(n_st.x) : n_st;
+    }
+    sturn = (sturn + 1) & 7;
   };
-  float acc[4 * TT], sum[4 * TT];
+  float acc[4 * TT];
 #pragma unroll
-  for (int i = 0; i < 4 * TT; ++i) acc[i] = sum[i] = 0.f;
+  for (int i = 0; i < 4 * TT; ++i) { acc[i] = 0.f; s_sum[i][threadIdx.x] = 0.f; }
   int ci = i0;  // first row of the tile computed next
   if (nt > 0) {
     load_tile();
@@ -198,6 +220,8 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   if (nt > 1) load_tile();
   for (int j = 0; j < nt; ++j) {
     const int buf = j & 1;
+    // (a wave whose keys no row of the tile sees has nothing to add)
+    if (!(listed && (j0 >= sq.len || (a.causal && sq.qs + min(ci + QT, t_end) - 1 < j0)))) {
     // some pair of the tile and the wave's keys is masked
     const bool edge = !listed || ci + QT > t_end || j0 + 16 * TT > sq.len ||
                       (a.causal && sq.qs + ci + 1 < j0 + 16 * TT);
@@ -228,7 +252,9 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
       for (int qb = 0; qb < QT / 16; ++qb) {
         if (qb + 1 < QT / 16) scores(qb + 1, s[(qb + 1) & 1]);
         const float2 st = s_st[buf][16 * qb + c16];
-        const int lim = s_lim[buf][16 * qb + c16] - j0 - 4 * g;  // token 16 tt + i of the lane is seen below it
+        const int i0c = ci + 16 * qb + c16;
+        const int see = !listed ? s_lim[buf][16 * qb + c16] : i0c < t_end ? mass_limit(a, sq, i0c) : 0;
+        const int lim = see - j0 - 4 * g;  // token 16 tt + i of the lane is seen below it
 #pragma unroll
         for (int i = 0; i < 4 * TT; ++i) {
           const float p = __builtin_amdgcn_exp2f(fmaf(s[qb & 1][i / 4][i % 4], a.sm_log2, -st.x));
@@ -236,9 +262,10 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
         }
       }
     }
+    }
     if ((j + 1) % kFlush == 0) {
 #pragma unroll
-      for (int i = 0; i < 4 * TT; ++i) { sum[i] += acc[i]; acc[i] = 0.f; }
+      for (int i = 0; i < 4 * TT; ++i) { s_sum[i][threadIdx.x] += acc[i]; acc[i] = 0.f; }
     }
     ci = ni;
     if (j + 1 < nt) store_tile((j + 1) & 1);
@@ -246,14 +273,14 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     __syncthreads();
   }
   // over the 16 query columns, in a fixed order
-  float* dst = a.parts > 1 ? a.opart + ((long)pt * nhb + hb) * a.Tk : a.out + b * a.o_sb + hk * a.o_sh;
 #pragma unroll
   for (int i = 0; i < 4 * TT; ++i) {
-    float v = sum[i] + acc[i];
+    float v = s_sum[i][threadIdx.x] + acc[i];
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
     const int key = j0 + 16 * (i / 4) + 4 * g + i % 4;
     if (c16 == 0 && key < a.Tk) dst[key] = a.accumulate && a.parts == 1 ? dst[key] + v : v;
+  }
   }
 }
 
@@ -271,16 +298,34 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassArgs a) {
 template <typename ET, int D>
 __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   using V8 = typename ET::V8;
-  constexpr int TT = 2, KT = kMassTile, KS = D / 32, KRS = 2 * D + 16, CHR = D / 8, NCH = KT * CHR / 512;
+  constexpr int TT = 2, KT = kMassTile, KS = D / 32, KRS = 2 * D + 32, CHR = D / 8, NCH = KT * CHR / 512;
   constexpr float kOver = 64.f;
   __shared__ __align__(16) char lds[2][KT * KRS];
   const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
-  const int sp = rest % a.nsk, qblk = a.nqb - 1 - rest / a.nsk;  // the longest walks (latest rows) first
+  const int np = (a.nqb + 1) / 2, pair = rest % np, sp = rest / np;
   const int b = hb / a.Hkv, hk = hb % a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int rows = a.G * a.Tq, r0 = qblk * 256 + 16 * TT * w;
+  const int rows = a.G * a.Tq;
   const MassSeq sq = mass_seq(a, b);
+  uint32_t off[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+    off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.k_st + (threadIdx.x % CHR) * 16);
+  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
+  // tiles of the keys that some row of block qb sees: its rows' furthest limit, a head's last row where it has one
+  auto tiles_of = [&](int qb) {
+    const int ra = qb * 256, rz = min(ra + 256, rows) - 1;
+    const int t = ra / a.Tq != rz / a.Tq || rz % a.Tq == a.Tq - 1 ? a.Tq - 1 : rz % a.Tq;
+    return (mass_limit(a, sq, t) + KT - 1) / KT;
+  };
+  // The pair's walks, one after the other, as one: this part's tiles of it.
+  const int qb_b = a.nqb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (qb_b > pair ? tiles_of(qb_b) : 0);
+  const int from = (int)((long)n_all * sp / a.nsk), to = (int)((long)n_all * (sp + 1) / a.nsk);
+#pragma unroll 1
+  for (int f = 0; f < (qb_b > pair ? 2 : 1); ++f) {
+  const int r0 = (f ? qb_b : pair) * 256 + 16 * TT * w;
+  const int t0 = max(from - (f ? n_a : 0), 0), nt = min(to, f ? n_all : n_a) - (f ? n_a : 0) - t0;
   V8 qf[TT][KS];
   int lim[4 * TT], lo = 0x7fffffff;
 #pragma unroll
@@ -308,21 +353,8 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
     lo = min(lo, __shfl_xor(lo, o, 64));
     hi = max(hi, __shfl_xor(hi, o, 64));
   }
-  __shared__ int s_hi[8];
-  if (lane == 0) s_hi[w] = hi;
-  __syncthreads();
   lo = __builtin_amdgcn_readfirstlane(lo);
-  int end = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) end = max(end, s_hi[i]);
-  const int all = (end + KT - 1) / KT;
-  const int t0 = (int)((long)all * sp / a.nsk), nt = (int)((long)all * (sp + 1) / a.nsk) - t0;
   uint32_t stg[NCH][4];
-  uint32_t off[NCH];
-#pragma unroll
-  for (int k = 0; k < NCH; ++k)
-    off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.k_st + (threadIdx.x % CHR) * 16);
-  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
   auto load_tile = [&](int j) {  // (keys behind the sequence's end read as zeros; they are masked)
     const int k0 = (t0 + j) * KT;
     const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + k0 * a.k_st, (uint32_t)((min(KT, sq.len - k0) - 1) * a.k_st + 2 * D));
@@ -411,6 +443,7 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
       p[0] = mm;
       p[1] = v;
     }
+  }
   }
 }
 
@@ -544,14 +577,26 @@ int check_mass(const carekv_mass_params* pp) {
   return CAREKV_OK;
 }
 
-// How a call is cut: the kernel of few rows, or parts of the walks, 2048
-// work-groups (four rounds of the resident 512, so that the unequal causal
-// walks even out) of at least 8 tiles each.
+// How a call is cut: the kernel of few rows, or walks.  A causal walk is the
+// longer the earlier its key block (the later its row block) lies; the first and
+// the last block, the second and the last but one .. make pairs of equal length,
+// each cut into equal parts.  All 512 work-groups that the GPU holds at once then
+// end together: the number of parts that makes rounds x (tiles of a part + 3, a
+// part's start) least is taken.
 struct MassPlan {
   bool few;
   int few_stride;
-  int nkb, psg, prow, nqb, nsk;
+  int nkb, parts, nqb, nsk;
 };
+int walk_parts(long pairs, long tiles) {
+  long best = 1;
+  double least = 1e300;
+  for (long p = 1; p <= 64 && (p == 1 || p * 4 <= tiles); ++p) {
+    const double c = (double)((pairs * p + 511) / 512) * ((double)tiles / p + 3);
+    if (c < least) { least = c; best = p; }
+  }
+  return (int)best;
+}
 MassPlan mass_plan(const carekv_mass_params& p) {
   MassPlan m{};
   const long G = p.n_heads / p.n_kv_heads, rows = G * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
@@ -561,18 +606,17 @@ MassPlan mass_plan(const carekv_mass_params& p) {
   m.nqb = (int)((rows + 255) / 256);
   const long seg = p.n_queries >= 32 ? p.n_queries : rows, nseg = p.n_queries >= 32 ? G : 1;
   const long tiles = (seg + kMassTile - 1) / kMassTile * nseg, ktiles = ((long)p.n_keys + kMassTile - 1) / kMassTile;
-  auto cut = [&](long wgs, long walk) { return (int)std::max(1L, std::min({2048 / std::max(1L, wgs), walk / 8, 64L})); };
-  const long parts = cut(hb * m.nkb, tiles);
-  m.psg = (int)std::min(parts, nseg);
-  m.prow = (int)std::max(1L, std::min(parts / m.psg, (seg + kMassTile - 1) / kMassTile));
-  m.nsk = cut(hb * m.nqb, ktiles);
+  // (a pair of causal walks over as many rows as keys has about the tiles of one whole walk)
+  const bool tri = p.causal && 2L * p.n_queries > p.n_keys;
+  m.parts = walk_parts(hb * ((m.nkb + 1) / 2), tri || m.nkb == 1 ? tiles : 2 * tiles);
+  m.nsk = walk_parts(hb * ((m.nqb + 1) / 2), tri || m.nqb == 1 ? ktiles : 2 * ktiles);
   return m;
 }
 long mass_ws(const carekv_mass_params& p, bool have_lse) {
   const MassPlan m = mass_plan(p);
   if (m.few) return 0;
   const long rows = (long)p.batch * p.n_heads * p.n_queries;
-  return (have_lse ? 0 : rows * 8 * (1 + m.nsk)) + (m.psg * m.prow > 1 ? (long)m.psg * m.prow * p.batch * p.n_kv_heads * p.n_keys * 4 : 0);
+  return (have_lse ? 0 : rows * 8 * (1 + m.nsk)) + (m.parts > 1 ? (long)m.parts * p.batch * p.n_kv_heads * p.n_keys * 4 : 0);
 }
 }  // namespace
 
@@ -609,7 +653,7 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.k_st = p.n_keys > 1 ? 2 * p.k_st : 0; a.o_sb = p.out_sb; a.o_sh = p.out_sh;
   a.B = p.batch; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.Tq = p.n_queries;
   a.Tk = p.n_keys; a.causal = p.causal != 0; a.accumulate = p.accumulate != 0;
-  a.nkb = m.nkb; a.psg = m.psg; a.prow = m.prow; a.parts = m.psg * m.prow; a.nqb = m.nqb; a.nsk = m.nsk;
+  a.nkb = m.nkb; a.parts = m.parts; a.nqb = m.nqb; a.nsk = m.nsk;
   if (p.n_queries >= 32) { a.nseg = a.G; a.seg = a.Tq; }
   else { a.nseg = 1; a.seg = a.G * a.Tq; }
   a.sm_log2 = (float)((double)p.sm_scale * 1.4426950408889634074);
@@ -618,7 +662,7 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.part = a.stat + (lse ? 0 : 2 * rows);
   a.opart = a.part + (lse ? 0 : 2 * rows * m.nsk);
   hipStream_t s = (hipStream_t)stream;
-  const long wgs = hb * m.nkb * a.parts, swgs = hb * m.nqb * m.nsk, sum = (hb * p.n_keys + 255) / 256;
+  const long wgs = hb * ((m.nkb + 1) / 2) * m.parts, swgs = hb * ((m.nqb + 1) / 2) * m.nsk, sum = (hb * p.n_keys + 255) / 256;
   CAREKV_REQUIRE(wgs < (1L << 31) && swgs < (1L << 31) && sum < (1L << 31) && (rows + 31) / 32 < (1L << 31),
                  "too many blocks");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {

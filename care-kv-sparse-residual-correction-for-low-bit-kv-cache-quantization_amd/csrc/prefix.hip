@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   using V8 = typename ET::V8;
   using E = typename ET::E;
   constexpr int WK = 4 / WQ, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
-  constexpr int KRS = 2 * D + 16, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
+  constexpr int KRS = 2 * D + 32, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
   constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / 256;
   constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WK == 1 ? 2 : 1;
   __shared__ __align__(16) char lds[NBUF * BUF];
