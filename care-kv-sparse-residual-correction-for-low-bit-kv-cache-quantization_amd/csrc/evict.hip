@@ -15,7 +15,10 @@
 // cleared and no sum depends on an order.  evict_gather_kernel copies the rows.
 //
 // Bound by memory: each weight and kept row read once, each kept row written;
-// the select's launches are latency.
+// the select is a chain of latencies.  Measured: 16 rows of 131072 weights, 16384
+// kept (279 MB): select 35 us in four launches (one work-group a row 251), gather
+// 45 us, 6.0 TB/s; 64 rows of 8192, 2048 kept (137 MB): 12.8 + 22 us; 4 rows of
+// 512 10 us in one launch.
 #include <algorithm>
 
 #include "common.h"

@@ -604,6 +604,8 @@ MassPlan mass_plan(const carekv_mass_params& p) {
   m.few = rows <= kFewRows && rows * m.few_stride * 4 <= kFewLds && (long)p.n_keys * p.head_dim * 2 <= (1 << 20);
   m.nkb = (p.n_keys + kMassKeys - 1) / kMassKeys;
   m.nqb = (int)((rows + 255) / 256);
+  m.parts = m.nsk = 1;
+  if (m.few) return m;
   const long seg = p.n_queries >= 32 ? p.n_queries : rows, nseg = p.n_queries >= 32 ? G : 1;
   const long tiles = (seg + kMassTile - 1) / kMassTile * nseg, ktiles = ((long)p.n_keys + kMassTile - 1) / kMassTile;
   // (a pair of causal walks over as many rows as keys has about the tiles of one whole walk)

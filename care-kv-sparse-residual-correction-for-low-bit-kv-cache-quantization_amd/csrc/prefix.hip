@@ -12,7 +12,17 @@
 // logits; the weights are rounded to the element type for the second product
 // and their sum is not.  The keys are split over work-groups until the GPU is
 // full; prefix_join_kernel then joins the splits' (maximum, sum, O), kept in
-// 32 bits, and the row's own part.
+// 32 bits, and the row's own part.  One split joins its own part itself.
+//
+// K and V rows are padded by 32 bytes in LDS: 16-byte reads of 16 rows then take
+// 5.6 cycles a wave, padded by 16 bytes 9.0.
+//
+// Measured: 16 x 128 rows, 40 heads, D = 128, 4097 keys (172 GFLOP) 198 us, 0.87
+// PFLOP/s: 640 equal work-groups on 768 places, products and exponentials
+// overlapping in part.  64 rows x 32 / 8 heads on 32768 keys (34 GFLOP, 134 MB
+// of K and V) 51 us + 11 us for the join: 48 splits, whose partials are 50 MB;
+// 32 splits 57 + 9, 16 splits 71 + 6.  4 x 8 rows a head on 1000 keys 12 us, one
+// launch.
 #include <algorithm>
 #include <cmath>
 

@@ -14,6 +14,11 @@
 // for all the heads of the walk (64-bit products are what would cost here);
 // where there are too few tokens to fill the GPU the walk is cut into shorter
 // ones.
+//
+// Measured: 4 x 8192 tokens of 80 heads, D = 128 (1.34 GB) 259 us, 5.18 TB/s, the
+// rate of a large copy (5.17); 8 x 2047 tokens of 40 heads, half of each turned
+// (336 MB), 72 us, 4.7 TB/s; one token 4 us.  Stores that pass the caches made
+// the first 245-250 us and the second, part of which stays in them, 83-85.
 #include "common.h"
 #include "host_util.h"
 
