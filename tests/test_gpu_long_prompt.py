@@ -255,6 +255,70 @@ def test_captured_and_replayed():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("correction", [False, True])
+def test_decode_behind_a_prefix_captured(correction, monkeypatch):
+    """decode_attention(prefix=...) in a graph, replayed over new queries and a
+    new prefix with eager calls between."""
+    import care_kv
+    monkeypatch.setenv("CAREKV_CHECK", "0")  # (the status word's read-back waits for the stream)
+    lay, cfg, g = _layer(care_kv)
+    cache = care_kv.CAREKVCache(cfg, n_seq=2)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").half()  # noqa: E731
+    cache.write_prefill(0, r(2, 2, 300, 64), r(2, 2, 300, 64))
+    q, k, v = r(2, 8, 64), r(2, 1500, 64), r(2, 1500, 64)
+
+    def call():
+        return care_kv.decode_attention(cache, 0, q, correction=correction, prefix=(k, v), return_lse=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for turn in range(4):
+        for x in (q, k, v):
+            x.copy_(r(*x.shape))
+        if turn % 2:
+            torch.cuda.synchronize()
+        graph.replay()
+        got = [o.clone() for o in out]
+        for a, b in zip(got, call()):
+            assert torch.equal(a, b)
+
+
+def test_hf_model_keeps_heavy_rows(monkeypatch):
+    """A patched model under CacheConfig.prefill_keep: generates from a long and
+    a padded prompt, its pages hold the kept rows and the decoded ones; a prompt
+    that fits generates the tokens of the unbounded cache."""
+    import care_kv
+    transformers = pytest.importorskip("transformers")
+    monkeypatch.setenv("CAREKV_PREFILL_MODE", "fp")
+    hf = transformers.LlamaConfig(vocab_size=300, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
+                                  num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
+    ids = torch.randint(3, 300, (2, 120), generator=torch.Generator().manual_seed(1)).cuda()
+    mask = torch.ones_like(ids)
+    mask[1, :30] = 0
+    outs = {}
+    for keep in (0, 48, 150):
+        torch.manual_seed(0)
+        model = transformers.LlamaForCausalLM(hf).half().cuda().eval()
+        cfg = care_kv.CacheConfig(num_layers=2, num_heads=4, num_kv_heads=2, head_dim=64, page_size=16, max_pages=16,
+                                  base_bits=4, group_size=32, packed_base=True, scale_quant="int8", prefill_keep=keep,
+                                  prefill_keep_sink=4, prefill_keep_recent=16)
+        model = care_kv.patch_llama_model(model, cfg)
+        with torch.no_grad():
+            outs[keep] = model.generate(ids, attention_mask=mask, max_new_tokens=6, do_sample=False, pad_token_id=0)
+        att = next(m for m in model.modules() if isinstance(m, care_kv.CAREKVLlamaAttention))
+        cache = att._shared.cache
+        rows = [cache.total_valid_tokens(1, 1, s) for s in range(2)]
+        assert rows == [(48 if keep == 48 else 120) + 5, (48 if keep == 48 else 90) + 5]
+        assert outs[keep].shape == (2, 126)
+    assert torch.equal(outs[0], outs[150])
+    assert torch.equal(outs[48][:, :121], outs[0][:, :121])  # the prompt's own attention sees every row
+
+
 def test_host_lists_are_refused_in_captured_code():
     """A captured call takes lengths on the device (or one int); host lists raise
     and leave the capture to go on."""

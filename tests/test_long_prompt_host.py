@@ -181,3 +181,28 @@ def test_config(monkeypatch):
     monkeypatch.setenv("CAREKV_PREFILL_KEEP_WINDOW", "64")
     c = care_kv.CacheConfig(**care_kv.apply_carekv_env_overrides({}))
     assert (c.prefill_keep, c.prefill_keep_sink, c.prefill_keep_recent, c.prefill_keep_window) == (256, 4, 32, 64)
+
+
+def test_launches_on_the_tensors_device(monkeypatch):
+    """Whatever device is current: the launch and its stream are those of the
+    tensors' device (the library and the guard are stand-ins)."""
+    entered, launched = [], []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+
+        def __exit__(self, *exc):
+            entered.pop()
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(_lib, "_raw_stream", lambda index: 100 + index)
+    fn = lambda *a: launched.append((list(entered), a)) or 0  # noqa: E731
+    _lib.call(torch.device("cuda", 1), "x", fn, 7)
+    _lib.call(torch.device("cuda", 0), "x", fn, 8)
+    assert launched == [([torch.device("cuda", 1)], (7, 101)), ([], (8, 100))] and not entered
+    with pytest.raises(_lib.CarekvError):
+        _lib.call(torch.device("cuda", 0), "x", lambda *a: -1)
