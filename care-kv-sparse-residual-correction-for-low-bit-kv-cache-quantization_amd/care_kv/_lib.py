@@ -353,13 +353,23 @@ def call(dev: torch.device, what: str, fn, *args):
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory that a and b span overlaps (the same tensor apart)."""
-    if not a.numel() or not b.numel() or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()):
+    """Whether a and b may share memory: their spans meet, and they are not
+    interleaved as the q and k heads of one fused projection are."""
+    def span(t, below=None):  # bytes that the dims of a stride below `below` step over
+        e = t.element_size()
+        return (sum((n - 1) * s for n, s in zip(t.shape, t.stride()) if below is None or s * e < below) + 1) * e
+    if not a.numel() or not b.numel():
         return False
-
-    def end(t):
-        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa >= pb + span(b) or pb >= pa + span(a):
+        return False
+    steps = [s * t.element_size() for t in (a, b) for n, s in zip(t.shape, t.stride()) if n > 1 and s > 0]
+    for p in set(steps):  # both lie in a period of p bytes, one behind the other
+        if all(s % p == 0 for s in steps if s >= p):
+            d = (pb - pa) % p
+            if span(a, p) <= d and d + span(b, p) <= p:
+                return False
+    return True
 
 
 def check_out(out: torch.Tensor, shape, dtype, name: str, *inputs: torch.Tensor):
@@ -371,7 +381,7 @@ def check_out(out: torch.Tensor, shape, dtype, name: str, *inputs: torch.Tensor)
             (out.shape[-1] > 1 and out.stride(-1) != 1) or
             any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride()))):
         raise ValueError(f"{name} needs the values of a row next to each other and no repeated rows")
-    if any(overlap(out, x) for x in inputs):
+    if any(overlap(out, x) for x in inputs if x.data_ptr() != out.data_ptr() or x.stride() != out.stride()):
         raise ValueError(f"{name} must be its input itself or not overlap it")
 
 

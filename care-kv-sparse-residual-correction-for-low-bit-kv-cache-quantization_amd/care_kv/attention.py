@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from .cache import CAREKVCache, get_sketch_proj, to_device
 from .config import CacheConfig, ReadKnobs, any_read_budget, resolve_read_knobs
-from .prefix import prefix_attention
+from .prefix import check_prefix, prefix_attention
 
 KIND_CODE = {"both": 0, "k": 1, "v": 2}
 
@@ -286,6 +286,11 @@ def decode_attention(cache: CAREKVCache, layer: int, q: torch.Tensor, seqs: Opti
     if knobs is None:
         knobs = resolve_read_knobs(cfg, layer)
     q = q.to(torch.float16).contiguous()
+    if prefix is not None:
+        check_prefix(prefix, Hq, D, torch.float16, q.device)
+        # (the prefix's pass reads q and the prefix after the cached rows' pass has written out)
+        if out is not None and any(_lib.overlap(out, x) for x in (q, *prefix)):
+            raise ValueError("decode_attention: out must not overlap q or the prefix")
     npages = cache.next_page[layer, 0, np.asarray(seqs, dtype=np.int64)].astype(np.int32)
     if n_pages is not None:
         npages = np.minimum(npages, np.asarray(list(n_pages), dtype=np.int32))

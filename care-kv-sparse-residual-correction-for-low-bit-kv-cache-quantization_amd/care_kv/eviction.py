@@ -67,7 +67,9 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is not None:
-        _lib.check_out(out, (B, Hkv, Tk), torch.float32, "out", q, k, *(() if lse is None else (lse,)))
+        _lib.check_out(out, (B, Hkv, Tk), torch.float32, "out")
+        if any(_lib.overlap(out, x) for x in (q, k, lse) if x is not None):
+            raise ValueError("out must not overlap q, k or lse")
     dev = _lib.same_device("attention_mass", q, k, lse, out)
     if out is None:
         out = q.new_empty((B, Hkv, Tk), dtype=torch.float32)
@@ -97,7 +99,7 @@ def evict_rows(mass: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, keep: in
 
     mass (B, Hkv, T) fp32; k and v (B, Hkv, T, D) of any 2- or 4-byte type and
     any strides ((Hkv, T) and (Hkv, T, D) of one sequence work alike, and give
-    results without the batch dim).  ``lengths``: rows of each sequence that
+    results without the batch dim, lengths with one value).  ``lengths``: rows of each sequence that
     count (default T), a device tensor of B integers or (not in captured code) a
     host sequence; what the rows behind them hold is not used.  The results have min(keep, T) places;
     sequences that are shorter keep every row."""

@@ -37,7 +37,7 @@ from .attention import (debug_stats_enabled, decode_attention, decode_read_mode,
                         get_imp_per_layer, importance_probe, prefill_correction, reset_debug_stats)
 from .cache import CAREKVCache
 from .eviction import attention_mass, evict_rows
-from .prefix import prefix_attention
+from .prefix import check_prefix, prefix_attention
 from .rotary import RotaryPlan, rotate_heads
 from .config import CacheConfig, any_read_budget, resolve_read_knobs
 from .prefill import eval_knobs, prefill_attention, prefill_eval, quant_dequant
@@ -133,8 +133,10 @@ class CAREKVLayer(nn.Module):
         Hq, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         Q, K, V = self._project(hidden)
         if position_embeddings is not None and isinstance(position_embeddings[0], RotaryPlan):
-            Q, K = rotate_heads(Q.to(F16), K.to(F16), position_embeddings[1], position_embeddings[0])
-            return Q, K, V.to(F16).contiguous()
+            # 32-bit heads are rounded after the turn; bf16 ones fit fp16 and are rounded by it once
+            Q, K = (x if x.dtype == torch.float32 else x.to(F16) for x in (Q, K))
+            Q, K = rotate_heads(Q, K, position_embeddings[1], position_embeddings[0])
+            return Q.to(F16), K.to(F16), V.to(F16).contiguous()
         cos, sin = (None, None) if position_embeddings is None else (x.to(Q.dtype) for x in position_embeddings)
         q, k, v = (x.transpose(1, 2) for x in (Q, K, V))  # the projections' own layout
         if (q.dtype == F16 and q.is_cuda and B * T > 0 and all(x.is_contiguous() for x in (q, k, v))
@@ -283,6 +285,8 @@ class CAREKVLayer(nn.Module):
             raise NotImplementedError(f"prefill_keep in prefill mode {mode!r} with base_quantizer="
                                       f"{cfg.base_quantizer!r}: the mode reads the pages of the whole prompt")
         Qh, Kh, Vh = self._heads(hidden, position_embeddings)
+        if prefix is not None:  # before anything is written
+            check_prefix(prefix, cfg.num_heads, cfg.head_dim, F16, Qh.device)
         hats = None
         if not evict:
             hats = cache.write_prefill(self.layer_id, Kh, Vh, token_start_abs=token_start_abs,
@@ -346,6 +350,8 @@ class CAREKVLayer(nn.Module):
         B = hidden.shape[0]
         Q, K, V = self._heads(hidden[:, -1:], position_embeddings)
         seqs = list(range(B)) if seqs is None else list(seqs)
+        if prefix is not None:
+            check_prefix(prefix, self.cfg.num_heads, self.cfg.head_dim, F16, Q.device)
         cache.append(self.layer_id, K[:, :, 0], V[:, :, 0], seqs=seqs)
         correction, knobs = decode_read_mode(self.cfg, self.layer_id)
         O = decode_attention(cache, self.layer_id, Q[:, :, 0], seqs=seqs, correction=correction,

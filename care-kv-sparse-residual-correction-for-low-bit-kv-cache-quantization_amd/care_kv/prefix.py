@@ -13,6 +13,22 @@ import torch
 from . import _lib
 
 
+def check_prefix(prefix, heads: int, head_dim: int, dtype, device):
+    """Refuse a (k, v) that prefix_attention would not take behind `heads` query heads."""
+    if len(prefix) != 2:
+        raise ValueError(f"prefix must be (k, v); got {len(prefix)} values")
+    k, v = prefix
+    if k.dim() != 3 or k.shape[2] != head_dim or v.shape != k.shape or not k.shape[0] or heads % k.shape[0]:
+        raise ValueError(f"prefix k {tuple(k.shape)} and v {tuple(v.shape)} must be (kv heads, P, {head_dim}) alike, "
+                         f"with kv heads dividing {heads}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"a prefix needs head_dim 64 or 128 (got {head_dim})")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"prefix k and v must be {dtype} (got {k.dtype}, {v.dtype})")
+    if k.device != device or v.device != device:
+        raise _lib.CarekvError(f"prefix on {k.device} / {v.device}, the queries on {device}")
+
+
 def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                      own: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, sm_scale: Optional[float] = None,
                      return_lse: bool = False, out: Optional[torch.Tensor] = None):

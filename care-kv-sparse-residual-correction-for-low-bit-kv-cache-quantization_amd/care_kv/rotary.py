@@ -137,6 +137,8 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         _lib.check_out(out[0], q.shape, q.dtype, "q_out", q)
         if k is not None:
             _lib.check_out(out[1], k.shape, k.dtype, "k_out", k)
+            if any(_lib.overlap(a, b) for a, b in ((out[0], out[1]), (out[0], k), (out[1], q))):
+                raise ValueError("q_out must not overlap k or k_out, nor k_out q")
     dev = _lib.same_device("rotate_heads", q, k, positions, plan.freqs, *(() if out is None else out))
     if out is None:
         qo = q.new_empty(q.shape)

@@ -389,7 +389,7 @@ int check_evict(const carekv_evict_params* pp) {
                  "keep must be positive, sink and recent not negative and at most keep together");
   CAREKV_REQUIRE(p.n_keys < (1 << 30), "n_keys must be below 2^30");
   CAREKV_REQUIRE(p.row_bytes > 0 && p.row_bytes % 4 == 0, "rows must be a multiple of 4 bytes");
-  CAREKV_REQUIRE((long)p.batch * p.n_kv_heads * evict_parts(p) < (1L << 31), "too many (sequence, kv head) rows");
+  CAREKV_REQUIRE(grid_fits((long)p.batch * p.n_kv_heads * evict_parts(p), kSel), "too many (sequence, kv head) rows");
   return CAREKV_OK;
 }
 }  // namespace
@@ -432,7 +432,7 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
   const bool wide = (bits & 15) == 0;
   const int per = p.row_bytes / (wide ? 16 : 4);
   const long n = bh * p.keep * per;
-  CAREKV_REQUIRE((n + 255) / 256 < (1L << 31), "too many kept rows");
+  CAREKV_REQUIRE(grid_fits((n + 255) / 256, 256), "too many kept rows");
   hipStream_t s = (hipStream_t)stream;
   if (parts == 1) {
     const dim3 grid((unsigned)bh), block(kSel);

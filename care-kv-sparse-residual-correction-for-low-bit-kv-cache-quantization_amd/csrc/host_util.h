@@ -42,6 +42,9 @@ inline uintptr_t operand_bits(const void* p, std::initializer_list<std::pair<int
   return bits;
 }
 
+// Whether a launch of `blocks` work-groups in x fits: the threads of a dimension are counted in 32 bits.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks < (1LL << 32) / threads; }
+
 // Validate the arena against what the kernels support.  On failure the
 // message is left in last_error_buf().
 bool check_arena(const carekv_arena& A);

@@ -665,7 +665,8 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.opart = a.part + (lse ? 0 : 2 * rows * m.nsk);
   hipStream_t s = (hipStream_t)stream;
   const long wgs = hb * ((m.nkb + 1) / 2) * m.parts, swgs = hb * ((m.nqb + 1) / 2) * m.nsk, sum = (hb * p.n_keys + 255) / 256;
-  CAREKV_REQUIRE(wgs < (1L << 31) && swgs < (1L << 31) && sum < (1L << 31) && (rows + 31) / 32 < (1L << 31),
+  CAREKV_REQUIRE(grid_fits(wgs, 512) && grid_fits(swgs, 512) && grid_fits(sum, 256) &&
+                     grid_fits((rows + 31) / 32, 256) && grid_fits(m.few ? hb : 0, 1024),
                  "too many blocks");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
     using ET = decltype(et);

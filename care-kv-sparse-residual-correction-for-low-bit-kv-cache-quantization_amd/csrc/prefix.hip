@@ -486,7 +486,7 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   a.al8 = (rows8 & 7) == 0;
   hipStream_t s = (hipStream_t)stream;
   const long wgs = (long)a.nqb * a.Hkv * ns;
-  CAREKV_REQUIRE(wgs < (1L << 31), "too many row blocks");
+  CAREKV_REQUIRE(grid_fits(wgs, 256) && (ns == 1 || grid_fits(rows / (256 / p.head_dim) + 1, 256)), "too many rows");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
     using ET = decltype(et);
     constexpr int D = decltype(d)::value;

@@ -166,7 +166,7 @@ extern "C" int carekv_rotate_heads(const carekv_rotary_params* pp, const void* q
   const bool wide = (bits & 15) == 0 && p.rotary_dim % 16 == 0 && p.head_dim % 16 == 0;
   const long threads = rows * (p.head_dim / 2 / (wide ? 8 : 1));
   const long blocks = (threads + 255) / 256;
-  CAREKV_REQUIRE(blocks < (1L << 31), "too many elements");
+  CAREKV_REQUIRE(grid_fits(blocks, 256), "too many elements");
   // walks over all heads, cut shorter until 2048 work-groups (8 a CU) are there
   long cuts = (2048 + blocks - 1) / blocks;
   if (cuts > heads) cuts = heads;

@@ -355,3 +355,49 @@ def test_two_streams_at_once():
         for outs in got[i]:
             for a, b in zip(outs, want[i]):
                 assert torch.equal(a, b)
+
+
+def test_refusals_leave_the_cache_alone(monkeypatch):
+    """A prefix that does not fit is refused before a prompt is written or a
+    token appended; an output over the queries or the prefix is refused too."""
+    import care_kv
+    monkeypatch.setenv("CAREKV_PREFILL_MODE", "fp")
+    lay, cfg, g = _layer(care_kv)
+    cache = care_kv.CAREKVCache(cfg, n_seq=2)
+    x = torch.randn(2, 9, 512, generator=g, device="cuda").half()
+    k = torch.randn(2, 33, 64, generator=g, device="cuda").half()
+    plan = care_kv.rotary_plan(64)
+    pe = (plan, torch.arange(33, 42, device="cuda"))
+    for bad in ((k, k[:, :5]), (k.bfloat16(), k.bfloat16()), (k[..., :32], k[..., :32]), (k,)):
+        with pytest.raises(ValueError):
+            lay.prefill(cache, x, position_embeddings=pe, prefix=bad)
+    assert cache.total_valid_tokens(0, 0, 0) == 0
+    lay.prefill(cache, x, position_embeddings=pe, prefix=(k, k))
+    for bad in ((k, k[:, :5]), (k.float(), k.float())):
+        with pytest.raises(ValueError):
+            lay.decode_step(cache, x[:, :1], position_embeddings=(plan, pe[1][:1]), prefix=bad)
+    assert cache.total_valid_tokens(0, 0, 0) == 9
+    q = torch.randn(2, 8, 64, generator=g, device="cuda").half()
+    for out in (q, k.view(-1)[:1024].view(2, 8, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            care_kv.decode_attention(cache, 0, q, prefix=(k, k), out=out)
+
+
+def test_layer_rounds_32_bit_heads_after_the_turn():
+    """fp32 projections: each head value is off by one fp16 rounding of the
+    turned value (half a step, 2^-11 of it; 2^-25 below 2^-14) and the 32-bit turn's own error."""
+    import care_kv
+    lay, _, g = _layer(care_kv)
+    for p in lay.parameters():
+        p.data = p.data.float()
+    x = torch.randn(2, 37, 512, generator=g, device="cuda")
+    plan = care_kv.rotary_plan(64)
+    pos = torch.arange(1000, 1037, device="cuda")
+    Q, K, _ = lay._project(x)
+    q, k, _ = lay._heads(x, (plan, pos))
+    for got, x0 in ((q, Q), (k, K)):
+        want = _rot64(x0, pos, plan)
+        m = x0.abs().double()
+        m = m + torch.cat((m[..., 32:], m[..., :32]), -1)
+        # angles off by 2^-26 turns (2 pi 2^-26 < 2^-23) and their 32-bit sine, cosine and products
+        assert got.dtype == F16 and ((got.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -21 * m).all()

@@ -206,3 +206,65 @@ def test_launches_on_the_tensors_device(monkeypatch):
     assert launched == [([torch.device("cuda", 1)], (7, 101)), ([], (8, 100))] and not entered
     with pytest.raises(_lib.CarekvError):
         _lib.call(torch.device("cuda", 0), "x", lambda *a: -1)
+
+
+def _brute(a, b):
+    """Whether two strided views share a byte, by listing both."""
+    def cells(t):
+        at = {t.data_ptr()}
+        for n, st in zip(t.shape, t.stride()):
+            at = {x + i * st * t.element_size() for x in at for i in range(n)}
+        return {x + j for x in at for j in range(t.element_size())}
+    return bool(cells(a) & cells(b))
+
+
+def test_overlap_of_views():
+    """Never missed, and the heads of fused projections in either order are told apart."""
+    a = torch.zeros(2, 5, 12, 8, dtype=torch.float16)  # (B, T, heads, D)
+    c = torch.zeros(2, 12, 5, 8, dtype=torch.float16)  # (B, heads, T, D)
+    split = lambda x: [x[:, :, :6].transpose(1, 2), x[:, :, 6:9].transpose(1, 2), x[:, :, 4:8].transpose(1, 2)]  # noqa: E731
+    views = split(a) + [c[:, :6], c[:, 6:9], c[:, 4:8], a[..., :4], a[..., 4:], a[:1], a[1:], a[:, 1:3], a[:, ::2],
+                        a[:, 1::2], a.float(), a.view(torch.float32), a[:, :0], a[0, 0, 0], a[:1].expand(3, 5, 12, 8)]
+    for x in views:
+        for y in views:
+            shared = bool(x.numel() and y.numel()) and _brute(x, y)
+            assert _lib.overlap(x, y) or not shared
+    for x, y in ((views[0], views[1]), (views[3], views[4]), (views[6], views[7]), (a[:, ::2], views[9])):
+        assert _lib.overlap(x, y) == _brute(x, y) == _lib.overlap(y, x)
+
+
+def test_outputs_over_inputs_are_refused():
+    q, k, pos = _half(2, 4, 3, 64), _half(2, 4, 3, 64), torch.zeros(2, 3, dtype=torch.int64)
+    buf = _half(2, 7, 3, 64)
+    for a, b, out in ((q, k, (k, q)), (q, q, (q, q)), (q, k, (_half(2, 4, 3, 64), q)), (q, k, (buf[:, :4], buf[:, 3:])),
+                      (buf[:, :4], buf[:, 3:], (buf[:, :4], buf[:, 3:]))):
+        with pytest.raises(ValueError, match="overlap"):
+            care_kv.rotate_heads(a, b, pos, _plan(), out=out)
+    lse = torch.zeros(2, 4, 3)  # of the output's own shape
+    with pytest.raises(ValueError, match="overlap"):
+        care_kv.attention_mass(q, k, lse=lse, out=lse)
+
+
+def test_prefix_is_checked_before_the_cache_changes():
+    from care_kv.prefix import check_prefix
+    k = _half(2, 9, 64)
+    check_prefix((k, k), 4, 64, torch.float16, k.device)
+    for p, h, d in (((k,), 4, 64), ((k, k[:, :8]), 4, 64), ((k, k), 3, 64), ((k, k), 4, 128), ((k, k.bfloat16()), 4, 64),
+                    ((k[..., :32], k[..., :32]), 4, 32), ((k[None], k[None]), 4, 64), ((k[:0], k[:0]), 4, 64)):
+        with pytest.raises(ValueError):
+            check_prefix(p, h, d, torch.float16, k.device)
+
+
+def test_launches_that_do_not_fit_are_refused():
+    """Grids of 2^32 threads and more: refused with a message, nothing launched."""
+    lib = _lib.load()
+    p = 4096
+    rot = _lib.RotaryParams(batch=1 << 15, seq_len=1 << 20, n_heads=1, n_kv_heads=0, head_dim=64, rotary_dim=64, dtype=0,
+                            pos_bits=64)
+    assert lib.carekv_rotate_heads(rot, p, None, p, p, p, None, None) == -1
+    mass = _lib.MassParams(batch=1 << 20, n_heads=8, n_kv_heads=8, n_queries=1, n_keys=9, head_dim=64, dtype=0)
+    assert lib.carekv_attention_mass(mass, p, p, None, None, None, p, p, 1 << 62, None) == -1
+    ev = _lib.EvictParams(batch=1 << 20, n_kv_heads=8, n_keys=9, row_bytes=128, keep=4)
+    assert lib.carekv_evict_rows(ev, p, p, p, None, p, p, p, p, p, p, 1 << 62, None) == -1
+    pre = _lib.PrefixParams(batch=1 << 20, n_heads=64, n_kv_heads=8, seq_len=8, prefix_len=0, head_dim=128)
+    assert lib.carekv_prefix_attn(pre, p, p, p, None, None, p, None, p, 1 << 62, None) == -1
