@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "fast_div.h"
 #include "host_util.h"
 
 namespace carekv {
@@ -38,6 +39,7 @@ struct EvictArgs {
   int32_t* kept;
   long m_sb, m_sh, k_sb, k_sh, k_st, v_sb, v_sh, v_st;  // bytes
   int H, T, keep, sink, recent, row_bytes;
+  FastDiv by_h, by_parts, by_per;  // per: threads of a kept row
 };
 
 // unsigned order of a weight: -inf < finite < +inf as unsigned integers, NaN lowest
@@ -196,8 +198,8 @@ __device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* ke
 
 // Row r of the (sequence, kv head) at km / vm, copied to its place by threads c of the row's `per`.
 template <typename V>
-__device__ __forceinline__ void copy_row(const EvictArgs& a, long bh, long r, int j, int c) {
-  const long b = bh / a.H, h = bh - b * a.H;
+__device__ __forceinline__ void copy_row(const EvictArgs& a, int bh, long r, int j, int c) {
+  const long b = bh / a.by_h, h = bh - b * a.H;
   V x{}, y{};
   if (j >= 0) {
     x = *reinterpret_cast<const V*>(a.k + b * a.k_sb + h * a.k_sh + j * a.k_st + c);
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   constexpr bool FUSE = !std::is_void<V>::value;
   __shared__ __align__(16) int hist[3][kBins];
   __shared__ SelectScratch sc;
-  const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x;
+  const int b = (int)blockIdx.x / a.by_h, h = blockIdx.x - b * a.H, tid = threadIdx.x;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
   for (int i = tid; i < 3 * kBins; i += kSel) hist[0][i] = 0;
   uint32_t key[kEpt];
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
     __syncthreads();  // (the indices, written by this work-group, are read back by it)
     const int per = a.row_bytes / (int)sizeof(V);
     for (int i = tid; i < a.keep * per; i += kSel) {
-      const int r = i / per;
+      const int r = i / a.by_per;
       copy_row<V>(a, blockIdx.x, (long)blockIdx.x * a.keep + r, index[r], (i - r * per) * (int)sizeof(V));
     }
   }
@@ -268,10 +270,10 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
                                                           int* state) {
   __shared__ int sh_hist[kBins];
   __shared__ SelectScratch sc;
-  const int bh = blockIdx.x / parts, pt = blockIdx.x % parts, tid = threadIdx.x;
-  const int b = bh / a.H, h = bh % a.H;
+  const int bh = (int)blockIdx.x / a.by_parts, pt = blockIdx.x - bh * parts, tid = threadIdx.x;
+  const int b = bh / a.by_h, h = bh - b * a.H;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
-  const int i0 = (int)((long)a.T * pt / parts), t1 = (int)((long)a.T * (pt + 1) / parts);
+  const int i0 = part_start(a.T, pt, a.by_parts), t1 = part_start(a.T, pt + 1, a.by_parts);
   // a turn's weights; the first turn's are on their way before anything else is known
   float x[kEpt];
   auto load_turn = [&](int c0) {
@@ -369,8 +371,8 @@ template <typename V>
 __global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a, long n, int per) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
-  const long r = i / per;  // (sequence, kv head, kept row)
-  copy_row<V>(a, r / a.keep, r, a.index[r], (int)(i - r * per) * (int)sizeof(V));
+  const uint32_t r = (uint32_t)i / (uint32_t)per;  // (sequence, kv head, kept row); n is below 2^32
+  copy_row<V>(a, (int)(r / (uint32_t)a.keep), r, a.index[r], (int)(i - (long)r * per) * (int)sizeof(V));
 }
 
 namespace {
@@ -432,6 +434,7 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
   const bool wide = (bits & 15) == 0;
   const int per = p.row_bytes / (wide ? 16 : 4);
   const long n = bh * p.keep * per;
+  a.by_h = FastDiv(p.n_kv_heads); a.by_parts = FastDiv(parts); a.by_per = FastDiv(per);
   CAREKV_REQUIRE(grid_fits((n + 255) / 256, 256), "too many kept rows");
   hipStream_t s = (hipStream_t)stream;
   if (parts == 1) {

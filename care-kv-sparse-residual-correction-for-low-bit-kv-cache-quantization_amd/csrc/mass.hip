@@ -41,6 +41,7 @@
 // for a given lse the part of lse log2(e) that a 32-bit M does not hold.
 #include <algorithm>
 
+#include "fast_div.h"
 #include "mfma16.h"
 
 namespace carekv {
@@ -60,6 +61,7 @@ struct MassArgs {
   int B, Hq, Hkv, G, Tq, Tk, causal, accumulate;
   int nkb, parts;          // mass walks: key blocks, parts that a pair of blocks' walk is cut into
   int nqb, nsk;            // statistics: row blocks, parts of a walk
+  FastDiv by_nhb, by_hkv, by_tq, by_kpairs, by_qpairs, by_parts, by_nsk;  // nhb = B Hkv, pairs of blocks
   int nseg, seg;           // a mass walk: nseg lists of seg rows
   float sm_log2;
 };
@@ -111,9 +113,9 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   __shared__ int s_lim[2][QT];
   __shared__ float s_sum[4 * TT][512];  // the outer sums: the registers they would take spill others
   // Sequences and heads go round the XCDs, the blocks of one part run together: they meet in one L2.
-  const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
-  const int np = (a.nkb + 1) / 2, pair = rest % np, pt = rest / np;
-  const int b = hb / a.Hkv, hk = hb % a.Hkv;
+  const int nhb = a.by_nhb.d, rest = (int)blockIdx.x / a.by_nhb, hb = blockIdx.x - rest * nhb;
+  const int pt = rest / a.by_kpairs, pair = rest - pt * a.by_kpairs.d;
+  const int b = hb / a.by_hkv, hk = hb - b * a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
   const MassSeq sq = mass_seq(a, b);
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   auto tiles_of = [&](int kb) { return (a.seg - first_row(kb) + QT - 1) / QT * a.nseg; };
   // The pair's walks, one after the other, as one: this part's tiles of it.
   const int kb_b = a.nkb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (kb_b > pair ? tiles_of(kb_b) : 0);
-  const int lo = (int)((long)n_all * pt / a.parts), hi = (int)((long)n_all * (pt + 1) / a.parts);
+  const int lo = part_start(n_all, pt, a.by_parts), hi = part_start(n_all, pt + 1, a.by_parts);
   float* dst = a.parts > 1 ? a.opart + ((long)pt * nhb + hb) * a.Tk : a.out + b * a.o_sb + hk * a.o_sh;
   const uint32_t off0 = (uint32_t)(threadIdx.x / CHR * a.q_st + (threadIdx.x % CHR) * 16);
   const char* qbase = a.q + b * a.q_sb + (long)hk * a.G * a.q_sh;
@@ -136,7 +138,9 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   const int kb = f ? kb_b : pair, j0 = kb * kMassKeys + 16 * TT * w;  // the block, the wave's first key
   const int t_first = first_row(kb), t_end = a.seg, per = max(1, (t_end - t_first + QT - 1) / QT);
   const int at = max(lo - (f ? n_a : 0), 0), nt = min(hi, f ? n_all : n_a) - (f ? n_a : 0) - at;
-  int sg = at / per, i0 = t_first + (at - sg * per) * QT;  // the tile loaded next
+  int sg = 0, i0 = at;  // the tile loaded next: list, first row
+  while (i0 >= per) { i0 -= per; ++sg; }  // (at most nseg turns)
+  i0 = t_first + i0 * QT;
   // K operands: tokens j0 + 16 tt + c16, dims 32 s + 8 g .. (keys past the end: the last one, masked below)
   V8 kf[TT][KS];
   if (nt > 0) {
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     } else {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int i = i0 + (int)threadIdx.x / CHR + 512 / CHR * k, h = i / a.Tq, t = i - h * a.Tq;
+        const int i = i0 + (int)threadIdx.x / CHR + 512 / CHR * k, h = i / a.by_tq, t = i - h * a.Tq;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (i < t_end)
           v = *reinterpret_cast<const uint4*>(qbase + h * a.q_sh + t * a.q_st + (threadIdx.x % CHR) * 16);
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
       const int i = i0 + lane;
       int h = sg, t = i;
       if (!listed) {
-        h = i / a.Tq;
+        h = i / a.by_tq;
         t = i - h * a.Tq;
         n_lim = i < t_end ? mass_limit(a, sq, t) : 0;
       }
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassArgs a) {
   if (i >= n) return;
   float v = 0.f;
   for (int p = 0; p < a.parts; ++p) v += a.opart[p * n + i];
-  const long hb = i / a.Tk, b = hb / a.Hkv;
+  const long hb = (uint32_t)i / (uint32_t)a.Tk, b = (int)hb / a.by_hkv;
   float* dst = a.out + b * a.o_sb + (hb - b * a.Hkv) * a.o_sh + (i - hb * a.Tk);
   *dst = a.accumulate ? *dst + v : v;
 }
@@ -301,9 +305,9 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   constexpr int TT = 2, KT = kMassTile, KS = D / 32, KRS = 2 * D + 32, CHR = D / 8, NCH = KT * CHR / 512;
   constexpr float kOver = 64.f;
   __shared__ __align__(16) char lds[2][KT * KRS];
-  const int nhb = a.Hkv * a.B, hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
-  const int np = (a.nqb + 1) / 2, pair = rest % np, sp = rest / np;
-  const int b = hb / a.Hkv, hk = hb % a.Hkv;
+  const int rest = (int)blockIdx.x / a.by_nhb, hb = blockIdx.x - rest * a.by_nhb.d;
+  const int sp = rest / a.by_qpairs, pair = rest - sp * a.by_qpairs.d;
+  const int b = hb / a.by_hkv, hk = hb - b * a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
   const int rows = a.G * a.Tq;
@@ -316,12 +320,12 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   // tiles of the keys that some row of block qb sees: its rows' furthest limit, a head's last row where it has one
   auto tiles_of = [&](int qb) {
     const int ra = qb * 256, rz = min(ra + 256, rows) - 1;
-    const int t = ra / a.Tq != rz / a.Tq || rz % a.Tq == a.Tq - 1 ? a.Tq - 1 : rz % a.Tq;
+    const int hz = rz / a.by_tq, t = ra < hz * a.Tq ? a.Tq - 1 : rz - hz * a.Tq;
     return (mass_limit(a, sq, t) + KT - 1) / KT;
   };
   // The pair's walks, one after the other, as one: this part's tiles of it.
   const int qb_b = a.nqb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (qb_b > pair ? tiles_of(qb_b) : 0);
-  const int from = (int)((long)n_all * sp / a.nsk), to = (int)((long)n_all * (sp + 1) / a.nsk);
+  const int from = part_start(n_all, sp, a.by_nsk), to = part_start(n_all, sp + 1, a.by_nsk);
 #pragma unroll 1
   for (int f = 0; f < (qb_b > pair ? 2 : 1); ++f) {
   const int r0 = (f ? qb_b : pair) * 256 + 16 * TT * w;
@@ -330,7 +334,7 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   int lim[4 * TT], lo = 0x7fffffff;
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
-    const int r = min(r0 + 16 * tt + c16, rows - 1), h = r / a.Tq, t = r - h * a.Tq;
+    const int r = min(r0 + 16 * tt + c16, rows - 1), h = r / a.by_tq, t = r - h * a.Tq;
     const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[tt][s] = load8<V8>(qp + (32 * s + 8 * g) * 2);
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   int hi = 0;
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
-    int r = r0 + 16 * tt + 4 * g, t = r % a.Tq;
+    int r = r0 + 16 * tt + 4 * g, t = r % a.by_tq;
 #pragma unroll
     for (int i = 0; i < 4; ++i, ++r) {
       lim[4 * tt + i] = r < rows ? mass_limit(a, sq, t) : 0;
@@ -480,10 +484,10 @@ __global__ __launch_bounds__(1024) void mass_few_kernel(MassArgs a, int stride) 
   __shared__ __align__(16) float sc[kFewLds / 4];  // [rows][stride] base-2 logits
   __shared__ float s_m[16][16], s_l[16][16];
   __shared__ float2 s_st[16];
-  const int hb = blockIdx.x, b = hb / a.Hkv, hk = hb % a.Hkv, rows = a.G * a.Tq;
+  const int hb = blockIdx.x, b = hb / a.by_hkv, hk = hb - b * a.Hkv, rows = a.G * a.Tq;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int r = min(c16, rows - 1), h = r / a.Tq, t = r - h * a.Tq;
+  const int r = min(c16, rows - 1), h = r / a.by_tq, t = r - h * a.Tq;
   V8 qf[KS];
   const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
 #pragma unroll
@@ -658,6 +662,9 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.nkb = m.nkb; a.parts = m.parts; a.nqb = m.nqb; a.nsk = m.nsk;
   if (p.n_queries >= 32) { a.nseg = a.G; a.seg = a.Tq; }
   else { a.nseg = 1; a.seg = a.G * a.Tq; }
+  a.by_nhb = FastDiv((long)p.batch * p.n_kv_heads); a.by_hkv = FastDiv(p.n_kv_heads);
+  a.by_tq = FastDiv(std::max(p.n_queries, 1)); a.by_parts = FastDiv(m.parts); a.by_nsk = FastDiv(m.nsk);
+  a.by_kpairs = FastDiv((m.nkb + 1) / 2); a.by_qpairs = FastDiv(std::max((m.nqb + 1) / 2, 1));
   a.sm_log2 = (float)((double)p.sm_scale * 1.4426950408889634074);
   const long rows = (long)p.batch * p.n_heads * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
   a.stat = (float*)workspace;

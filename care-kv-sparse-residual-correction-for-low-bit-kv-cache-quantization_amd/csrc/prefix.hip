@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "fast_div.h"
 #include "host_util.h"
 #include "mfma16.h"
 
@@ -44,6 +45,7 @@ struct PrefixArgs {
   long q_sb, q_sh, q_st, k_sh, k_st, v_sh, v_st, o_sb, o_sh, o_st, w_sb, w_sh, w_st;  // bytes
   long rows;             // n_kv_heads * M
   int B, Hq, Hkv, G, T, P, M, nqb, nsplit;
+  FastDiv by_t, by_g, by_nqb, by_nsplit, by_m;
   float sm_log2;         // |scale| log2(e), 1 where that is 0
   uint32_t q_sign;       // sign bits of two elements where the scale is negative
   uint32_t q_keep;       // 0 where the scale is 0 (0 times the -inf of a masked score would be NaN), else all bits
@@ -56,9 +58,9 @@ struct PrefixRow {
 };
 __device__ __forceinline__ PrefixRow prefix_row(const PrefixArgs& a, int hk, int r) {
   PrefixRow x;
-  const int bg = r / a.T;
+  const int bg = r / a.by_t;
   x.t = r - bg * a.T;
-  x.b = bg / a.G;
+  x.b = bg / a.by_g;
   x.h = hk * a.G + bg - x.b * a.G;
   return x;
 }
@@ -127,13 +129,13 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   const int n = gridDim.x;
   int it = blockIdx.x;
   if (n % 8 == 0) it = it % 8 * (n / 8) + it / 8;
-  const int qblk = it % a.nqb, sp = it / a.nqb % a.nsplit, hk = it / a.nqb / a.nsplit;
+  const int blk = it / a.by_nqb, qblk = it - blk * a.nqb, hk = blk / a.by_nsplit, sp = blk - hk * a.nsplit;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
   const int r0 = qblk * QB + QW * (WK == 1 ? w : 0), wk = WK == 1 ? 0 : w;  // first row, key quarter of the wave
   const int tiles = (a.P + KT - 1) / KT;
-  const int tile0 = (int)((long)sp * tiles / a.nsplit), tile1 = (int)((long)(sp + 1) * tiles / a.nsplit);
+  const int tile0 = part_start(tiles, sp, a.by_nsplit), tile1 = part_start(tiles, sp + 1, a.by_nsplit);
   const int j0 = tile0 * KT, keys = min(tile1 * KT, a.P) - j0;  // the split's keys (at least one)
   const char* kbase = a.k + hk * a.k_sh + j0 * a.k_st;
   const char* vbase = a.v + hk * a.v_sh + j0 * a.v_st;
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
     LL += s_ml[rw][i].y * f;
     O += s_o[(rw * JG + i) * D4 + d4] * f;
   }
-  const int hk = (int)(pr / a.M);
+  const int hk = (int)pr / a.by_m;
   const PrefixRow x = prefix_row(a, hk, (int)(pr - (long)hk * a.M));
   const PrefixOwn<ET> own(a, x, mm);
   own.write(a, x, 4 * d4, O, LL);
@@ -475,6 +477,8 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   a.w_sb = 2 * p.own_sb; a.w_sh = 2 * p.own_sh; a.w_st = 2 * p.own_st;
   a.B = p.batch; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.T = p.seq_len;
   a.P = p.prefix_len; a.M = p.batch * a.G * p.seq_len; a.rows = rows; a.nqb = plan.nqb; a.nsplit = ns;
+  a.by_t = FastDiv(a.T); a.by_g = FastDiv(a.G); a.by_m = FastDiv(a.M);
+  a.by_nqb = FastDiv(std::max(a.nqb, 1)); a.by_nsplit = FastDiv(std::max(ns, 1));
   a.po = (float*)workspace;
   a.pml = a.po + ns * rows * p.head_dim;
   a.sm_log2 = (float)(std::fabs((double)p.sm_scale) * 1.4426950408889634074);

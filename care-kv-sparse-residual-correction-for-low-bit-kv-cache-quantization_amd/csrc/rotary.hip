@@ -78,11 +78,10 @@ template <typename E, int PV, bool IL, bool P64>
 __global__ __launch_bounds__(256) void rotate_heads_kernel(RotaryArgs a) {
   constexpr bool W = PV > 1;
   const int per = a.D / 2 / PV, nrot = a.R / 2 / PV;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = i / per;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / (uint32_t)per;  // (a grid's threads are below 2^32)
   if (row >= a.rows) return;
   const int u = (int)(i - row * per);
-  const long b = row / a.T, t = row - b * a.T;
+  const long b = row / (uint32_t)a.T, t = row - b * a.T;
   const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.H);
   const bool rot = u < nrot;
   float c[PV], s[PV];
