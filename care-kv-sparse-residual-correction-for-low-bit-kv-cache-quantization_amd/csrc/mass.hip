@@ -18,7 +18,8 @@
 // stationary, key tiles walked, each lane with its own (reference, sum) per row.
 // The reference is no maximum, only a value that no logit passes by 2^64: sums
 // stay in 32-bit range, their accuracy is relative, so that it need not move
-// with every larger score.  mass_join_kernel joins the walks' parts.
+// with every larger score.  mass_join_kernel joins the walks' parts; those of few
+// rows are joined by the mass walks.
 //
 // mass_few_kernel, at most 16 rows a kv head (a decode step): a work-group a
 // (sequence, kv head), the scores of all keys in LDS, K read once, one launch.
@@ -32,8 +33,9 @@
 // pairs, 2048 work-groups: 350; LDS rows padded by 16 bytes (9.0 cycles a read
 // against 5.6): 360; masked wave tiles not skipped: 337; 4 waves of 64 keys or
 // 32 x 32 products were slower (363 and 374 before these).  A window of 64 rows
-// on 4 x 8191 keys: 28 us statistics, 31 us weights, each reading K (67 MB, 13
-// us at the copy rate).
+// on 4 x 8191 keys: 27 us statistics, 32 us weights, 8 us each before the first
+// products and 1.1 us a tile and CU, which two work-groups a CU (or two tiles on
+// their way) change by little: K (67 MB) is not what bounds them.
 //
 // Sums: a lane adds at most kFlush tiles' weights before they go to an outer
 // sum, so that a key's total over 2^15 rows keeps the accuracy of a short sum.
@@ -61,12 +63,13 @@ struct MassArgs {
   int B, Hq, Hkv, G, Tq, Tk, causal, accumulate;
   int nkb, parts;          // mass walks: key blocks, parts that a pair of blocks' walk is cut into
   int nqb, nsk;            // statistics: row blocks, parts of a walk
+  int fold;                // mass_kernel joins the parts of its rows' statistics itself
   FastDiv by_nhb, by_hkv, by_tq, by_kpairs, by_qpairs, by_parts, by_nsk;  // nhb = B Hkv, pairs of blocks
   int nseg, seg;           // a mass walk: nseg lists of seg rows
   float sm_log2;
 };
 
-constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072;
+constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072, kFoldRows = 256;
 
 // A sequence's visible keys: row t sees j < min(len, qs + t + 1), not causal: j < len.
 struct MassSeq {
@@ -103,6 +106,32 @@ __device__ __forceinline__ V8 load8(const char* p) {
   return x;
 }
 
+// (M, w) of a row, given to the first of its N lanes (u = 0 .. N - 1), from the parts of its walk, eight of a lane's
+// loads in flight.  A row that sees nothing has (inf, 0): weights of 0.
+template <int N>
+__device__ __forceinline__ float2 join_parts(const float2* p, int nsk, int u) {
+  float mx = kLowest, l = 0.f;
+  for (int s0 = u; s0 < nsk; s0 += 8 * N) {
+    float2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[min(s0 + N * i, nsk - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (s0 + N * i >= nsk) break;
+      const float m = fmaxf(mx, v[i].x);
+      l = l * __builtin_amdgcn_exp2f(mx - m) + v[i].y * __builtin_amdgcn_exp2f(v[i].x - m);
+      mx = m;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    const float m = fmaxf(mx, __shfl_xor(mx, o, 64)), f = l * __builtin_amdgcn_exp2f(mx - m);
+    l = f + __shfl_xor(f, o, 64);
+    mx = m;
+  }
+  return l != 0.f ? make_float2(mx, 1.f / l) : make_float2(INFINITY, 0.f);
+}
+
 template <typename ET, int D>
 __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   using V8 = typename ET::V8;
@@ -111,6 +140,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   static_assert(QT == 64, "a wave has a tile's rows");
   __shared__ float2 s_st[2][QT];
   __shared__ int s_lim[2][QT];
+  __shared__ float2 s_row[kFoldRows];  // every row's (M, w), where the statistics' parts are joined here
   __shared__ float s_sum[4 * TT][512];  // the outer sums: the registers they would take spill others
   // Sequences and heads go round the XCDs, the blocks of one part run together: they meet in one L2.
   const int nhb = a.by_nhb.d, rest = (int)blockIdx.x / a.by_nhb, hb = blockIdx.x - rest * nhb;
@@ -118,6 +148,13 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   const int b = hb / a.by_hkv, hk = hb - b * a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
+  if (a.fold) {  // (256 rows, two lanes each; before the length is known)
+    const int r = threadIdx.x / 2, rows = a.G * a.Tq;
+    const float2 st = join_parts<2>(reinterpret_cast<const float2*>(a.part) + ((long)hb * rows + min(r, rows - 1)) * a.nsk,
+                                    a.nsk, threadIdx.x & 1);
+    if (threadIdx.x % 2 == 0) s_row[r] = st;
+    __syncthreads();
+  }
   const MassSeq sq = mass_seq(a, b);
   const long hrow = (long)hb * a.G * a.Tq;  // first row of this (sequence, kv head) in stat / lse
   const bool listed = a.nseg > 1 || a.G == 1;  // a list is a head's rows
@@ -191,6 +228,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
       n_st = make_float2(INFINITY, 0.f);
       if (i < t_end) {
         if (a.lse) n_st.x = a.lse[r];
+        else if (a.fold) n_st = s_row[h * a.Tq + t];
         else n_st = *reinterpret_cast<const float2*>(a.stat + 2 * r);
       }
     }
@@ -451,28 +489,12 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   }
 }
 
-// (M, w) of every row from the parts of its walk.  A row that sees nothing
-// has (inf, 0): weights of 0.
+// (M, w) of every row from the parts of its walk.
 __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a) {
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) / 8;  // 8 lanes a row
-  const int u = threadIdx.x & 7;
   const bool in = i < (long)a.B * a.Hq * a.Tq;
-  const float2* p = reinterpret_cast<const float2*>(a.part) + (in ? i : 0) * a.nsk;
-  float mx = kLowest, l = 0.f;
-  for (int s = u; s < a.nsk; s += 8) {
-    const float2 v = p[s];
-    const float m = fmaxf(mx, v.x);
-    l = l * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
-    mx = m;
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    const float m = fmaxf(mx, __shfl_xor(mx, o, 64)), f = l * __builtin_amdgcn_exp2f(mx - m);
-    l = f + __shfl_xor(f, o, 64);
-    mx = m;
-  }
-  if (in && u == 0)
-    reinterpret_cast<float2*>(a.stat)[i] = l != 0.f ? make_float2(mx, 1.f / l) : make_float2(INFINITY, 0.f);
+  const float2 st = join_parts<8>(reinterpret_cast<const float2*>(a.part) + (in ? i : 0) * a.nsk, a.nsk, threadIdx.x & 7);
+  if (in && threadIdx.x % 8 == 0) reinterpret_cast<float2*>(a.stat)[i] = st;
 }
 
 // At most 16 rows a kv head: 16 waves take 64 keys each in turn.  Lane: keys
@@ -584,19 +606,29 @@ int check_mass(const carekv_mass_params* pp) {
 // How a call is cut: the kernel of few rows, or walks.  A causal walk is the
 // longer the earlier its key block (the later its row block) lies; the first and
 // the last block, the second and the last but one .. make pairs of equal length,
-// each cut into equal parts.  All 512 work-groups that the GPU holds at once then
-// end together: the number of parts that makes rounds x (tiles of a part + 3, a
-// part's start) least is taken.
+// each cut into equal parts, so that all work-groups end together.
+//
+// The number of parts that costs least is taken, in times of a tile: a round of
+// 512 work-groups (2 a CU) starts in 7 of them; two on a CU take its tiles by
+// turns, 2.5 % faster than one alone; the sum of a mass walk's parts costs 3, each
+// part that a row's statistics are joined from 0.06.
+// Measured (D = 128, 32 / 8 heads, 4 x 64 rows, one WG a CU and tile 1.1 us): K of
+// 2048, 1 / 2 / 4 / 8 parts 22.6 / 21.0 / 19.2 / 29.7 us with the sum, of 4096 23.4
+// / 24.8 / 32.7, of 8192 32.0 / 42.4; statistics of 1024 keys, 2 / 4 / 8 / 16 parts
+// 18.0 / 13.5 / 11.3 / 12.2, of 8192 4 / 8 / 16 / 24 45.7 / 27.9 / 26.5 / 30.4.
 struct MassPlan {
   bool few;
   int few_stride;
   int nkb, parts, nqb, nsk;
+  bool fold;
 };
-int walk_parts(long pairs, long tiles) {
+int walk_parts(long pairs, long tiles, double sum, double each) {
   long best = 1;
   double least = 1e300;
-  for (long p = 1; p <= 64 && (p == 1 || p * 4 <= tiles); ++p) {
-    const double c = (double)((pairs * p + 511) / 512) * ((double)tiles / p + 3);
+  for (long p = 1; p <= 64 && (p == 1 || p * 2 <= tiles); ++p) {
+    const long wgs = pairs * p;
+    const double turns = wgs <= 256 ? 1 : 0.975 * ((wgs + 255) / 256);
+    const double c = 7.0 * ((wgs + 511) / 512) + turns * tiles / p + (p > 1 ? sum : 0) + each * p;
     if (c < least) { least = c; best = p; }
   }
   return (int)best;
@@ -614,8 +646,12 @@ MassPlan mass_plan(const carekv_mass_params& p) {
   const long tiles = (seg + kMassTile - 1) / kMassTile * nseg, ktiles = ((long)p.n_keys + kMassTile - 1) / kMassTile;
   // (a pair of causal walks over as many rows as keys has about the tiles of one whole walk)
   const bool tri = p.causal && 2L * p.n_queries > p.n_keys;
-  m.parts = walk_parts(hb * ((m.nkb + 1) / 2), tri || m.nkb == 1 ? tiles : 2 * tiles);
-  m.nsk = walk_parts(hb * ((m.nqb + 1) / 2), tri || m.nqb == 1 ? ktiles : 2 * ktiles);
+  m.parts = walk_parts(hb * ((m.nkb + 1) / 2), tri || m.nkb == 1 ? tiles : 2 * tiles, 3, 0);
+  m.nsk = walk_parts(hb * ((m.nqb + 1) / 2), tri || m.nqb == 1 ? ktiles : 2 * ktiles, 0, 0.06);
+  // Few rows' statistics are joined by the mass walks themselves where one round of them is at work and the parts are
+  // at most half of a block's K: 4 x 64 rows on 8191 keys, 16 parts, 60.7 us with the 5 us launch, 59.9 without; 1 x 64
+  // rows on 8192 keys, 32 parts, 33 with it, 40 without.
+  m.fold = rows > 0 && rows <= kFoldRows && rows * m.nsk <= 16 * kFoldRows && hb * ((m.nkb + 1) / 2) * m.parts <= 512;
   return m;
 }
 long mass_ws(const carekv_mass_params& p, bool have_lse) {
@@ -667,6 +703,7 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.by_kpairs = FastDiv((m.nkb + 1) / 2); a.by_qpairs = FastDiv(std::max((m.nqb + 1) / 2, 1));
   a.sm_log2 = (float)((double)p.sm_scale * 1.4426950408889634074);
   const long rows = (long)p.batch * p.n_heads * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
+  a.fold = m.fold && !lse;
   a.stat = (float*)workspace;
   a.part = a.stat + (lse ? 0 : 2 * rows);
   a.opart = a.part + (lse ? 0 : 2 * rows * m.nsk);
@@ -686,8 +723,10 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
     if (!lse && rows > 0) {
       hipLaunchKernelGGL((stats_kernel<ET, D>), dim3((unsigned)swgs), dim3(512), 0, s, a);
       CAREKV_CHECK_LAUNCH("mass_stats");
-      hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, a);
-      CAREKV_CHECK_LAUNCH("mass_join");
+      if (!a.fold) {
+        hipLaunchKernelGGL(mass_join_kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, a);
+        CAREKV_CHECK_LAUNCH("mass_join");
+      }
     }
     hipLaunchKernelGGL((mass_kernel<ET, D>), dim3((unsigned)wgs), dim3(512), 0, s, a);
     CAREKV_CHECK_LAUNCH("mass");
