@@ -20,8 +20,9 @@
 // Measured: 16 x 128 rows, 40 heads, D = 128, 4097 keys (172 GFLOP) 198 us, 0.87
 // PFLOP/s: 640 equal work-groups on 768 places, products and exponentials
 // overlapping in part.  64 rows x 32 / 8 heads on 32768 keys (34 GFLOP, 134 MB
-// of K and V) 51 us + 11 us for the join: 48 splits, whose partials are 50 MB;
-// 32 splits 57 + 9, 16 splits 71 + 6.  4 x 8 rows a head on 1000 keys 12 us, one
+// of K and V) 55 us + 6 us for the join: 16 splits of three sets of waves, whose
+// partials are 17 MB; without the sets 48 splits and 50 MB 53 + 11, 32 splits 57 +
+// 9, 16 splits 71 + 6.  4 x 8 rows a head on 1000 keys 12 us, one
 // launch.
 #include <algorithm>
 #include <cmath>
@@ -109,17 +110,17 @@ struct PrefixOwn {
   }
 };
 
-// WQ waves share the keys of a tile, each with 32 rows of its own; with WQ = 1
-// the four waves have the same 32 rows and a quarter of the tile's 128 keys
-// each, joined in LDS at the end: few rows then still use every wave.
-template <typename ET, int D, int WQ>
-__global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(PrefixArgs a) {
+// WQ waves have 32 rows each, WK sets of them 32 keys of the tile each, joined
+// in LDS at the end: with WQ = 1, WK = 4 few rows still use every wave, with WK =
+// 3 three sets write one partial.
+template <typename ET, int D, int WQ, int WK>
+__global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void prefix_attn_kernel(PrefixArgs a) {
   using V8 = typename ET::V8;
   using E = typename ET::E;
-  constexpr int WK = 4 / WQ, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
+  constexpr int NT = 64 * WQ * WK, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
   constexpr int KRS = 2 * D + 32, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
-  constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / 256;
-  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WK == 1 ? 2 : 1;
+  constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / NT;
+  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WQ == 4 ? 2 : 1;
   __shared__ __align__(16) char lds[NBUF * BUF];
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int r0 = qblk * QB + QW * (WK == 1 ? w : 0), wk = WK == 1 ? 0 : w;  // first row, key quarter of the wave
+  const int wq = w % WQ, wk = w / WQ, r0 = qblk * QB + QW * wq;  // the wave's share of rows and keys, its first row
   const int tiles = (a.P + KT - 1) / KT;
   const int tile0 = part_start(tiles, sp, a.by_nsplit), tile1 = part_start(tiles, sp + 1, a.by_nsplit);
   const int j0 = tile0 * KT, keys = min(tile1 * KT, a.P) - j0;  // the split's keys (at least one)
@@ -156,11 +157,11 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   }
 
   uint32_t stg[NCH][4];
-  const int srow = threadIdx.x / CHR, scol = threadIdx.x % CHR * 16;  // (chunk k: row srow + 256 / CHR k of K, then V)
+  const int srow = threadIdx.x / CHR, scol = threadIdx.x % CHR * 16;  // (chunk k: row srow + NT / CHR k of K, then V)
   uint32_t off[NCH];
 #pragma unroll
   for (int k = 0; k < NCH; ++k)
-    off[k] = (uint32_t)((srow + 256 / CHR * (k % (NCH / 2))) * (k < NCH / 2 ? a.k_st : a.v_st) + scol);
+    off[k] = (uint32_t)((srow + NT / CHR * (k % (NCH / 2))) * (k < NCH / 2 ? a.k_st : a.v_st) + scol);
   // A tile is a buffer resource of its rows, a thread's offsets in it stay the same; rows past the split read zeros.
   auto load_tile = [&](int j) {
     const int last = min(KT, keys - j * KT) - 1;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   auto store_tile = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int row = srow + 256 / CHR * (k % (NCH / 2));
+      const int row = srow + NT / CHR * (k % (NCH / 2));
       char* dst = lds + buf * BUF + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + scol;
       *reinterpret_cast<uint4*>(dst) = make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
     }
@@ -288,20 +289,22 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
   for (int qb = 0; qb < NQ; ++qb) lt[qb] = col_sum(l_run[qb]);
   if constexpr (WK > 1) {
     // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum,
-    // 16 rows at a time in the tile's LDS, added in wave order; wave w keeps the dims of tiles w DT/4 ..
-    __shared__ float s_ml[WK][QW][2];
-    float* so = reinterpret_cast<float*>(lds);  // [WK][DT][64 lanes][4]
+    // 16 rows at a time in the tiles' LDS, added in wave order; a wave keeps the dims of tiles wk, wk + WK ..
+    __shared__ float s_ml[WK][QB][2];
+    float* so = reinterpret_cast<float*>(lds);  // [waves][DT][64 lanes][4]
+    static_assert(WQ * WK * DT * 1024 <= NBUF * BUF, "the waves' O fits the tiles' LDS");
+    const int rr = QW * wq + c16;
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb)
-      if (g == 0) { s_ml[w][16 * qb + c16][0] = m_run[qb]; s_ml[w][16 * qb + c16][1] = lt[qb]; }
+      if (g == 0) { s_ml[wk][16 * qb + rr][0] = m_run[qb]; s_ml[wk][16 * qb + rr][1] = lt[qb]; }
     __syncthreads();
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
       float m = kLowest, l = 0.f;
 #pragma unroll
-      for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + c16][0]);
+      for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + rr][0]);
 #pragma unroll
-      for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + c16][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + c16][0] - m);
+      for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + rr][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + rr][0] - m);
       const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((w * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
@@ -309,35 +312,37 @@ __global__ __launch_bounds__(256, WQ == 4 ? 3 : 2) void prefix_attn_kernel(Prefi
       lt[qb] = l;
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < DT / 4; ++u) {
-        const int dt = w * (DT / 4) + u;
-        float4_t v = *reinterpret_cast<const float4_t*>(so + (dt * 64 + lane) * 4);
+      for (int u = 0; u < (DT + WK - 1) / WK; ++u) {
+        const int dt = wk + WK * u;
+        if (dt >= DT) break;
+        float4_t v = *reinterpret_cast<const float4_t*>(so + ((wq * DT + dt) * 64 + lane) * 4);
 #pragma unroll
-        for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + ((i * DT + dt) * 64 + lane) * 4);
+        for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + (((i * WQ + wq) * DT + dt) * 64 + lane) * 4);
         o[qb][u] = v;
       }
       __syncthreads();
     }
   }
   // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
-  constexpr int OT = WK == 1 ? DT : DT / 4;
-  const int dt0 = WK == 1 ? 0 : w * OT;
+  constexpr int OT = (DT + WK - 1) / WK;
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) {
     const int r = r0 + 16 * qb + c16;
     if (r >= a.M) continue;
-    const bool first = g == 0 && (WK == 1 || w == 0);
+    const bool first = g == 0 && wk == 0;
     if (a.nsplit == 1) {
       const PrefixRow x = prefix_row(a, hk, r);
       const PrefixOwn<ET> own(a, x, m_run[qb]);
 #pragma unroll
-      for (int u = 0; u < OT; ++u) own.write(a, x, 16 * (dt0 + u) + 4 * g, o[qb][u], lt[qb]);
+      for (int u = 0; u < OT; ++u)
+        if (wk + WK * u < DT) own.write(a, x, 16 * (wk + WK * u) + 4 * g, o[qb][u], lt[qb]);
       if (a.lse && first) own.write_lse(a, x, lt[qb]);
     } else {
       const long pr = (long)sp * a.rows + (long)hk * a.M + r;
       float* dst = a.po + pr * D + 4 * g;
 #pragma unroll
-      for (int u = 0; u < OT; ++u) *reinterpret_cast<float4_t*>(dst + 16 * (dt0 + u)) = o[qb][u];
+      for (int u = 0; u < OT; ++u)
+        if (wk + WK * u < DT) *reinterpret_cast<float4_t*>(dst + 16 * (wk + WK * u)) = o[qb][u];
       if (first) {
         a.pml[2 * pr] = m_run[qb];
         a.pml[2 * pr + 1] = lt[qb];
@@ -401,22 +406,37 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
 
 namespace {
 // How a call is cut.  At most 32 rows a kv head: the four waves of a work-group
-// split a tile's keys (wq = 1); more: they split the rows.  Key splits until
-// 768 work-groups (3 a CU) are there, each of at least 4 tiles; up to 8 tiles
-// one split, whose launch writes the results (4 x 8 rows on 1000 keys: two
-// splits and their join 8 + 4 us).
+// split a tile's keys (wq = 1, wk = 4); more: they split the rows (wq = 4, wk =
+// 1).  Key splits until 768 work-groups (3 a CU) are there, each of at least 4
+// tiles; up to 8 tiles one split, whose launch writes the results (4 x 8 rows on
+// 1000 keys: two splits and their join 8 + 4 us).
+//
+// Many splits of a long prefix: work-groups of 12 waves, a CU each, whose three
+// sets of waves share the rows and are joined in LDS (wk = 3): a third of the
+// partials.  us a call, one set / three: 64 rows x 32 / 8 heads, D = 128, on 32768
+// keys (48 splits) 72.5 / 67, 8192 35 / 30, 4096 27 / 26.5, 2048 (16 splits) 21.3 /
+// 22.5; 16 rows on 32768 40 / 36, on 4096 17 / 18; D = 64, 32 / 4 heads, 64 rows on
+// 4096 21.7 / 18.3, on 1500 13.4 / 14.8, 16 rows on 32768 38 / 26.
 struct PrefixPlan {
-  int wq, nqb, nsplit;
+  int wq, wk, nqb, nsplit;
 };
 PrefixPlan prefix_plan(const carekv_prefix_params& p) {
   PrefixPlan r{};
   const long M = (long)p.batch * p.seq_len * (p.n_heads / p.n_kv_heads);
   r.wq = M <= 32 ? 1 : 4;
+  r.wk = M <= 32 ? 4 : 1;
   r.nqb = (int)((M + 32 * r.wq - 1) / (32 * r.wq));
-  const long kt = 128 / r.wq, wgs = (long)r.nqb * p.n_kv_heads, tiles = (p.prefix_len + kt - 1) / kt;
-  if (tiles == 0 || wgs == 0) return r;
-  const long s = tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
-  r.nsplit = (int)std::min(s, tiles);
+  const long wgs = (long)r.nqb * p.n_kv_heads;
+  auto tiles = [&]() { return ((long)p.prefix_len + 32 * r.wk - 1) / (32 * r.wk); };
+  if (tiles() == 0 || wgs == 0) return r;
+  auto splits = [&](long places, long least) {
+    return (int)(tiles() <= 8 ? 1 : std::min(tiles(), std::max(1L, std::min(places / wgs, (tiles() + least - 1) / least))));
+  };
+  r.nsplit = splits(768, 4);
+  if (r.wq == 4 && r.nsplit >= 12 && tiles() >= 128) {
+    r.wk = 3;
+    r.nsplit = splits(256, 3);
+  }
   return r;
 }
 int check_prefix(const carekv_prefix_params* pp) {
@@ -490,14 +510,15 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   a.al8 = (rows8 & 7) == 0;
   hipStream_t s = (hipStream_t)stream;
   const long wgs = (long)a.nqb * a.Hkv * ns;
-  CAREKV_REQUIRE(grid_fits(wgs, 256) && (ns == 1 || grid_fits(rows / (256 / p.head_dim) + 1, 256)), "too many rows");
+  CAREKV_REQUIRE(grid_fits(wgs, 768) && (ns == 1 || grid_fits(rows / (256 / p.head_dim) + 1, 256)), "too many rows");
   return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
     using ET = decltype(et);
     constexpr int D = decltype(d)::value;
     if (ns > 0) {
-      const dim3 grid((unsigned)wgs), block(256);
-      if (plan.wq == 4) hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 4>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 1>), grid, block, 0, s, a);
+      const dim3 grid((unsigned)wgs), block(64 * plan.wq * plan.wk);
+      if (plan.wq == 1) hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 1, 4>), grid, block, 0, s, a);
+      else if (plan.wk == 1) hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 4, 1>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((prefix_attn_kernel<ET, D, 4, 3>), grid, block, 0, s, a);
       CAREKV_CHECK_LAUNCH("prefix_attn");
     }
     if (ns != 1) {

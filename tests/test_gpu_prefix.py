@@ -244,3 +244,18 @@ def test_decode_behind_a_prefix(correction, monkeypatch):
     assert torch.equal(with_diag[0], got[0]) and with_diag[1].shape == (3, 8, 8)
     with pytest.raises(ValueError):
         care_kv.decode_attention(cache, 0, q, prefix=(k, v), no_alloc=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,T,P", [(40, 4, 2, 64, 1, 5000), (9, 8, 1, 64, 5, 12345), (33, 1, 1, 128, 1, 4096),
+                                            (1, 6, 2, 128, 50, 4111), (2, 3, 3, 64, 40, 33000)])
+def test_long_prefixes_of_many_rows(dtype, B, Hq, Hkv, D, T, P):
+    """Prefixes long enough that the waves of a work-group share the rows as well as the keys."""
+    import care_kv
+    print(f"prefix {dtype} B={B} {Hq}/{Hkv} D={D} T={T} P={P}", flush=True)
+    q, k, v, own = _inputs(P, B, Hq, Hkv, D, T, P, dtype)
+    own[1][0] = -torch.inf
+    got = care_kv.prefix_attention(q, k, v, own=own, return_lse=True)
+    _check(got, _ref(q, k, v, own))
+    for a, b in zip(got, care_kv.prefix_attention(q, k, v, own=own, return_lse=True)):
+        assert torch.equal(a, b)
