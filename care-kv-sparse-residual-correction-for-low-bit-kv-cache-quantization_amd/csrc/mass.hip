@@ -23,6 +23,14 @@
 //
 // mass_few_kernel, at most 16 rows a kv head (a decode step): a work-group a
 // (sequence, kv head), the scores of all keys in LDS, K read once, one launch.
+// Past kFewBytes of K a head the keys are cut into parts (mass_scores_kernel: K
+// read once, the scores to memory; mass_weigh_kernel: their weights), up to 2048
+// work-groups.  us a call in a graph, one launch / two: 8 heads, D = 128, 4 rows
+// on 512 keys (128 KB) 8.3 / 7.8, 1024 11.5 / 8.0, 2048 18.9 / 8.4, 4096 33.7 / 8.4;
+// 128 heads, D = 64, 8 rows on 2303 keys (288 KB) 14.9 / 16.4, 4000 22.0 / 21.2;
+// a launch more costs an eager call 3 us of host time.  Decode steps on 8 x 8192
+// keys, 32 / 8 heads (134 MB) 27 us, on 16 x 6000, 32 / 32 heads (786 MB) 160, 4.9
+// TB/s (as walks 64 and 374).
 //
 // Measured, D = 128, 8192 causal rows with lse: 32 / 8 heads 321 us + 5 for the
 // sum of the parts (275 GFLOP of visible products, 1.07e9 exponentials: 0.84
@@ -69,7 +77,7 @@ struct MassArgs {
   float sm_log2;
 };
 
-constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072, kFoldRows = 256;
+constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072, kFewBytes = 320 << 10, kFoldRows = 256;
 
 // A sequence's visible keys: row t sees j < min(len, qs + t + 1), not causal: j < len.
 struct MassSeq {
@@ -586,6 +594,106 @@ __global__ __launch_bounds__(1024) void mass_few_kernel(MassArgs a, int stride) 
   }
 }
 
+// At most 16 rows a kv head on more keys than a work-group should read alone: the keys are cut into parts, a
+// work-group (4 waves of 64 keys in turn) each.  Its base-2 logits go to `sc` [B Hkv][rows][stride] (masked: -inf),
+// every row's (reference, sum) to part [B Hkv][rows][nsk].
+template <typename ET, int D>
+__global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a, float* sc, int stride) {
+  using V8 = typename ET::V8;
+  constexpr int KS = D / 32, TT = 4, KT = 16 * TT;
+  __shared__ float s_m[4][16], s_l[4][16];
+  const int hb = (int)blockIdx.x / a.by_nsk, sp = blockIdx.x - hb * a.nsk;
+  const int b = hb / a.by_hkv, hk = hb - b * a.Hkv, rows = a.G * a.Tq;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int r = min(c16, rows - 1), h = r / a.by_tq, t = r - h * a.Tq;
+  const int all = (a.Tk + KT - 1) / KT, j0 = part_start(all, sp, a.by_nsk), j1 = part_start(all, sp + 1, a.by_nsk);
+  V8 qf[KS];
+  const char* qp = a.q + b * a.q_sb + ((long)hk * a.G + h) * a.q_sh + (long)t * a.q_st;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = load8<V8>(qp + (32 * s + 8 * g) * 2);
+  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
+  V8 kf[TT][KS];
+  auto load_keys = [&](int j) {  // (keys behind the sequence are masked, whatever they hold)
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      const char* kp = kbase + (long)min(KT * j + 16 * tt + c16, a.Tk - 1) * a.k_st;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[tt][s] = load8<V8>(kp + (32 * s + 8 * g) * 2);
+    }
+  };
+  load_keys(j0 + w);  // on their way before the length is known
+  const MassSeq sq = mass_seq(a, b);
+  const int lim = c16 < rows ? mass_limit(a, sq, t) : 0;
+  const int end = min(j1, (sq.len + KT - 1) / KT);  // turns with keys
+  float* dst = sc + ((long)hb * rows + c16) * stride;
+  float m = kLowest, l = 0.f;
+  for (int j = j0 + w; j < end; j += 4) {
+    float4_t s[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) s[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) s[tt] = ET::mfma(kf[tt][ks], qf[ks], s[tt]);
+    if (j + 4 < end) load_keys(j + 4);
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 4 * TT; ++i) {
+      const float x = s[i / 4][i % 4] * a.sm_log2;
+      s[i / 4][i % 4] = KT * j + 16 * (i / 4) + 4 * g + i % 4 < lim ? x : -INFINITY;
+      mx = fmaxf(mx, s[i / 4][i % 4]);
+    }
+    l *= __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+#pragma unroll
+    for (int i = 0; i < 4 * TT; ++i) l += __builtin_amdgcn_exp2f(s[i / 4][i % 4] - m);
+    if (c16 < rows) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<float4_t*>(dst + KT * j + 16 * tt + 4 * g) = s[tt];
+    }
+  }
+  const float mw = col_max(m), lw = col_sum(l * __builtin_amdgcn_exp2f(m - mw));
+  if (g == 0) { s_m[w][c16] = mw; s_l[w][c16] = lw; }
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    float mx = kLowest, ls = 0.f;
+    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s_m[i][threadIdx.x]);
+    for (int i = 0; i < 4; ++i) ls += s_l[i][threadIdx.x] * __builtin_amdgcn_exp2f(s_m[i][threadIdx.x] - mx);
+    float* p = a.part + 2 * (((long)hb * rows + threadIdx.x) * a.nsk + sp);
+    p[0] = mx;
+    p[1] = ls;
+  }
+}
+
+// The weights of those logits: a work-group 1024 keys, a thread four of them.
+__global__ __launch_bounds__(256) void mass_weigh_kernel(MassArgs a, const float* sc, int stride) {
+  __shared__ float2 s_st[kFewRows];
+  const int hb = (int)blockIdx.x / a.by_kpairs, key = (blockIdx.x - hb * a.by_kpairs.d) * 1024 + 4 * (int)threadIdx.x;
+  const int b = hb / a.by_hkv, rows = a.G * a.Tq, r = threadIdx.x / 16;
+  if (r < rows) {  // (16 lanes a row; a wave's rows that are not there leave it whole groups)
+    const float2 st = a.lse ? lse_stat(a.lse[(long)hb * rows + r])
+                            : join_parts<16>(reinterpret_cast<const float2*>(a.part) + ((long)hb * rows + r) * a.nsk, a.nsk,
+                                             threadIdx.x & 15);
+    if (threadIdx.x % 16 == 0) s_st[r] = st;
+  }
+  __syncthreads();
+  const MassSeq sq = mass_seq(a, b);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (key < sq.len)
+    for (int i = 0; i < rows; ++i) {
+      const float4_t x = *reinterpret_cast<const float4_t*>(sc + ((long)hb * rows + i) * stride + key);
+      const float2 st = s_st[i];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (x[u] != -INFINITY) v[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - st.x), st.y, v[u]);  // (masked: -inf; NaN goes on)
+    }
+  float* dst = a.out + b * a.o_sb + (hb - b * a.Hkv) * a.o_sh + key;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (key + u < a.Tk) dst[u] = a.accumulate ? dst[u] + v[u] : v[u];
+}
+
 namespace {
 int check_mass(const carekv_mass_params* pp) {
   CAREKV_REQUIRE(pp, "null argument");
@@ -620,7 +728,7 @@ struct MassPlan {
   bool few;
   int few_stride;
   int nkb, parts, nqb, nsk;
-  bool fold;
+  bool fold, split;  // split: few rows on many keys, nsk parts
 };
 int walk_parts(long pairs, long tiles, double sum, double each) {
   long best = 1;
@@ -637,11 +745,17 @@ MassPlan mass_plan(const carekv_mass_params& p) {
   MassPlan m{};
   const long G = p.n_heads / p.n_kv_heads, rows = G * p.n_queries, hb = (long)p.batch * p.n_kv_heads;
   m.few_stride = (p.n_keys + 63) / 64 * 64 + 4;
-  m.few = rows <= kFewRows && rows * m.few_stride * 4 <= kFewLds && (long)p.n_keys * p.head_dim * 2 <= (1 << 20);
+  m.few = rows <= kFewRows && rows * m.few_stride * 4 <= kFewLds && (long)p.n_keys * p.head_dim * 2 <= kFewBytes;
   m.nkb = (p.n_keys + kMassKeys - 1) / kMassKeys;
   m.nqb = (int)((rows + 255) / 256);
   m.parts = m.nsk = 1;
   if (m.few) return m;
+  m.split = hb > 0 && rows > 0 && rows <= kFewRows;
+  if (m.split) {
+    m.few_stride = (p.n_keys + 63) / 64 * 64;
+    m.nsk = (int)std::max(1L, std::min({64L, 2048 / hb, ((long)p.n_keys + 255) / 256}));
+    return m;
+  }
   const long seg = p.n_queries >= 32 ? p.n_queries : rows, nseg = p.n_queries >= 32 ? G : 1;
   const long tiles = (seg + kMassTile - 1) / kMassTile * nseg, ktiles = ((long)p.n_keys + kMassTile - 1) / kMassTile;
   // (a pair of causal walks over as many rows as keys has about the tiles of one whole walk)
@@ -658,6 +772,7 @@ long mass_ws(const carekv_mass_params& p, bool have_lse) {
   const MassPlan m = mass_plan(p);
   if (m.few) return 0;
   const long rows = (long)p.batch * p.n_heads * p.n_queries;
+  if (m.split) return rows * 4 * (m.few_stride + 2L * m.nsk);
   return (have_lse ? 0 : rows * 8 * (1 + m.nsk)) + (m.parts > 1 ? (long)m.parts * p.batch * p.n_kv_heads * p.n_keys * 4 : 0);
 }
 }  // namespace
@@ -707,6 +822,11 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   a.stat = (float*)workspace;
   a.part = a.stat + (lse ? 0 : 2 * rows);
   a.opart = a.part + (lse ? 0 : 2 * rows * m.nsk);
+  if (m.split) {  // the logits, then the parts' statistics
+    a.opart = (float*)workspace;
+    a.part = a.opart + rows * m.few_stride;
+    a.by_kpairs = FastDiv((p.n_keys + 1023) / 1024);
+  }
   hipStream_t s = (hipStream_t)stream;
   const long wgs = hb * ((m.nkb + 1) / 2) * m.parts, swgs = hb * ((m.nqb + 1) / 2) * m.nsk, sum = (hb * p.n_keys + 255) / 256;
   CAREKV_REQUIRE(grid_fits(wgs, 512) && grid_fits(swgs, 512) && grid_fits(sum, 256) &&
@@ -718,6 +838,13 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
     if (m.few && rows > 0) {
       hipLaunchKernelGGL((mass_few_kernel<ET, D>), dim3((unsigned)hb), dim3(1024), 0, s, a, m.few_stride);
       CAREKV_CHECK_LAUNCH("mass_few");
+      return CAREKV_OK;
+    }
+    if (m.split) {
+      hipLaunchKernelGGL((mass_scores_kernel<ET, D>), dim3((unsigned)(hb * m.nsk)), dim3(256), 0, s, a, a.opart, m.few_stride);
+      CAREKV_CHECK_LAUNCH("mass_scores");
+      hipLaunchKernelGGL(mass_weigh_kernel, dim3((unsigned)(hb * a.by_kpairs.d)), dim3(256), 0, s, a, a.opart, m.few_stride);
+      CAREKV_CHECK_LAUNCH("mass_weigh");
       return CAREKV_OK;
     }
     if (!lse && rows > 0) {

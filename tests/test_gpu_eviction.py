@@ -286,3 +286,35 @@ def test_offsets_past_32_bits():
     _check_mass(mass[None], ref, rel, 1)
     got = care_kv.evict_rows(mass, k, k, keep=4)
     assert torch.equal(got.index[0].long(), hot) and torch.equal(got.k[0], k[0, hot])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,Tq,Tk", [(3, 8, 2, 128, 1, 5003), (2, 16, 1, 64, 1, 2500), (2, 3, 3, 128, 5, 4500),
+                                              (1, 2, 1, 64, 8, 20000), (70, 8, 8, 64, 1, 8200)])
+def test_mass_of_few_rows_on_many_keys(dtype, B, Hq, Hkv, D, Tq, Tk):
+    """Decode steps and short windows on long contexts: ragged lengths with NaN behind them, starts of every kind,
+    given log-sum-exps, sums added to; the same bits twice."""
+    import care_kv
+    print(f"mass {dtype} B={B} {Hq}/{Hkv} D={D} Tq={Tq} Tk={Tk}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(Tk)
+    q = torch.randn(B, Hq, Tq, D, generator=g, device="cuda").to(dtype)
+    k = torch.randn(B, Hkv, Tk, D, generator=g, device="cuda").to(dtype)
+    lengths = ([Tk, 0, 1, Tk - 1, 1025, 64, 65] * 10)[:B]
+    starts = [n - Tq if i % 3 < 2 else n // 2 for i, n in enumerate(lengths)]
+    for b, n in enumerate(lengths):
+        k[b, :, n:] = float("nan")
+    ln, st = torch.tensor(lengths, device="cuda"), torch.tensor(starts, device="cuda")
+    ref, lse, rel = _mass_ref(q, k, lengths=lengths, q_start=starts)
+    n = Hq // Hkv * Tq
+    got = care_kv.attention_mass(q, k, lengths=ln, q_start=st)
+    _check_mass(got, ref, rel, n)
+    assert torch.equal(got, care_kv.attention_mass(q, k, lengths=ln, q_start=st))
+    for b, m in enumerate(lengths):
+        assert not got[b, :, m:].any()
+    out = torch.ones(B, Hkv, Tk + 3, device="cuda")[:, :, 1:Tk + 1]
+    care_kv.attention_mass(q, k, lengths=ln, q_start=st, out=out, accumulate=True)
+    assert torch.equal(out, got + 1.0)
+    with_lse, _, _ = _mass_ref(q, k, lengths=lengths, q_start=starts, lse=lse.float())
+    _check_mass(care_kv.attention_mass(q, k, lengths=ln, q_start=st, lse=lse.float()), with_lse, rel, n)
+    whole, _, rel = _mass_ref(q[:1], k[:1], causal=False)
+    _check_mass(care_kv.attention_mass(q[:1], k[:1], causal=False), whole, rel, n)
