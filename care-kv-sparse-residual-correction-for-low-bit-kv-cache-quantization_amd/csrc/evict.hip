@@ -7,9 +7,9 @@
 // three histograms of 11, 11 and 10 bits find the key of the last kept row and
 // how many of its equals are kept; a scan in index order places the kept rows.
 //
-// Up to 8192 rows: evict_select_kernel, one work-group a (sequence, kv head),
-// the keys in registers, everything in one launch, small results gathered there
-// too.  Longer: the rows are cut into parts of 8192 (at most 64 parts), a
+// Up to 16384 rows: evict_select_kernel, one work-group a (sequence, kv head),
+// the keys in registers (8 a thread, past 8192 rows 16), everything in one launch,
+// small results gathered there too.  Longer: the rows are cut into parts of 8192 (at most 64 parts), a
 // work-group each, and every histogram is a launch (evict_part_kernel): each
 // part writes its own, the next launch adds up its row's, so that nothing is
 // cleared and no sum depends on an order.  evict_gather_kernel copies the rows.
@@ -18,7 +18,9 @@
 // the select is a chain of latencies.  Measured: 16 rows of 131072 weights, 16384
 // kept (279 MB): select 35 us in four launches (one work-group a row 251), gather
 // 45 us, 6.0 TB/s; 64 rows of 8192, 2048 kept (137 MB): 12.8 + 22 us; 4 rows of
-// 512 10 us in one launch.
+// 512 10 us in one launch.  One launch or four and the gather, in a graph: 4 rows of
+// 12000, 1024 kept 17.7 / 27.8 us, 64 of 16384, 4096 kept 59 / 67, 512 of 9000, 1024
+// kept 145 / 198; with 32 keys a thread 4 rows of 24000 30.3, in four 28.8.
 #include <algorithm>
 
 #include "common.h"
@@ -50,7 +52,7 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 }
 
 constexpr int kSel = 1024;           // threads of a select work-group
-constexpr int kEpt = 8;              // keys a thread holds
+constexpr int kEpt = 8;              // keys a thread holds, or twice as many of rows in one launch
 constexpr int kChunk = kSel * kEpt;  // rows of a part's turn
 constexpr int kBins = 2048;
 constexpr int kMaxParts = 64;
@@ -150,22 +152,23 @@ __device__ __forceinline__ void find_bin_wave(const int* hist, int nb, int need,
 }
 
 // Row e of this thread in a turn that starts at c0: a wave's loads are consecutive rows.
+template <int EPT>
 __device__ __forceinline__ int turn_row(int c0, int e) {
-  return c0 + (int)(threadIdx.x >> 6) * 64 * kEpt + 64 * e + (int)(threadIdx.x & 63);
+  return c0 + (int)(threadIdx.x >> 6) * 64 * EPT + 64 * e + (int)(threadIdx.x & 63);
 }
 
 // Places of a turn's rows, given their keys, in index order: those kept for
 // certain or above thr, and the first `left` of its equals.  base: places taken
 // before the turn, eqb: equals seen before it.
-template <typename F>
-__device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* key, int c0, int end, uint32_t thr,
+template <int EPT, typename F>
+__device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t (&key)[EPT], int c0, int end, uint32_t thr,
                                            int left, int& base, int& eqb, SelectScratch& sc, F&& put) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  uint64_t sure[kEpt], eq[kEpt];
+  uint64_t sure[EPT], eq[EPT];
   int ts = 0, te = 0;
 #pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    const int i = turn_row(c0, e);
+  for (int e = 0; e < EPT; ++e) {
+    const int i = turn_row<EPT>(c0, e);
     const bool in = i < end, by = in && i >= q.lo && i < q.hi;
     sure[e] = __ballot((in && !by) || (by && q.need > 0 && key[e] > thr));
     eq[e] = __ballot(by && q.need > 0 && key[e] == thr);
@@ -185,10 +188,10 @@ __device__ __forceinline__ void place_rows(const EvictSeq& q, const uint32_t* ke
   const uint64_t below = (1ull << lane) - 1;
   const int eq_in = min(eqb, left);  // kept equals that base counts already
 #pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
+  for (int e = 0; e < EPT; ++e) {
     const int rank = e0 + __popcll(eq[e] & below), pos = s0 + __popcll(sure[e] & below) + min(rank, left) - eq_in;
     const bool is_eq = (eq[e] >> lane) & 1;
-    if (((sure[e] >> lane) & 1) || (is_eq && rank < left)) put(pos, turn_row(c0, e));
+    if (((sure[e] >> lane) & 1) || (is_eq && rank < left)) put(pos, turn_row<EPT>(c0, e));
     s0 += __popcll(sure[e]);
     e0 += __popcll(eq[e]);
   }
@@ -210,8 +213,8 @@ __device__ __forceinline__ void copy_row(const EvictArgs& a, int bh, long r, int
   if (c == 0) a.mo[r] = j >= 0 ? *reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh + j * 4L) : 0.f;
 }
 
-// V: bytes a thread moves at once, void: no gather here.
-template <typename V>
+// V: bytes a thread moves at once, void: no gather here.  EPT: keys a thread holds.
+template <typename V, int EPT>
 __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   constexpr bool FUSE = !std::is_void<V>::value;
   __shared__ __align__(16) int hist[3][kBins];
@@ -219,10 +222,10 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
   const int b = (int)blockIdx.x / a.by_h, h = blockIdx.x - b * a.H, tid = threadIdx.x;
   const float* m = reinterpret_cast<const float*>(a.mass + b * a.m_sb + h * a.m_sh);
   for (int i = tid; i < 3 * kBins; i += kSel) hist[0][i] = 0;
-  uint32_t key[kEpt];
+  uint32_t key[EPT];
 #pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    const int i = turn_row(0, e);
+  for (int e = 0; e < EPT; ++e) {
+    const int i = turn_row<EPT>(0, e);
     key[e] = i < a.T ? weight_key(m[i]) : 0u;
   }
   const EvictSeq q = evict_seq(a, b);
@@ -236,8 +239,8 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
     for (int pass = 0; pass < 3; ++pass) {
       const int nb = pass_bins(pass), sh = pass_shift(pass), up = pass == 0 ? 0 : pass_shift(pass - 1);
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        const int i = turn_row(0, e);
+      for (int e = 0; e < EPT; ++e) {
+        const int i = turn_row<EPT>(0, e);
         if (i >= q.lo && i < q.hi && (pass == 0 || (key[e] >> up) == (thr >> up)))
           atomicAdd(&hist[pass][(key[e] >> sh) & (nb - 1)], 1);
       }
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
   auto load_turn = [&](int c0) {
 #pragma unroll
     for (int e = 0; e < kEpt; ++e) {
-      const int i = turn_row(c0, e);
+      const int i = turn_row<kEpt>(c0, e);
       x[e] = i < t1 ? m[i] : 0.f;
     }
   };
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(kSel) void evict_part_kernel(EvictArgs a, int pass,
       if (c0 > i0) load_turn(c0);
 #pragma unroll
       for (int e = 0; e < kEpt; ++e) {
-        const int i = turn_row(c0, e);
+        const int i = turn_row<kEpt>(c0, e);
         const uint32_t key = weight_key(x[e]);
         if (i >= q.lo && i < min(i1, q.hi) && (pass == 0 || (key >> up) == (thr >> up)))
           atomicAdd(&sh_hist[(key >> sh) & (nb - 1)], 1);
@@ -377,7 +380,8 @@ __global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a, long n, 
 
 namespace {
 int evict_parts(const carekv_evict_params& p) {
-  return (int)std::min((long)kMaxParts, std::max(1L, ((long)p.n_keys + kChunk - 1) / kChunk));
+  if (p.n_keys <= 2 * kChunk) return 1;
+  return (int)std::min((long)kMaxParts, ((long)p.n_keys + kChunk - 1) / kChunk);
 }
 long evict_ws(const carekv_evict_params& p) {
   const long parts = evict_parts(p);
@@ -438,15 +442,18 @@ extern "C" int carekv_evict_rows(const carekv_evict_params* pp, const float* mas
   CAREKV_REQUIRE(grid_fits((n + 255) / 256, 256), "too many kept rows");
   hipStream_t s = (hipStream_t)stream;
   if (parts == 1) {
-    const dim3 grid((unsigned)bh), block(kSel);
-    if ((long)p.keep * p.row_bytes <= kFuseBytes) {
-      if (wide) hipLaunchKernelGGL(evict_select_kernel<uint4>, grid, block, 0, s, a);
-      else hipLaunchKernelGGL(evict_select_kernel<uint32_t>, grid, block, 0, s, a);
-      CAREKV_CHECK_LAUNCH("evict_select");
-      return CAREKV_OK;
-    }
-    hipLaunchKernelGGL(evict_select_kernel<void>, grid, block, 0, s, a);
+    const bool fuse = (long)p.keep * p.row_bytes <= kFuseBytes;
+    auto select = [&](auto ept) {
+      constexpr int EPT = decltype(ept)::value;
+      const dim3 grid((unsigned)bh), block(kSel);
+      if (!fuse) hipLaunchKernelGGL((evict_select_kernel<void, EPT>), grid, block, 0, s, a);
+      else if (wide) hipLaunchKernelGGL((evict_select_kernel<uint4, EPT>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((evict_select_kernel<uint32_t, EPT>), grid, block, 0, s, a);
+    };
+    if (p.n_keys <= kChunk) select(std::integral_constant<int, kEpt>{});
+    else select(std::integral_constant<int, 2 * kEpt>{});
     CAREKV_CHECK_LAUNCH("evict_select");
+    if (fuse) return CAREKV_OK;
   } else {
     int* hist = (int*)workspace;
     int* above = hist + bh * 3 * parts * kBins;

@@ -318,3 +318,18 @@ def test_mass_of_few_rows_on_many_keys(dtype, B, Hq, Hkv, D, Tq, Tk):
     _check_mass(care_kv.attention_mass(q, k, lengths=ln, q_start=st, lse=lse.float()), with_lse, rel, n)
     whole, _, rel = _mass_ref(q[:1], k[:1], causal=False)
     _check_mass(care_kv.attention_mass(q[:1], k[:1], causal=False), whole, rel, n)
+
+
+@pytest.mark.parametrize("T", [8192, 8193, 12001, 16384, 16385])
+@pytest.mark.parametrize("D,keep", [(64, 40), (64, 5000), (6, 300)])
+def test_evict_around_one_launch(T, D, keep):
+    """The sizes where the keys a thread holds and the launches change; ragged, with equal weights and NaN."""
+    import care_kv
+    print(f"evict T={T} D={D} keep={keep}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    mass = torch.randn(4, 3, T, generator=g, device="cuda").mul(4).round()
+    mass[:, :, 3::70] = float("nan")
+    k, v = (torch.randn(4, 3, T, D, generator=g, device="cuda").half() for _ in range(2))
+    for lengths in (None, [T, T - 1, 7, 8200]):
+        _check_evict(care_kv, mass, k, v, keep, 4, keep // 4, lengths)
+        _check_evict(care_kv, torch.zeros_like(mass), k, v, keep, 0, 0, lengths)
