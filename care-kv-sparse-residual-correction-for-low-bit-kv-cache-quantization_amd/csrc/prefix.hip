@@ -477,6 +477,7 @@ extern "C" int carekv_prefix_attn(const carekv_prefix_params* pp, const void* q,
   const long rows = (long)p.batch * p.seq_len * p.n_heads;
   if (rows == 0) return CAREKV_OK;
   CAREKV_REQUIRE(q && out && (workspace || prefix_plan(p).nsplit < 2) && (p.prefix_len == 0 || (k && v)) && !own == !own_lse, "null argument");
+  CAREKV_REQUIRE(!lse || lse != own_lse, "lse must not be own_lse");
   const uintptr_t bits = operand_bits(q, {{p.batch, 2 * p.q_sb}, {p.n_heads, 2 * p.q_sh}, {p.seq_len, 2 * p.q_st}}) |
                          operand_bits(k, {{p.n_kv_heads, 2 * p.k_sh}, {p.prefix_len, 2 * p.k_st}}) |
                          operand_bits(v, {{p.n_kv_heads, 2 * p.v_sh}, {p.prefix_len, 2 * p.v_st}}) |

@@ -637,8 +637,8 @@ int64_t carekv_evict_rows_workspace_bytes(const carekv_evict_params* params);
  * joined with the row's attention over tokens of its own (own, own_lse; NULL:
  * none) as one softmax: own like q, own_lse fp32 [batch][n_heads][seq_len]
  * contiguous, the natural log-sum-exp behind own (finite; -inf: no tokens, the
- * row of own is not used).  lse (optional, laid out like own_lse) receives the
- * joint log-sum-exp.  A row that sees nothing is 0 with lse -inf.  fp16 or
+ * row of own is not used).  lse (optional, laid out like own_lse, but not own_lse
+ * itself) receives the joint log-sum-exp.  A row that sees nothing is 0 with lse -inf.  fp16 or
  * bf16, strides in elements, rows of q, k and v 16-byte aligned; head_dim 64
  * or 128.  out may be own (the same pointer and strides). */
 typedef struct carekv_prefix_params {

@@ -268,3 +268,11 @@ def test_launches_that_do_not_fit_are_refused():
     assert lib.carekv_evict_rows(ev, p, p, p, None, p, p, p, p, p, p, 1 << 62, None) == -1
     pre = _lib.PrefixParams(batch=1 << 20, n_heads=64, n_kv_heads=8, seq_len=8, prefix_len=0, head_dim=128)
     assert lib.carekv_prefix_attn(pre, p, p, p, None, None, p, None, p, 1 << 62, None) == -1
+
+
+def test_prefix_refuses_its_own_lse_as_output():
+    lib, p = _lib.load(), 4096
+    pp = _lib.PrefixParams(batch=2, n_heads=4, n_kv_heads=2, seq_len=1, prefix_len=9, head_dim=64, q_sb=256, q_sh=64,
+                           k_sh=576, k_st=64, v_sh=576, v_st=64, out_sb=256, out_sh=64, own_sb=256, own_sh=64)
+    assert lib.carekv_prefix_attn(pp, p, p, p, p, p, p, p, p, 1 << 40, None) == -1
+    assert "own_lse" in lib.carekv_last_error().decode()
