@@ -95,7 +95,8 @@ __device__ __forceinline__ int mass_limit(const MassArgs& a, const MassSeq& s, i
 }
 
 // (M, w) of a row with log-sum-exp l: l log2(e) = M + rest, M the rounded
-// product, rest what it lost.  Infinite l: weights of 0.  NaN goes on as NaN.
+// product, rest what it lost.  Infinite l: (inf, 0), whose row is masked (0 times what it holds may be NaN).  NaN
+// goes on as NaN.
 __device__ __forceinline__ float2 lse_stat(float l) {
   float2 st = make_float2(INFINITY, 0.f);
   if (!(fabsf(l) >= 1e30f)) {
@@ -140,7 +141,8 @@ __device__ __forceinline__ float2 join_parts(const float2* p, int nsk, int u) {
   return l != 0.f ? make_float2(mx, 1.f / l) : make_float2(INFINITY, 0.f);
 }
 
-template <typename ET, int D>
+// GIVEN: with the rows' log-sum-exp.
+template <typename ET, int D, bool GIVEN>
 __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   using V8 = typename ET::V8;
   constexpr int TT = kMassKeys / 128, QT = kMassTile, KS = D / 32, QRS = 2 * D + 32, CHR = D / 8, NCH = QT * CHR / 512;
@@ -148,6 +150,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   static_assert(QT == 64, "a wave has a tile's rows");
   __shared__ float2 s_st[2][QT];
   __shared__ int s_lim[2][QT];
+  __shared__ int s_off[8];  // a wave's share of the rows has one of infinite lse
   __shared__ float2 s_row[kFoldRows];  // every row's (M, w), where the statistics' parts are joined here
   __shared__ float s_sum[4 * TT][512];  // the outer sums: the registers they would take spill others
   // Sequences and heads go round the XCDs, the blocks of one part run together: they meet in one L2.
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   const int b = hb / a.by_hkv, hk = hb - b * a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  if (a.fold) {  // (256 rows, two lanes each; before the length is known)
+  if (!GIVEN && a.fold) {  // (256 rows, two lanes each; before the length is known)
     const int r = threadIdx.x / 2, rows = a.G * a.Tq;
     const float2 st = join_parts<2>(reinterpret_cast<const float2*>(a.part) + ((long)hb * rows + min(r, rows - 1)) * a.nsk,
                                     a.nsk, threadIdx.x & 1);
@@ -166,6 +169,21 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
   const MassSeq sq = mass_seq(a, b);
   const long hrow = (long)hb * a.G * a.Tq;  // first row of this (sequence, kv head) in stat / lse
   const bool listed = a.nseg > 1 || a.G == 1;  // a list is a head's rows
+  // Rows of infinite lse are masked, whatever they hold: where there are any, every tile looks for them.  (Found here,
+  // 1 % of a prompt's walks; a flag of each tile's rows, read before its first branch, cost 4 %.)
+  bool off = false;
+  if (GIVEN && listed)
+    for (int r0 = threadIdx.x; r0 < a.G * a.Tq; r0 += 512 * 8) {
+      float l[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l[i] = a.lse[hrow + min(r0 + 512 * i, a.G * a.Tq - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) off |= fabsf(l[i]) >= 1e30f;
+    }
+  if (GIVEN) {
+    off = __any(off);
+    if (lane == 0) s_off[w] = off;
+  }
   // rows of a list below first_row see nothing of block kb
   auto first_row = [&](int kb) {
     if (kb * kMassKeys >= sq.len) return a.seg;
@@ -235,7 +253,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
       const long r = hrow + (long)h * a.Tq + t;
       n_st = make_float2(INFINITY, 0.f);
       if (i < t_end) {
-        if (a.lse) n_st.x = a.lse[r];
+        if (GIVEN) n_st.x = a.lse[r];
         else if (a.fold) n_st = s_row[h * a.Tq + t];
         else n_st = *reinterpret_cast<const float2*>(a.stat + 2 * r);
       }
@@ -253,7 +271,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     }
     if (w == sturn) {
       if (!listed) s_lim[buf][lane] = n_lim;
-      s_st[buf][lane] = a.lse ? lse_stat(n_st.x) : n_st;
+      s_st[buf][lane] = a.lse ? lse_stat(n_st.x) : n_st;  // (with GIVEN the form without lse spills four registers)
     }
     sturn = (sturn + 1) & 7;
   };
@@ -266,6 +284,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     store_tile(0);
   }
   __syncthreads();
+  const bool care = GIVEN && __any(s_off[lane & 7] != 0);
   int ni = i0;
   if (nt > 1) load_tile();
   for (int j = 0; j < nt; ++j) {
@@ -274,7 +293,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     if (!(listed && (j0 >= sq.len || (a.causal && sq.qs + min(ci + QT, t_end) - 1 < j0)))) {
     // some pair of the tile and the wave's keys is masked
     const bool edge = !listed || ci + QT > t_end || j0 + 16 * TT > sq.len ||
-                      (a.causal && sq.qs + ci + 1 < j0 + 16 * TT);
+                      (a.causal && sq.qs + ci + 1 < j0 + 16 * TT) || care;
     // the next 16 rows' products are issued before this one's exponentials: they run side by side
     float4_t s[2][TT];
     auto scores = [&](int qb, float4_t* x) {
@@ -303,7 +322,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
         if (qb + 1 < QT / 16) scores(qb + 1, s[(qb + 1) & 1]);
         const float2 st = s_st[buf][16 * qb + c16];
         const int i0c = ci + 16 * qb + c16;
-        const int see = !listed ? s_lim[buf][16 * qb + c16] : i0c < t_end ? mass_limit(a, sq, i0c) : 0;
+        const int see = GIVEN && st.y == 0.f ? 0 : !listed ? s_lim[buf][16 * qb + c16] : i0c < t_end ? mass_limit(a, sq, i0c) : 0;
         const int lim = see - j0 - 4 * g;  // token 16 tt + i of the lane is seen below it
 #pragma unroll
         for (int i = 0; i < 4 * TT; ++i) {
@@ -588,7 +607,8 @@ __global__ __launch_bounds__(1024) void mass_few_kernel(MassArgs a, int stride) 
       for (int i = 0; i < rows; ++i) {
         const float x = sc[i * stride + key];
         const float2 st = s_st[i];
-        if (x != -INFINITY) v = fmaf(__builtin_amdgcn_exp2f(x - st.x), st.y, v);  // (masked: -inf; NaN goes on)
+        // (masked: -inf; NaN goes on, but not from a row of infinite lse)
+        if (x != -INFINITY && st.y != 0.f) v = fmaf(__builtin_amdgcn_exp2f(x - st.x), st.y, v);
       }
     dst[key] = a.accumulate ? dst[key] + v : v;
   }
@@ -686,7 +706,8 @@ __global__ __launch_bounds__(256) void mass_weigh_kernel(MassArgs a, const float
       const float2 st = s_st[i];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (x[u] != -INFINITY) v[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - st.x), st.y, v[u]);  // (masked: -inf; NaN goes on)
+        // (masked: -inf; NaN goes on, but not from a row of infinite lse)
+        if (x[u] != -INFINITY && st.y != 0.f) v[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - st.x), st.y, v[u]);
     }
   float* dst = a.out + b * a.o_sb + (hb - b * a.Hkv) * a.o_sh + key;
 #pragma unroll
@@ -855,7 +876,8 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
         CAREKV_CHECK_LAUNCH("mass_join");
       }
     }
-    hipLaunchKernelGGL((mass_kernel<ET, D>), dim3((unsigned)wgs), dim3(512), 0, s, a);
+    if (lse) hipLaunchKernelGGL((mass_kernel<ET, D, true>), dim3((unsigned)wgs), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((mass_kernel<ET, D, false>), dim3((unsigned)wgs), dim3(512), 0, s, a);
     CAREKV_CHECK_LAUNCH("mass");
     if (a.parts > 1) {
       hipLaunchKernelGGL(mass_sum_kernel, dim3((unsigned)sum), dim3(256), 0, s, a);

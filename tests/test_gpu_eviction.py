@@ -333,3 +333,48 @@ def test_evict_around_one_launch(T, D, keep):
     for lengths in (None, [T, T - 1, 7, 8200]):
         _check_evict(care_kv, mass, k, v, keep, 4, keep // 4, lengths)
         _check_evict(care_kv, torch.zeros_like(mass), k, v, keep, 0, 0, lengths)
+
+
+# Each form of the weights' kernels: all scores in LDS, scores to memory, walks over a head's rows, over rows of several
+# heads, and 64-row windows whose statistics the walks join.
+FORMS = [(2, 4, 2, 64, 3, 300), (1, 8, 2, 128, 2, 5000), (2, 3, 3, 64, 200, 333), (2, 8, 2, 128, 64, 900),
+         (3, 12, 3, 64, 9, 700), (1, 2, 1, 128, 700, 700)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,Tq,Tk", FORMS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_mass_rows_of_infinite_lse_add_nothing(dtype, B, Hq, Hkv, D, Tq, Tk, causal):
+    """Whatever they hold: NaN, infinities, values whose logits are infinite."""
+    import care_kv
+    print(f"mass {dtype} B={B} {Hq}/{Hkv} D={D} Tq={Tq} Tk={Tk} causal={causal}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(Tq + Tk)
+    q = torch.randn(B, Hq, Tq, D, generator=g, device="cuda").to(dtype)
+    k = torch.randn(B, Hkv, Tk, D, generator=g, device="cuda").to(dtype)
+    off = torch.rand(B, Hq, Tq, generator=g, device="cuda") < 0.2
+    off[0, 0, Tq - 1] = True
+    q[off] = 0
+    _, lse, _ = _mass_ref(q, k, causal)
+    lse = lse.float()
+    lse[off] = -float("inf")
+    lse[off & (torch.rand(B, Hq, Tq, generator=g, device="cuda") < 0.3)] = float("inf")
+    ref, _, rel = _mass_ref(q, k, causal, lse=lse)
+    for bad in (float("nan"), float("inf"), torch.finfo(dtype).max):
+        q[off] = bad
+        got = care_kv.attention_mass(q, k, lse=lse, causal=causal)
+        _check_mass(got, ref, rel, Hq // Hkv * Tq)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,Tq,Tk", FORMS)
+def test_mass_infinite_logits_stay_with_the_keys_they_see(B, Hq, Hkv, D, Tq, Tk):
+    """A row without a given lse whose logits pass 32 bits: NaN at every key it sees, as the formula has it, and at no other."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(Tk)
+    q = torch.randn(B, Hq, Tq, D, generator=g, device="cuda").bfloat16()
+    k = torch.randn(B, Hkv, Tk, D, generator=g, device="cuda").abs().bfloat16()
+    row = Tq // 2
+    q[0, 0, row] = torch.finfo(torch.bfloat16).max
+    got = care_kv.attention_mass(q, k)
+    sees = Tk - Tq + row + 1
+    assert torch.isnan(got[0, 0, :sees]).all() and not torch.isnan(got[0, 0, sees:]).any()
+    assert not torch.isnan(got[0, 1:]).any() and not torch.isnan(got[1:]).any()
