@@ -93,7 +93,8 @@ class RotaryParams(C.Structure):
 class MassParams(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "n_queries", "n_keys", "head_dim", "dtype",
                                          "causal", "accumulate")] + [("sm_scale", C.c_float)] + \
-        [(n, C.c_int64) for n in ("q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "out_sb", "out_sh")]
+        [(n, C.c_int64) for n in ("q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "out_sb", "out_sh")] + \
+        [("q_lengths", C.c_void_p)]
 
 
 class EvictParams(C.Structure):

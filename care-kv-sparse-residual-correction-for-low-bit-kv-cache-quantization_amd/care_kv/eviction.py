@@ -25,25 +25,29 @@ class EvictedRows(NamedTuple):
 
 
 def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tensor] = None, causal: bool = True,
-                   sm_scale: Optional[float] = None, q_start=None, lengths=None, out: Optional[torch.Tensor] = None,
-                   accumulate: bool = False) -> torch.Tensor:
+                   sm_scale: Optional[float] = None, q_start=None, lengths=None, q_lengths=None,
+                   out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """The attention weight each key has gathered, fp32 (B, Hkv, Tk):
     mass[b, g, j] = sum over the query heads of kv head g and the query rows i
     that see key j of exp(sm_scale q_i . k_j - lse_i).
 
     q (B, Hq, Tq, D) and k (B, Hkv, Tk, D), fp16 or bf16, any strides; (Hq, Tq,
     D) and (Hkv, Tk, D) of one sequence work alike.  Query row i of sequence b
-    stands at position ``q_start[b] + i`` (default: the last Tq of the sequence)
-    and sees the keys below ``lengths[b]`` (default Tk) and, with ``causal``, up
-    to its own position: Tq = Tk is a prompt, a few last rows are a voting
-    window, Tq = 1 a decode step.  q_start and lengths: a device tensor of B
-    integers, one int for all, or (not in captured code) a host sequence.  lse (B, Hq, Tq) fp32: the
+    stands at position ``q_start[b] + i`` and sees the keys below ``lengths[b]``
+    (default Tk) and, with ``causal``, up to its own position: Tq = Tk is a
+    prompt, a few last rows are a voting window, Tq = 1 a decode step.  Rows from
+    ``q_lengths[b]`` on are padding and see nothing.  Default of q_lengths: Tq,
+    but where neither it nor q_start is given and Tq = Tk, the lengths (row i of
+    q and of k are one token of a right-padded prompt); of q_start: the rows are
+    the last of the sequence, lengths[b] - q_lengths[b] + i.  q_start, lengths
+    and q_lengths: a device tensor of B integers, one int for all, or (not in
+    captured code) a host sequence.  lse (B, Hq, Tq) fp32: the
     rows' log-sum-exp as ``prefill_attention(..., return_lse=True)`` gives it;
     without it an extra pass computes it.  ``accumulate`` adds to ``out``, whose
     values of a head must lie next to each other.
 
-    Rows that see nothing, or whose lse is infinite, add nothing; what masked
-    rows of q and k hold is never used (NaN included).  Sums run in a fixed
+    Rows that see nothing, or whose lse is infinite, add nothing; what they and
+    the keys behind a length hold is never used (NaN included).  Sums run in a fixed
     order.  The result carries no autograd history."""
     squeeze = q.dim() == 3
     if squeeze:
@@ -81,6 +85,9 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
         lib = _lib.load()
         qs = _lib.row_counts(q_start, B, dev, "q_start")
         ln = _lib.row_counts(lengths, B, dev, "lengths")
+        ql = ln if q_lengths is None and q_start is None and Tq == Tk else \
+            _lib.row_counts(q_lengths, B, dev, "q_lengths")
+        pp.q_lengths = None if ql is None else ql.data_ptr()
         nbytes = lib.carekv_attention_mass_workspace_bytes(pp, lse is not None)
         if nbytes < 0:
             _lib.check(-1, "carekv_attention_mass_workspace_bytes")

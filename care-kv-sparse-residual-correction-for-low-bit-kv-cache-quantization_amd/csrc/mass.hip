@@ -3,7 +3,8 @@
 //   i that see key j of e^(scale q_i . k_j - lse_i)
 // with lse_i the log-sum-exp of row i's visible scores, given or computed here.
 // Query row i stands at position q_start + i and sees the keys j below
-// min(length, position + 1) (not causal: below the length).
+// min(length, position + 1) (not causal: below the length); rows from q_length
+// on (the padding of a ragged batch) see nothing.
 //
 // mass_kernel, key-stationary: a work-group keeps 256 keys (8 waves of 32, the
 // A operand of S^T = K Q^T in registers) and walks over 64-row tiles of q
@@ -60,8 +61,9 @@ struct MassArgs {
   const char* q;
   const char* k;
   const float* lse;        // [B][Hq][Tq], or null
-  const int32_t* q_start;  // [B], or null: the last Tq of the length
+  const int32_t* q_start;  // [B], or null: the rows are the last of the length
   const int32_t* lengths;  // [B], or null
+  const int32_t* q_lengths;  // [B], or null
   float* out;
   float* part;             // [B][Hkv][rows][nsk][2] reference (base 2), sum
   float* stat;             // [B][Hkv][rows][2] M, w (no lse)
@@ -79,19 +81,20 @@ struct MassArgs {
 
 constexpr int kMassKeys = 256, kMassTile = 64, kFlush = 8, kFewRows = 16, kFewLds = 131072, kFewBytes = 320 << 10, kFoldRows = 256;
 
-// A sequence's visible keys: row t sees j < min(len, qs + t + 1), not causal: j < len.
+// A sequence's visible keys: row t < nq sees j < min(len, qs + t + 1), not causal: j < len.
 struct MassSeq {
-  int len;
+  int len, nq;
   long qs;
 };
 __device__ __forceinline__ MassSeq mass_seq(const MassArgs& a, int b) {
   MassSeq s;
   s.len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-  s.qs = a.q_start ? (long)a.q_start[b] : (long)s.len - a.Tq;
+  s.nq = a.q_lengths ? min(max(a.q_lengths[b], 0), a.Tq) : a.Tq;
+  s.qs = a.q_start ? (long)a.q_start[b] : (long)s.len - s.nq;
   return s;
 }
 __device__ __forceinline__ int mass_limit(const MassArgs& a, const MassSeq& s, int t) {
-  return a.causal ? (int)max(0L, min((long)s.len, s.qs + t + 1)) : s.len;
+  return t >= s.nq ? 0 : a.causal ? (int)max(0L, min((long)s.len, s.qs + t + 1)) : s.len;
 }
 
 // (M, w) of a row with log-sum-exp l: l log2(e) = M + rest, M the rounded
@@ -178,18 +181,20 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) l[i] = a.lse[hrow + min(r0 + 512 * i, a.G * a.Tq - 1)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) off |= fabsf(l[i]) >= 1e30f;
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(l[i]) >= 1e30f) off |= min(r0 + 512 * i, a.G * a.Tq - 1) % a.by_tq < sq.nq;
     }
   if (GIVEN) {
     off = __any(off);
     if (lane == 0) s_off[w] = off;
   }
-  // rows of a list below first_row see nothing of block kb
+  const int seg = listed ? sq.nq : a.seg;  // rows of a list
+  // those below first_row see nothing of block kb
   auto first_row = [&](int kb) {
-    if (kb * kMassKeys >= sq.len) return a.seg;
-    return a.causal && listed ? (int)min((long)a.seg, max(0L, (long)kb * kMassKeys - sq.qs)) : 0;
+    if (kb * kMassKeys >= sq.len) return seg;
+    return a.causal && listed ? (int)min((long)seg, max(0L, (long)kb * kMassKeys - sq.qs)) : 0;
   };
-  auto tiles_of = [&](int kb) { return (a.seg - first_row(kb) + QT - 1) / QT * a.nseg; };
+  auto tiles_of = [&](int kb) { return (seg - first_row(kb) + QT - 1) / QT * a.nseg; };
   // The pair's walks, one after the other, as one: this part's tiles of it.
   const int kb_b = a.nkb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (kb_b > pair ? tiles_of(kb_b) : 0);
   const int lo = part_start(n_all, pt, a.by_parts), hi = part_start(n_all, pt + 1, a.by_parts);
@@ -199,7 +204,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
 #pragma unroll 1
   for (int f = 0; f < (kb_b > pair ? 2 : 1); ++f) {
   const int kb = f ? kb_b : pair, j0 = kb * kMassKeys + 16 * TT * w;  // the block, the wave's first key
-  const int t_first = first_row(kb), t_end = a.seg, per = max(1, (t_end - t_first + QT - 1) / QT);
+  const int t_first = first_row(kb), t_end = seg, per = max(1, (t_end - t_first + QT - 1) / QT);
   const int at = max(lo - (f ? n_a : 0), 0), nt = min(hi, f ? n_all : n_a) - (f ? n_a : 0) - at;
   int sg = 0, i0 = at;  // the tile loaded next: list, first row
   while (i0 >= per) { i0 -= per; ++sg; }  // (at most nseg turns)
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     store_tile(0);
   }
   __syncthreads();
-  const bool care = GIVEN && __any(s_off[lane & 7] != 0);
+  const int care = GIVEN ? __builtin_amdgcn_readfirstlane(__any(s_off[lane & 7] != 0)) : 0;
   int ni = i0;
   if (nt > 1) load_tile();
   for (int j = 0; j < nt; ++j) {
@@ -293,7 +298,7 @@ __global__ __launch_bounds__(512, 4) void mass_kernel(MassArgs a) {
     if (!(listed && (j0 >= sq.len || (a.causal && sq.qs + min(ci + QT, t_end) - 1 < j0)))) {
     // some pair of the tile and the wave's keys is masked
     const bool edge = !listed || ci + QT > t_end || j0 + 16 * TT > sq.len ||
-                      (a.causal && sq.qs + ci + 1 < j0 + 16 * TT) || care;
+                      (a.causal && sq.qs + ci + 1 < j0 + 16 * TT) || care != 0;
     // the next 16 rows' products are issued before this one's exponentials: they run side by side
     float4_t s[2][TT];
     auto scores = [&](int qb, float4_t* x) {
@@ -382,11 +387,12 @@ __global__ __launch_bounds__(512, 4) void stats_kernel(MassArgs a) {
   for (int k = 0; k < NCH; ++k)
     off[k] = (uint32_t)((threadIdx.x / CHR + 512 / CHR * k) * a.k_st + (threadIdx.x % CHR) * 16);
   const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
-  // tiles of the keys that some row of block qb sees: its rows' furthest limit, a head's last row where it has one
+  // tiles of the keys that some row of block qb sees: its rows' furthest limit, a head's last row below nq where it
+  // has one
   auto tiles_of = [&](int qb) {
     const int ra = qb * 256, rz = min(ra + 256, rows) - 1;
-    const int hz = rz / a.by_tq, t = ra < hz * a.Tq ? a.Tq - 1 : rz - hz * a.Tq;
-    return (mass_limit(a, sq, t) + KT - 1) / KT;
+    const int hz = rz / a.by_tq, ta = ra - hz * a.Tq, t = min(ta < 0 ? a.Tq - 1 : rz - hz * a.Tq, sq.nq - 1);
+    return t < max(ta, 0) ? 0 : (mass_limit(a, sq, t) + KT - 1) / KT;
   };
   // The pair's walks, one after the other, as one: this part's tiles of it.
   const int qb_b = a.nqb - 1 - pair, n_a = tiles_of(pair), n_all = n_a + (qb_b > pair ? tiles_of(qb_b) : 0);
@@ -826,7 +832,8 @@ extern "C" int carekv_attention_mass(const carekv_mass_params* pp, const void* q
   }
   const MassPlan m = mass_plan(p);
   MassArgs a{};
-  a.q = (const char*)q; a.k = (const char*)k; a.lse = lse; a.q_start = q_start; a.lengths = lengths; a.out = out;
+  a.q = (const char*)q; a.k = (const char*)k; a.lse = lse; a.q_start = q_start; a.lengths = lengths; a.q_lengths = p.q_lengths;
+  a.out = out;
   a.q_sb = 2 * p.q_sb; a.q_sh = 2 * p.q_sh; a.q_st = p.n_queries > 1 ? 2 * p.q_st : 0; a.k_sb = 2 * p.k_sb; a.k_sh = 2 * p.k_sh;
   a.k_st = p.n_keys > 1 ? 2 * p.k_st : 0; a.o_sb = p.out_sb; a.o_sh = p.out_sh;
   a.B = p.batch; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.Tq = p.n_queries;

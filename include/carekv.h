@@ -592,12 +592,14 @@ int carekv_rotate_heads(const carekv_rotary_params* params, const void* q, const
  * [n_queries][head_dim], k [batch][n_kv_heads][n_keys][head_dim], fp16 or bf16,
  * strides in elements, rows 16-byte aligned; out fp32, a (sequence, kv head)'s
  * n_keys values next to each other.  Query row i of sequence b stands at
- * position q_start[b] + i (NULL: length - n_queries + i) and sees the keys
- * j < lengths[b] (NULL: n_keys), with causal only j <= its position.  lse: fp32
- * [batch][n_heads][n_queries] contiguous (carekv_prefill_attn's), or NULL:
- * computed here.  A row that sees nothing, or whose lse is infinite, adds
- * nothing; keys no row sees get 0; values of masked keys and rows are never
- * used.  accumulate != 0 adds to out.  head_dim 64 or 128.  The order of every
+ * position q_start[b] + i and sees the keys j < lengths[b] (NULL: n_keys), with
+ * causal only j <= its position.  Rows i >= q_lengths[b] (NULL: n_queries) are
+ * padding and see nothing: a right-padded prompt, n_queries = n_keys, gives its
+ * lengths as q_lengths too.  q_start NULL: the rows are the sequence's last,
+ * lengths[b] - q_lengths[b] + i.  lse: fp32 [batch][n_heads][n_queries]
+ * contiguous (carekv_prefill_attn's), or NULL: computed here.  A row that sees
+ * nothing, or whose lse is infinite, adds nothing; keys no row sees get 0; what
+ * such rows, and keys behind the length, hold is never used.  accumulate != 0 adds to out.  head_dim 64 or 128.  The order of every
  * sum is fixed. */
 typedef struct carekv_mass_params {
   int32_t batch, n_heads, n_kv_heads, n_queries, n_keys, head_dim;
@@ -605,6 +607,7 @@ typedef struct carekv_mass_params {
   int32_t causal, accumulate;
   float sm_scale;
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, out_sb, out_sh;
+  const int32_t* q_lengths; /* device [batch], or NULL                         */
 } carekv_mass_params;
 
 int carekv_attention_mass(const carekv_mass_params* params, const void* q, const void* k, const float* lse,

@@ -378,3 +378,58 @@ def test_mass_infinite_logits_stay_with_the_keys_they_see(B, Hq, Hkv, D, Tq, Tk)
     sees = Tk - Tq + row + 1
     assert torch.isnan(got[0, 0, :sees]).all() and not torch.isnan(got[0, 0, sees:]).any()
     assert not torch.isnan(got[0, 1:]).any() and not torch.isnan(got[1:]).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,Tq,Tk", [
+    (5, 4, 2, 64, 7, 7), (5, 2, 2, 64, 333, 333), (4, 8, 2, 128, 96, 96), (5, 12, 3, 64, 9, 9), (5, 8, 2, 128, 700, 700),
+    (5, 4, 2, 64, 3, 300), (4, 8, 2, 128, 4, 5000), (5, 4, 1, 64, 31, 900), (4, 8, 2, 128, 64, 2000), (5, 2, 2, 64, 100, 400)])
+@pytest.mark.parametrize("causal,given", [(True, False), (True, True), (False, False), (False, True)])
+def test_mass_right_padded_queries(dtype, B, Hq, Hkv, D, Tq, Tk, causal, given):
+    """Rows of q behind q_lengths do not vote, and nothing that padded rows of q, k and lse hold is used: each sequence
+    is what it is alone.  A prompt (Tq = Tk) takes its lengths for its queries' too."""
+    import care_kv
+    print(f"mass {dtype} B={B} {Hq}/{Hkv} D={D} Tq={Tq} Tk={Tk} causal={causal} lse={given}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(Tq * 3 + Tk)
+    q = torch.randn(B, Hq, Tq, D, generator=g, device="cuda").to(dtype)
+    k = torch.randn(B, Hkv, Tk, D, generator=g, device="cuda").to(dtype)
+    lengths = [Tk, Tk // 2 + 1, 0, Tk - 1, 1][:B]
+    qn = lengths if Tq == Tk else [min(n, m) for n, m in zip([Tq, Tq // 2 + 1, 0, 1, Tq], lengths)]
+    ref, lse, rel = torch.zeros(B, Hkv, Tk, dtype=torch.float64, device="cuda"), torch.full((B, Hq, Tq), float("nan")).cuda(), 0.0
+    for b, (n, m) in enumerate(zip(lengths, qn)):
+        if m:
+            x, y = q[b:b + 1, :, :m], k[b:b + 1, :, :n]
+            r, l, e = _mass_ref(x, y, causal)
+            if given:  # a given log-sum-exp is rounded to 32 bits
+                lse[b, :, :m] = l[0].float()
+                r, _, _ = _mass_ref(x, y, causal, lse=lse[b:b + 1, :, :m])
+            ref[b, :, :n], rel = r[0], max(rel, e)
+        q[b, :, m:] = float("nan")
+        q[b, :, m:, ::3] = float("inf")
+        k[b, :, n:] = float("nan")
+    for dev in (False, True):
+        ln, ql = (torch.tensor(x, device="cuda") for x in (lengths, qn)) if dev else (lengths, qn)
+        kw = dict(lse=lse if given else None, causal=causal, lengths=ln)
+        got = care_kv.attention_mass(q, k, q_lengths=ql, **kw)
+        _check_mass(got, ref, rel, Hq // Hkv * Tq)
+        for b, n in enumerate(lengths):
+            assert not got[b, :, n if qn[b] else 0:].any()
+        if Tq == Tk:
+            assert torch.equal(got, care_kv.attention_mass(q, k, **kw))
+        at = [n - m for n, m in zip(lengths, qn)]  # the default start, said
+        assert torch.equal(got, care_kv.attention_mass(q, k, q_lengths=ql, q_start=at, **kw))
+
+
+def test_mass_query_lengths_of_every_kind():
+    """Below zero, past the rows, one int for all, with starts of their own."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(3, 4, 40, 64, generator=g, device="cuda").half()
+    k = torch.randn(3, 2, 300, 64, generator=g, device="cuda").half()
+    got = care_kv.attention_mass(q, k, q_lengths=[-5, 99, 40])
+    want = care_kv.attention_mass(q, k)
+    assert not got[0].any() and torch.equal(got[1:], want[1:])
+    got = care_kv.attention_mass(q, k, q_lengths=17, q_start=[3, 283, -2])
+    ref, _, rel = _mass_ref(q[:, :, :17], k, q_start=[3, 283, -2])
+    _check_mass(got, ref, rel, 2 * 17)
+    assert torch.equal(care_kv.attention_mass(q[0], k[0], q_lengths=17, q_start=3), got[0])
