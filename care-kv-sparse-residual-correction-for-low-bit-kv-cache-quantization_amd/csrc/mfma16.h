@@ -8,14 +8,18 @@ namespace carekv {
 
 typedef __bf16 bhalf8_t __attribute__((ext_vector_type(8)));
 
+// kUp: a weight of 2^kUp at most is held where the largest is the row's, so that small ones stay normal (fp16: those
+// down to 2^-29 of it).
 struct ElemF16 {
   using E = _Float16;
   using V8 = half8_t;
+  static constexpr float kUp = 15.f;
   static __device__ __forceinline__ float4_t mfma(V8 a, V8 b, float4_t c) { return mfma16x32(a, b, c); }
 };
 struct ElemBF16 {
   using E = __bf16;
   using V8 = bhalf8_t;
+  static constexpr float kUp = 0.f;
   static __device__ __forceinline__ float4_t mfma(V8 a, V8 b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }

@@ -10,8 +10,13 @@
 // buffered, one barrier a tile), S^T = K Q^T and O^T += V^T P^T on
 // v_mfma_f32_16x16x32, the softmax over a query's column in 32 bits on base-2
 // logits; the weights are rounded to the element type for the second product
-// and their sum is not.  The keys are split over work-groups until the GPU is
-// full; prefix_join_kernel then joins the splits' (maximum, sum, O), kept in
+// and their sum is not: each is off by half a step at most (2^-11 or 2^-8 of
+// it).  A row's reference is its maximum less 15 in fp16, so that weights are
+// up to 2^15: with the maximum itself those below 2^-14 would be subnormal and
+// those below 2^-25 zero, and a long tail under one key would be lost from the
+// result but not from the sum.  What is subnormal now is off by 2^-40 of the
+// largest.  The keys are split over work-groups until the GPU is
+// full; prefix_join_kernel then joins the splits' (reference, sum, O), kept in
 // 32 bits, and the row's own part.  One split joins its own part itself.
 //
 // K and V rows are padded by 32 bytes in LDS: 16-byte reads of 16 rows then take
@@ -41,7 +46,7 @@ struct PrefixArgs {
   const float* own_lse;  // [B][Hq][T]
   char* out;
   float* lse;            // [B][Hq][T], or null
-  float* pml;            // [nsplit][rows][2] maximum (base 2), sum
+  float* pml;            // [nsplit][rows][2] reference (base 2), sum
   float* po;             // [nsplit][rows][D]
   long q_sb, q_sh, q_st, k_sh, k_st, v_sh, v_st, o_sb, o_sh, o_st, w_sb, w_sh, w_st;  // bytes
   long rows;             // n_kv_heads * M
@@ -73,7 +78,7 @@ __device__ __forceinline__ PrefixRow prefix_row(const PrefixArgs& a, int hk, int
 template <typename ET>
 struct PrefixOwn {
   using E = typename ET::E;
-  float lo, m, f, fo;  // own log-sum-exp (base 2), joint maximum, factors of the prefix's and the own part
+  float lo, m, f, fo;  // own log-sum-exp (base 2), joint reference, factors of the prefix's and the own part
   __device__ __forceinline__ PrefixOwn(const PrefixArgs& a, const PrefixRow& x, float mp) {
     lo = a.own ? a.own_lse[((long)x.b * a.Hq + x.h) * a.T + x.t] * kLog2e : -INFINITY;
     m = fmaxf(lo, mp);
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void prefix_attn_ker
 #pragma unroll
               for (int qb = 0; qb < NQ; ++qb) s[tt][qb][i] = -INFINITY;
       }
-      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -max)
+      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
       float mx[NQ];
       bool any_over = false, over[NQ];
 #pragma unroll
@@ -237,14 +242,14 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void prefix_attn_ker
         mx[qb] = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
-        over[qb] = mx[qb] * c > m_run[qb];
+        over[qb] = fmaf(mx[qb], c, -ET::kUp) > m_run[qb];
         any_over |= over[qb];
       }
       if (__any(any_over)) {
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) {
-          if (!__any(over[qb])) continue;  // columns that keep their maximum get a factor of exactly 1
-          const float m_new = fmaxf(m_run[qb], col_max(mx[qb]) * c);
+          if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
+          const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c, -ET::kUp));
           const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
           m_run[qb] = m_new;
           l_run[qb] *= f;

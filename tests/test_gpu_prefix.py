@@ -259,3 +259,24 @@ def test_long_prefixes_of_many_rows(dtype, B, Hq, Hkv, D, T, P):
     _check(got, _ref(q, k, v, own))
     for a, b in zip(got, care_kv.prefix_attention(q, k, v, own=own, return_lse=True)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nats", [9.0, 17.5, 21.0, 27.0])
+@pytest.mark.parametrize("B,D,P", [(1, 64, 1024), (4, 128, 1000), (64, 64, 256), (40, 128, 9000)])
+def test_a_long_tail_below_one_key(dtype, nats, B, D, P):
+    """One key far above a long flat prefix, and a value of 0 there: the result is the tail's, whose weights keep their
+    rounding of half a step each.  fp16 weights that are subnormal even times 2^15 are off by half of 2^-24 of
+    2^-15 of the largest."""
+    import care_kv
+    print(f"prefix {dtype} {nats} nats B={B} D={D} P={P}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(P)
+    q = torch.ones(B, 4, 1, D, device="cuda").to(dtype)
+    k = (0.1 * torch.randn(2, P, D, generator=g, device="cuda")).to(dtype)
+    k[:, P // 3] = nats / D ** 0.5
+    v = (200 + 100 * torch.rand(2, P, D, generator=g, device="cuda")).to(dtype)
+    v[:, P // 3] = 0
+    o, lse, tol = _ref(q, k, v)
+    if dtype == torch.float16:
+        tol = tol + P * 2.0 ** -40 * float(v.max())
+    _check(care_kv.prefix_attention(q, k, v, return_lse=True), (o, lse, tol))
