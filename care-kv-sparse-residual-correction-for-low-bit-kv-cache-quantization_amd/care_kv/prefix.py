@@ -70,7 +70,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         o_own = o_own if o_own.stride(3) == 1 else o_own.contiguous()
         l_own = l_own.contiguous()
     if out is not None:
-        _lib.check_out(out, q.shape, q.dtype, "out", q, k, v, *(() if own is None else (o_own,)))
+        _lib.check_out(out, q.shape, q.dtype, "out", q, k, v, *(() if own is None else (o_own, l_own)))
     dev = _lib.same_device("prefix_attention", q, k, v, o_own, l_own, out)
     if out is None:
         out = q.new_empty(q.shape)

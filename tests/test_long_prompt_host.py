@@ -276,3 +276,11 @@ def test_prefix_refuses_its_own_lse_as_output():
                            k_sh=576, k_st=64, v_sh=576, v_st=64, out_sb=256, out_sh=64, own_sb=256, own_sh=64)
     assert lib.carekv_prefix_attn(pp, p, p, p, p, p, p, p, p, 1 << 40, None) == -1
     assert "own_lse" in lib.carekv_last_error().decode()
+
+
+def test_prefix_output_over_its_own_lse_is_refused():
+    q, k = _half(2, 4, 3, 64), _half(2, 9, 64)
+    out = _half(2, 4, 3, 64)
+    lse = out.view(-1)[:48].view(torch.float32).view(2, 4, 3)
+    with pytest.raises(ValueError, match="overlap"):
+        care_kv.prefix_attention(q, k, k, own=(_half(2, 4, 3, 64), lse), out=out)
