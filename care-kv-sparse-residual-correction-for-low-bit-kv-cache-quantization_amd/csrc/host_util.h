@@ -34,11 +34,14 @@ void set_error(const char* fmt, ...);
   } while (0)
 
 // The bits of an operand's address and of the strides (bytes) of the dims it
-// steps: those of one entry do not count, whatever the caller has there.
+// steps: those of one entry do not count, whatever the caller has there, and
+// nothing does of an operand without entries.
 inline uintptr_t operand_bits(const void* p, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
   uintptr_t bits = (uintptr_t)p;
-  for (const auto& d : dims)
+  for (const auto& d : dims) {
+    if (d.first == 0) return 0;
     if (d.first > 1) bits |= (uintptr_t)d.second;
+  }
   return bits;
 }
 

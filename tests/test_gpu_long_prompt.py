@@ -401,3 +401,16 @@ def test_layer_rounds_32_bit_heads_after_the_turn():
         m = m + torch.cat((m[..., 32:], m[..., :32]), -1)
         # angles off by 2^-26 turns (2 pi 2^-26 < 2^-23) and their 32-bit sine, cosine and products
         assert got.dtype == F16 and ((got.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -21 * m).all()
+
+
+def test_empty_operands_of_any_strides():
+    """No query rows, or no prefix: what their views' strides are does not count."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").half()  # noqa: E731
+    q, k = r(2, 4, 7, 65)[..., 1:], r(2, 2, 9, 64)
+    assert not care_kv.attention_mass(q[:, :, :0], k).any()
+    o, lse = r(2, 4, 7, 64), torch.randn(2, 4, 7, generator=g, device="cuda")
+    p = r(2, 5, 65)[:, :0, 1:]
+    got, l = care_kv.prefix_attention(q, p, p, own=(o, lse), return_lse=True)
+    assert torch.equal(got, o) and float((l - lse).abs().max()) < 1e-5
