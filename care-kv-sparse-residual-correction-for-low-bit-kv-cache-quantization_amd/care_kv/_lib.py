@@ -309,11 +309,18 @@ def stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def aligned_rows(x: torch.Tensor, n: int = 16) -> torch.Tensor:
+# elements between rows that kernels which count them in 32 bits take
+MAX_ROW_STEP = 1 << 22
+
+
+def aligned_rows(x: torch.Tensor, n: int = 16, near: bool = False) -> torch.Tensor:
     """x with the values of a row (the last dim) next to each other and every
-    row on a multiple of n bytes: x itself, or a packed copy."""
+    row on a multiple of n bytes, with ``near`` rows less than MAX_ROW_STEP
+    elements apart: x itself, or a packed copy."""
     bits, e = x.data_ptr(), x.element_size()
     st = x.stride()
+    if near and st[-2] >= MAX_ROW_STEP and x.shape[-2] > 1:
+        return x.clone(memory_format=torch.contiguous_format)
     for s in st[:-1]:
         bits |= s * e
     if st[-1] == 1 and not bits % n:

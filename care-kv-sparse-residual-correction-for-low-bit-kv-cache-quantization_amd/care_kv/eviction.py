@@ -78,7 +78,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, *, lse: Optional[torch.Tens
     if out is None:
         out = q.new_empty((B, Hkv, Tk), dtype=torch.float32)
     if B and Tk:
-        q, k = _lib.aligned_rows(q), _lib.aligned_rows(k)
+        q, k = _lib.aligned_rows(q, near=True), _lib.aligned_rows(k, near=True)
         pp = _lib.MassParams(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], bool(causal), bool(accumulate),
                              1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *q.stride()[:3],
                              *k.stride()[:3], *out.stride()[:2])

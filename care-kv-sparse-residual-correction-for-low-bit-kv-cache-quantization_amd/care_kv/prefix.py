@@ -76,7 +76,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         out = q.new_empty(q.shape)
     lse = q.new_empty((B, Hq, T), dtype=torch.float32) if return_lse else None
     if out.numel():
-        q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k), _lib.aligned_rows(v)
+        q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k, near=True), _lib.aligned_rows(v, near=True)
         pp = _lib.PrefixParams(B, Hq, Hkv, T, P, D, _lib.DTYPE_CODE[q.dtype],
                                1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *q.stride()[:3],
                                *k.stride()[:2], *v.stride()[:2], *out.stride()[:3],

@@ -414,3 +414,16 @@ def test_empty_operands_of_any_strides():
     p = r(2, 5, 65)[:, :0, 1:]
     got, l = care_kv.prefix_attention(q, p, p, own=(o, lse), return_lse=True)
     assert torch.equal(got, o) and float((l - lse).abs().max()) < 1e-5
+
+
+def test_rows_far_apart():
+    """Rows 2^22 elements apart and more: copied like any rows that the kernels do not read as they lie."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(4)
+    far = lambda n: torch.randn(n * ((1 << 22) + 64), generator=g, device="cuda", dtype=torch.float16).as_strided(  # noqa: E731
+        (2, n, 64), (64, (1 << 22) + 64, 1))
+    q, k, v = far(3)[None], far(5), far(5)
+    assert torch.equal(care_kv.attention_mass(q, k[None]), care_kv.attention_mass(q.contiguous(), k[None].contiguous()))
+    got = care_kv.prefix_attention(q, k, v, return_lse=True)
+    for a, b in zip(got, care_kv.prefix_attention(q.contiguous(), k.contiguous(), v.contiguous(), return_lse=True)):
+        assert torch.equal(a, b)

@@ -284,3 +284,10 @@ def test_prefix_output_over_its_own_lse_is_refused():
     lse = out.view(-1)[:48].view(torch.float32).view(2, 4, 3)
     with pytest.raises(ValueError, match="overlap"):
         care_kv.prefix_attention(q, k, k, own=(_half(2, 4, 3, 64), lse), out=out)
+
+
+def test_rows_far_apart_are_copied():
+    far = torch.empty(0, dtype=torch.float16).set_(torch.zeros(1 << 24, dtype=torch.float16).untyped_storage(), 0, (2, 3, 64),
+                                                   (64, _lib.MAX_ROW_STEP, 1))
+    assert _lib.aligned_rows(far) is far and _lib.aligned_rows(far[:, :1], near=True).data_ptr() == far.data_ptr()
+    assert _lib.aligned_rows(far, near=True).is_contiguous()
