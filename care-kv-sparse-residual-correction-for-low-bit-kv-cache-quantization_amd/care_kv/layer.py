@@ -273,20 +273,22 @@ class CAREKVLayer(nn.Module):
         mode = resolve_prefill_mode()
         seqs = list(range(B)) if seqs is None else list(seqs)
         runs = self._key_runs(attention_mask, B, T)
+        # before anything is written, for a padded batch before its first sequence
+        longest = T if runs is None else max((e - s for s, e in runs), default=0)
+        if prefix is not None:
+            if mode not in ("fp", "base_quant"):
+                raise NotImplementedError(f"a shared prefix in prefill mode {mode!r}: the correction weighs a prompt's own "
+                                          "rows alone (fp and base_quant take one)")
+            check_prefix(prefix, cfg.num_heads, cfg.head_dim, F16, self.W_Q.device)
+        if 0 < cfg.prefill_keep < longest and (mode == "carekv_stored" or (cache.hat and mode != "fp")):
+            raise NotImplementedError(f"prefill_keep in prefill mode {mode!r} with base_quantizer="
+                                      f"{cfg.base_quantizer!r}: the mode reads the pages of the whole prompt")
         if runs is not None:
             out = self._prefill_runs(cache, hidden, runs, sink_tokens, position_embeddings, token_start_abs, seqs,
                                      prefix)
             return out[0] if squeeze else out
         evict = 0 < cfg.prefill_keep < T
-        if prefix is not None and mode not in ("fp", "base_quant"):
-            raise NotImplementedError(f"a shared prefix in prefill mode {mode!r}: the correction weighs a prompt's own "
-                                      "rows alone (fp and base_quant take one)")
-        if evict and (mode == "carekv_stored" or (cache.hat and mode != "fp")):
-            raise NotImplementedError(f"prefill_keep in prefill mode {mode!r} with base_quantizer="
-                                      f"{cfg.base_quantizer!r}: the mode reads the pages of the whole prompt")
         Qh, Kh, Vh = self._heads(hidden, position_embeddings)
-        if prefix is not None:  # before anything is written
-            check_prefix(prefix, cfg.num_heads, cfg.head_dim, F16, Qh.device)
         hats = None
         if not evict:
             hats = cache.write_prefill(self.layer_id, Kh, Vh, token_start_abs=token_start_abs,

@@ -291,3 +291,24 @@ def test_rows_far_apart_are_copied():
                                                    (64, _lib.MAX_ROW_STEP, 1))
     assert _lib.aligned_rows(far) is far and _lib.aligned_rows(far[:, :1], near=True).data_ptr() == far.data_ptr()
     assert _lib.aligned_rows(far, near=True).is_contiguous()
+
+
+@pytest.mark.parametrize("mode,kw,prefix", [("carekv_stored", dict(prefill_keep=40), False),
+                                            ("base_quant", dict(prefill_keep=40, base_quantizer="kivi_style", base_bits=2), False),
+                                            ("carekv_eval", {}, True), ("carekv_stored", {}, True), ("fp", {}, "short")])
+def test_padded_prompts_are_refused_before_any_is_written(mode, kw, prefix, monkeypatch):
+    """What a mode does not take of any sequence of a padded batch is refused before the first one is computed."""
+    monkeypatch.setenv("CAREKV_PREFILL_MODE", mode)
+    cfg = care_kv.CacheConfig(num_layers=1, num_heads=4, num_kv_heads=2, head_dim=64, prefill_keep_sink=4,
+                              prefill_keep_recent=8, **kw)
+    w = [torch.zeros(o, 256, dtype=torch.float16) for o in (256, 128, 128, 256)]
+    lay = care_kv.CAREKVLayer(cfg, 0, *w)
+    monkeypatch.setattr(lay, "_heads", lambda *a: pytest.fail("a prompt was computed"))
+    mask = torch.ones(3, 60, dtype=torch.int64)
+    mask[0, :50] = 0  # 10 rows, 59, 30
+    mask[1, 59:] = 0
+    mask[2, 30:] = 0
+    cache = type("Cache", (), {"hat": "kivi_style" in kw.values()})()
+    pre = None if not prefix else (_half(2, 9, 64), _half(2, 8 if prefix == "short" else 9, 64))
+    with pytest.raises(ValueError if prefix == "short" else NotImplementedError):
+        lay.prefill(cache, _half(3, 60, 256), attention_mask=mask, prefix=pre)
