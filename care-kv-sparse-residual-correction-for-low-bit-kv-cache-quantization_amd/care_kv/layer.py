@@ -133,8 +133,8 @@ class CAREKVLayer(nn.Module):
         Hq, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         Q, K, V = self._project(hidden)
         if position_embeddings is not None and isinstance(position_embeddings[0], RotaryPlan):
-            # 32-bit heads are rounded after the turn; bf16 ones fit fp16 and are rounded by it once
-            Q, K = (x if x.dtype == torch.float32 else x.to(F16) for x in (Q, K))
+            # rounded to fp16 once, after the turn: bf16 heads, whose range is wider, are turned in 32 bits
+            Q, K = (x if x.dtype == F16 else x.float() for x in (Q, K))
             Q, K = rotate_heads(Q, K, position_embeddings[1], position_embeddings[0])
             return Q.to(F16), K.to(F16), V.to(F16).contiguous()
         cos, sin = (None, None) if position_embeddings is None else (x.to(Q.dtype) for x in position_embeddings)

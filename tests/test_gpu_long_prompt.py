@@ -427,3 +427,28 @@ def test_rows_far_apart():
     got = care_kv.prefix_attention(q, k, v, return_lse=True)
     for a, b in zip(got, care_kv.prefix_attention(q.contiguous(), k.contiguous(), v.contiguous(), return_lse=True)):
         assert torch.equal(a, b)
+
+
+def test_layer_rounds_bf16_heads_once():
+    """bf16 projections past fp16's range in both directions: what a turn brings back into it is rounded once, after
+    the turn (half a step, 2^-11 of it; 2^-25 below 2^-14), beside the 32-bit turn's own error."""
+    import care_kv
+    lay, _, g = _layer(care_kv)
+    for p in lay.parameters():
+        p.data = p.data.bfloat16()
+    lay.W_K.data *= 40000
+    lay.W_Q.data *= 2.0 ** -20
+    x = torch.randn(2, 37, 512, generator=g, device="cuda").bfloat16()
+    plan = care_kv.rotary_plan(64)
+    pos = torch.arange(1000, 1037, device="cuda")
+    Q, K, _ = lay._project(x)
+    q, k, v = lay._heads(x, (plan, pos))
+    assert (K.abs() > 65504).any() and (Q.abs() < 2.0 ** -24).any() and q.dtype == k.dtype == v.dtype == F16
+    for got, x0 in ((q, Q), (k, K)):
+        want = _rot64(x0, pos, plan)
+        m = x0.abs().double()
+        m = m + torch.cat((m[..., 32:], m[..., :32]), -1)
+        fits = want.abs() + 2.0 ** -21 * m < 65504
+        assert float(fits.double().mean()) > 0.5
+        err = (got.double() - want).abs()
+        assert (err[fits] <= (2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -21 * m)[fits]).all()
