@@ -1,8 +1,8 @@
 """Rows of a prompt kept by the attention they get (no reference counterpart):
 ``attention_mass`` adds up the weight that each key gathers from the query
 rows that see it, ``evict_rows`` keeps the first, the last and the heaviest
-rows and gathers their K and V, ready for ``CAREKVCache.write_prefill`` or as
-the shared prefix of ``prefix_attention``.
+rows and gathers their K and V for ``CAREKVCache.write_prefill`` or as the
+shared prefix of ``prefix_attention``.
 """
 from __future__ import annotations
 
@@ -16,7 +16,9 @@ from . import _lib
 
 class EvictedRows(NamedTuple):
     """What ``evict_rows`` kept, in index order; places past a sequence's kept
-    rows hold zeros and index -1."""
+    rows hold zeros and index -1.  ``write_prefill`` and ``prefix_attention``
+    know no lengths and would take those zeros for rows: of a sequence shorter
+    than keep they are given k[b, :, :n] and v[b, :, :n], n = lengths[b]."""
     k: torch.Tensor        # (B, Hkv, keep, D)
     v: torch.Tensor
     mass: torch.Tensor     # (B, Hkv, keep) fp32

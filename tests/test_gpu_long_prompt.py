@@ -452,3 +452,25 @@ def test_layer_rounds_bf16_heads_once():
         assert float(fits.double().mean()) > 0.5
         err = (got.double() - want).abs()
         assert (err[fits] <= (2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -21 * m)[fits]).all()
+
+
+def test_kept_rows_of_a_short_sequence():
+    """A ragged batch, one sequence shorter than keep: cut to its kept length, its rows are a prefix of its own rows
+    alone, and what the pages store."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").half()  # noqa: E731
+    k, v, q, lens = r(2, 2, 200, 64), r(2, 2, 200, 64), r(3, 8, 64), [200, 17]
+    kept = care_kv.evict_rows(torch.rand(2, 2, 200, generator=g, device="cuda"), k, v, keep=50, sink=4, recent=8, lengths=lens)
+    n = int(kept.lengths[1])
+    assert n == 17 and not kept.k[1][:, n:].any()
+    for a, b in zip(care_kv.prefix_attention(q, kept.k[1][:, :n], kept.v[1][:, :n], return_lse=True),
+                    care_kv.prefix_attention(q, k[1, :, :17], v[1, :, :17], return_lse=True)):
+        assert torch.equal(a, b)
+    _, cfg, _ = _layer(care_kv)
+    a, b = care_kv.CAREKVCache(cfg, n_seq=1), care_kv.CAREKVCache(cfg, n_seq=1)
+    a.write_prefill(0, kept.k[1:, :, :n], kept.v[1:, :, :n])
+    b.write_prefill(0, k[1:, :, :17], v[1:, :, :17])
+    assert a.total_valid_tokens(0, 0, 0) == 17
+    for nm in ("kcodes", "vcodes", "kscale", "valid"):
+        assert torch.equal(getattr(a, nm), getattr(b, nm)), nm
