@@ -40,9 +40,6 @@ struct RotaryArgs {
   long rows;           // batch * T
 };
 
-template <typename E>
-__device__ __forceinline__ float to_f32(E v) { return (float)v; }
-
 // N elements at p: 16-byte pieces where WIDE (the host checked the alignment), else one by one
 template <typename E, int N, bool WIDE>
 __device__ __forceinline__ void load_vec(E* x, const char* p) {
