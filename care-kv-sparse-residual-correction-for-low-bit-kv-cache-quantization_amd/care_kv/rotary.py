@@ -111,6 +111,8 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     gradient of the forward call, and with scale 1 its inverse.  ``out``: (q_out,
     k_out), which may be (q, k) themselves; by default new contiguous tensors.
     The results carry no autograd history."""
+    if out is not None and (len(out) != 2 or out[0] is None or (out[1] is None) != (k is None)):
+        raise ValueError("out must be (q_out, k_out), k_out None only without k")
     squeeze = q.dim() == 3
     if squeeze:
         qo, ko = (None, None) if out is None else out
@@ -131,8 +133,6 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     pos = positions.unsqueeze(0) if positions.dim() == 1 else positions
     if pos.dim() != 2 or pos.shape[0] not in (1, B) or pos.shape[1] != T:
         raise ValueError(f"positions must be ({B}, {T}), (1, {T}) or ({T},); got {tuple(positions.shape)}")
-    if out is not None and (len(out) != 2 or out[0] is None or (out[1] is None) != (k is None)):
-        raise ValueError("out must be (q_out, k_out), k_out None only without k")
     if out is not None:
         _lib.check_out(out[0], q.shape, q.dtype, "q_out", q)
         if k is not None:

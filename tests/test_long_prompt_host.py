@@ -312,3 +312,12 @@ def test_padded_prompts_are_refused_before_any_is_written(mode, kw, prefix, monk
     pre = None if not prefix else (_half(2, 9, 64), _half(2, 8 if prefix == "short" else 9, 64))
     with pytest.raises(ValueError if prefix == "short" else NotImplementedError):
         lay.prefill(cache, _half(3, 60, 256), attention_mask=mask, prefix=pre)
+
+
+def test_rotate_refusals_of_one_sequence():
+    q, k, pos = _half(4, 3, 64), _half(2, 3, 64), torch.zeros(3, dtype=torch.int64)
+    for out in ((None, k), (q, None), (q,), (q, k, k), (q[:2], k)):
+        with pytest.raises(ValueError):
+            care_kv.rotate_heads(q, k, pos, _plan(), out=out)
+    with pytest.raises(ValueError):
+        care_kv.rotate_heads(q, None, pos, _plan(), out=(q, k))
