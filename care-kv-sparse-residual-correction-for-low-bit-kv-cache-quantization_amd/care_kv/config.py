@@ -144,8 +144,9 @@ class CacheConfig:
     # only so many rows per kv head go to the pages, the first
     # prefill_keep_sink, the last prefill_keep_recent and the rows that gathered
     # the most attention weight (attention_mass / evict_rows) from the prompt's
-    # last prefill_keep_window queries (0: all of them).  The prompt's own
-    # attention sees every row.
+    # last prefill_keep_window queries (0: all of them), each query's weights
+    # summing to 1 over the prompt's rows, also behind a shared prefix.  The
+    # prompt's own attention sees every row.
     prefill_keep: int = 0
     prefill_keep_sink: int = 4
     prefill_keep_recent: int = 32

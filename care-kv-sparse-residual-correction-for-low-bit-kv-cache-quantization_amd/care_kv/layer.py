@@ -264,7 +264,8 @@ class CAREKVLayer(nn.Module):
         post-RoPE rows before every sequence's first token; the caller's
         position_embeddings start behind them.  cfg.prefill_keep (every mode
         but ``carekv_stored``, whose correction needs all pages of the prompt)
-        writes only the rows kept to the pages."""
+        writes only the rows kept to the pages; a query's weights for that are
+        those over the prompt's own rows, also behind a prefix."""
         squeeze = hidden.dim() == 2
         if squeeze:
             hidden = hidden.unsqueeze(0)
