@@ -433,3 +433,33 @@ def test_mass_query_lengths_of_every_kind():
     ref, _, rel = _mass_ref(q[:, :, :17], k, q_start=[3, 283, -2])
     _check_mass(got, ref, rel, 2 * 17)
     assert torch.equal(care_kv.attention_mass(q[0], k[0], q_lengths=17, q_start=3), got[0])
+
+
+def test_mass_query_lengths_captured():
+    """Lengths on the device may change between replays of a captured call, as the tensors may."""
+    import care_kv
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q = torch.randn(3, 4, 200, 64, generator=g, device="cuda").half()
+    k = torch.randn(3, 2, 200, 64, generator=g, device="cuda").half()
+    n = torch.tensor([200, 50, 120], device="cuda", dtype=torch.int32)
+    lse = torch.full((3, 4, 200), 5.0, device="cuda")
+
+    def call():
+        return care_kv.attention_mass(q, k, lengths=n), care_kv.attention_mass(q, k, lse=lse, lengths=n, q_lengths=n)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for turn, lens in enumerate(([200, 50, 120], [1, 200, 0], [64, 65, 199], [0, 0, 7])):
+        n.copy_(torch.tensor(lens))
+        lse[:, :, turn::5] = -float("inf")
+        q[:, :, turn::5] = float("nan")
+        graph.replay()
+        got = [o.clone() for o in out]
+        for a, b in zip(got, call()):
+            assert torch.equal(torch.nan_to_num(a, 7.0), torch.nan_to_num(b, 7.0))
+        assert not torch.isnan(got[1]).any()
