@@ -26,23 +26,27 @@
 // (sequence, kv head), the scores of all keys in LDS, K read once, one launch.
 // Past kFewBytes of K a head the keys are cut into parts (mass_scores_kernel: K
 // read once, the scores to memory; mass_weigh_kernel: their weights), up to 2048
-// work-groups.  us a call in a graph, one launch / two: 8 heads, D = 128, 4 rows
-// on 512 keys (128 KB) 8.3 / 7.8, 1024 11.5 / 8.0, 2048 18.9 / 8.4, 4096 33.7 / 8.4;
-// 128 heads, D = 64, 8 rows on 2303 keys (288 KB) 14.9 / 16.4, 4000 22.0 / 21.2;
-// a launch more costs an eager call 3 us of host time.  Decode steps on 8 x 8192
+// work-groups.  The limit is that of an eager call, where the second launch and
+// the workspace cost 4 us of host time: 8 heads, D = 128, 4 rows on 1280 keys (320
+// KB) 13.8 us in one launch, 15.7 in two whatever the keys up to 4096.  In a graph
+// it depends on the heads too, one launch / two: 8 heads, D = 128, 4 rows on 512
+// keys (128 KB) 8.3 / 7.8, 1024 11.5 / 8.0, 2048 18.9 / 8.4, 4096 33.7 / 8.4; 128
+// heads, D = 64, 8 rows on 2303 keys (288 KB) 14.9 / 16.4, 4000 22.0 / 21.2: few
+// heads lose up to 5 us there below the limit.  Decode steps on 8 x 8192
 // keys, 32 / 8 heads (134 MB) 27 us, on 16 x 6000, 32 / 32 heads (786 MB) 160, 4.9
 // TB/s (as walks 64 and 374).
 //
-// Measured, D = 128, 8192 causal rows with lse: 32 / 8 heads 321 us + 5 for the
+// Measured, D = 128, 8192 causal rows with lse: 32 / 8 heads 324 us + 5 for the
 // sum of the parts (275 GFLOP of visible products, 1.07e9 exponentials: 0.84
-// PFLOP/s), 32 / 32 heads 304; long uncut walks reach 1.0 PFLOP/s.  Bound: a
-// 16 x 16 x 32 product with the exponential and two fused multiply-adds of its
-// four scores a lane takes a SIMD 25 cycles at best (measured in registers
-// alone; the product itself 16), 180 us of the 321.  Blocks in order instead of
-// pairs, 2048 work-groups: 350; LDS rows padded by 16 bytes (9.0 cycles a read
-// against 5.6): 360; masked wave tiles not skipped: 337; 4 waves of 64 keys or
-// 32 x 32 products were slower (363 and 374 before these).  A window of 64 rows
-// on 4 x 8191 keys: 27 us statistics, 32 us weights, 8 us each before the first
+// PFLOP/s; in bursts after a pause 340-360), 32 / 32 heads 318, without lse 32 / 8
+// heads 632; long uncut walks reach 1.0 PFLOP/s.  Bound: a 16 x 16 x 32 product
+// with the exponential and two fused multiply-adds of its four scores a lane takes
+// a SIMD 25 cycles at best (measured in registers alone; the product itself 16),
+// 180 us of the 324.  Against 321 then: blocks in order instead of pairs, 2048
+// work-groups, 350; LDS rows padded by 16 bytes (9.0 cycles a read against 5.6)
+// 360; masked wave tiles not skipped 337.  Before these, against 355-370: 4 waves
+// of 64 keys 363, 32 x 32 products 374; not measured since.  A window of 64 rows
+// on 4 x 8191 keys: 29 us statistics, 31 us weights, 8 us each before the first
 // products and 1.1 us a tile and CU, which two work-groups a CU (or two tiles on
 // their way) change by little: K (67 MB) is not what bounds them.
 //

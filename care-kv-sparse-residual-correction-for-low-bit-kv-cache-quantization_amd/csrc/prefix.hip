@@ -22,8 +22,8 @@
 // K and V rows are padded by 32 bytes in LDS: 16-byte reads of 16 rows then take
 // 5.6 cycles a wave, padded by 16 bytes 9.0.
 //
-// Measured: 16 x 128 rows, 40 heads, D = 128, 4097 keys (172 GFLOP) 198 us, 0.87
-// PFLOP/s: 640 equal work-groups on 768 places, products and exponentials
+// Measured: 16 x 128 rows, 40 heads, D = 128, 4097 keys (172 GFLOP) 206 us, 0.83
+// PFLOP/s (in bursts after a pause 217): 640 equal work-groups on 768 places, products and exponentials
 // overlapping in part.  64 rows x 32 / 8 heads on 32768 keys (34 GFLOP, 134 MB
 // of K and V) 55 us + 6 us for the join: 16 splits of three sets of waves, whose
 // partials are 17 MB; without the sets 48 splits and 50 MB 53 + 11, 32 splits 57 +
