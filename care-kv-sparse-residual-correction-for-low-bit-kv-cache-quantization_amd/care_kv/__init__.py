@@ -8,7 +8,8 @@ in ``libcarekv_hip.so`` through a C ABI (include/carekv.h).  Additions of
 this build: the batched entry points ``decode_attention`` /
 ``prefill_correction`` / ``prefill_attention``, ``CAREKVAdapter`` and
 ``CarekvError``, and for long prompts ``rotate_heads``, ``attention_mass`` /
-``evict_rows`` and ``prefix_attention``.
+``evict_rows`` and ``prefix_attention``; for serving on pages of 4-bit rows
+``append_pages``, ``paged_attention``, ``window_attention`` and ``verify_drafts``.
 """
 from .config import (CacheConfig, apply_carekv_env_overrides, layer_budget_multiplier,
                      resolve_read_knobs, resolve_store_knobs)
@@ -24,6 +25,9 @@ from .prefill import dequantize_rows, prefill_attention, prefill_eval, quant_deq
 from .rotary import RotaryPlan, rotary_plan, rotate_heads
 from .eviction import EvictedRows, attention_mass, evict_rows
 from .prefix import prefix_attention
+from .pages import Int4Pages, append_pages, int4_pages, paged_attention
+from .window import window_attention
+from .drafts import VerifiedDrafts, verify_drafts
 from .layer import CAREKVLayer
 from .attention import get_imp_per_layer
 from .utils import (ABLATION_VARIANTS, budget_sweep, calibrate_layer_sensitivity, compute_boundary_risk_stats,
@@ -57,4 +61,5 @@ __all__ = [
     "decode_attention", "prefill_correction", "prefill_attention", "prefill_eval", "quantize_rows", "dequantize_rows",
     "quant_dequant", "CAREKVAdapter", "CarekvError", "CAREKVHFCache",
     "RotaryPlan", "rotary_plan", "rotate_heads", "EvictedRows", "attention_mass", "evict_rows", "prefix_attention",
+    "Int4Pages", "int4_pages", "append_pages", "paged_attention", "window_attention", "VerifiedDrafts", "verify_drafts",
 ]

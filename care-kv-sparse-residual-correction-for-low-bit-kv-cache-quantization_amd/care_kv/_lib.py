@@ -109,6 +109,31 @@ class PrefixParams(C.Structure):
                                   "own_sb", "own_sh", "own_st")]
 
 
+class AppendParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "seq_len", "head_dim", "rotary_dim", "dtype",
+                                         "interleaved", "pos_bits", "n_pages", "max_pages")] + [("scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("pos_batch", "table_sb", "q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "v_sb", "v_sh",
+                                  "v_st", "qo_sb", "qo_sh", "qo_st")]
+
+
+class PagedParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "seq_len", "head_dim", "dtype", "n_pages",
+                                         "max_pages", "window", "sink")] + [("sm_scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("table_sb", "q_sb", "q_sh", "q_st", "out_sb", "out_sh", "out_st")]
+
+
+class WindowParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_heads", "n_kv_heads", "seq_len", "n_keys", "head_dim", "dtype",
+                                         "window", "sink")] + [("sm_scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("q_sb", "q_sh", "q_st", "k_sb", "k_sh", "k_st", "v_sb", "v_sh", "v_st", "out_sb", "out_sh",
+                                  "out_st")]
+
+
+class VerifyParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_drafts", "vocab", "dtype")] + \
+        [(n, C.c_int64) for n in ("target_sb", "target_st", "draft_probs_sb", "draft_probs_st", "draft_sb", "u_sb")]
+
+
 # page job: int32 x 6 (seq, kv_head, page, num_valid, token_start, is_recent)
 PAGE_JOB_INTS = 6
 
@@ -120,7 +145,9 @@ EXPORTS = ["carekv_store_pages", "carekv_store_prefill", "carekv_store_workspace
            "carekv_quantize_rows_f32", "carekv_dequantize_rows_f32", "carekv_kivi_codes", "carekv_read_hat_pages",
            "carekv_prefill_eval", "carekv_rotate_heads", "carekv_attention_mass",
            "carekv_attention_mass_workspace_bytes", "carekv_evict_rows", "carekv_evict_rows_workspace_bytes", "carekv_prefix_attn",
-           "carekv_prefix_attn_workspace_bytes", "carekv_last_error"]
+           "carekv_prefix_attn_workspace_bytes", "carekv_page4_bytes", "carekv_append_pages", "carekv_paged_attn",
+           "carekv_paged_attn_workspace_bytes", "carekv_window_attn", "carekv_window_attn_workspace_bytes",
+           "carekv_verify_drafts", "carekv_verify_drafts_workspace_bytes", "carekv_last_error"]
 
 # bytes of the per-GPU static workspace of carekv_decode_attn_static
 # (CAREKV_STATIC_SCRATCH_BYTES in include/carekv.h)
@@ -218,6 +245,22 @@ def load(path: str | None = None):
         lib.carekv_prefix_attn.argtypes = [C.POINTER(PrefixParams), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.carekv_prefix_attn_workspace_bytes.restype = i64
         lib.carekv_prefix_attn_workspace_bytes.argtypes = [C.POINTER(PrefixParams)]
+        lib.carekv_page4_bytes.restype = i64
+        lib.carekv_page4_bytes.argtypes = [i32]
+        lib.carekv_append_pages.restype = C.c_int
+        lib.carekv_append_pages.argtypes = [C.POINTER(AppendParams)] + [vp] * 13
+        lib.carekv_paged_attn.restype = C.c_int
+        lib.carekv_paged_attn.argtypes = [C.POINTER(PagedParams), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_paged_attn_workspace_bytes.restype = i64
+        lib.carekv_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedParams)]
+        lib.carekv_window_attn.restype = C.c_int
+        lib.carekv_window_attn.argtypes = [C.POINTER(WindowParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_window_attn_workspace_bytes.restype = i64
+        lib.carekv_window_attn_workspace_bytes.argtypes = [C.POINTER(WindowParams)]
+        lib.carekv_verify_drafts.restype = C.c_int
+        lib.carekv_verify_drafts.argtypes = [C.POINTER(VerifyParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_verify_drafts_workspace_bytes.restype = i64
+        lib.carekv_verify_drafts_workspace_bytes.argtypes = [C.POINTER(VerifyParams)]
         _lib = lib
         return lib
 

@@ -1,0 +1,293 @@
+// New tokens into pages of 4-bit rows, q and k under rotary positions on the way
+// (append_pages): for pair i of a head and position p, t = p f_i,
+//   y1 = a (x1 cos t - x2 sin t),  y2 = a (x2 cos t + x1 sin t),
+// then per 32 values s = half(max|y| / 7), c = clamp(rint(half(y / s)), -8, 7).
+//
+// Angles and products are 64 bits, rounded to 32 and then to the type: a product
+// rounded to 32 bits first puts one k in some 10^6 into the neighbouring code,
+// which is a seventh of the group's largest value.
+//
+// Bound by memory: each value is read and written once.  A work-group takes 4
+// (D = 64: 8) consecutive places of a sequence, whose sines and cosines its
+// threads compute once, one each, and its waves walk over the heads; a lane owns
+// 8 dims of one token, so that the angles stay in registers over the walk.
+// V's words hold four tokens of a dim: the places of a wave start at a multiple
+// of four, so that no other wave writes a word of it, and a word of which only
+// some tokens are new is read and joined.
+#include <algorithm>
+
+#include "common.h"
+#include "host_util.h"
+#include "pages4.h"
+
+namespace carekv {
+
+struct AppendArgs {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* qo;
+  uint16_t* k_hat;       // [B][Hkv][T][D], or null
+  uint16_t* v_hat;
+  const void* pos;       // or null: start + t
+  const double* freqs;
+  const int32_t* start;
+  const int32_t* counts; // or null: T
+  const int32_t* table;
+  char* pages;
+  long pos_batch, table_sb, q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st;  // (q .. o: bytes)
+  int T, Hq, Hkv, R, nu, n_pages, max_pages, pos64, interleaved;
+  int partner_wide;      // the other halves of a lane's pairs are one aligned run
+  float scale;
+};
+
+// 8 elements at p: one 16-byte load where the host checked the alignment
+template <typename E, bool W>
+__device__ __forceinline__ void load8(E* x, const char* p, bool wide = true) {
+  if (W && wide) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    __builtin_memcpy(x, &v, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const E*>(p)[i];
+  }
+}
+
+// A lane's 8 fp16 values as codes: u[e] = c + 8, and the group's scale (its 4 lanes hold the other values)
+struct Coded {
+  uint32_t u[8];
+  _Float16 s;
+};
+__device__ __forceinline__ Coded code8(const _Float16* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, (uint32_t)(half2bits(x[e]) & 0x7fff));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+  Coded r;
+  const bool bad = m >= 0x7c00;
+  r.s = bad ? bits2half(0x7e00) : (_Float16)(h2f((uint16_t)m) / 7.f);
+  const float s = (float)r.s;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float c = rintf((float)(_Float16)((float)x[e] / s));  // (0 / 0: NaN, which fmaxf drops below)
+    r.u[e] = bad || c != c ? 8u : (uint32_t)((int)fminf(fmaxf(c, -8.f), 7.f) + 8);
+  }
+  return r;
+}
+
+template <typename E, int D, bool W>
+__global__ __launch_bounds__(256) void append_pages_kernel(AppendArgs a) {
+  using P = Page4<D>;
+  constexpr int CH = D / 8, TPW = 64 / CH;  // lanes of a token, tokens of a wave
+  __shared__ double2 tab[256];              // [TPW][D / 2] cosine, sine
+  __shared__ __align__(8) uint8_t codes[4][TPW * D];
+  const int b = blockIdx.x / a.nu, unit = blockIdx.x - b * a.nu;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int start = min(max(a.start[b], -(1 << 29)), 1 << 29);
+  const int slot0 = (start & ~(TPW - 1)) + unit * TPW;
+  if (slot0 >= start + a.T) return;
+  const int count = min(a.counts ? a.counts[b] : a.T, a.T);
+  const int half = a.R / 2;
+  {
+    const int i = threadIdx.x % (D / 2), t = slot0 + (int)threadIdx.x / (D / 2) - start;
+    if (i < half && t >= 0 && t < a.T) {
+      const long pi = b * a.pos_batch + t;
+      const double p = !a.pos ? (double)(start + t)
+                              : a.pos64 ? (double)reinterpret_cast<const int64_t*>(a.pos)[pi]
+                                        : (double)reinterpret_cast<const int32_t*>(a.pos)[pi];
+      // t less its whole turns (2 pi in two parts), in half turns
+      const double x = p * a.freqs[i], n = rint(x * 0.15915494309189533577);
+      const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586477, x));
+      double s, c;
+      sincospi(r * 0.31830988618379067154, &s, &c);
+      tab[threadIdx.x] = make_double2(c * (double)a.scale, s * (double)a.scale);
+    }
+  }
+  __syncthreads();
+  const int j = lane / CH, c = lane % CH, slot = slot0 + j, t = slot - start;
+  const bool in = t >= 0 && t < a.T, fresh = t >= 0 && t < count;
+  // y[e] = x[e] cs[e] + x[partner] sn[e]
+  double cs[8], sn[8];
+  const bool rot = 8 * c < a.R;
+  // (half: a lane's dims may lie in both halves or behind R where R is no multiple of 16)
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = 8 * c + e;
+    const int i = a.interleaved ? d / 2 : d < half ? d : d - half;
+    const bool second = a.interleaved ? d & 1 : d >= half;
+    const double2 w = tab[j * (D / 2) + min(i, D / 2 - 1)];
+    cs[e] = d < a.R ? w.x : 1.0;
+    sn[e] = d < a.R ? (second ? w.y : -w.y) : 0.0;
+  }
+  auto turned = [&](float* y, const E* x, const char* row) {
+    E o[8];
+    if (rot) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = x[e ^ 1];
+      } else if (a.partner_wide) {
+        load8<E, W>(o, row + 2 * (8 * c < half ? 8 * c + half : 8 * c - half));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = 8 * c + e;
+          o[e] = reinterpret_cast<const E*>(row)[d >= a.R ? d : d < half ? d + half : d - half];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      y[e] = 8 * c + e < a.R ? (float)fma((double)(float)x[e], cs[e], (double)(float)o[e] * sn[e]) : (float)x[e];
+  };
+  const int page = slot0 >= 0 && slot0 / kPage < a.max_pages ? a.table[b * a.table_sb + slot0 / kPage] : -1;
+  const bool there = page >= 0 && page < a.n_pages;
+  for (int w = blockIdx.y * 4 + wave; w < a.Hkv + a.Hq; w += 4 * gridDim.y) {
+    if (w >= a.Hkv) {
+      if (!in) continue;
+      const int h = w - a.Hkv;
+      const char* row = a.q + b * a.q_sb + h * a.q_sh + t * a.q_st;
+      E x[8], z[8];
+      float y[8];
+      load8<E, W>(x, row + 16 * c);
+      turned(y, x, row);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (E)y[e];
+      char* dst = a.qo + b * a.o_sb + h * a.o_sh + t * a.o_st + 16 * c;
+      if (W) {
+        uint4 u;
+        __builtin_memcpy(&u, z, 16);
+        *reinterpret_cast<uint4*>(dst) = u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) reinterpret_cast<E*>(dst)[e] = z[e];
+      }
+      continue;
+    }
+    char* block = a.pages + ((long)page * a.Hkv + w) * P::kBytes;
+    _Float16 kx[8], vx[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kx[e] = vx[e] = (_Float16)0.f;
+    if (fresh) {
+      const char* krow = a.k + b * a.k_sb + w * a.k_sh + t * a.k_st;
+      const char* vrow = a.v + b * a.v_sb + w * a.v_sh + t * a.v_st;
+      E x[8], z[8];
+      float y[8];
+      load8<E, W>(x, krow + 16 * c);
+      load8<E, W>(z, vrow + 16 * c);
+      turned(y, x, krow);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { kx[e] = (_Float16)y[e]; vx[e] = (_Float16)(float)z[e]; }
+    }
+    const Coded kc = code8(kx), vc = code8(vx);
+    if (a.k_hat && in) {
+      const long at = (((long)b * a.Hkv + w) * a.T + t) * D + 8 * c;
+      _Float16 kh[8], vh[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { kh[e] = dq((int)kc.u[e] - 8, kc.s); vh[e] = dq((int)vc.u[e] - 8, vc.s); }
+      uint4 u;
+      __builtin_memcpy(&u, kh, 16);
+      *reinterpret_cast<uint4*>(a.k_hat + at) = u;
+      __builtin_memcpy(&u, vh, 16);
+      *reinterpret_cast<uint4*>(a.v_hat + at) = u;
+    }
+    if (!there) continue;  // (the same for the whole wave)
+    const int place = slot & (kPage - 1);
+    if (fresh) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word |= kc.u[e] << nib4(e);
+      *reinterpret_cast<uint32_t*>(block + place * (D / 2) + 4 * c) = word;
+      if ((c & 3) == 0) {
+        *reinterpret_cast<uint16_t*>(block + P::kKS + ((c >> 2) * kPage + place) * 2) = half2bits(kc.s);
+        *reinterpret_cast<uint16_t*>(block + P::kVS + (((place >> 2) * P::G + (c >> 2)) * 4 + (place & 3)) * 2) = half2bits(vc.s);
+      }
+    }
+    uint8_t* mine = codes[wave];
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { lo |= vc.u[e] << (8 * e); hi |= vc.u[e + 4] << (8 * e); }
+    lds_sync_wave();  // (the last head's bytes have been read)
+    *reinterpret_cast<uint2*>(mine + j * D + 8 * c) = make_uint2(lo, hi);
+    lds_sync_wave();
+    // lane: word lane % (D / 2) of token quad lane / (D / 2)
+    constexpr int WQ = D / 2;  // words of a quad
+    const int quad = lane / WQ, l = lane % WQ, c16 = l / P::G, gr = l % P::G;
+    const int s0 = slot0 + 4 * quad - start;  // the quad's first token
+    uint32_t word = 0, put = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int tok = e & 3;
+      word |= (uint32_t)mine[(4 * quad + tok) * D + 16 * (2 * gr + e / 4) + c16] << nib4(e);
+      if (s0 + tok >= 0 && s0 + tok < count) put |= 15u << nib4(e);
+    }
+    if (put) {
+      uint32_t* dst = reinterpret_cast<uint32_t*>(block + P::kV + (((slot0 + 4 * quad) & (kPage - 1)) / 4) * (WQ * 4)) + l;
+      if (put != ~0u) word = (word & put) | (*dst & ~put);
+      *dst = word;
+    }
+  }
+}
+
+}  // namespace carekv
+
+using namespace carekv;
+
+extern "C" int64_t carekv_page4_bytes(int32_t head_dim) {
+  return head_dim == 64 ? Page4<64>::kBytes : head_dim == 128 ? Page4<128>::kBytes : -1;
+}
+
+extern "C" int carekv_append_pages(const carekv_append_params* pp, const void* q, const void* k, const void* v,
+                                   const void* positions, const double* freqs, const int32_t* start,
+                                   const int32_t* counts, const int32_t* table, void* pages, void* q_out,
+                                   void* k_hat, void* v_hat, void* stream) {
+  CAREKV_REQUIRE(pp, "null argument");
+  const carekv_append_params& p = *pp;
+  CAREKV_REQUIRE(p.head_dim == 64 || p.head_dim == 128, "head_dim must be 64 or 128");
+  CAREKV_REQUIRE(p.dtype == CAREKV_F16 || p.dtype == CAREKV_BF16, "dtype must be CAREKV_F16 or CAREKV_BF16");
+  CAREKV_REQUIRE(p.batch >= 0 && p.seq_len >= 0 && p.n_heads >= 0 && p.n_kv_heads > 0 && p.n_pages >= 0 && p.max_pages >= 0,
+                 "negative counts");
+  CAREKV_REQUIRE(p.rotary_dim >= 0 && p.rotary_dim % 2 == 0 && p.rotary_dim <= p.head_dim,
+                 "rotary_dim must be even, 0 <= rotary_dim <= head_dim");
+  CAREKV_REQUIRE(p.pos_bits == 32 || p.pos_bits == 64 || !positions, "pos_bits must be 32 or 64");
+  CAREKV_REQUIRE(p.seq_len < (1 << 29) && p.max_pages < (1 << 25), "seq_len must be below 2^29, max_pages below 2^25");
+  if (p.batch == 0 || p.seq_len == 0) return CAREKV_OK;
+  CAREKV_REQUIRE(k && v && start && (p.rotary_dim == 0 || freqs) && (p.n_heads == 0 || (q && q_out)) &&
+                     (p.max_pages == 0 || table) && (p.n_pages == 0 || pages) && !k_hat == !v_hat, "null argument");
+  CAREKV_REQUIRE((((uintptr_t)pages | (uintptr_t)k_hat | (uintptr_t)v_hat) & 15) == 0, "pages, k_hat and v_hat must be 16-byte aligned");
+  AppendArgs a{};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.qo = (char*)q_out;
+  a.k_hat = (uint16_t*)k_hat; a.v_hat = (uint16_t*)v_hat;
+  a.pos = positions; a.freqs = freqs; a.start = start; a.counts = counts; a.table = table; a.pages = (char*)pages;
+  a.pos_batch = p.pos_batch; a.table_sb = p.table_sb;
+  a.q_sb = 2 * p.q_sb; a.q_sh = 2 * p.q_sh; a.q_st = 2 * p.q_st; a.k_sb = 2 * p.k_sb; a.k_sh = 2 * p.k_sh; a.k_st = 2 * p.k_st;
+  a.v_sb = 2 * p.v_sb; a.v_sh = 2 * p.v_sh; a.v_st = 2 * p.v_st; a.o_sb = 2 * p.qo_sb; a.o_sh = 2 * p.qo_sh; a.o_st = 2 * p.qo_st;
+  const int tpw = 64 / (p.head_dim / 8);
+  a.T = p.seq_len; a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.R = p.rotary_dim; a.n_pages = p.n_pages; a.max_pages = p.max_pages;
+  a.pos64 = p.pos_bits == 64; a.interleaved = p.interleaved != 0; a.scale = p.scale;
+  a.nu = (p.seq_len + 2 * tpw - 2) / tpw;
+  uintptr_t bits = operand_bits(k, {{p.batch, a.k_sb}, {p.n_kv_heads, a.k_sh}, {p.seq_len, a.k_st}}) |
+                   operand_bits(v, {{p.batch, a.v_sb}, {p.n_kv_heads, a.v_sh}, {p.seq_len, a.v_st}});
+  if (p.n_heads)
+    bits |= operand_bits(q, {{p.batch, a.q_sb}, {p.n_heads, a.q_sh}, {p.seq_len, a.q_st}}) |
+            operand_bits(q_out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}});
+  const bool wide = (bits & 15) == 0;
+  a.partner_wide = wide && p.rotary_dim % 16 == 0;
+  const long units = (long)p.batch * a.nu;
+  CAREKV_REQUIRE(grid_fits(units, 256), "too many tokens");
+  const long heads = (long)p.n_heads + p.n_kv_heads;
+  CAREKV_REQUIRE(heads < 65536, "too many heads");
+  // walks cut until 1024 work-groups (4 a CU) are there
+  const long cuts = std::max(1L, std::min((heads + 3) / 4, 1024 / units));
+  const dim3 grid((unsigned)units, (unsigned)cuts);
+  hipStream_t s = (hipStream_t)stream;
+  const int rc = dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
+    using E = typename decltype(et)::E;
+    constexpr int D = decltype(d)::value;
+    if (wide) hipLaunchKernelGGL((append_pages_kernel<E, D, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((append_pages_kernel<E, D, false>), grid, dim3(256), 0, s, a);
+    return CAREKV_OK;
+  });
+  CAREKV_CHECK_LAUNCH("append_pages");
+  return rc;
+}

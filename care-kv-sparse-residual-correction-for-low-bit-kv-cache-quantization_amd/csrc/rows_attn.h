@@ -1,0 +1,181 @@
+// What the rows of windowed attention see (paged_attention, window_attention),
+// and how parts of their keys are joined.
+//
+// Query row t of sequence b, t < q_lengths[b], stands at position p = q_start[b]
+// + t and sees the keys j <= p, j < lengths[b], with j > p - window or j < sink.
+// The rows of a kv head are numbered r = t G + h over its G query heads, so that
+// rows next to each other see nearly the same keys.
+#pragma once
+
+#include <cmath>
+
+#include "fast_div.h"
+#include "mfma16.h"
+
+namespace carekv {
+
+constexpr int kMaxPos = 1 << 29;  // keys, query rows and the distance of q_start from 0 are below it, a window at most twice
+
+struct RowsArgs {
+  const char* q;
+  char* out;
+  float* lse;                // [B][Hq][T], or null
+  const int32_t* lengths;    // or null: max_keys
+  const int32_t* q_lengths;  // or null: T
+  const int32_t* q_start;    // or null: the rows are the sequence's last
+  float* pml;                // [nsplit][rows][2] reference (base 2), sum
+  float* po;                 // [nsplit][rows][D]
+  long q_sb, q_sh, q_st, o_sb, o_sh, o_st;  // bytes
+  long rows;                 // B * Hkv * M
+  int Hq, Hkv, G, T, M, max_keys, window, sink, nqb, nsplit, qb_rows;
+  int tps;                   // tiles of a split
+  FastDiv by_g, by_nqb, by_hkv, by_nsplit, by_m;
+  float sm_log2;             // |scale| log2(e), 1 where that is 0
+  uint32_t q_sign, q_keep;   // sign bits of two elements where the scale is negative; 0 where it is 0
+  int al8;                   // rows of out on 8 bytes
+};
+
+// Sequence b's counts, kept where sums of them stay in 32 bits.
+struct SeqRows {
+  int len, qlen, base;  // keys, rows that are no padding, position of row 0
+  __device__ __forceinline__ SeqRows(const RowsArgs& a, int b) {
+    len = a.lengths ? min(max(a.lengths[b], 0), a.max_keys) : a.max_keys;
+    qlen = a.q_lengths ? min(max(a.q_lengths[b], 0), a.T) : a.T;
+    base = a.q_start ? min(max(a.q_start[b], -kMaxPos), kMaxPos) : len - qlen;
+  }
+};
+
+// The keys that rows t0 .. t1 - 1 see between them, as tiles of KT keys: the
+// first n_sink tiles, then those from tile0 on.
+template <int KT>
+struct Span {
+  int first, last;  // positions of the first and the last row
+  int hi;           // last key that is seen
+  int n_sink, tile0, n;
+  __device__ __forceinline__ Span(const RowsArgs& a, const SeqRows& s, int t0, int t1) {
+    t1 = min(t1, s.qlen);
+    first = s.base + t0;
+    last = s.base + t1 - 1;
+    hi = min(last, s.len - 1);
+    n_sink = tile0 = n = 0;
+    if (t0 >= t1 || hi < 0) return;
+    tile0 = max(0, first - a.window + 1) / KT;
+    n_sink = min((min(a.sink, hi + 1) + KT - 1) / KT, tile0);
+    n = n_sink + max(0, hi / KT - tile0 + 1);
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : i - n_sink + tile0; }
+  // whether every row sees every key of the tile at j0
+  __device__ __forceinline__ bool whole(const RowsArgs& a, int j0) const {
+    return j0 + KT - 1 <= min(first, hi) && (j0 > last - a.window || j0 + KT <= a.sink);
+  }
+};
+
+// Position of row r, below every key where it is padding or there is none; and its bounds: the row sees key j where
+// j <= top and (j >= low or j < sink).
+struct RowSight {
+  int top, low;
+  RowSight() = default;
+  __device__ __forceinline__ RowSight(const RowsArgs& a, const SeqRows& s, int r) {
+    const int t = r / a.by_g;
+    const bool there = r < a.M && t < s.qlen;
+    top = there ? min(s.base + t, s.len - 1) : -1;
+    low = s.base + t - a.window + 1;
+  }
+  __device__ __forceinline__ bool sees(const RowsArgs& a, int j) const { return j <= top && (j >= low || j < a.sink); }
+};
+
+// Row r of kv head hk of sequence b: where its output starts, and its place in lse.
+__device__ __forceinline__ char* out_row(const RowsArgs& a, int b, int hk, int r) {
+  const int t = r / a.by_g, h = hk * a.G + r - t * a.G;
+  return a.out + b * a.o_sb + h * a.o_sh + t * a.o_st;
+}
+__device__ __forceinline__ void write_lse(const RowsArgs& a, int b, int hk, int r, float m, float l) {
+  const int t = r / a.by_g, h = hk * a.G + r - t * a.G;
+  a.lse[((long)b * a.Hq + h) * a.T + t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+// four neighbouring dims of a row, o / l (0 for a row that sees nothing)
+template <typename E>
+__device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, float4_t o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  E w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (E)(o[i] * inv);
+  E* dst = reinterpret_cast<E*>(row) + d;
+  if (a.al8) __builtin_memcpy(__builtin_assume_aligned(dst, 8), w, 8);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = w[i];
+}
+
+// The splits' partials of a row: 256 / D rows a work-group, four groups of D / 4
+// threads that take every fourth split, added up in LDS in group order.  Splits
+// behind the rows' last tile wrote nothing and are not read.
+template <typename E, int D, int KT>
+__global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
+  constexpr int D4 = D / 4, JG = 4, RW = 256 / (D4 * JG);
+  __shared__ float4_t s_o[256];
+  __shared__ float2 s_ml[RW][JG];
+  const int d4 = threadIdx.x % D4, grp = threadIdx.x / D4 % JG, rw = threadIdx.x / (D4 * JG);
+  const long pr = (long)blockIdx.x * RW + rw;
+  const bool in = pr < a.rows;
+  float m = kLowest, L = 0.f;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+  int b = 0, hk = 0, r = 0;
+  bool pad = false;
+  if (in) {
+    const int bh = (int)pr / a.by_m;
+    r = (int)pr - bh * a.M;
+    b = bh / a.by_hkv;
+    hk = bh - b * a.Hkv;
+    const SeqRows s(a, b);
+    const int r0 = r / a.qb_rows * a.qb_rows, r1 = min(r0 + a.qb_rows, a.M);
+    const Span<KT> span(a, s, r0 / a.by_g, (r1 - 1) / a.by_g + 1);
+    const int ns = (span.n + a.tps - 1) / a.tps;
+    pad = r / a.by_g >= s.qlen;
+    for (int s0 = grp; s0 < ns; s0 += 4 * JG) {  // four splits' loads in flight
+      float2 ml[4];
+      float4_t v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long at = min(s0 + u * JG, ns - 1) * a.rows + pr;
+        ml[u] = *reinterpret_cast<const float2*>(a.pml + 2 * at);
+        v[u] = *reinterpret_cast<const float4_t*>(a.po + at * D + 4 * d4);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u * JG >= ns) break;
+        const float mn = fmaxf(m, ml[u].x), f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[u].x - mn);
+        o = o * f + v[u] * e;
+        L = L * f + ml[u].y * e;
+        m = mn;
+      }
+    }
+  }
+  s_o[threadIdx.x] = o;
+  if (d4 == 0) s_ml[rw][grp] = make_float2(m, L);
+  __syncthreads();
+  if (!in || grp != 0) return;
+  float mm = kLowest, LL = 0.f;
+  float4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < JG; ++i) mm = fmaxf(mm, s_ml[rw][i].x);
+#pragma unroll
+  for (int i = 0; i < JG; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_ml[rw][i].x - mm);
+    LL += s_ml[rw][i].y * f;
+    O += s_o[(rw * JG + i) * D4 + d4] * f;
+  }
+  if (pad) { LL = 0.f; O = float4_t{0.f, 0.f, 0.f, 0.f}; }  // (what a row of padding holds is not used)
+  write4<E>(a, out_row(a, b, hk, r), 4 * d4, O, LL);
+  if (a.lse && d4 == 0) write_lse(a, b, hk, r, mm, LL);
+}
+
+// The scale as the kernels take it.
+inline void set_scale(RowsArgs& a, float scale) {
+  a.sm_log2 = (float)(std::fabs((double)scale) * 1.4426950408889634074);
+  a.q_sign = scale < 0.f ? 0x80008000u : 0u;
+  a.q_keep = a.sm_log2 == 0.f ? 0u : ~0u;
+  if (a.sm_log2 == 0.f) a.sm_log2 = 1.f;
+}
+
+}  // namespace carekv

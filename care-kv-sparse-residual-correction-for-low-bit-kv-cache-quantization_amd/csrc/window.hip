@@ -1,0 +1,427 @@
+// Attention of (ragged) prompts and single tokens over 16-bit rows, inside a
+// window and over the first tokens (window_attention):
+//   o = sum_j e^(s_j) v_j / sum_j e^(s_j), s_j = scale q . k_j,
+// over the keys that the row sees (rows_attn.h).
+//
+// A work-group has 128 rows of a kv head (4 waves of 32; all query heads of a
+// token side by side, so that their keys are the same) and walks over the tiles
+// of 32 keys that any of them sees: K and V in LDS (double buffered, one barrier
+// a tile), S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32, the softmax
+// over a query's column in 32 bits on base-2 logits.  The weights are rounded to
+// the element type for the second product (half a step, 2^-11 or 2^-8; their sum
+// is not); in fp16 against a reference 15 below the row's maximum, so that a
+// weight of 2^-29 of the largest is still normal.  Masks are applied where a
+// wave's tile has a key that some row of the wave does not see, tiles that none
+// sees are left out.  Up to 32 rows: the four waves split a tile of 128 keys.
+// Where work-groups are few the tiles are split over more of them and joined.
+#include <algorithm>
+#include <cmath>
+
+#include "host_util.h"
+#include "rows_attn.h"
+
+namespace carekv {
+
+struct WindowArgs : RowsArgs {
+  const char* k;
+  const char* v;
+  long k_sb, k_sh, k_st, v_sb, v_sh, v_st;  // bytes
+};
+
+// Whether one of two elements is infinite or no number: its exponent's bits all set.
+template <typename ET>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
+  constexpr uint32_t e = std::is_same<typename ET::E, _Float16>::value ? 0x7c007c00u : 0x7f807f80u, one = e & (~e << 1);
+  return ((x & e) + one) & 0x80008000u;
+}
+
+template <typename ET, int D, int WQ, int WK>
+__global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_kernel(WindowArgs a) {
+  using V8 = typename ET::V8;
+  using E = typename ET::E;
+  constexpr int NT = 64 * WQ * WK, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
+  constexpr int KRS = 2 * D + 32, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
+  constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / NT;
+  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WQ == 4 ? 2 : 1;
+  __shared__ __align__(16) char lds[NBUF * BUF];
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) short4_t lds_short4;
+
+  const int n = gridDim.x;
+  int it = blockIdx.x;
+  it = n / 8 * (it & 7) + min(it & 7, n & 7) + (it >> 3);  // an XCD takes consecutive items: blocks of the same keys
+  const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
+  const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
+  const int b = bh / a.by_hkv, hk = bh - b * a.Hkv;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int wq = w % WQ, wk = w / WQ, r0 = qblk * QB + QW * wq;  // the wave's share of rows and keys, its first row
+  const SeqRows seq(a, b);
+  const int b0 = qblk * QB, b1 = min(b0 + QB, a.M);
+  const Span<KT> span(a, seq, b0 / a.by_g, (b1 - 1) / a.by_g + 1);
+  const int w1 = min(r0 + QW, a.M);
+  const Span<32> mine(a, seq, r0 / a.by_g, w1 > r0 ? (w1 - 1) / a.by_g + 1 : 0);
+  const int i0 = sp * a.tps, i1 = min(i0 + a.tps, span.n), nt = i1 - i0;
+  if (a.nsplit > 1 && nt <= 0) return;  // (the join does not read it)
+  const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
+  const char* vbase = a.v + b * a.v_sb + hk * a.v_sh;
+
+  // Q^T operands: sub-block qb, step s -> row r0 + 16 qb + c16, dims 32s + 8g ..; negated for a negative scale
+  V8 qf[NQ][KS];
+  RowSight sight[NQ];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    sight[qb] = RowSight(a, seq, r0 + 16 * qb + c16);
+    const int r = min(r0 + 16 * qb + c16, a.M - 1), t = r / a.by_g, h = hk * a.G + r - t * a.G;
+    const char* qp = a.q + b * a.q_sb + h * a.q_sh + t * a.q_st;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint4 v = *reinterpret_cast<const uint4*>(qp + (32 * s + 8 * g) * 2);
+      v.x = (v.x ^ a.q_sign) & a.q_keep; v.y = (v.y ^ a.q_sign) & a.q_keep;
+      v.z = (v.z ^ a.q_sign) & a.q_keep; v.w = (v.w ^ a.q_sign) & a.q_keep;
+      __builtin_memcpy(&qf[qb][s], &v, 16);
+    }
+  }
+
+  uint32_t stg[NCH][4];
+  const int srow = threadIdx.x / CHR, scol = threadIdx.x % CHR * 16;  // (chunk k: row srow + NT / CHR k of K, then V)
+  uint32_t off[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+    off[k] = (uint32_t)((srow + NT / CHR * (k % (NCH / 2))) * (k < NCH / 2 ? a.k_st : a.v_st) + scol);
+  // A tile is a buffer resource of its rows, a thread's offsets in it stay the same; rows past the length read zeros.
+  auto load_tile = [&](int i) {
+    const int j0 = span.tile(i0 + i) * KT, last = min(KT, seq.len - j0) - 1;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + (long)j0 * a.k_st, (uint32_t)(last * a.k_st + 2 * D));
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vbase + (long)j0 * a.v_st, (uint32_t)(last * a.v_st + 2 * D));
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(k < NCH / 2 ? rk : rv, off[k], 0, 0);
+      stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
+    }
+  };
+  auto store_tile = [&](int buf) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int row = srow + NT / CHR * (k % (NCH / 2));
+      char* dst = lds + buf * BUF + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + scol;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
+    }
+  };
+
+  float m_run[NQ], l_run[NQ];
+  float4_t o[NQ][DT];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    m_run[qb] = kLowest;
+    l_run[qb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const float c = a.sm_log2;  // (not negative)
+  if (nt > 0) {
+    load_tile(0);
+    store_tile(0);
+  }
+  __syncthreads();
+  if (nt > 1) load_tile(1);
+  for (int i = 0; i < nt; ++i) {
+    const int jw = span.tile(i0 + i) * KT + 32 * wk;  // the wave's first key of the tile
+    const char* kb = lds + (NBUF == 2 ? (i & 1) * BUF : 0) + 32 * wk * KRS;
+    const char* vb = lds + (NBUF == 2 ? (i & 1) * BUF : 0) + KBUF + 32 * wk * VRS;
+    if (mine.n > 0 && jw <= mine.hi && (jw + 31 > mine.first - a.window || jw < a.sink)) {
+      // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
+      __builtin_amdgcn_s_setprio(1);
+      float4_t s[TT][NQ];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          V8 ak;
+          *reinterpret_cast<uint4*>(&ak) = *reinterpret_cast<const uint4*>(kb + (16 * tt + c16) * KRS + (32 * ks + 8 * g) * 2);
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = ET::mfma(ak, qf[qb][ks], s[tt][qb]);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      const bool whole = mine.whole(a, jw);
+      if (!whole) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb)
+              if (!sight[qb].sees(a, jw + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
+      }
+      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
+      float mx[NQ];
+      bool any_over = false, over[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
+        mx[qb] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
+        over[qb] = fmaf(mx[qb], c, -ET::kUp) > m_run[qb];
+        any_over |= over[qb];
+      }
+      if (__any(any_over)) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
+          const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c, -ET::kUp));
+          const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+          m_run[qb] = m_new;
+          l_run[qb] *= f;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
+        }
+      }
+      V8 bp[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
+        float ls = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[k / 4][qb][k % 4], c, -m_run[qb]));
+          ls += p;
+          bp[qb][k] = (E)p;
+        }
+        l_run[qb] += ls;
+      }
+      const __attribute__((address_space(3))) char* vrow =
+          (const __attribute__((address_space(3))) char*)vb + (4 * g + (c16 >> 2)) * VRS + (c16 & 3) * 8;
+      auto v_operand = [&](int dt) {
+        const short4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrow + 32 * dt));
+        const short4_t v2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrow + 16 * VRS + 32 * dt));
+        V8 av;
+        __builtin_memcpy(&av, &v1, 8);
+        __builtin_memcpy(reinterpret_cast<char*>(&av) + 8, &v2, 8);
+        return av;
+      };
+      uint32_t odd = 0;
+      if (!whole) {  // a masked weight of 0 times an infinite value would be no number
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const V8 av = v_operand(dt);
+          uint32_t x[4];
+          __builtin_memcpy(x, &av, 16);
+          odd |= not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]) | not_finite2<ET>(x[2]) | not_finite2<ET>(x[3]);
+        }
+      }
+      if (__builtin_expect(__any(odd != 0), 0)) {
+        // key by key, into the rows that see it alone
+        for (int kg = 0; kg < 4; ++kg) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int key = 16 * (k / 4) + 4 * kg + k % 4;
+            float p[NQ];
+            bool see[NQ];
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb) {
+              p[qb] = __shfl((float)bp[qb][k], 16 * kg + c16, 64);
+              see[qb] = sight[qb].sees(a, jw + key);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              E v[4];
+              __builtin_memcpy(v, vb + key * VRS + (16 * dt + 4 * g) * 2, 8);
+#pragma unroll
+              for (int qb = 0; qb < NQ; ++qb)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[qb][dt][x] = see[qb] ? fmaf(p[qb], (float)v[x], o[qb][dt][x]) : o[qb][dt][x];
+            }
+          }
+        }
+      } else {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const V8 av = v_operand(dt);
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
+        }
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (NBUF == 1) __syncthreads();
+    if (i + 1 < nt) store_tile(NBUF == 2 ? (i + 1) & 1 : 0);
+    if (i + 2 < nt) load_tile(i + 2);
+    __syncthreads();
+  }
+  float lt[NQ];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) lt[qb] = col_sum(l_run[qb]);
+  if constexpr (WK > 1) {
+    // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum, 16 rows at a time
+    // in the tiles' LDS, added in wave order; a wave keeps the dims of tiles wk, wk + WK ..
+    __shared__ float s_ml[WK][QB][2];
+    float* so = reinterpret_cast<float*>(lds);  // [waves][DT][64 lanes][4]
+    static_assert(WQ * WK * DT * 1024 <= NBUF * BUF, "the waves' O fits the tiles' LDS");
+    const int rr = QW * wq + c16;
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb)
+      if (g == 0) { s_ml[wk][16 * qb + rr][0] = m_run[qb]; s_ml[wk][16 * qb + rr][1] = lt[qb]; }
+    __syncthreads();
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+      float m = kLowest, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + rr][0]);
+#pragma unroll
+      for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + rr][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + rr][0] - m);
+      const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((w * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
+      m_run[qb] = m;
+      lt[qb] = l;
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < (DT + WK - 1) / WK; ++u) {
+        const int dt = wk + WK * u;
+        if (dt >= DT) break;
+        float4_t v = *reinterpret_cast<const float4_t*>(so + ((wq * DT + dt) * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + (((i * WQ + wq) * DT + dt) * 64 + lane) * 4);
+        o[qb][u] = v;
+      }
+      __syncthreads();
+    }
+  }
+  // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
+  constexpr int OT = (DT + WK - 1) / WK;
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    const int r = r0 + 16 * qb + c16;
+    if (r >= a.M) continue;
+    const bool first = g == 0 && wk == 0;
+    if (a.nsplit == 1) {
+      const bool pad = sight[qb].top < 0;  // (what a row of padding holds is not used)
+      const float l = pad ? 0.f : lt[qb];
+      char* row = out_row(a, b, hk, r);
+#pragma unroll
+      for (int u = 0; u < OT; ++u)
+        if (wk + WK * u < DT) write4<E>(a, row, 16 * (wk + WK * u) + 4 * g, pad ? float4_t{0.f, 0.f, 0.f, 0.f} : o[qb][u], l);
+      if (a.lse && first) write_lse(a, b, hk, r, m_run[qb], l);
+    } else {
+      const long pr = (long)sp * a.rows + (long)bh * a.M + r;
+      float* dst = a.po + pr * D + 4 * g;
+#pragma unroll
+      for (int u = 0; u < OT; ++u)
+        if (wk + WK * u < DT) *reinterpret_cast<float4_t*>(dst + 16 * (wk + WK * u)) = o[qb][u];
+      if (first) {
+        a.pml[2 * pr] = m_run[qb];
+        a.pml[2 * pr + 1] = lt[qb];
+      }
+    }
+  }
+}
+
+namespace {
+// How a call is cut: at most 32 rows a kv head share the work-group's waves by
+// keys (wq = 1, wk = 4), more by rows; key splits, each of at least 4 tiles, until
+// 768 work-groups (3 a CU) are there.
+struct WindowPlan {
+  int wq, wk, nqb, nsplit, tps;
+};
+WindowPlan window_plan(const carekv_window_params& p) {
+  WindowPlan r{};
+  const long M = (long)p.seq_len * (p.n_heads / p.n_kv_heads);
+  r.wq = M <= 32 ? 1 : 4;
+  r.wk = M <= 32 ? 4 : 1;
+  r.nqb = (int)((M + 32 * r.wq - 1) / (32 * r.wq));
+  const int kt = 32 * r.wk;
+  long keys = p.n_keys;  // that a block of rows may see
+  if (p.window > 0) keys = std::min(keys, (long)p.window + std::min<long>(p.seq_len, 32L * r.wq) + p.sink + 2 * kt);
+  const long tiles = std::max(1L, (keys + kt - 1) / kt), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
+  const long ns = tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
+  r.tps = (int)((tiles + ns - 1) / ns);
+  r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
+  return r;
+}
+long window_ws(const carekv_window_params& p, const WindowPlan& r) {
+  const long rows = (long)p.batch * p.seq_len * p.n_heads;
+  return r.nsplit > 1 ? r.nsplit * rows * (2 + p.head_dim) * 4 : 0;
+}
+int check_window(const carekv_window_params* pp) {
+  CAREKV_REQUIRE(pp, "null argument");
+  const carekv_window_params& p = *pp;
+  CAREKV_REQUIRE(p.head_dim == 64 || p.head_dim == 128, "head_dim must be 64 or 128");
+  CAREKV_REQUIRE(p.dtype == CAREKV_F16 || p.dtype == CAREKV_BF16, "dtype must be CAREKV_F16 or CAREKV_BF16");
+  CAREKV_REQUIRE(p.batch >= 0 && p.seq_len >= 0 && p.n_keys >= 0 && p.window >= 0 && p.sink >= 0, "negative counts");
+  CAREKV_REQUIRE(p.n_heads > 0 && p.n_kv_heads > 0 && p.n_heads % p.n_kv_heads == 0,
+                 "n_heads must be a positive multiple of n_kv_heads");
+  CAREKV_REQUIRE((long)p.batch * p.seq_len * p.n_heads < (1L << 30), "too many rows");
+  CAREKV_REQUIRE(p.n_keys < kMaxPos && p.seq_len < kMaxPos, "n_keys and seq_len must be below 2^29");
+  CAREKV_REQUIRE(p.n_keys < 2 || (p.k_st >= 0 && p.v_st >= 0 && p.k_st < (1 << 22) && p.v_st < (1 << 22)),
+                 "K and V row strides must be in 0 .. 2^22 elements");
+  return CAREKV_OK;
+}
+}  // namespace
+
+}  // namespace carekv
+
+using namespace carekv;
+
+extern "C" int64_t carekv_window_attn_workspace_bytes(const carekv_window_params* pp) {
+  if (check_window(pp) != CAREKV_OK) return -1;
+  return window_ws(*pp, window_plan(*pp));
+}
+
+extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q, const void* k, const void* v,
+                                  const int32_t* lengths, const int32_t* q_lengths, const int32_t* q_start, void* out,
+                                  float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_window(pp);
+  if (rc != CAREKV_OK) return rc;
+  const carekv_window_params& p = *pp;
+  const long rows = (long)p.batch * p.seq_len * p.n_heads;
+  if (rows == 0) return CAREKV_OK;
+  const WindowPlan plan = window_plan(p);
+  CAREKV_REQUIRE(q && out && (p.n_keys == 0 || (k && v)) && (workspace || plan.nsplit < 2), "null argument");
+  const uintptr_t bits = operand_bits(q, {{p.batch, 2 * p.q_sb}, {p.n_heads, 2 * p.q_sh}, {p.seq_len, 2 * p.q_st}}) |
+                         operand_bits(k, {{p.batch, 2 * p.k_sb}, {p.n_kv_heads, 2 * p.k_sh}, {p.n_keys, 2 * p.k_st}}) |
+                         operand_bits(v, {{p.batch, 2 * p.v_sb}, {p.n_kv_heads, 2 * p.v_sh}, {p.n_keys, 2 * p.v_st}}) |
+                         (uintptr_t)workspace;
+  CAREKV_REQUIRE((bits & 15) == 0, "q, k and v rows must be 16-byte aligned");
+  if (workspace_bytes < window_ws(p, plan)) {
+    set_error("carekv_window_attn: workspace too small (%lld < %lld)", (long long)workspace_bytes, (long long)window_ws(p, plan));
+    return CAREKV_ESPACE;
+  }
+  WindowArgs a{};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)out; a.lse = lse;
+  a.lengths = lengths; a.q_lengths = q_lengths; a.q_start = q_start;
+  a.q_sb = 2 * p.q_sb; a.q_sh = 2 * p.q_sh; a.q_st = 2 * p.q_st; a.o_sb = 2 * p.out_sb; a.o_sh = 2 * p.out_sh; a.o_st = 2 * p.out_st;
+  a.k_sb = 2 * p.k_sb; a.k_sh = 2 * p.k_sh; a.k_st = 2 * p.k_st; a.v_sb = 2 * p.v_sb; a.v_sh = 2 * p.v_sh; a.v_st = 2 * p.v_st;
+  a.Hq = p.n_heads; a.Hkv = p.n_kv_heads; a.G = p.n_heads / p.n_kv_heads; a.T = p.seq_len; a.M = a.G * p.seq_len;
+  a.rows = rows; a.max_keys = p.n_keys;
+  a.window = p.window > 0 ? std::min(p.window, 2 * kMaxPos) : 2 * kMaxPos;
+  a.sink = p.sink;
+  a.nqb = plan.nqb; a.nsplit = plan.nsplit; a.tps = plan.tps; a.qb_rows = 32 * plan.wq;
+  a.by_g = FastDiv(a.G); a.by_nqb = FastDiv(a.nqb); a.by_hkv = FastDiv(a.Hkv); a.by_nsplit = FastDiv(a.nsplit); a.by_m = FastDiv(a.M);
+  a.po = (float*)workspace;
+  a.pml = a.po + plan.nsplit * rows * p.head_dim;
+  set_scale(a, p.sm_scale);
+  a.al8 = (operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}}) & 7) == 0;
+  hipStream_t s = (hipStream_t)stream;
+  const long wgs = (long)p.batch * a.Hkv * a.nqb * a.nsplit;
+  CAREKV_REQUIRE(grid_fits(wgs, 256) && grid_fits(rows / (256 / p.head_dim) + 1, 256), "too many rows");
+  return dispatch_elem_d(p.dtype, p.head_dim, [&](auto et, auto d) {
+    using ET = decltype(et);
+    constexpr int D = decltype(d)::value;
+    const dim3 grid((unsigned)wgs), block(256);
+    if (plan.wq == 1) hipLaunchKernelGGL((window_attn_kernel<ET, D, 1, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((window_attn_kernel<ET, D, 4, 1>), grid, block, 0, s, a);
+    CAREKV_CHECK_LAUNCH("window_attn");
+    if (a.nsplit > 1) {
+      constexpr int RW = 256 / D;
+      const dim3 jg((unsigned)((rows + RW - 1) / RW));
+      if (plan.wk == 4) hipLaunchKernelGGL((rows_join_kernel<typename ET::E, D, 128>), jg, dim3(256), 0, s, (RowsArgs)a);
+      else hipLaunchKernelGGL((rows_join_kernel<typename ET::E, D, 32>), jg, dim3(256), 0, s, (RowsArgs)a);
+      CAREKV_CHECK_LAUNCH("rows_join");
+    }
+    return CAREKV_OK;
+  });
+}

@@ -657,6 +657,98 @@ int carekv_prefix_attn(const carekv_prefix_params* params, const void* q, const 
                        int64_t workspace_bytes, void* stream);
 int64_t carekv_prefix_attn_workspace_bytes(const carekv_prefix_params* params);
 
+/* Pages of 4-bit rows: a page holds 16 tokens of a sequence, a block of
+ * carekv_page4_bytes(head_dim) bytes for each of its n_kv_heads.  Of a row every
+ * 32 values x (fp16) are kept as s = half(max|x| / 7) and c = clamp(rint(half(x
+ * / s)), -8, 7), c = 0 where x / s is 0 / 0, and stand for half(c s); a group
+ * with a value that is not finite stands for NaN.  Page tables: device int32
+ * [batch][max_pages], entry i of a sequence the page of its tokens 16 i ..; an
+ * entry outside 0 .. n_pages - 1 is a page that is not there: what is appended
+ * to it is dropped, its tokens are seen by no row. */
+int64_t carekv_page4_bytes(int32_t head_dim); /* head_dim 64 or 128, else -1   */
+
+/* seq_len new tokens of every sequence, the first counts[b] of them (NULL:
+ * seq_len) written behind its start[b] tokens: token t to place start[b] + t.
+ * q [batch][n_heads][seq_len][head_dim] and k (n_kv_heads) are turned as by
+ * carekv_rotate_heads, at positions (device int32 or int64, NULL: start[b] + t),
+ * in 64 bits, rounded to 32 and then to the type (q_out) or fp16 (k); rotary_dim
+ * 0: not at all.  n_heads 0: no q.  k_hat, v_hat (both or neither): fp16 [batch]
+ * [n_kv_heads][seq_len][head_dim], the values that the new rows stand for, 0
+ * behind the counts.  fp16 or bf16, strides in elements, pages, k_hat and v_hat
+ * 16-byte aligned.  No two sequences of a call may write to one page. */
+typedef struct carekv_append_params {
+  int32_t batch, n_heads, n_kv_heads, seq_len, head_dim, rotary_dim;
+  int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
+  int32_t interleaved, pos_bits, n_pages, max_pages;
+  float scale;             /* on the turned values                             */
+  int64_t pos_batch;       /* elements; 0: one row of positions for all        */
+  int64_t table_sb;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, qo_sb, qo_sh, qo_st;
+} carekv_append_params;
+
+int carekv_append_pages(const carekv_append_params* params, const void* q, const void* k, const void* v,
+                        const void* positions, const double* freqs, const int32_t* start, const int32_t* counts,
+                        const int32_t* table, void* pages, void* q_out, void* k_hat, void* v_hat, void* stream);
+
+/* Attention of the rows of q [batch][n_heads][seq_len][head_dim] over their
+ * sequence's pages.  lengths[b]: its tokens, those of q among them; row t <
+ * q_lengths[b] (NULL: seq_len) is token p = lengths[b] - q_lengths[b] + t and
+ * sees the tokens j <= p with j > p - window (0: no bound) or j < sink.  Rows of
+ * padding and rows that see nothing are 0, their log-sum-exp (lse, optional:
+ * fp32 [batch][n_heads][seq_len]) -inf; what places that a row does not see
+ * hold is not used.  Strides in elements, rows of q 16-byte aligned. */
+typedef struct carekv_paged_params {
+  int32_t batch, n_heads, n_kv_heads, seq_len, head_dim;
+  int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
+  int32_t n_pages, max_pages, window, sink;
+  float sm_scale;
+  int64_t table_sb;
+  int64_t q_sb, q_sh, q_st, out_sb, out_sh, out_st;
+} carekv_paged_params;
+
+int carekv_paged_attn(const carekv_paged_params* params, const void* q, const void* pages, const int32_t* table,
+                      const int32_t* lengths, const int32_t* q_lengths, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int64_t carekv_paged_attn_workspace_bytes(const carekv_paged_params* params);
+
+/* The same over 16-bit rows k, v [batch][n_kv_heads][n_keys][head_dim] of q's
+ * type: lengths NULL: n_keys; row t stands at q_start[b] + t (NULL: the rows are
+ * the sequence's last).  Rows of q, k and v 16-byte aligned. */
+typedef struct carekv_window_params {
+  int32_t batch, n_heads, n_kv_heads, seq_len, n_keys, head_dim;
+  int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
+  int32_t window, sink;
+  float sm_scale;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, out_sb, out_sh, out_st;
+} carekv_window_params;
+
+int carekv_window_attn(const carekv_window_params* params, const void* q, const void* k, const void* v,
+                       const int32_t* lengths, const int32_t* q_lengths, const int32_t* q_start, void* out, float* lse,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int64_t carekv_window_attn_workspace_bytes(const carekv_window_params* params);
+
+/* Drafted tokens x_t = draft[b][t], t < counts[b] (NULL: n_drafts), against the
+ * model's probabilities target_probs [batch][n_drafts + 1][vocab] and those that
+ * they were drawn from, draft_probs [batch][n_drafts][vocab] (NULL: all of q_t on
+ * x_t): x_t is accepted while u[b][t] q_t(x_t) < p_t(x_t); behind the n accepted
+ * ones, tokens[b][n] is the smallest i with w_0 + .. + w_i > u_next[b] sum(w), w =
+ * max(p_n - q_n, 0) where x_n was rejected and any of it is over 0, else p_n (-1
+ * if none of that is; the last i with a weight for u_next >= 1).  tokens int32
+ * [batch][n_drafts + 1], -1 behind them, accepted int32 [batch].  Products and
+ * sums are 64 bits; weights that are NaN or below 0 count as 0, a token outside
+ * the vocabulary is rejected.  Strides in elements, the values of a row next to
+ * each other. */
+typedef struct carekv_verify_params {
+  int32_t batch, n_drafts, vocab;
+  int32_t dtype;           /* of both probabilities: CAREKV_F16, _BF16 or _F32 */
+  int64_t target_sb, target_st, draft_probs_sb, draft_probs_st, draft_sb, u_sb;
+} carekv_verify_params;
+
+int carekv_verify_drafts(const carekv_verify_params* params, const int64_t* draft, const void* target_probs,
+                         const void* draft_probs, const float* u, const float* u_next, const int32_t* counts,
+                         int32_t* tokens, int32_t* accepted, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t carekv_verify_drafts_workspace_bytes(const carekv_verify_params* params);
+
 const char* carekv_last_error(void);
 
 #ifdef __cplusplus
