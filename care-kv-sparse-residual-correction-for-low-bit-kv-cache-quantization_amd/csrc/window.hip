@@ -44,6 +44,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / NT;
   constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WQ == 4 ? 2 : 1;
   __shared__ __align__(16) char lds[NBUF * BUF];
+  __shared__ int s_odd[NBUF];  // the last tile in the buffer that held a V value that is not finite
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
 
@@ -101,7 +102,25 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
       stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
     }
   };
-  auto store_tile = [&](int buf) {
+  // (a masked weight of 0 times a value that is not finite would be no number: such a value is 0 in the tile, its tile
+  // noted and its rows' results set from the value itself)
+  auto store_tile = [&](int i) {
+    const int buf = NBUF == 2 ? i & 1 : 0;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int k = NCH / 2; k < NCH; ++k)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) odd |= not_finite2<ET>(stg[k][x]);
+    if (__builtin_expect(odd != 0, 0)) {
+      s_odd[buf] = i;
+#pragma unroll
+      for (int k = NCH / 2; k < NCH; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t n = not_finite2<ET>(stg[k][x]);
+          stg[k][x] &= (n & 0x8000u ? 0u : 0xffffu) | (n >> 31 ? 0u : 0xffff0000u);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int row = srow + NT / CHR * (k % (NCH / 2));
@@ -120,6 +139,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   const float c = a.sm_log2;  // (not negative)
+  if (threadIdx.x < NBUF) s_odd[threadIdx.x] = -1;
+  __syncthreads();
   if (nt > 0) {
     load_tile(0);
     store_tile(0);
@@ -194,61 +215,43 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
       }
       const __attribute__((address_space(3))) char* vrow =
           (const __attribute__((address_space(3))) char*)vb + (4 * g + (c16 >> 2)) * VRS + (c16 & 3) * 8;
-      auto v_operand = [&](int dt) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
         const short4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrow + 32 * dt));
         const short4_t v2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vrow + 16 * VRS + 32 * dt));
         V8 av;
         __builtin_memcpy(&av, &v1, 8);
         __builtin_memcpy(reinterpret_cast<char*>(&av) + 8, &v2, 8);
-        return av;
-      };
-      uint32_t odd = 0;
-      if (!whole) {  // a masked weight of 0 times an infinite value would be no number
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const V8 av = v_operand(dt);
-          uint32_t x[4];
-          __builtin_memcpy(x, &av, 16);
-          odd |= not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]) | not_finite2<ET>(x[2]) | not_finite2<ET>(x[3]);
-        }
+        for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
       }
-      if (__builtin_expect(__any(odd != 0), 0)) {
-        // key by key, into the rows that see it alone
-        for (int kg = 0; kg < 4; ++kg) {
+      if (__builtin_expect(s_odd[NBUF == 2 ? i & 1 : 0] == i, 0)) {
+        // values that are not finite, from where they came, into the rows that see them: with a weight over 0 they
+        // are the result whatever it is
+#pragma unroll 1
+        for (int key = 0; key < min(32, seq.len - jw); ++key) {
+          const char* src = vbase + (long)(jw + key) * a.v_st + 8 * g;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int key = 16 * (k / 4) + 4 * kg + k % 4;
-            float p[NQ];
-            bool see[NQ];
+          for (int dt = 0; dt < DT; ++dt) {
+            asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
+            uint32_t x[2];
+            __builtin_memcpy(x, __builtin_assume_aligned(src + 32 * dt, 8), 8);
+            if (!(not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]))) continue;
+            E v[4];
+            __builtin_memcpy(v, x, 8);
 #pragma unroll
-            for (int qb = 0; qb < NQ; ++qb) {
-              p[qb] = __shfl((float)bp[qb][k], 16 * kg + c16, 64);
-              see[qb] = sight[qb].sees(a, jw + key);
-            }
+            for (int qb = 0; qb < NQ; ++qb)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              E v[4];
-              __builtin_memcpy(v, vb + key * VRS + (16 * dt + 4 * g) * 2, 8);
-#pragma unroll
-              for (int qb = 0; qb < NQ; ++qb)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[qb][dt][x] = see[qb] ? fmaf(p[qb], (float)v[x], o[qb][dt][x]) : o[qb][dt][x];
-            }
+              for (int y = 0; y < 4; ++y)
+                if (sight[qb].sees(a, jw + key) && !(fabsf((float)v[y]) < INFINITY)) o[qb][dt][y] += (float)v[y];
           }
-        }
-      } else {
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const V8 av = v_operand(dt);
-#pragma unroll
-          for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
         }
       }
     }
     __builtin_amdgcn_s_setprio(0);
     if (NBUF == 1) __syncthreads();
-    if (i + 1 < nt) store_tile(NBUF == 2 ? (i + 1) & 1 : 0);
+    if (i + 1 < nt) store_tile(i + 1);
     if (i + 2 < nt) load_tile(i + 2);
     __syncthreads();
   }
