@@ -64,9 +64,10 @@ def verify_drafts(draft: torch.Tensor, target_probs: torch.Tensor, u: torch.Tens
         nbytes = lib.carekv_verify_drafts_workspace_bytes(pp)
         if nbytes < 0:
             _lib.check(-1, "carekv_verify_drafts_workspace_bytes")
-        ws = p.new_empty(nbytes, dtype=torch.uint8)
+        ws = p.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         ct = _lib.row_counts(counts, B, dev, "counts")
         _lib.call(dev, "carekv_verify_drafts", lib.carekv_verify_drafts, pp, draft.data_ptr(), p.data_ptr(),
                   None if q is None else q.data_ptr(), u.data_ptr(), u_next.data_ptr(),
-                  None if ct is None else ct.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nbytes)
+                  None if ct is None else ct.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
+                  None if ws is None else ws.data_ptr(), nbytes)
     return VerifiedDrafts(tokens, accepted)

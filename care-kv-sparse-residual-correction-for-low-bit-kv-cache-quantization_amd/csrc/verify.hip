@@ -7,8 +7,10 @@
 // between tokens by 2^-50 of the sum, in 32 bits by as much as a token holds.
 //
 // Bound by reading the one row of p and q that the next token is drawn from.  A
-// row is cut over work-groups, which add up their parts; a second launch finds
-// the part and the place in it.
+// row is cut into segments of 1024 values, whose sums a wave takes each; from the
+// segments' sums one wave finds the segment and then the place in it.  Short rows
+// and large batches do both in one work-group a sequence, few long rows in two
+// launches, the first over the whole GPU.
 #include <algorithm>
 
 #include "common.h"
@@ -25,19 +27,21 @@ struct VerifyArgs {
   const int32_t* counts; // or null
   int32_t* tokens;       // [B][T + 1]
   int32_t* accepted;     // [B]
-  double* sums;          // [B][parts][2]: of max(p - q, 0), of p
+  double2* sums;         // [B][segs]: of max(p - q, 0), of p; null: kept in LDS
   long p_sb, p_st, q_sb, q_st, draft_sb, u_sb;  // elements
-  int T, V, parts, step; // a part is step values
+  int T, V, segs;
 };
 
-// How many of sequence b's tokens are accepted, by the work-group's first wave, to all of its threads.
+constexpr int kSeg = 1024;      // values of a segment
+constexpr int kSegsInLds = 512; // at most
+
+// How many of sequence b's tokens are accepted (every wave for itself).
 template <typename E>
 __device__ __forceinline__ int count_accepted(const VerifyArgs& a, int b, int count) {
-  __shared__ int s_n;
-  if (threadIdx.x < 64) {
+  {
     int n = 0;
     for (; n < count; n += 64) {
-      const int t = n + threadIdx.x;
+      const int t = n + (threadIdx.x & 63);
       bool ok = false;
       if (t < count) {
         const long x = a.draft[b * a.draft_sb + t];
@@ -53,10 +57,8 @@ __device__ __forceinline__ int count_accepted(const VerifyArgs& a, int b, int co
         break;
       }
     }
-    if (threadIdx.x == 0) s_n = min(n, count);
+    return min(n, count);
   }
-  __syncthreads();
-  return s_n;
 }
 
 // The weights of row n: max(p - q, 0) and p, 0 where they are not over 0.
@@ -72,10 +74,13 @@ struct Weights {
     if (a.q) q = reinterpret_cast<const E*>(a.q) + b * a.q_sb + n * a.q_st;
     else x = a.draft[b * a.draft_sb + n];
   }
-  __device__ __forceinline__ void at(int i, double& r, double& w) const {
-    const double v = (double)(float)p[i], d = q ? v - (double)(float)q[i] : i == x ? 0.0 : v;
+  __device__ __forceinline__ void of(int i, double v, double less, double& r, double& w) const {
+    const double d = i == x ? 0.0 : v - less;
     w = v > 0.0 ? v : 0.0;
     r = rest ? (d > 0.0 ? d : 0.0) : w;
+  }
+  __device__ __forceinline__ void at(int i, double& r, double& w) const {
+    of(i, (double)(float)p[i], q ? (double)(float)q[i] : 0.0, r, w);
   }
 };
 
@@ -85,123 +90,154 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return v;
 }
 
+// The sums of segment seg, by a wave: sixteen loads of each row in flight.
+template <typename E>
+__device__ __forceinline__ double2 segment_sums(const VerifyArgs& a, const Weights<E>& w, int seg) {
+  const int lane = threadIdx.x & 63, i0 = seg * kSeg + lane;
+  double r = 0.0, s = 0.0;
+  if (i0 - lane + kSeg <= a.V) {
+    E p[kSeg / 64], q[kSeg / 64];
+#pragma unroll
+    for (int k = 0; k < kSeg / 64; ++k) p[k] = w.p[i0 + 64 * k];
+    if (w.q)
+#pragma unroll
+      for (int k = 0; k < kSeg / 64; ++k) q[k] = w.q[i0 + 64 * k];
+#pragma unroll
+    for (int k = 0; k < kSeg / 64; ++k) {
+      double x, y;
+      w.of(i0 + 64 * k, (double)(float)p[k], w.q ? (double)(float)q[k] : 0.0, x, y);
+      r += x;
+      s += y;
+    }
+  } else {
+    for (int i = i0; i < a.V; i += 64) {
+      double x, y;
+      w.at(i, x, y);
+      r += x;
+      s += y;
+    }
+  }
+  return make_double2(wave_sum_d(r), wave_sum_d(s));
+}
+
+// The first of the wave's 64 runs (lane by lane) at whose end the sum passes the goal, of those with any weight; where
+// none does (a number of 1 and more), the last one.  base: the sum before it.  -1: no run has any.
+__device__ __forceinline__ int find_run(double mine, double before, double goal, double& base) {
+  double end = mine;  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double x = __shfl_up(end, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) end += x;
+  }
+  const unsigned long long some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && before + end > goal);
+  const int who = past ? __ffsll((long long)past) - 1 : some ? 63 - __clzll((long long)some) : -1;
+  base = before + __shfl(end - mine, max(who, 0), 64);
+  return who;
+}
+
+// The token behind the accepted ones, by a wave, from the segments' sums.
+template <typename E>
+__device__ __forceinline__ int pick_token(const VerifyArgs& a, const Weights<E>& w, const double2* sums, float u) {
+  const int lane = threadIdx.x & 63, per = (a.segs + 63) / 64, s0 = min(lane * per, a.segs), s1 = min(s0 + per, a.segs);
+  double r = 0.0, s = 0.0;
+  for (int i = s0; i < s1; ++i) {
+    const double2 x = sums[i];
+    r += x.x;
+    s += x.y;
+  }
+  const double all_r = wave_sum_d(r), all_s = wave_sum_d(s);
+  const bool rest = all_r > 0.0;
+  double goal = (double)u * (rest ? all_r : all_s), base;
+  if (!(goal >= 0.0)) goal = 0.0;
+  const int who = find_run(rest ? r : s, 0.0, goal, base);
+  if (who < 0) return -1;
+  // the segment among that lane's
+  int seg = -1;
+  double at = base, before = base;
+  for (int i = s0; i < s1; ++i) {
+    const double x = rest ? sums[i].x : sums[i].y;
+    if (x > 0.0) {
+      seg = i;
+      before = at;
+      if (at + x > goal) break;
+    }
+    at += x;
+  }
+  seg = __shfl(seg, who, 64);
+  before = __shfl(before, who, 64);
+  // sixteen values a lane, and the place among those of the lane that passes the goal
+  const int i0 = seg * kSeg + lane * (kSeg / 64);
+  double v[kSeg / 64], mine = 0.0;
+#pragma unroll
+  for (int k = 0; k < kSeg / 64; ++k) {
+    double x = 0.0, y = 0.0;
+    if (i0 + k < a.V) w.at(i0 + k, x, y);
+    v[k] = rest ? x : y;
+    mine += v[k];
+  }
+  const int lane_of = find_run(mine, before, goal, base);
+  int token = -1;
+  bool done = false;
+  at = base;
+#pragma unroll
+  for (int k = 0; k < kSeg / 64; ++k) {
+    at += v[k];
+    if (v[k] > 0.0 && !done) {
+      token = i0 + k;
+      done = at > goal;
+    }
+  }
+  return __shfl(token, max(lane_of, 0), 64);
+}
+
+// Sequence b's results, by a wave.
+__device__ __forceinline__ void write_verdict(const VerifyArgs& a, int b, int n, int token) {
+  for (int t = threadIdx.x & 63; t <= a.T; t += 64)
+    a.tokens[(long)b * (a.T + 1) + t] = t < n ? (int32_t)a.draft[b * a.draft_sb + t] : t == n ? token : -1;
+  if ((threadIdx.x & 63) == 0) a.accepted[b] = n;
+}
+
+__device__ __forceinline__ int count_of(const VerifyArgs& a, int b) {
+  return a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
+}
+
 template <typename E>
 __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
-  const int b = blockIdx.y;
-  const int count = min(max(a.counts ? a.counts[b] : a.T, 0), a.T);
-  const int n = count_accepted<E>(a, b, count);
+  const int b = blockIdx.y, count = count_of(a, b), n = count_accepted<E>(a, b, count);
   const Weights<E> w(a, b, n, count);
-  const int i0 = blockIdx.x * a.step, i1 = min(i0 + a.step, a.V);
-  double r = 0.0, s = 0.0;
-  for (int i = i0 + threadIdx.x; i < i1; i += 256) {
-    double x, y;
-    w.at(i, x, y);
-    r += x;
-    s += y;
-  }
-  __shared__ double s_r[4], s_s[4];
-  r = wave_sum_d(r);
-  s = wave_sum_d(s);
-  if ((threadIdx.x & 63) == 0) { s_r[threadIdx.x >> 6] = r; s_s[threadIdx.x >> 6] = s; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double* dst = a.sums + 2 * ((long)b * a.parts + blockIdx.x);
-    dst[0] = (s_r[0] + s_r[1]) + (s_r[2] + s_r[3]);
-    dst[1] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+  for (int seg = blockIdx.x * 4 + (threadIdx.x >> 6); seg < a.segs; seg += 4 * gridDim.x) {
+    const double2 x = segment_sums(a, w, seg);
+    if ((threadIdx.x & 63) == 0) a.sums[(long)b * a.segs + seg] = x;
   }
 }
 
 template <typename E>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-  const int b = blockIdx.x;
-  const int count = min(max(a.counts ? a.counts[b] : a.T, 0), a.T);
-  const int n = count_accepted<E>(a, b, count);
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+  const int b = blockIdx.x, count = count_of(a, b), n = count_accepted<E>(a, b, count);
   const Weights<E> w(a, b, n, count);
-  __shared__ double s_base, s_goal;
-  __shared__ int s_part, s_kind;
-  if (threadIdx.x == 0) {
-    const double* sums = a.sums + 2 * (long)b * a.parts;
-    double r = 0.0, s = 0.0;
-    for (int i = 0; i < a.parts; ++i) { r += sums[2 * i]; s += sums[2 * i + 1]; }
-    const int kind = r > 0.0 ? 0 : 1;
-    const double total = kind ? s : r;
-    // the first part whose end passes the goal; none does for u_next of 1 and more: the last with any weight
-    double goal = (double)a.u_next[b] * total, base = 0.0, at = 0.0;
-    if (!(goal >= 0.0)) goal = 0.0;
-    int part = -1;
-    for (int i = 0; i < a.parts; ++i) {
-      const double x = sums[2 * i + kind];
-      if (x > 0.0) {
-        part = i;
-        base = at;
-        if (at + x > goal) break;
-      }
-      at += x;
-    }
-    s_base = base;
-    s_goal = goal;
-    s_part = total > 0.0 ? part : -1;
-    s_kind = kind;
+  write_verdict(a, b, n, pick_token(a, w, a.sums + (long)b * a.segs, a.u_next[b]));
+}
+
+template <typename E>
+__global__ __launch_bounds__(1024) void verify_kernel(VerifyArgs a) {
+  __shared__ double2 s_sums[kSegsInLds];
+  const int b = blockIdx.x, count = count_of(a, b), n = count_accepted<E>(a, b, count);
+  const Weights<E> w(a, b, n, count);
+  for (int seg = threadIdx.x >> 6; seg < a.segs; seg += 16) {
+    const double2 x = segment_sums(a, w, seg);
+    if ((threadIdx.x & 63) == 0) s_sums[seg] = x;
   }
   __syncthreads();
-  const int part = s_part, kind = s_kind;
-  int token = -1;
-  if (part >= 0) {
-    // a thread's run of the part, the runs' sums, and the place in the run that passes the goal
-    const int i0 = part * a.step, i1 = min(i0 + a.step, a.V), run = (i1 - i0 + 255) / 256;
-    const int j0 = min(i0 + (int)threadIdx.x * run, i1), j1 = min(j0 + run, i1);
-    double mine = 0.0;
-    for (int i = j0; i < j1; ++i) {
-      double x[2];
-      w.at(i, x[0], x[1]);
-      mine += x[kind];
-    }
-    __shared__ double s_run[256];
-    __shared__ int s_who;
-    s_run[threadIdx.x] = mine;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double at = s_base;
-      int who = 0;
-      double base = at;
-      for (int i = 0; i < 256; ++i) {
-        if (s_run[i] > 0.0) {
-          who = i;
-          base = at;
-          if (at + s_run[i] > s_goal) break;
-        }
-        at += s_run[i];
-      }
-      s_who = who;
-      s_base = base;
-    }
-    __syncthreads();
-    if ((int)threadIdx.x == s_who) {
-      double at = s_base;
-      for (int i = j0; i < j1; ++i) {
-        double x[2];
-        w.at(i, x[0], x[1]);
-        at += x[kind];
-        if (x[kind] > 0.0) {
-          token = i;
-          if (at > s_goal) break;
-        }
-      }
-      s_part = token;
-    }
-    __syncthreads();
-    token = s_part;
-  }
-  for (int t = threadIdx.x; t <= a.T; t += 256)
-    a.tokens[(long)b * (a.T + 1) + t] = t < n ? (int32_t)a.draft[b * a.draft_sb + t] : t == n ? token : -1;
-  if (threadIdx.x == 0) a.accepted[b] = n;
+  if (threadIdx.x < 64) write_verdict(a, b, n, pick_token(a, w, s_sums, a.u_next[b]));
 }
 
 namespace {
-// Parts of a row: until 1024 work-groups are there, of at least 2048 values each.
-int verify_parts(const carekv_verify_params& p) {
-  const long most = (p.vocab + 2047L) / 2048, want = std::max(1L, 1024L / std::max(p.batch, 1));
-  return (int)std::max(1L, std::min(most, want));
+int verify_segs(const carekv_verify_params& p) { return (p.vocab + kSeg - 1) / kSeg; }
+// One work-group a sequence where its waves have at most four segments each, or where there are sequences for half of
+// the CUs; else two launches.
+bool verify_fused(const carekv_verify_params& p) {
+  const int segs = verify_segs(p);
+  return segs <= 64 || (p.batch >= 128 && segs <= kSegsInLds);
 }
 int check_verify(const carekv_verify_params* pp) {
   CAREKV_REQUIRE(pp, "null argument");
@@ -219,7 +255,7 @@ using namespace carekv;
 
 extern "C" int64_t carekv_verify_drafts_workspace_bytes(const carekv_verify_params* pp) {
   if (check_verify(pp) != CAREKV_OK) return -1;
-  return 16L * pp->batch * verify_parts(*pp);
+  return verify_fused(*pp) ? 0 : 16L * pp->batch * verify_segs(*pp);
 }
 
 extern "C" int carekv_verify_drafts(const carekv_verify_params* pp, const int64_t* draft, const void* target_probs,
@@ -230,26 +266,31 @@ extern "C" int carekv_verify_drafts(const carekv_verify_params* pp, const int64_
   if (rc != CAREKV_OK) return rc;
   const carekv_verify_params& p = *pp;
   if (p.batch == 0) return CAREKV_OK;
-  CAREKV_REQUIRE(target_probs && u_next && tokens && accepted && workspace && (p.n_drafts == 0 || (draft && u)), "null argument");
+  CAREKV_REQUIRE(target_probs && u_next && tokens && accepted && (workspace || verify_fused(p)) && (p.n_drafts == 0 || (draft && u)), "null argument");
   VerifyArgs a{};
   a.p = (const char*)target_probs; a.q = p.n_drafts ? (const char*)draft_probs : nullptr; a.draft = draft; a.u = u;
-  a.u_next = u_next; a.counts = counts; a.tokens = tokens; a.accepted = accepted; a.sums = (double*)workspace;
+  a.u_next = u_next; a.counts = counts; a.tokens = tokens; a.accepted = accepted; a.sums = (double2*)workspace;
   a.p_sb = p.target_sb; a.p_st = p.target_st; a.q_sb = p.draft_probs_sb; a.q_st = p.draft_probs_st;
   a.draft_sb = p.draft_sb; a.u_sb = p.u_sb;
-  a.T = p.n_drafts; a.V = p.vocab; a.parts = verify_parts(p);
-  a.step = (p.vocab + a.parts - 1) / a.parts;
-  a.parts = (p.vocab + a.step - 1) / a.step;  // (no part without values)
-  if (workspace_bytes < 16L * p.batch * a.parts) {
-    set_error("carekv_verify_drafts: workspace too small (%lld < %lld)", (long long)workspace_bytes,
-              (long long)(16L * p.batch * a.parts));
+  a.T = p.n_drafts; a.V = p.vocab; a.segs = verify_segs(p);
+  const bool fused = verify_fused(p);
+  const int64_t need = carekv_verify_drafts_workspace_bytes(pp);
+  if (workspace_bytes < need) {
+    set_error("carekv_verify_drafts: workspace too small (%lld < %lld)", (long long)workspace_bytes, (long long)need);
     return CAREKV_ESPACE;
   }
-  CAREKV_REQUIRE(((uintptr_t)workspace & 7) == 0, "workspace must be 8-byte aligned");
+  CAREKV_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
+  // work-groups of a sequence: each wave a segment, until 1024 are there
+  const int wgs = std::max(1, std::min((a.segs + 3) / 4, 1024 / p.batch));
   auto go = [&](auto e) {
     using E = decltype(e);
-    hipLaunchKernelGGL(verify_sums_kernel<E>, dim3(a.parts, p.batch), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(verify_pick_kernel<E>, dim3(p.batch), dim3(256), 0, s, a);
+    if (fused) {
+      hipLaunchKernelGGL(verify_kernel<E>, dim3(p.batch), dim3(1024), 0, s, a);
+      return;
+    }
+    hipLaunchKernelGGL(verify_sums_kernel<E>, dim3(wgs, p.batch), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(verify_pick_kernel<E>, dim3(p.batch), dim3(64), 0, s, a);
   };
   if (p.dtype == CAREKV_F16) go(_Float16{});
   else if (p.dtype == CAREKV_BF16) go(__bf16{});
