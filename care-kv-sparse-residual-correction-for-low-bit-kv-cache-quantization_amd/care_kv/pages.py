@@ -74,6 +74,22 @@ def int4_pages(n_pages: int, n_kv_heads: int, head_dim: int, *, device=None) -> 
     return Int4Pages(torch.zeros(n_pages, n_kv_heads, block_bytes(head_dim), dtype=torch.uint8, device=device), head_dim)
 
 
+_NONE = (0, 0, 0)
+
+
+def _ptr(x: Optional[torch.Tensor]):
+    return None if x is None else x.data_ptr()
+
+
+def _outside(x: torch.Tensor, block: torch.Tensor) -> bool:
+    """Whether x has no memory in common with the packed block."""
+    at, lo = x.data_ptr(), block.data_ptr()
+    if at >= lo + block.nbytes:
+        return True
+    reach = sum([(n - 1) * s for n, s in zip(x.shape, x.stride())])
+    return at + (reach + 1) * x.element_size() <= lo or not _lib.overlap(block, x)
+
+
 def _check_table(table: torch.Tensor, batch: int) -> torch.Tensor:
     if table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32:
         raise ValueError(f"table must be ({batch}, max_pages) int32; got {tuple(table.shape)} {table.dtype}")
@@ -111,58 +127,66 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
     Tokens before place 0, behind the table or on pages that are not there are
     dropped.  No two sequences of a call may write to one page.  The results
     carry no autograd history."""
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError(f"k and v must be (B, Hkv, T, D) of one type; got {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} "
-                         f"{v.dtype}")
-    B, Hkv, T, D = k.shape
-    if k.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"append_pages: fp16 or bf16 rows (got {k.dtype})")
-    if (Hkv, D) != (pages.n_kv_heads, pages.head_dim):
-        raise ValueError(f"k {tuple(k.shape)} does not fit pages of {pages.n_kv_heads} kv heads, head_dim {pages.head_dim}")
-    if q is not None and (q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, T, D) or q.dtype != k.dtype):
-        raise ValueError(f"q must be ({B}, heads, {T}, {D}) {k.dtype}; got {tuple(q.shape)} {q.dtype}")
+    kd, ks, dev = k.dtype, k.shape, k.device
+    if len(ks) != 4 or v.shape != ks or v.dtype != kd:
+        raise ValueError(f"k and v must be (B, Hkv, T, D) of one type; got {tuple(ks)} {kd}, {tuple(v.shape)} {v.dtype}")
+    B, Hkv, T, D = ks
+    if kd != torch.float16 and kd != torch.bfloat16:
+        raise ValueError(f"append_pages: fp16 or bf16 rows (got {kd})")
+    data = pages.data
+    n_pages, heads, _ = data.shape
+    if Hkv != heads or D != pages.head_dim:
+        raise ValueError(f"k {tuple(ks)} does not fit pages of {heads} kv heads, head_dim {pages.head_dim}")
+    Hq, qo, sq, so = 0, None, _NONE, _NONE
+    if q is not None:
+        if q.dim() != 4 or q.dtype != kd or (q.shape[0], q.shape[2], q.shape[3]) != (B, T, D):
+            raise ValueError(f"q must be ({B}, heads, {T}, {D}) {kd}; got {tuple(q.shape)} {q.dtype}")
+        Hq = q.shape[1]
     table = _check_table(table, B)
-    if plan is None and positions is not None:
+    R, layout, scale, freqs = 0, False, 1.0, None
+    if plan is not None:
+        R, layout, scale, freqs = plan.rotary_dim, plan.layout == "interleaved", plan.scale, plan.freqs
+        if R > D:
+            raise ValueError(f"head_dim {D} must be at least the plan's rotary_dim {R}")
+    elif positions is not None:
         raise ValueError("positions need a plan")
-    if plan is not None and plan.rotary_dim > D:
-        raise ValueError(f"head_dim {D} must be at least the plan's rotary_dim {plan.rotary_dim}")
-    pos = positions
+    pos, pos_bits, pos_batch = positions, 64, 0
     if pos is not None:
         pos = pos.unsqueeze(0) if pos.dim() == 1 else pos
         if pos.dtype not in (torch.int32, torch.int64) or pos.dim() != 2 or pos.shape[0] not in (1, B) or pos.shape[1] != T:
             raise ValueError(f"positions must be int32 or int64 ({B}, {T}), (1, {T}) or ({T},); got "
                              f"{tuple(positions.shape)} {positions.dtype}")
         pos = pos if pos.stride(1) == 1 or T == 1 else pos.contiguous()
-    if any(_lib.overlap(pages.data, x) for x in (k, v, q) if x is not None):
+        pos_bits, pos_batch = 64 if pos.dtype == torch.int64 else 32, pos.stride(0) if pos.shape[0] > 1 else 0
+    if not (_outside(k, data) and _outside(v, data) and (q is None or _outside(q, data))):
         raise ValueError("k, v and q must not overlap the pages")
-    dev = _lib.same_device("append_pages", k, v, q, pages.data, table, pos, None if plan is None else plan.freqs)
+    _lib.same_device("append_pages", k, v, q, data, table, pos, freqs)
     if start is None:
         raise ValueError("append_pages needs start, the tokens that the sequences hold")
-    qo = None if q is None else q.new_empty(q.shape)
+    if q is not None:
+        qo = q.new_empty(q.shape)
     kh = vh = None
     if return_hat:
-        kh = k.new_empty(k.shape, dtype=torch.float16)
-        vh = k.new_empty(k.shape, dtype=torch.float16)
+        kh, vh = k.new_empty(ks, dtype=torch.float16), k.new_empty(ks, dtype=torch.float16)
     if B and T:
-        if k.stride(3) != 1:
+        sk, sv = k.stride(), v.stride()
+        if sk[3] != 1:
             k = k.contiguous()
-        if v.stride(3) != 1:
+            sk = k.stride()
+        if sv[3] != 1:
             v = v.contiguous()
-        if q is not None and q.stride(3) != 1:
-            q = q.contiguous()
-        st = _lib.row_counts(start, B, dev, "start")
-        ct = _lib.row_counts(counts, B, dev, "counts")
-        pp = _lib.AppendParams(B, 0 if q is None else q.shape[1], Hkv, T, D, 0 if plan is None else plan.rotary_dim,
-                               _lib.DTYPE_CODE[k.dtype], plan is not None and plan.layout == "interleaved",
-                               64 if pos is None or pos.dtype == torch.int64 else 32, pages.n_pages, table.shape[1],
-                               1.0 if plan is None else plan.scale,
-                               pos.stride(0) if pos is not None and pos.shape[0] > 1 else 0, table.stride(0),
-                               *((0, 0, 0) if q is None else q.stride()[:3]), *k.stride()[:3], *v.stride()[:3],
-                               *((0, 0, 0) if q is None else qo.stride()[:3]))
-        ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-        _lib.call(dev, "carekv_append_pages", _lib.load().carekv_append_pages, pp, ptr(q), k.data_ptr(), v.data_ptr(),
-                  ptr(pos), None if plan is None else plan.freqs.data_ptr(), st.data_ptr(), ptr(ct), table.data_ptr(),
-                  pages.data.data_ptr(), ptr(qo), ptr(kh), ptr(vh))
+            sv = v.stride()
+        if q is not None:
+            if q.stride(3) != 1:
+                q = q.contiguous()
+            sq, so = q.stride(), qo.stride()
+        st, ct = _lib.row_counts(start, B, dev, "start"), _lib.row_counts(counts, B, dev, "counts")
+        pp = _lib.AppendParams(B, Hq, Hkv, T, D, R, _lib.DTYPE_CODE[kd], layout, pos_bits, n_pages, table.shape[1], scale,
+                               pos_batch, table.stride(0), sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
+                               so[0], so[1], so[2])
+        _lib.call(dev, "carekv_append_pages", _lib.load().carekv_append_pages, pp, _ptr(q), k.data_ptr(), v.data_ptr(),
+                  _ptr(pos), _ptr(freqs), st.data_ptr(), _ptr(ct), table.data_ptr(), data.data_ptr(), _ptr(qo), _ptr(kh),
+                  _ptr(vh))
     return (qo, kh, vh) if return_hat else qo
 
 

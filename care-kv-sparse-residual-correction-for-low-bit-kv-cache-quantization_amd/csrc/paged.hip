@@ -20,7 +20,7 @@
 
 #include "host_util.h"
 #include "pages4.h"
-#include "rows_attn.h"
+#include "tile_attn.h"
 
 namespace carekv {
 
@@ -86,11 +86,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
   using P = Page4<D>;
   constexpr int W = D / 32, KS = D / 32, DT = D / 16, QB = 16 * NQ;
   constexpr float kUp = ElemF16::kUp;
-  const int n = gridDim.x;
-  int it = blockIdx.x;
-  it = n / 8 * (it & 7) + min(it & 7, n & 7) + (it >> 3);  // an XCD takes consecutive items
-  const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
-  const int bh = sp_blk / a.by_nqb, qblk = sp_blk - bh * a.nqb, b = bh / a.by_hkv, hk = bh - b * a.Hkv;
+  const int it = xcd_item(a);
+  // a group: the kv heads' blocks of a sequence's split, which lie side by side in its pages
+  const int unit = it / a.by_group, b = unit / a.by_nsplit, sp = unit - b * a.nsplit;
+  const int in = it - unit * a.by_group.d, hk = in / a.by_nqb, qblk = in - hk * a.nqb, bh = b * a.Hkv + hk;
   const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r0 = qblk * QB, r1 = min(r0 + QB, a.M);
@@ -176,6 +175,12 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
     const bool whole = span.whole(a, j0) && p0 >= 0 && p1 >= 0;
     uint32_t see[NQ] = {};
     if (!whole) {
+      RowSight row[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
+        row[qb] = sight[qb];
+        row[qb].stay_here();
+      }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
         const bool there = (tt ? p1 : p0) >= 0;
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
           const int j = j0 + 16 * tt + 4 * g + k;
 #pragma unroll
           for (int qb = 0; qb < NQ; ++qb) {
-            const bool v = there && sight[qb].sees(a, j);
+            const bool v = there && row[qb].sees(a, j);
             see[qb] |= (uint32_t)v << (4 * tt + k);
             s[tt][qb][k] = v ? s[tt][qb][k] : -INFINITY;
           }
@@ -289,14 +294,14 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((w * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
     __syncthreads();
     const int r = r0 + 16 * qb + c16;
-    const bool in = r < a.M, pad = sight[qb].top < 0;
+    const bool is_row = r < a.M, pad = sight[qb].top < 0;
 #pragma unroll
     for (int u = 0; u < DT / 4; ++u) {
       const int dt = w + 4 * u;
       float4_t v = *reinterpret_cast<const float4_t*>(so + (dt * 64 + lane) * 4);
 #pragma unroll
       for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const float4_t*>(so + ((k * DT + dt) * 64 + lane) * 4);
-      if (!in) continue;
+      if (!is_row) continue;
       if (a.nsplit == 1) {
         if (pad) v = float4_t{0.f, 0.f, 0.f, 0.f};
         write4<E>(a, out_row(a, b, hk, r), 16 * dt + 4 * g, v, pad ? 0.f : l);
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
         *reinterpret_cast<float4_t*>(a.po + pr * D + 16 * dt + 4 * g) = v;
       }
     }
-    if (in && g == 0 && w == 0) {
+    if (is_row && g == 0 && w == 0) {
       if (a.nsplit > 1) {
         const long pr = (long)sp * a.rows + (long)bh * a.M + r;
         a.pml[2 * pr] = m;
@@ -318,76 +323,62 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
   }
 }
 
-// Many rows: bound by the products, so that the codes are turned into fp16 once
-// for 128 rows (4 waves of 32).  A wave takes half of one page's codes of a tile
-// of 32 keys and writes them to LDS as the operands that all four read, 1 KB each
-// in the lanes' order (double buffered, one barrier a tile; the next tile's codes
-// are on their way while this one is used).
-template <typename E, int D>
-__global__ __launch_bounds__(256, 3) void paged_tile_kernel(PagedArgs a) {
-  using P = Page4<D>;
-  constexpr int W = D / 32, KS = D / 32, DT = D / 16, NQ = 2, QW = 32, QB = 128, NW = W / 2;
-  constexpr int KBUF = 2 * KS * 1024, BUF = KBUF + DT * 1024;
-  constexpr float kUp = ElemF16::kUp;
-  __shared__ __align__(16) char lds[2 * BUF];
-  __shared__ int s_odd[2];  // the last tile in the buffer with a V scale that is no number
-  const int n = gridDim.x;
-  int it = blockIdx.x;
-  it = n / 8 * (it & 7) + min(it & 7, n & 7) + (it >> 3);  // an XCD takes consecutive items
-  const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
-  const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb), b = bh / a.by_hkv, hk = bh - b * a.Hkv;
-  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b0 = qblk * QB, b1 = min(b0 + QB, a.M), r0 = b0 + QW * w, r1 = min(r0 + QW, a.M);
-  const SeqRows seq(a, b);
-  const Span<kTile> span(a, seq, b0 / a.by_g, (b1 - 1) / a.by_g + 1);
-  const Span<kTile> mine(a, seq, r0 / a.by_g, r1 > r0 ? (r1 - 1) / a.by_g + 1 : 0);
-  const int i0 = sp * a.tps, i1 = min(i0 + a.tps, span.n), nt = i1 - i0;
-  if (a.nsplit > 1 && nt <= 0) return;  // (the join does not read it)
-
-  half8_t qf[NQ][KS];
-  float c[NQ];
-  RowSight sight[NQ];
-#pragma unroll
-  for (int qb = 0; qb < NQ; ++qb) {
-    sight[qb] = RowSight(a, seq, r0 + 16 * qb + c16);
-    c[qb] = load_q4<E, D>(qf[qb], a, b, hk, r0 + 16 * qb + c16, g);
-  }
-
-  const char* pool = a.pages + (long)hk * P::kBytes;
-  const long page_bytes = (long)a.Hkv * P::kBytes;
-  const int32_t* table = a.table + b * a.table_sb;
-  auto page_of = [&](int at) {  // -1: not there
-    const int p = table[min(at, a.max_pages - 1)];
-    return at < a.max_pages && p >= 0 && p < a.n_pages ? p : -1;
-  };
-  const int pg = w >> 1, half = w & 1;  // the wave's page of a tile and half of its words
+// Many rows: bound by the products, so that the codes are turned into fp16 once for
+// the 128 rows of tile_attn.h.  A wave takes half of one page's codes of a tile of 32
+// keys and writes them to LDS as the operands that all four read, 1 KB each in the
+// lanes' order.
+template <typename E_, int D_>
+struct Pages4 {
+  using Args = PagedArgs;
+  using ET = ElemF16;
+  using Out = E_;
+  using V8 = half8_t;
+  using P = Page4<D_>;
+  static constexpr int D = D_, W = D / 32, KS = D / 32, NW = W / 2, kK = 2 * KS * 1024, kV = D / 16 * 1024;
+  const char* pool;
+  const int32_t* table;
+  long page_bytes;
+  int n_pages, max_pages, hi, lane, g, c16, pg, half;  // pg, half: the wave's page of a tile and half of its words
   uint32_t kw[NW], vw[NW];
   half2_t vs[2 * NW];
   uint16_t ks;
-  int there = 0;  // of the tile whose codes are on their way: bit i, page i
-  auto load_tile = [&](int i) {
-    const int tile = span.tile(i0 + i), p0 = page_of(2 * tile), p1 = page_of(2 * tile + 1);
-    there = (p0 >= 0) | (p1 >= 0) << 1;
+  int p0, p1;        // the next tile's pages
+  int loaded, held;  // which pages of the tile on its way, of the tile stored last, are there: bit i, page i
+
+  __device__ __forceinline__ Pages4(const Args& a, int b, int hk, const SeqRows&, int hi_, int w, int lane_)
+      : pool(a.pages + (long)hk * P::kBytes), table(a.table + b * a.table_sb), page_bytes((long)a.Hkv * P::kBytes),
+        n_pages(a.n_pages), max_pages(a.max_pages), hi(hi_), lane(lane_), g(lane_ >> 4), c16(lane_ & 15), pg(w >> 1),
+        half(w & 1), loaded(0), held(0) {}
+  static __device__ __forceinline__ float load_q(V8* qf, const Args& a, int b, int hk, int r, int g) {
+    return load_q4<E_, D>(qf, a, b, hk, r, g);
+  }
+  __device__ __forceinline__ int page_of(int at) const {  // -1: not there
+    const int p = table[min(at, max_pages - 1)];
+    return at < max_pages && p >= 0 && p < n_pages ? p : -1;
+  }
+  __device__ __forceinline__ void look(int tile) {
+    p0 = page_of(2 * tile);
+    p1 = page_of(2 * tile + 1);
+  }
+  __device__ __forceinline__ void load() {
+    loaded = (p0 >= 0) | (p1 >= 0) << 1;
     const char* blk = pool + (long)max(pg ? p1 : p0, 0) * page_bytes;
     __builtin_memcpy(kw, __builtin_assume_aligned(blk + c16 * (D / 2) + (g * W + half * NW) * 4, 4 * NW), 4 * NW);
     __builtin_memcpy(vw, __builtin_assume_aligned(blk + P::kV + (lane * W + half * NW) * 4, 4 * NW), 4 * NW);
     __builtin_memcpy(vs, __builtin_assume_aligned(blk + P::kVS + (g * W + half * NW) * 8, 8 * NW), 8 * NW);
     ks = *reinterpret_cast<const uint16_t*>(blk + P::kKS + ((D == 128 ? g : g >> 1) * kPage + c16) * 2);
-  };
-  auto store_tile = [&](int i) {
-    char* buf = lds + (i & 1) * BUF;
-    const int j0 = span.tile(i0 + i) * kTile;
-    // a weight of 0 times a scale that is no number would be NaN: such scales, and what lies where no row looks, are 0
-    // here, and the rows that do see such a key are set below
-    uint32_t odd = 0;
-    if (j0 + kTile - 1 > span.hi || there != 3) {
+  }
+  __device__ __forceinline__ bool store(char* kb, char* vb, int tile) {
+    held = loaded;
+    const int j0 = tile * kTile;
+    if (j0 + kTile - 1 > hi || held != 3) {  // what lies where no row looks
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (!(there >> pg & 1) || j0 + 16 * pg + 4 * g + k > span.hi)
+        if (!(held >> pg & 1) || j0 + 16 * pg + 4 * g + k > hi)
 #pragma unroll
           for (int x = 0; x < NW; ++x) vs[2 * x + k / 2][k & 1] = (_Float16)0.f;
     }
+    uint32_t odd = 0;
 #pragma unroll
     for (int x = 0; x < 2 * NW; ++x) {
       uint32_t bits;
@@ -395,7 +386,6 @@ __global__ __launch_bounds__(256, 3) void paged_tile_kernel(PagedArgs a) {
       odd |= ((bits & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
     }
     if (__builtin_expect(odd != 0, 0)) {
-      s_odd[i & 1] = i;
 #pragma unroll
       for (int x = 0; x < 4 * NW; ++x)
         if ((half2bits(vs[x / 2][x & 1]) & 0x7c00) == 0x7c00) vs[x / 2][x & 1] = (_Float16)0.f;
@@ -408,158 +398,61 @@ __global__ __launch_bounds__(256, 3) void paged_tile_kernel(PagedArgs a) {
       dequant4(v, kw[x], kss);
       uint4 u;
       __builtin_memcpy(&u, v, 16);
-      *reinterpret_cast<uint4*>(buf + (pg * KS + half * NW + x) * 1024 + lane * 16) = u;
+      *reinterpret_cast<uint4*>(kb + (pg * KS + half * NW + x) * 1024 + lane * 16) = u;
       const half2_t sc[4] = {vs[2 * x], vs[2 * x + 1], vs[2 * x], vs[2 * x + 1]};
       dequant4(v, vw[x], sc);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {  // four tokens of dims 16 dt + c16: half of an operand
         uint2 t;
         __builtin_memcpy(&t, v + 2 * y, 8);
-        *reinterpret_cast<uint2*>(buf + KBUF + (2 * (half * NW + x) + y) * 1024 + lane * 16 + 8 * pg) = t;
+        *reinterpret_cast<uint2*>(vb + (2 * (half * NW + x) + y) * 1024 + lane * 16 + 8 * pg) = t;
       }
     }
-  };
-
-  float m_run[NQ], l_run[NQ];
-  float4_t o[NQ][DT];
-#pragma unroll
-  for (int qb = 0; qb < NQ; ++qb) {
-    m_run[qb] = kLowest;
-    l_run[qb] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    return odd != 0;
   }
-  if (threadIdx.x < 2) s_odd[threadIdx.x] = -1;
-  __syncthreads();
-  int here = 0;  // the current tile's pages
-  if (nt > 0) {
-    load_tile(0);
-    here = there;
-    store_tile(0);
+  __device__ __forceinline__ V8 k_op(const char* kb, int tt, int st) const {
+    V8 r;
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(kb + (tt * KS + st) * 1024 + lane * 16);
+    return r;
   }
-  __syncthreads();
-  if (nt > 1) load_tile(1);
-  for (int i = 0; i < nt; ++i) {
-    const int j0 = span.tile(i0 + i) * kTile;
-    const char* buf = lds + (i & 1) * BUF + lane * 16;
-    if (mine.n > 0 && j0 <= mine.hi && (j0 + kTile - 1 > mine.first - a.window || j0 < a.sink)) {
-      // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
-      __builtin_amdgcn_s_setprio(1);
-      float4_t s[2][NQ];
+  __device__ __forceinline__ V8 v_op(const char* vb, int dt) const {
+    V8 r;
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(vb + dt * 1024 + lane * 16);
+    return r;
+  }
+  __device__ __forceinline__ int there() const { return held; }
+  // groups that stand for NaN
+  template <int NQ, int DT>
+  __device__ __forceinline__ void odd_values(const Args& a, float4_t (&o)[NQ][DT], const RowSight (&sight)[NQ], int tile) const {
+#pragma unroll 1
+    for (int key = 0; key < kTile; ++key) {
+      const int p = page_of(2 * tile + key / kPage);
+      if (p < 0) continue;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(pool + (long)p * page_bytes + P::kVS) + key % 16 / 4 * W * 4 + key % 4;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          half8_t ak;
-          *reinterpret_cast<uint4*>(&ak) = *reinterpret_cast<const uint4*>(buf + (tt * KS + st) * 1024);
-#pragma unroll
-          for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = mfma16x32(ak, qf[qb][st], s[tt][qb]);
-        }
-      }
-      __builtin_amdgcn_s_setprio(0);
-      if (!mine.whole(a, j0) || here != 3) {
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int qb = 0; qb < NQ; ++qb)
-              if (!(here >> tt & 1) || !sight[qb].sees(a, j0 + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
-      }
-      float mx[NQ];
-      bool any_over = false, over[NQ];
-#pragma unroll
-      for (int qb = 0; qb < NQ; ++qb) {
-        mx[qb] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
-        over[qb] = fmaf(mx[qb], c[qb], -kUp) > m_run[qb];
-        any_over |= over[qb];
-      }
-      if (__any(any_over)) {
+      for (int gr = 0; gr < W; ++gr) {
+        asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
+        if ((src[4 * gr] & 0x7c00) != 0x7c00) continue;
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) {
-          if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
-          const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c[qb], -kUp));
-          const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
-          m_run[qb] = m_new;
-          l_run[qb] *= f;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
-        }
-      }
-      half8_t bp[NQ];
-#pragma unroll
-      for (int qb = 0; qb < NQ; ++qb) {
-        float ls = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[k / 4][qb][k % 4], c[qb], -m_run[qb]));
-          ls += p;
-          bp[qb][k] = (_Float16)p;
-        }
-        l_run[qb] += ls;
-      }
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        half8_t av;
-        *reinterpret_cast<uint4*>(&av) = *reinterpret_cast<const uint4*>(buf + KBUF + dt * 1024);
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = mfma16x32(av, bp[qb], o[qb][dt]);
-      }
-      if (__builtin_expect(s_odd[i & 1] == i, 0)) {
-#pragma unroll 1
-        for (int key = 0; key < kTile; ++key) {
-          const int p = page_of(j0 / kPage + key / kPage);
-          if (p < 0) continue;
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(pool + (long)p * page_bytes + P::kVS) + key % 16 / 4 * W * 4 + key % 4;
-#pragma unroll
-          for (int gr = 0; gr < W; ++gr) {
-            asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
-            if ((src[4 * gr] & 0x7c00) != 0x7c00) continue;
-#pragma unroll
-            for (int qb = 0; qb < NQ; ++qb)
-              if (sight[qb].sees(a, j0 + key)) o[qb][2 * gr] += NAN, o[qb][2 * gr + 1] += NAN;
-          }
+          RowSight row = sight[qb];
+          row.stay_here();
+          if (row.sees(a, kTile * tile + key)) o[qb][2 * gr] += NAN, o[qb][2 * gr + 1] += NAN;
         }
       }
     }
-    __builtin_amdgcn_s_setprio(0);
-    here = there;
-    if (i + 1 < nt) store_tile(i + 1);
-    if (i + 2 < nt) load_tile(i + 2);
-    __syncthreads();
   }
-#pragma unroll
-  for (int qb = 0; qb < NQ; ++qb) {
-    const int r = r0 + 16 * qb + c16;
-    const bool pad = sight[qb].top < 0;  // (what a row of padding holds is not used)
-    const float l = col_sum(l_run[qb]);
-    if (r >= a.M) continue;
-    if (a.nsplit == 1) {
-      char* row = out_row(a, b, hk, r);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        write4<E>(a, row, 16 * dt + 4 * g, pad ? float4_t{0.f, 0.f, 0.f, 0.f} : o[qb][dt], pad ? 0.f : l);
-      if (a.lse && g == 0) write_lse(a, b, hk, r, m_run[qb], pad ? 0.f : l);
-    } else {
-      const long pr = (long)sp * a.rows + (long)bh * a.M + r;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(a.po + pr * D + 16 * dt + 4 * g) = o[qb][dt];
-      if (g == 0) {
-        a.pml[2 * pr] = m_run[qb];
-        a.pml[2 * pr + 1] = l;
-      }
-    }
-  }
-}
+};
 
 namespace {
-// How a call is cut: 16 rows of a kv head at once or 32, more in blocks of 128;
-// key splits of at least 8 tiles until 1024 work-groups (768 of many rows) are there.
+// How a call is cut: 16 rows of a kv head at once or 32, more in blocks of 128.  Key
+// splits of at least 8 tiles (two a wave), at most 32: the join reads every split's
+// partials.  us a call, by splits: one row of 32 / 4 heads, D = 64, on 2303 keys 1 / 4
+// / 8 / 16 / 32: 17.2 / 10.3 / 9.1 / 8.7 / 9.2, on 8000 8 / 16 / 32 / 64: 12.4 / 10.0 /
+// 9.9 / 12.3; 32 / 8 heads, D = 128, on 16000 16 / 32 / 64: 16.7 / 14.1 / 16.6; 16 x 5 rows
+// on 8191 through a window of 4096 2 / 4 / 6 / 8: 39 / 34 / 39 / 39; 64 rows on 32768 2 / 4
+// / 6 / 8: 479 / 461 / 460 / 463.  512 rows of 40 heads on 16896 1 / 2 / 3 / 4 / 6: 877 / 568 /
+// 608 / 533 / 548.
 struct PagedPlan {
   int nq, nqb, nsplit, tps;  // nq: 16-row sub-blocks, 8 for the kernel of many rows
 };
@@ -574,7 +467,8 @@ PagedPlan paged_plan(const carekv_paged_params& p) {
     keys = std::min(keys, sees);
   }
   const long tiles = std::max(1L, (keys + kTile - 1) / kTile), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
-  const long ns = std::max(1L, std::min((r.nq == 8 ? 768 : 1024) / wgs, (tiles + 7) / 8));
+  const long at = r.nq == 8 ? 1280 : wgs * tiles < 512 * 64 ? 512 : 2048;  // work-groups
+  const long ns = std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
   return r;
@@ -636,9 +530,11 @@ extern "C" int carekv_paged_attn(const carekv_paged_params* pp, const void* q, c
   a.sink = p.sink;
   a.nqb = plan.nqb; a.nsplit = plan.nsplit; a.tps = plan.tps; a.qb_rows = 16 * plan.nq;
   a.by_g = FastDiv(a.G); a.by_nqb = FastDiv(a.nqb); a.by_hkv = FastDiv(a.Hkv); a.by_nsplit = FastDiv(a.nsplit); a.by_m = FastDiv(a.M);
+  a.by_group = FastDiv((long)a.nqb * (plan.nq == 8 ? a.nsplit : a.Hkv));
   a.po = (float*)workspace;
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);
+  set_period(a, p.window, (a.qb_rows + a.G - 1) / a.G, kTile);
   a.al8 = (operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}}) & 7) == 0;
   a.table = table; a.pages = (const char*)pages; a.table_sb = p.table_sb; a.n_pages = p.n_pages; a.max_pages = p.max_pages;
   hipStream_t s = (hipStream_t)stream;
@@ -650,7 +546,7 @@ extern "C" int carekv_paged_attn(const carekv_paged_params* pp, const void* q, c
     const dim3 grid((unsigned)wgs), block(256);
     if (plan.nq == 1) hipLaunchKernelGGL((paged_rows_kernel<E, D, 1>), grid, block, 0, s, a);
     else if (plan.nq == 2) hipLaunchKernelGGL((paged_rows_kernel<E, D, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((paged_tile_kernel<E, D>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tile_attn_kernel<Pages4<E, D>>), grid, block, 0, s, a);
     CAREKV_CHECK_LAUNCH("paged_rows");
     if (a.nsplit > 1) {
       constexpr int RW = 256 / D;

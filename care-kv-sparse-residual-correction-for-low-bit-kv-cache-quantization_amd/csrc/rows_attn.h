@@ -7,6 +7,7 @@
 // rows next to each other see nearly the same keys.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 
 #include "fast_div.h"
@@ -30,10 +31,28 @@ struct RowsArgs {
   int Hq, Hkv, G, T, M, max_keys, window, sink, nqb, nsplit, qb_rows;
   int tps;                   // tiles of a split
   FastDiv by_g, by_nqb, by_hkv, by_nsplit, by_m;
+  FastDiv by_group;          // items of a group (see xcd_item)
+  FastDiv by_period;         // tiles of a window and a block's tokens (see Span)
   float sm_log2;             // |scale| log2(e), 1 where that is 0
   uint32_t q_sign, q_keep;   // sign bits of two elements where the scale is negative; 0 where it is 0
   int al8;                   // rows of out on 8 bytes
 };
+
+// The work-group's item.  Items come in groups of a.by_group that read the same
+// memory; work-groups go round the 8 XCDs, and an XCD takes one group of every
+// eight, each time another one of them, so that the items of a group meet in its
+// L2 and each XCD has some of every (ragged) sequence; of the groups that are left
+// over each XCD takes a share.
+__device__ __forceinline__ int xcd_item(const RowsArgs& a) {
+  const int idx = blockIdx.x, n = gridDim.x, x = idx & 7, per = a.by_group.d;
+  const int whole = n / a.by_group / 8 * 8 * per;
+  if (idx < whole) {
+    const int j = (idx >> 3) / a.by_group;
+    return (8 * j + (x + j & 7)) * per + (idx >> 3) - j * per;
+  }
+  const int left = n - whole;
+  return whole + left / 8 * x + min(x, left & 7) + ((idx - whole) >> 3);
+}
 
 // Sequence b's counts, kept where sums of them stay in 32 bits.
 struct SeqRows {
@@ -46,24 +65,32 @@ struct SeqRows {
 };
 
 // The keys that rows t0 .. t1 - 1 see between them, as tiles of KT keys: the
-// first n_sink tiles, then those from tile0 on.
+// first n_sink tiles, then those from tile0 on, begun at the multiple of the
+// period among them: blocks that run side by side then read the same one or two
+// tiles at a time whatever their windows start with, and those come from the L2.
 template <int KT>
 struct Span {
   int first, last;  // positions of the first and the last row
   int hi;           // last key that is seen
-  int n_sink, tile0, n;
+  int n_sink, tile0, n_main, turn, n;
   __device__ __forceinline__ Span(const RowsArgs& a, const SeqRows& s, int t0, int t1) {
     t1 = min(t1, s.qlen);
     first = s.base + t0;
     last = s.base + t1 - 1;
     hi = min(last, s.len - 1);
-    n_sink = tile0 = n = 0;
+    n_sink = tile0 = n_main = turn = n = 0;
     if (t0 >= t1 || hi < 0) return;
     tile0 = max(0, first - a.window + 1) / KT;
     n_sink = min((min(a.sink, hi + 1) + KT - 1) / KT, tile0);
-    n = n_sink + max(0, hi / KT - tile0 + 1);
+    n_main = max(0, hi / KT - tile0 + 1);
+    n = n_sink + n_main;
+    turn = (tile0 + a.by_period.d - 1) / a.by_period * a.by_period.d - tile0;
+    if (turn >= n_main) turn = 0;
   }
-  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : i - n_sink + tile0; }
+  __device__ __forceinline__ int tile(int i) const {
+    const int j = i - n_sink + turn;
+    return i < n_sink ? i : tile0 + (j < n_main ? j : j - n_main);
+  }
   // whether every row sees every key of the tile at j0
   __device__ __forceinline__ bool whole(const RowsArgs& a, int j0) const {
     return j0 + KT - 1 <= min(first, hi) && (j0 > last - a.window || j0 + KT <= a.sink);
@@ -81,6 +108,8 @@ struct RowSight {
     top = there ? min(s.base + t, s.len - 1) : -1;
     low = s.base + t - a.window + 1;
   }
+  // in a branch that few tiles take: without it the compiler compares for every tile
+  __device__ __forceinline__ void stay_here() { asm volatile("" : "+v"(top), "+v"(low)); }
   __device__ __forceinline__ bool sees(const RowsArgs& a, int j) const { return j <= top && (j >= low || j < a.sink); }
 };
 
@@ -168,6 +197,11 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
   if (pad) { LL = 0.f; O = float4_t{0.f, 0.f, 0.f, 0.f}; }  // (what a row of padding holds is not used)
   write4<E>(a, out_row(a, b, hk, r), 4 * d4, O, LL);
   if (a.lse && d4 == 0) write_lse(a, b, hk, r, mm, LL);
+}
+
+// The period of blocks of `tokens` tokens and tiles of kt keys.
+inline void set_period(RowsArgs& a, int window, int tokens, int kt) {
+  a.by_period = FastDiv(window > 0 ? std::min(((long)window + tokens) / kt + 2, (long)kMaxPos) : kMaxPos);
 }
 
 // The scale as the kernels take it.

@@ -1,0 +1,182 @@
+// The main loop of windowed attention with many rows (window_attention's 16-bit
+// rows, paged_attention's 4-bit pages): a work-group has 128 rows of a kv head (4
+// waves of 32) and walks over the tiles of 32 keys that any of them sees, K and V
+// in LDS (double buffered, one barrier a tile): S^T = K Q^T and O^T += V^T P^T on
+// v_mfma_f32_16x16x32, the softmax over a query's column in 32 bits on base-2
+// logits.  The weights are rounded to the operands' type (half a step; their sum
+// is not), in fp16 against a reference 15 below the row's maximum, so that a weight
+// of 2^-29 of the largest is still normal.
+//
+// Masks are applied where a wave's tile has a key that some row of the wave does
+// not see, tiles that none sees are left out.
+#pragma once
+
+#include "rows_attn.h"
+
+namespace carekv {
+
+// Src: where K and V come from.  look says which tile is loaded next, load starts its loads into registers, store
+// writes them to LDS (and says whether the thread had a V value that is not finite: it writes 0 for it, so that a masked
+// weight of 0 times it is no NaN), k_op / v_op read operands, there() tells which halves of the tile stored last exist,
+// odd_values() brings the values that are not finite to the rows that see them.
+template <class Src>
+__global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a) {
+  using ET = typename Src::ET;
+  using V8 = typename ET::V8;
+  using E = typename Src::Out;
+  constexpr int D = Src::D, NQ = 2, QW = 32, QB = 128, KT = 32, KS = D / 32, DT = D / 16;
+  constexpr int BUF = Src::kK + Src::kV;
+  __shared__ __align__(16) char lds[2 * BUF];
+  __shared__ int s_odd[2];  // the last tile in the buffer that held a V value that is not finite
+  const int it = xcd_item(a);
+  const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
+  const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
+  const int b = bh / a.by_hkv, hk = bh - b * a.Hkv;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b0 = qblk * QB, b1 = min(b0 + QB, a.M), r0 = b0 + QW * w, r1 = min(r0 + QW, a.M);
+  const SeqRows seq(a, b);
+  const Span<KT> span(a, seq, b0 / a.by_g, (b1 - 1) / a.by_g + 1);
+  const Span<KT> mine(a, seq, r0 / a.by_g, r1 > r0 ? (r1 - 1) / a.by_g + 1 : 0);
+  const int i0 = sp * a.tps, i1 = min(i0 + a.tps, span.n), nt = i1 - i0;
+  if (a.nsplit > 1 && nt <= 0) return;  // (the join does not read it)
+
+  V8 qf[NQ][KS];
+  float c[NQ];
+  RowSight sight[NQ];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    sight[qb] = RowSight(a, seq, r0 + 16 * qb + c16);
+    c[qb] = Src::load_q(qf[qb], a, b, hk, r0 + 16 * qb + c16, g);
+  }
+  float m_run[NQ], l_run[NQ];
+  float4_t o[NQ][DT];
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    m_run[qb] = kLowest;
+    l_run[qb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  Src src(a, b, hk, seq, span.hi, w, lane);
+  auto tile = [&](int i) { return span.tile(i0 + i); };
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = -1;
+  __syncthreads();
+  if (nt > 0) {
+    src.look(tile(0));
+    src.load();
+    src.look(tile(min(1, nt - 1)));
+    if (src.store(lds, lds + Src::kK, tile(0))) s_odd[0] = 0;
+  }
+  __syncthreads();
+  if (nt > 1) src.load();
+  for (int i = 0; i < nt; ++i) {
+    const int j0 = tile(i) * KT, here = src.there();
+    src.look(tile(min(i + 2, nt - 1)));
+    const char* kb = lds + (i & 1) * BUF;
+    const char* vb = kb + Src::kK;
+    if (mine.n > 0 && j0 <= mine.hi && (j0 + KT - 1 > mine.first - a.window || j0 < a.sink)) {
+      // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
+      __builtin_amdgcn_s_setprio(1);
+      float4_t s[2][NQ];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const V8 ak = src.k_op(kb, tt, ks);
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = ET::mfma(ak, qf[qb][ks], s[tt][qb]);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if (!mine.whole(a, j0) || here != 3) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          RowSight row = sight[qb];
+          row.stay_here();
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (!(here >> tt & 1) || !row.sees(a, j0 + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
+        }
+      }
+      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
+      float mx[NQ];
+      bool any_over = false, over[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
+        mx[qb] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
+        over[qb] = fmaf(mx[qb], c[qb], -ET::kUp) > m_run[qb];
+        any_over |= over[qb];
+      }
+      if (__any(any_over)) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
+          const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c[qb], -ET::kUp));
+          const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+          m_run[qb] = m_new;
+          l_run[qb] *= f;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
+        }
+      }
+      V8 bp[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) {
+        float ls = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[k / 4][qb][k % 4], c[qb], -m_run[qb]));
+          ls += p;
+          bp[qb][k] = (typename ET::E)p;
+        }
+        l_run[qb] += ls;
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const V8 av = src.v_op(vb, dt);
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
+      }
+      if (__builtin_expect(s_odd[i & 1] == i, 0)) src.odd_values(a, o, sight, tile(i));
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (i + 1 < nt && src.store(lds + (i + 1 & 1) * BUF, lds + (i + 1 & 1) * BUF + Src::kK, tile(i + 1)))
+      s_odd[(i + 1) & 1] = i + 1;
+    if (i + 2 < nt) src.load();
+    __syncthreads();
+  }
+
+  // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    const int r = r0 + 16 * qb + c16;
+    const bool pad = sight[qb].top < 0;  // (what a row of padding holds is not used)
+    const float l = col_sum(l_run[qb]);
+    if (r >= a.M) continue;
+    if (a.nsplit == 1) {
+      char* row = out_row(a, b, hk, r);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        write4<E>(a, row, 16 * dt + 4 * g, pad ? float4_t{0.f, 0.f, 0.f, 0.f} : o[qb][dt], pad ? 0.f : l);
+      if (a.lse && g == 0) write_lse(a, b, hk, r, m_run[qb], pad ? 0.f : l);
+    } else {
+      const long pr = (long)sp * a.rows + (long)bh * a.M + r;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(a.po + pr * D + 16 * dt + 4 * g) = o[qb][dt];
+      if (g == 0) {
+        a.pml[2 * pr] = m_run[qb];
+        a.pml[2 * pr + 1] = l;
+      }
+    }
+  }
+}
+
+}  // namespace carekv

@@ -18,7 +18,7 @@
 #include <cmath>
 
 #include "host_util.h"
-#include "rows_attn.h"
+#include "tile_attn.h"
 
 namespace carekv {
 
@@ -35,6 +35,144 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
   return ((x & e) + one) & 0x80008000u;
 }
 
+// Whether any of 2 n elements is: 0 times it, added up, is no number then.
+template <typename ET, int N>
+__device__ __forceinline__ bool not_finite(const uint32_t* x) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (std::is_same<typename ET::E, _Float16>::value) {
+      half2_t h;
+      __builtin_memcpy(&h, &x[i], 4);
+      sum = __builtin_amdgcn_fdot2(h, half2_t{}, sum, false);
+    } else {
+      typedef __bf16 bhalf2_t __attribute__((ext_vector_type(2)));
+      bhalf2_t h;
+      __builtin_memcpy(&h, &x[i], 4);
+      sum = __builtin_amdgcn_fdot2_f32_bf16(h, bhalf2_t{}, sum, false);
+    }
+  }
+  return !(sum == 0.f);
+}
+
+// 16-bit rows as the tiles' source.  LDS rows are padded by 32 bytes: every bank once per read pattern.
+template <typename ET_, int D_>
+struct Rows16 {
+  using Args = WindowArgs;
+  using ET = ET_;
+  using Out = typename ET::E;
+  using V8 = typename ET::V8;
+  static constexpr int D = D_, RS = 2 * D + 32, kK = 32 * RS, kV = 32 * RS, CHR = D / 8, NCH = 32 * CHR / 256;
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) short4_t lds_short4;
+  const char* kbase;
+  const char* vbase;
+  long k_st, v_st;
+  int len, lane, at, next;    // keys; the thread's place in a tile of LDS; the tile to be loaded
+  uint32_t k_off[NCH], v_off[NCH];
+  uint32_t k[NCH][4], v[NCH][4];
+
+  __device__ __forceinline__ Rows16(const Args& a, int b, int hk, const SeqRows& seq, int, int, int lane_)
+      : kbase(a.k + b * a.k_sb + hk * a.k_sh), vbase(a.v + b * a.v_sb + hk * a.v_sh), k_st(a.k_st), v_st(a.v_st),
+        len(seq.len), lane(lane_) {
+    const int row = threadIdx.x / CHR, col = threadIdx.x % CHR * 16;
+    at = row * RS + col;
+#pragma unroll
+    for (int x = 0; x < NCH; ++x) {
+      k_off[x] = (uint32_t)((row + 256 / CHR * x) * k_st + col);
+      v_off[x] = (uint32_t)((row + 256 / CHR * x) * v_st + col);
+    }
+  }
+  static __device__ __forceinline__ float load_q(V8* qf, const Args& a, int b, int hk, int r, int g) {
+    r = min(r, a.M - 1);
+    const int t = r / a.by_g, h = hk * a.G + r - t * a.G;
+    const char* qp = a.q + b * a.q_sb + h * a.q_sh + t * a.q_st;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      uint4 x = *reinterpret_cast<const uint4*>(qp + (32 * s + 8 * g) * 2);
+      x.x = (x.x ^ a.q_sign) & a.q_keep; x.y = (x.y ^ a.q_sign) & a.q_keep;
+      x.z = (x.z ^ a.q_sign) & a.q_keep; x.w = (x.w ^ a.q_sign) & a.q_keep;
+      __builtin_memcpy(&qf[s], &x, 16);
+    }
+    return a.sm_log2;
+  }
+  // a tile is a buffer resource of its rows, a thread's offsets in it stay the same; rows past the length read zeros
+  static __device__ __forceinline__ void load(uint32_t (&x)[NCH][4], const char* base, long st, const uint32_t (&off)[NCH],
+                                              int j0, int len) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (long)j0 * st, (uint32_t)((min(32, len - j0) - 1) * st + 2 * D));
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const auto u = __builtin_amdgcn_raw_buffer_load_b128(r, off[i], 0, 0);
+      x[i][0] = u[0]; x[i][1] = u[1]; x[i][2] = u[2]; x[i][3] = u[3];
+    }
+  }
+  __device__ __forceinline__ void look(int tile) { next = tile; }
+  __device__ __forceinline__ void load() {
+    load(k, kbase, k_st, k_off, 32 * next, len);
+    load(v, vbase, v_st, v_off, 32 * next, len);
+  }
+  __device__ __forceinline__ bool store(char* kb, char* vb, int) {
+    const bool odd = not_finite<ET, 4 * NCH>(&v[0][0]);
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t u = not_finite2<ET>(v[i][x]);
+          v[i][x] &= (u & 0x8000u ? 0u : 0xffffu) | (u >> 31 ? 0u : 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      *reinterpret_cast<uint4*>(kb + at + 256 / CHR * i * RS) = make_uint4(k[i][0], k[i][1], k[i][2], k[i][3]);
+      *reinterpret_cast<uint4*>(vb + at + 256 / CHR * i * RS) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+    }
+    return odd;
+  }
+  __device__ __forceinline__ V8 k_op(const char* buf, int tt, int ks) const {
+    V8 r;
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(buf + (16 * tt + (lane & 15)) * RS + (32 * ks + 8 * (lane >> 4)) * 2);
+    return r;
+  }
+  __device__ __forceinline__ V8 v_op(const char* buf, int dt) const {
+    const __attribute__((address_space(3))) char* row = (const __attribute__((address_space(3))) char*)buf +
+                                                        (4 * (lane >> 4) + ((lane & 15) >> 2)) * RS + (lane & 3) * 8;
+    const short4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(row + 32 * dt));
+    const short4_t v2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(row + 16 * RS + 32 * dt));
+    V8 r;
+    __builtin_memcpy(&r, &v1, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &v2, 8);
+    return r;
+  }
+  __device__ __forceinline__ int there() const { return 3; }
+  // from where they came: with a weight over 0 they are the result whatever it is
+  template <int NQ, int DT>
+  __device__ __forceinline__ void odd_values(const Args& a, float4_t (&o)[NQ][DT], const RowSight (&sight)[NQ], int tile) const {
+    const int j0 = 32 * tile;
+#pragma unroll 1
+    for (int key = 0; key < min(32, len - j0); ++key) {
+      const char* src = vbase + (long)(j0 + key) * v_st + 8 * (lane >> 4);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
+        uint32_t x[2];
+        __builtin_memcpy(x, __builtin_assume_aligned(src + 32 * dt, 8), 8);
+        if (!(not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]))) continue;
+        Out e[4];
+        __builtin_memcpy(e, x, 8);
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          RowSight row = sight[qb];
+          row.stay_here();
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (row.sees(a, j0 + key) && !(fabsf((float)e[y]) < INFINITY)) o[qb][dt][y] += (float)e[y];
+        }
+      }
+    }
+  }
+};
+
 template <typename ET, int D, int WQ, int WK>
 __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_kernel(WindowArgs a) {
   using V8 = typename ET::V8;
@@ -48,9 +186,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
 
-  const int n = gridDim.x;
-  int it = blockIdx.x;
-  it = n / 8 * (it & 7) + min(it & 7, n & 7) + (it >> 3);  // an XCD takes consecutive items: blocks of the same keys
+  const int it = xcd_item(a);
   const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
   const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
   const int b = bh / a.by_hkv, hk = bh - b * a.Hkv;
@@ -106,12 +242,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   // noted and its rows' results set from the value itself)
   auto store_tile = [&](int i) {
     const int buf = NBUF == 2 ? i & 1 : 0;
-    uint32_t odd = 0;
-#pragma unroll
-    for (int k = NCH / 2; k < NCH; ++k)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) odd |= not_finite2<ET>(stg[k][x]);
-    if (__builtin_expect(odd != 0, 0)) {
+    if (__builtin_expect(not_finite<ET, 2 * NCH>(&stg[NCH / 2][0]), 0)) {
       s_odd[buf] = i;
 #pragma unroll
       for (int k = NCH / 2; k < NCH; ++k)
@@ -404,9 +535,11 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
   a.sink = p.sink;
   a.nqb = plan.nqb; a.nsplit = plan.nsplit; a.tps = plan.tps; a.qb_rows = 32 * plan.wq;
   a.by_g = FastDiv(a.G); a.by_nqb = FastDiv(a.nqb); a.by_hkv = FastDiv(a.Hkv); a.by_nsplit = FastDiv(a.nsplit); a.by_m = FastDiv(a.M);
+  a.by_group = FastDiv((long)a.nqb * a.nsplit);
   a.po = (float*)workspace;
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);
+  set_period(a, p.window, (a.qb_rows + a.G - 1) / a.G, 32 * plan.wk);
   a.al8 = (operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}}) & 7) == 0;
   hipStream_t s = (hipStream_t)stream;
   const long wgs = (long)p.batch * a.Hkv * a.nqb * a.nsplit;
@@ -416,7 +549,7 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
     constexpr int D = decltype(d)::value;
     const dim3 grid((unsigned)wgs), block(256);
     if (plan.wq == 1) hipLaunchKernelGGL((window_attn_kernel<ET, D, 1, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((window_attn_kernel<ET, D, 4, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tile_attn_kernel<Rows16<ET, D>>), grid, block, 0, s, a);
     CAREKV_CHECK_LAUNCH("window_attn");
     if (a.nsplit > 1) {
       constexpr int RW = 256 / D;
