@@ -81,15 +81,6 @@ def _ptr(x: Optional[torch.Tensor]):
     return None if x is None else x.data_ptr()
 
 
-def _outside(x: torch.Tensor, block: torch.Tensor) -> bool:
-    """Whether x has no memory in common with the packed block."""
-    at, lo = x.data_ptr(), block.data_ptr()
-    if at >= lo + block.nbytes:
-        return True
-    reach = sum([(n - 1) * s for n, s in zip(x.shape, x.stride())])
-    return at + (reach + 1) * x.element_size() <= lo or not _lib.overlap(block, x)
-
-
 def _check_table(table: torch.Tensor, batch: int) -> torch.Tensor:
     if table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32:
         raise ValueError(f"table must be ({batch}, max_pages) int32; got {tuple(table.shape)} {table.dtype}")
@@ -158,8 +149,6 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
                              f"{tuple(positions.shape)} {positions.dtype}")
         pos = pos if pos.stride(1) == 1 or T == 1 else pos.contiguous()
         pos_bits, pos_batch = 64 if pos.dtype == torch.int64 else 32, pos.stride(0) if pos.shape[0] > 1 else 0
-    if not (_outside(k, data) and _outside(v, data) and (q is None or _outside(q, data))):
-        raise ValueError("k, v and q must not overlap the pages")
     _lib.same_device("append_pages", k, v, q, data, table, pos, freqs)
     if start is None:
         raise ValueError("append_pages needs start, the tokens that the sequences hold")
@@ -232,7 +221,7 @@ def paged_attention(q: torch.Tensor, pages: Int4Pages, table: torch.Tensor, leng
         out = q.new_empty(q.shape)
     lse = q.new_empty((B, Hq, T), dtype=torch.float32) if return_lse else None
     if out.numel():
-        qq = _lib.aligned_rows(q)
+        qq = _lib.aligned_rows(q) if not q.is_contiguous() or q.data_ptr() % 16 else q
         ln = _lib.row_counts(lengths, B, dev, "lengths")
         ql = _lib.row_counts(q_lengths, B, dev, "q_lengths")
         pp = _lib.PagedParams(B, Hq, pages.n_kv_heads, T, D, _lib.DTYPE_CODE[q.dtype], pages.n_pages, table.shape[1],

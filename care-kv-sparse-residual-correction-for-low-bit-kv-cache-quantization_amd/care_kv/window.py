@@ -58,7 +58,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         out = q.new_empty(q.shape)
     lse = q.new_empty((B, Hq, Tq), dtype=torch.float32) if return_lse else None
     if out.numel():
-        q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k, near=True), _lib.aligned_rows(v, near=True)
+        if not q.is_contiguous() or q.data_ptr() % 16:
+            q = _lib.aligned_rows(q)
+        k, v = (x if x.is_contiguous() and x.data_ptr() % 16 == 0 else _lib.aligned_rows(x, near=True) for x in (k, v))
         ln = _lib.row_counts(lengths, B, dev, "lengths")
         qs = _lib.row_counts(q_start, B, dev, "q_start")
         ql = ln if q_lengths is None and q_start is None and Tq == Tk else \

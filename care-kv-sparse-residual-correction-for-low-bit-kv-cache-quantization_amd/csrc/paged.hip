@@ -82,7 +82,7 @@ __device__ __forceinline__ float load_q4(half8_t* qf, const RowsArgs& a, int b, 
 }
 
 template <typename E, int D, int NQ>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedArgs a) {
   using P = Page4<D>;
   constexpr int W = D / 32, KS = D / 32, DT = D / 16, QB = 16 * NQ;
   constexpr float kUp = ElemF16::kUp;
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
 
   const char* pool = a.pages + (long)hk * P::kBytes;
   const long page_bytes = (long)a.Hkv * P::kBytes;
-  const int32_t* table = a.table + b * a.table_sb;
+  // (scalar loads: vector ones come back in order, behind the codes on their way)
+  const cint32_t* table = (const cint32_t*)(a.table + b * a.table_sb);
   auto page_of = [&](int tile, int i) {  // -1: not there
     const int at = 2 * tile + i;
     const int p = table[min(at, a.max_pages - 1)];
@@ -136,24 +137,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
     }
   };
 
-  Tile4<D> cur;
-  int p0 = -1, p1 = -1;
-  if (i0 + w < i1) {
-    const int tile = span.tile(i0 + w);
-    p0 = page_of(tile, 0);
-    p1 = page_of(tile, 1);
-    load(cur, p0, p1);
-  }
-  for (int i = i0 + w; i < i1; i += 4) {
+  const Unpack4 dequant4;
+  // tile i, whose codes are in cur, of pages p0 and p1
+  auto work = [&](Tile4<D>& cur, int p0, int p1, int i) {
     const int j0 = span.tile(i) * kTile;
-    Tile4<D> next;
-    int n0 = -1, n1 = -1;
-    if (i + 4 < i1) {
-      const int tile = span.tile(i + 4);
-      n0 = page_of(tile, 0);
-      n1 = page_of(tile, 1);
-      load(next, n0, n1);
-    }
     float4_t s[2][NQ];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -266,9 +253,24 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
         }
       }
     }
-    cur = next;
-    p0 = n0;
-    p1 = n1;
+  };
+  // the next tile's codes are on their way while one is worked on, two tiles a turn: nothing is moved between them
+  Tile4<D> x, y;
+  int x0 = -1, x1 = -1, y0 = -1, y1 = -1;
+  auto fetch = [&](Tile4<D>& t, int& p0, int& p1, int i) {
+    if (i >= i1) return;
+    const int tile = span.tile(i);
+    p0 = page_of(tile, 0);
+    p1 = page_of(tile, 1);
+    load(t, p0, p1);
+  };
+  fetch(x, x0, x1, i0 + w);
+  for (int i = i0 + w; i < i1; i += 8) {
+    fetch(y, y0, y1, i + 4);
+    work(x, x0, x1, i);
+    if (i + 4 >= i1) break;
+    fetch(x, x0, x1, i + 8);
+    work(y, y0, y1, i + 4);
   }
 
   // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum, 16 rows at a time,
@@ -336,7 +338,7 @@ struct Pages4 {
   using P = Page4<D_>;
   static constexpr int D = D_, W = D / 32, KS = D / 32, NW = W / 2, kK = 2 * KS * 1024, kV = D / 16 * 1024;
   const char* pool;
-  const int32_t* table;
+  const cint32_t* table;  // (scalar loads)
   long page_bytes;
   int n_pages, max_pages, hi, lane, g, c16, pg, half;  // pg, half: the wave's page of a tile and half of its words
   uint32_t kw[NW], vw[NW];
@@ -346,7 +348,7 @@ struct Pages4 {
   int loaded, held;  // which pages of the tile on its way, of the tile stored last, are there: bit i, page i
 
   __device__ __forceinline__ Pages4(const Args& a, int b, int hk, const SeqRows&, int hi_, int w, int lane_)
-      : pool(a.pages + (long)hk * P::kBytes), table(a.table + b * a.table_sb), page_bytes((long)a.Hkv * P::kBytes),
+      : pool(a.pages + (long)hk * P::kBytes), table((const cint32_t*)(a.table + b * a.table_sb)), page_bytes((long)a.Hkv * P::kBytes),
         n_pages(a.n_pages), max_pages(a.max_pages), hi(hi_), lane(lane_), g(lane_ >> 4), c16(lane_ & 15), pg(w >> 1),
         half(w & 1), loaded(0), held(0) {}
   static __device__ __forceinline__ float load_q(V8* qf, const Args& a, int b, int hk, int r, int g) {
@@ -390,6 +392,7 @@ struct Pages4 {
       for (int x = 0; x < 4 * NW; ++x)
         if ((half2bits(vs[x / 2][x & 1]) & 0x7c00) == 0x7c00) vs[x / 2][x & 1] = (_Float16)0.f;
     }
+    const Unpack4 dequant4;
     const _Float16 kf = bits2half(ks);
     const half2_t ks2 = {kf, kf}, kss[4] = {ks2, ks2, ks2, ks2};
 #pragma unroll
@@ -535,7 +538,7 @@ extern "C" int carekv_paged_attn(const carekv_paged_params* pp, const void* q, c
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);
   set_period(a, p.window, (a.qb_rows + a.G - 1) / a.G, kTile);
-  a.al8 = (operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}}) & 7) == 0;
+  set_alignment(a, p.batch);
   a.table = table; a.pages = (const char*)pages; a.table_sb = p.table_sb; a.n_pages = p.n_pages; a.max_pages = p.max_pages;
   hipStream_t s = (hipStream_t)stream;
   const long wgs = (long)p.batch * a.Hkv * a.nqb * a.nsplit;

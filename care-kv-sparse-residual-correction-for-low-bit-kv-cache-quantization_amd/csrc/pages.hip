@@ -255,6 +255,14 @@ extern "C" int carekv_append_pages(const carekv_append_params* pp, const void* q
   CAREKV_REQUIRE(k && v && start && (p.rotary_dim == 0 || freqs) && (p.n_heads == 0 || (q && q_out)) &&
                      (p.max_pages == 0 || table) && (p.n_pages == 0 || pages) && !k_hat == !v_hat, "null argument");
   CAREKV_REQUIRE((((uintptr_t)pages | (uintptr_t)k_hat | (uintptr_t)v_hat) & 15) == 0, "pages, k_hat and v_hat must be 16-byte aligned");
+  // the bytes from an operand's first value to behind its last
+  auto apart = [&](const void* x, int heads, int64_t sb, int64_t sh, int64_t st) {
+    const int64_t reach = 2 * ((p.batch - 1) * sb + (heads - 1) * sh + (p.seq_len - 1) * st + p.head_dim);
+    const uintptr_t lo = (uintptr_t)pages, hi = lo + (uintptr_t)p.n_pages * p.n_kv_heads * carekv_page4_bytes(p.head_dim);
+    return (uintptr_t)x >= hi || (uintptr_t)x + reach <= lo;
+  };
+  CAREKV_REQUIRE(apart(k, p.n_kv_heads, p.k_sb, p.k_sh, p.k_st) && apart(v, p.n_kv_heads, p.v_sb, p.v_sh, p.v_st) &&
+                     (p.n_heads == 0 || apart(q, p.n_heads, p.q_sb, p.q_sh, p.q_st)), "k, v and q must not overlap the pages");
   AppendArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.qo = (char*)q_out;
   a.k_hat = (uint16_t*)k_hat; a.v_hat = (uint16_t*)v_hat;

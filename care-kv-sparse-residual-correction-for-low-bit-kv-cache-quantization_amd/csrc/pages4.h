@@ -40,18 +40,24 @@ __host__ __device__ constexpr int nib4(int e) { return 4 * ((e & 1) * 4 + (e >> 
 // The codes of a word as fp16: 1024 + u in the mantissa of each half, then - 1032
 // (a nibble four bits up: 1024 + 16 u, times 1 / 16, - 72), both exact; times
 // their scales, rounded once as the definition has it.  s[i]: codes 2i and 2i + 1.
-__device__ __forceinline__ void dequant4(half2_t* v, uint32_t w, const half2_t* s) {
-  const half2_t one16 = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-1032.f, (_Float16)-1032.f},
-                off16 = {(_Float16)-72.f, (_Float16)-72.f};
+// The masks sit in vector registers, the exponents in a scalar one: an instruction
+// takes one scalar operand and no literal, and the compiler else spends an AND and
+// an OR on each pair.
+struct Unpack4 {
+  uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;
+  __device__ __forceinline__ Unpack4() { asm volatile("" : "+v"(lo), "+v"(hi), "+s"(one)); }
+  __device__ __forceinline__ void operator()(half2_t* v, uint32_t w, const half2_t* s) const {
+    const half2_t one16 = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-1032.f, (_Float16)-1032.f},
+                  off16 = {(_Float16)-72.f, (_Float16)-72.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = i < 2 ? w : w >> 8;
-    const uint32_t bits = (x & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
-    half2_t h;
-    __builtin_memcpy(&h, &bits, 4);
-    h = i & 1 ? __builtin_elementwise_fma(h, one16, off16) : h + off;
-    v[i] = h * s[i];
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = ((i < 2 ? w : w >> 8) & (i & 1 ? hi : lo)) | one;
+      half2_t h;
+      __builtin_memcpy(&h, &bits, 4);
+      h = i & 1 ? __builtin_elementwise_fma(h, one16, off16) : h + off;
+      v[i] = h * s[i];
+    }
   }
-}
+};
 
 }  // namespace carekv

@@ -35,7 +35,7 @@ struct RowsArgs {
   FastDiv by_period;         // tiles of a window and a block's tokens (see Span)
   float sm_log2;             // |scale| log2(e), 1 where that is 0
   uint32_t q_sign, q_keep;   // sign bits of two elements where the scale is negative; 0 where it is 0
-  int al8;                   // rows of out on 8 bytes
+  int al8, al16;             // rows of out on 8, on 16 bytes
 };
 
 // The work-group's item.  Items come in groups of a.by_group that read the same
@@ -197,6 +197,13 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
   if (pad) { LL = 0.f; O = float4_t{0.f, 0.f, 0.f, 0.f}; }  // (what a row of padding holds is not used)
   write4<E>(a, out_row(a, b, hk, r), 4 * d4, O, LL);
   if (a.lse && d4 == 0) write_lse(a, b, hk, r, mm, LL);
+}
+
+// Whether rows of out lie on 8 and on 16 bytes.
+inline void set_alignment(RowsArgs& a, int batch) {
+  const uintptr_t bits = operand_bits(a.out, {{batch, a.o_sb}, {a.Hq, a.o_sh}, {a.T, a.o_st}});
+  a.al8 = (bits & 7) == 0;
+  a.al16 = (bits & 15) == 0;
 }
 
 // The period of blocks of `tokens` tokens and tiles of kt keys.

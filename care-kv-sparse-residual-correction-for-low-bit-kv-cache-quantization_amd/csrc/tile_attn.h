@@ -154,18 +154,27 @@ __global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a)
     __syncthreads();
   }
 
-  // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
+  // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..).  Results go through the
+  // wave's part of LDS, 16-byte pieces exchanged against bank conflicts, so that whole rows are written.
+  char* turned = lds + w * (QW * 2 * D);
+  static_assert(4 * QW * 2 * D <= 2 * BUF, "the waves' results fit the tiles' LDS");
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) {
     const int r = r0 + 16 * qb + c16;
     const bool pad = sight[qb].top < 0;  // (what a row of padding holds is not used)
     const float l = col_sum(l_run[qb]);
+    const float inv = pad || l == 0.f ? 0.f : 1.f / l;
+    if (a.nsplit == 1) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        E e[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) e[x] = pad ? (E)0.f : (E)(o[qb][dt][x] * inv);
+        __builtin_memcpy(turned + (16 * qb + c16) * (2 * D) + ((2 * dt + (g >> 1)) ^ (c16 & (D / 8 - 1))) * 16 + (g & 1) * 8, e, 8);
+      }
+    }
     if (r >= a.M) continue;
     if (a.nsplit == 1) {
-      char* row = out_row(a, b, hk, r);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        write4<E>(a, row, 16 * dt + 4 * g, pad ? float4_t{0.f, 0.f, 0.f, 0.f} : o[qb][dt], pad ? 0.f : l);
       if (a.lse && g == 0) write_lse(a, b, hk, r, m_run[qb], pad ? 0.f : l);
     } else {
       const long pr = (long)sp * a.rows + (long)bh * a.M + r;
@@ -176,6 +185,18 @@ __global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a)
         a.pml[2 * pr + 1] = l;
       }
     }
+  }
+  if (a.nsplit > 1) return;
+  lds_sync_wave();
+  constexpr int CH = D / 8, RP = 64 / CH;  // pieces of a row, rows at a time
+#pragma unroll
+  for (int x = 0; x < QW / RP; ++x) {
+    const int row = RP * x + lane / CH, piece = lane % CH, r = r0 + row;
+    if (r >= a.M) break;
+    const uint4 u = *reinterpret_cast<const uint4*>(turned + row * (2 * D) + (piece ^ (row & (CH - 1))) * 16);
+    char* dst = out_row(a, b, hk, r) + 16 * piece;
+    if (a.al16) *reinterpret_cast<uint4*>(dst) = u;
+    else __builtin_memcpy(dst, &u, 16);
   }
 }
 

@@ -456,8 +456,13 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
 
 namespace {
 // How a call is cut: at most 32 rows a kv head share the work-group's waves by
-// keys (wq = 1, wk = 4), more by rows; key splits, each of at least 4 tiles, until
-// 768 work-groups (3 a CU) are there.
+// keys (wq = 1, wk = 4, tiles of 128 keys), more by rows (wq = 4, wk = 1, 32 keys).
+// Few rows: key splits until 512 work-groups (2 a CU) are there, down to a tile
+// each, at most 32 for the join's sake; us a call, by splits: 32 / 4 heads, D = 64,
+// on 1000 keys 1 / 4 / 8: 12.9 / 8.9 / 8.1, on 4097 4 / 8 / 16 / 32: 16.6 / 12.5 / 10.7 /
+// 10.3; 16 x 32 / 8 heads, D = 128, on 4097 2 / 4 / 8 / 16: 47.9 / 46.9 / 48.4 / 50.9.  Many: of
+// at least 4 tiles until 768 (3 a CU) are there: 300 rows of 32 / 8 heads on 4097 3 / 6 /
+// 8 / 12 / 16: 67.6 / 51.5 / 54.7 / 58.7 / 60.5.
 struct WindowPlan {
   int wq, wk, nqb, nsplit, tps;
 };
@@ -471,7 +476,8 @@ WindowPlan window_plan(const carekv_window_params& p) {
   long keys = p.n_keys;  // that a block of rows may see
   if (p.window > 0) keys = std::min(keys, (long)p.window + std::min<long>(p.seq_len, 32L * r.wq) + p.sink + 2 * kt);
   const long tiles = std::max(1L, (keys + kt - 1) / kt), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
-  const long ns = tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
+  const long ns = r.wq == 1 ? (tiles <= 2 ? 1 : std::max(1L, std::min(std::min(32L, 512 / wgs), tiles)))
+                            : tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
   return r;
@@ -540,7 +546,7 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);
   set_period(a, p.window, (a.qb_rows + a.G - 1) / a.G, 32 * plan.wk);
-  a.al8 = (operand_bits(out, {{p.batch, a.o_sb}, {p.n_heads, a.o_sh}, {p.seq_len, a.o_st}}) & 7) == 0;
+  set_alignment(a, p.batch);
   hipStream_t s = (hipStream_t)stream;
   const long wgs = (long)p.batch * a.Hkv * a.nqb * a.nsplit;
   CAREKV_REQUIRE(grid_fits(wgs, 256) && grid_fits(rows / (256 / p.head_dim) + 1, 256), "too many rows");

@@ -51,9 +51,6 @@ def test_append_refusals():
     for kw in bad:
         with pytest.raises(ValueError):
             care_kv.append_pages(**{**base, **kw})
-    inside = pg.data.view(-1)[:2 * 2 * 3 * 64 * 2].view(torch.float16).view(2, 2, 3, 64)
-    with pytest.raises(ValueError):
-        care_kv.append_pages(pg, tb, 0, inside, v)
     with pytest.raises(_lib.CarekvError):  # no device tensors
         care_kv.append_pages(**base)
 
@@ -114,6 +111,11 @@ def test_c_refusals():
         assert append(**kw) == -1 and "carekv_append_pages" in _last()
     assert append(batch=0) == 0 and append(seq_len=0) == 0
     assert lib.carekv_append_pages(None, *none12, None) == -1
+    p = _lib.AppendParams(1, 0, 2, 1, 64, 0, 0, 0, 64, 4, 2, 1.0, 0, 2, 0, 0, 0, 128, 64, 128, 128, 64, 128, 0, 0, 0)
+    pool = 1 << 20  # (an address that nothing is read from: the calls are refused first)
+    for k, v in ((pool + 4 * 2304 - 16, pool - 4096), (pool - 4096, pool), (pool - 240, pool - 4096), (pool - 4096, pool - 128)):
+        assert lib.carekv_append_pages(p, None, k, v, None, None, pool, None, pool, pool, None, None, None, None) == -1
+        assert "overlap" in _last()
 
     def paged(**kw):
         f = dict(batch=1, n_heads=4, n_kv_heads=2, seq_len=1, head_dim=64, dtype=0, n_pages=4, max_pages=200, sm_scale=1.0)
