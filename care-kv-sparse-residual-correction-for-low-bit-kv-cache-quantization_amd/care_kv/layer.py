@@ -21,8 +21,10 @@ the HIP library:
 Without a reference counterpart: ``position_embeddings`` may be (RotaryPlan,
 positions) instead of (cos, sin) tables (``rotate_heads``), ``prefix`` =
 (k, v) puts a prefix that the whole batch shares before every sequence
-(``prefix_attention``), and cfg.prefill_keep keeps only the rows of a prompt
-that its queries attend to (``attention_mass``, ``evict_rows``).
+(``prefix_attention``), cfg.prefill_keep keeps only the rows of a prompt
+that its queries attend to (``attention_mass``, ``evict_rows``), and
+``paged_step`` runs the layer over pages of 4-bit rows instead of the CARE-KV
+cache (``append_pages``, ``paged_attention``, ``window_attention``).
 """
 from __future__ import annotations
 
@@ -37,7 +39,9 @@ from .attention import (debug_stats_enabled, decode_attention, decode_read_mode,
                         get_imp_per_layer, importance_probe, prefill_correction, reset_debug_stats)
 from .cache import CAREKVCache
 from .eviction import attention_mass, evict_rows
+from .pages import Int4Pages, append_pages, paged_attention
 from .prefix import check_prefix, prefix_attention
+from .window import window_attention
 from .rotary import RotaryPlan, rotate_heads
 from .config import CacheConfig, any_read_budget, resolve_read_knobs
 from .prefill import eval_knobs, prefill_attention, prefill_eval, quant_dequant
@@ -361,3 +365,46 @@ class CAREKVLayer(nn.Module):
                              knobs=knobs, prefix=prefix)  # (B, Hq, D)
         out = self._out(O.unsqueeze(2), hidden.dtype).to(hidden.dtype)  # (B, 1, model_dim)
         return out[0] if squeeze else out
+
+    # ------------------------------------------------------------ pages of 4-bit rows
+    def paged_step(self, pages: Int4Pages, hidden: Tensor, table: Tensor, lengths,
+                   position_embeddings: Optional[Tuple[RotaryPlan, Optional[Tensor]]] = None, *, counts=None,
+                   window: Optional[int] = None, sink: int = 0, fresh: bool = False) -> Tensor:
+        """The layer over pages of 4-bit rows (no reference counterpart): T new
+        tokens of every sequence, hidden (B, T, model_dim) -> same shape.  Their
+        K and V go behind the ``lengths[b]`` tokens that the sequence holds in
+        ``pages`` (``append_pages``), their queries attend to all of them, with
+        ``window`` to the last ``window`` and the first ``sink``
+        (``paged_attention``).  Of a ragged batch the first ``counts[b]`` tokens
+        count; what the others' rows of the result hold means nothing.  The caller
+        adds the tokens that stay to lengths: one of a decode step, the accepted
+        ones of drafts and the one behind them, all of a prompt's chunk.
+
+        position_embeddings: (RotaryPlan, positions), positions as
+        ``append_pages`` takes them or None for places in the sequence.  ``fresh``: a
+        prompt of sequences that hold nothing yet (lengths are not looked at),
+        whose attention runs over its rows as they are (``window_attention``, the
+        ``fp`` mode of ``prefill``).  Nothing waits for the device, and with tensors
+        for lengths and counts the call can be captured."""
+        plan, pos = (None, None) if position_embeddings is None else position_embeddings
+        if plan is not None and not isinstance(plan, RotaryPlan):
+            raise ValueError("paged_step: position_embeddings must be (RotaryPlan, positions or None)")
+        if hidden.dim() != 3:
+            raise ValueError(f"paged_step: hidden must be (B, T, model_dim); got {tuple(hidden.shape)}")
+        B, T, _ = hidden.shape
+        Q, K, V = self._project(hidden)
+        if Q.dtype not in (F16, torch.bfloat16):
+            Q, K, V = Q.to(F16), K.to(F16), V.to(F16)
+        n = _lib.row_counts(counts, B, Q.device, "counts")
+        if fresh:
+            if plan is not None:
+                Q, K = rotate_heads(Q, K, torch.arange(T, device=Q.device) if pos is None else pos, plan)
+            append_pages(pages, table, 0, K, V, counts=n)
+            O = window_attention(Q, K, V, window=window, sink=sink, lengths=n, q_lengths=n)
+        else:
+            if lengths is None:
+                raise ValueError("paged_step needs lengths, the tokens that the sequences hold")
+            start = _lib.row_counts(lengths, B, Q.device, "lengths")
+            Q = append_pages(pages, table, start, K, V, q=Q, plan=plan, positions=pos, counts=n)
+            O = paged_attention(Q, pages, table, start + (T if n is None else n), q_lengths=n, window=window, sink=sink)
+        return self._out(O, hidden.dtype).to(hidden.dtype)

@@ -116,8 +116,8 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
     stand for, zeros behind the counts.
 
     Tokens before place 0, behind the table or on pages that are not there are
-    dropped.  No two sequences of a call may write to one page.  The results
-    carry no autograd history."""
+    dropped.  A call may write to a page for one sequence only, and for one entry of
+    its table.  The results carry no autograd history."""
     kd, ks, dev = k.dtype, k.shape, k.device
     if len(ks) != 4 or v.shape != ks or v.dtype != kd:
         raise ValueError(f"k and v must be (B, Hkv, T, D) of one type; got {tuple(ks)} {kd}, {tuple(v.shape)} {v.dtype}")

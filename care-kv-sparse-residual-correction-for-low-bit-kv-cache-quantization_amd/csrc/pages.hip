@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendArgs a) {
     const int i = threadIdx.x % (D / 2), t = slot0 + (int)threadIdx.x / (D / 2) - start;
     if (i < half && t >= 0 && t < a.T) {
       const long pi = b * a.pos_batch + t;
-      const double p = !a.pos ? (double)(start + t)
+      const double p = !a.pos ? (double)((long)a.start[b] + t)
                               : a.pos64 ? (double)reinterpret_cast<const int64_t*>(a.pos)[pi]
                                         : (double)reinterpret_cast<const int32_t*>(a.pos)[pi];
       // t less its whole turns (2 pi in two parts), in half turns

@@ -675,8 +675,8 @@ int64_t carekv_page4_bytes(int32_t head_dim); /* head_dim 64 or 128, else -1   *
  * 0: not at all.  n_heads 0: no q.  k_hat, v_hat (both or neither): fp16 [batch]
  * [n_kv_heads][seq_len][head_dim], the values that the new rows stand for, 0
  * behind the counts.  fp16 or bf16, strides in elements, pages, k_hat and v_hat
- * 16-byte aligned; q, k and v apart from the pages.  No two sequences of a call may
- * write to one page. */
+ * 16-byte aligned; q, k and v apart from the pages.  A call may write to a page
+ * for one sequence only, and for one entry of its table. */
 typedef struct carekv_append_params {
   int32_t batch, n_heads, n_kv_heads, seq_len, head_dim, rotary_dim;
   int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */

@@ -157,7 +157,7 @@ def test_append_positions():
     plan = care_kv.rotary_plan(64, base=500000.0)
     table, n = _table(B, 2, g)
     at = torch.randint(0, 1 << 20, (B, T), generator=g, device="cuda")
-    for pos in (at, at.int(), at[:1], at[0], at.t().contiguous().t(), -at):
+    for pos in (at, at.int(), at[:1], at[0], at.t().contiguous().t(), -at, at + (1 << 31)):
         pages = care_kv.int4_pages(n, H, D)
         before = pages.data.clone()
         out = care_kv.append_pages(pages, table, 3, k, v, q=q, plan=plan, positions=pos)
@@ -207,6 +207,24 @@ def test_pages_that_are_not_there():
     care_kv.append_pages(none, table, 0, k, v)
     o = care_kv.paged_attention(r(B, 4, 3, D).half(), none, table, 5)
     assert not o.any()
+
+
+def test_nothing_to_do():
+    """No sequences, no tokens, no heads of q."""
+    import care_kv
+    pages, h = care_kv.int4_pages(4, 2, 64), lambda *s: torch.zeros(*s, dtype=F16, device="cuda")
+    before = pages.data.clone()
+    for B, T in ((0, 3), (2, 0), (0, 0)):
+        table = torch.zeros(B, 2, dtype=torch.int32, device="cuda")
+        out, kh, vh = care_kv.append_pages(pages, table, 0, h(B, 2, T, 64), h(B, 2, T, 64), q=h(B, 4, T, 64), return_hat=True)
+        assert out.shape == (B, 4, T, 64) and kh.shape == vh.shape == (B, 2, T, 64)
+        o, lse = care_kv.paged_attention(h(B, 4, T, 64), pages, table, 0, return_lse=True)
+        assert o.shape == (B, 4, T, 64) and lse.shape == (B, 4, T)
+    assert torch.equal(pages.data, before)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    assert care_kv.append_pages(pages, table, 0, h(1, 2, 1, 64), h(1, 2, 1, 64)) is None
+    o, lse = care_kv.paged_attention(h(1, 4, 3, 64), pages, table, 0, return_lse=True)
+    assert not o.any() and (lse == -math.inf).all()
 
 
 def _case(seed, B, Hq, Hkv, D, T, N, dtype, mul=1.0):

@@ -110,6 +110,15 @@ def test_not_a_number_where_a_row_does_not_look(dtype, Tq, Tk, G):
                 assert ((got[1].double() - ref[1]).abs() <= ref[3])[0, hs][:, ~hit & see[0].any(-1)].all()
 
 
+def test_nothing_to_see():
+    """No sequences, no rows, no keys."""
+    import care_kv
+    for B, Tq, Tk in ((0, 3, 4), (2, 0, 4), (2, 3, 0), (2, 0, 0)):
+        q, k, v = _inputs(1, B, 4, 2, 64, Tq, Tk, F16)
+        o, lse = care_kv.window_attention(q, k, v, window=4, return_lse=True)
+        assert o.shape == q.shape and lse.shape == (B, 4, Tq) and not o.any() and (lse == -math.inf).all()
+
+
 def test_extreme_logits():
     import care_kv
     q, k, v = _inputs(7, 2, 4, 2, 64, 50, 400, F16)
