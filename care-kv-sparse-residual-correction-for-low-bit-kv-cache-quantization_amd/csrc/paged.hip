@@ -456,6 +456,9 @@ namespace {
 // on 8191 through a window of 4096 2 / 4 / 6 / 8: 39 / 34 / 39 / 39; 64 rows on 32768 2 / 4
 // / 6 / 8: 479 / 461 / 460 / 463.  512 rows of 40 heads on 16896 1 / 2 / 3 / 4 / 6: 877 / 568 /
 // 608 / 533 / 548.
+// Up to 1024 keys (D = 128: 512) of few rows one split: the join's launch costs the
+// host 4 us, its splits save less (one row on 500 keys split 7.9 / 9.3 us on the GPU,
+// whole 6.9 / 9.1, with the host 16.8 and 12.6; on 1000 keys 7.9 / 9.3 and 9.9 / 13.1).
 struct PagedPlan {
   int nq, nqb, nsplit, tps;  // nq: 16-row sub-blocks, 8 for the kernel of many rows
 };
@@ -471,7 +474,8 @@ PagedPlan paged_plan(const carekv_paged_params& p) {
   }
   const long tiles = std::max(1L, (keys + kTile - 1) / kTile), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
   const long at = r.nq == 8 ? 1280 : wgs * tiles < 512 * 64 ? 512 : 2048;  // work-groups
-  const long ns = std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
+  const bool whole = r.nq < 8 && tiles * p.head_dim <= 32 * 64;
+  const long ns = whole ? 1 : std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
   return r;
