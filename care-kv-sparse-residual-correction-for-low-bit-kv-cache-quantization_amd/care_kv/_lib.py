@@ -9,6 +9,7 @@ import collections
 import ctypes as C
 import operator
 import os
+import struct
 import threading
 import warnings
 
@@ -134,6 +135,18 @@ class VerifyParams(C.Structure):
         [(n, C.c_int64) for n in ("target_sb", "target_st", "draft_probs_sb", "draft_probs_st", "draft_sb", "u_sb")]
 
 
+_LETTERS = {C.c_int32: "i", C.c_float: "f", C.c_int64: "q", C.c_void_p: "P"}
+
+
+def _packer(cls):
+    """The structure's bytes from its values in order: a quarter of the time that ctypes takes to fill in one of two
+    dozen members (0.5 against 2.1 us), in calls whose kernels take five."""
+    return struct.Struct("@" + "".join(_LETTERS[t] for _, t in cls._fields_)).pack
+
+
+append_params, paged_params, window_params, verify_params = map(_packer, (AppendParams, PagedParams, WindowParams,
+                                                                           VerifyParams))
+
 # page job: int32 x 6 (seq, kv_head, page, num_valid, token_start, is_recent)
 PAGE_JOB_INTS = 6
 
@@ -248,19 +261,19 @@ def load(path: str | None = None):
         lib.carekv_page4_bytes.restype = i64
         lib.carekv_page4_bytes.argtypes = [i32]
         lib.carekv_append_pages.restype = C.c_int
-        lib.carekv_append_pages.argtypes = [C.POINTER(AppendParams)] + [vp] * 13
+        lib.carekv_append_pages.argtypes = [vp] + [vp] * 13
         lib.carekv_paged_attn.restype = C.c_int
-        lib.carekv_paged_attn.argtypes = [C.POINTER(PagedParams), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_paged_attn.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.carekv_paged_attn_workspace_bytes.restype = i64
-        lib.carekv_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedParams)]
+        lib.carekv_paged_attn_workspace_bytes.argtypes = [vp]
         lib.carekv_window_attn.restype = C.c_int
-        lib.carekv_window_attn.argtypes = [C.POINTER(WindowParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_window_attn.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.carekv_window_attn_workspace_bytes.restype = i64
-        lib.carekv_window_attn_workspace_bytes.argtypes = [C.POINTER(WindowParams)]
+        lib.carekv_window_attn_workspace_bytes.argtypes = [vp]
         lib.carekv_verify_drafts.restype = C.c_int
-        lib.carekv_verify_drafts.argtypes = [C.POINTER(VerifyParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+        lib.carekv_verify_drafts.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.carekv_verify_drafts_workspace_bytes.restype = i64
-        lib.carekv_verify_drafts_workspace_bytes.argtypes = [C.POINTER(VerifyParams)]
+        lib.carekv_verify_drafts_workspace_bytes.argtypes = [vp]
         _lib = lib
         return lib
 

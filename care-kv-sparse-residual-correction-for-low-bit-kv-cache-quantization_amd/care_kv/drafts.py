@@ -58,7 +58,7 @@ def verify_drafts(draft: torch.Tensor, target_probs: torch.Tensor, u: torch.Tens
             return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
         draft, p, u, u_next = packed(draft.to(torch.int64)), packed(target_probs), packed(u), packed(u_next)
         q = None if draft_probs is None or T == 0 else packed(draft_probs)
-        pp = _lib.VerifyParams(B, T, V, _lib.DTYPE_CODE[p.dtype], *p.stride()[:2],
+        pp = _lib.verify_params(B, T, V, _lib.DTYPE_CODE[p.dtype], *p.stride()[:2],
                                *((0, 0) if q is None else q.stride()[:2]), draft.stride(0), u.stride(0))
         lib = _lib.load()
         nbytes = lib.carekv_verify_drafts_workspace_bytes(pp)

@@ -153,10 +153,11 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
     if start is None:
         raise ValueError("append_pages needs start, the tokens that the sequences hold")
     if q is not None:
-        qo = q.new_empty(q.shape)
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     kh = vh = None
     if return_hat:
-        kh, vh = k.new_empty(ks, dtype=torch.float16), k.new_empty(ks, dtype=torch.float16)
+        kh = torch.empty_like(k, dtype=torch.float16, memory_format=torch.contiguous_format)
+        vh = torch.empty_like(kh)
     if B and T:
         sk, sv = k.stride(), v.stride()
         if sk[3] != 1:
@@ -170,7 +171,7 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
                 q = q.contiguous()
             sq, so = q.stride(), qo.stride()
         st, ct = _lib.row_counts(start, B, dev, "start"), _lib.row_counts(counts, B, dev, "counts")
-        pp = _lib.AppendParams(B, Hq, Hkv, T, D, R, _lib.DTYPE_CODE[kd], layout, pos_bits, n_pages, table.shape[1], scale,
+        pp = _lib.append_params(B, Hq, Hkv, T, D, R, _lib.DTYPE_CODE[kd], layout, pos_bits, n_pages, table.shape[1], scale,
                                pos_batch, table.stride(0), sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                                so[0], so[1], so[2])
         _lib.call(dev, "carekv_append_pages", _lib.load().carekv_append_pages, pp, _ptr(q), k.data_ptr(), v.data_ptr(),
@@ -218,13 +219,13 @@ def paged_attention(q: torch.Tensor, pages: Int4Pages, table: torch.Tensor, leng
     if lengths is None:
         raise ValueError("paged_attention needs lengths")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, Hq, T), dtype=torch.float32) if return_lse else None
     if out.numel():
         qq = _lib.aligned_rows(q) if not q.is_contiguous() or q.data_ptr() % 16 else q
         ln = _lib.row_counts(lengths, B, dev, "lengths")
         ql = _lib.row_counts(q_lengths, B, dev, "q_lengths")
-        pp = _lib.PagedParams(B, Hq, pages.n_kv_heads, T, D, _lib.DTYPE_CODE[q.dtype], pages.n_pages, table.shape[1],
+        pp = _lib.paged_params(B, Hq, pages.n_kv_heads, T, D, _lib.DTYPE_CODE[q.dtype], pages.n_pages, table.shape[1],
                               window, sink, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), table.stride(0),
                               *qq.stride()[:3], *out.stride()[:3])
         lib = _lib.load()

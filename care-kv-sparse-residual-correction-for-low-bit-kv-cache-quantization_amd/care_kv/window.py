@@ -55,7 +55,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
             raise ValueError("out must not overlap k or v")
     dev = _lib.same_device("window_attention", q, k, v, out)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, Hq, Tq), dtype=torch.float32) if return_lse else None
     if out.numel():
         if not q.is_contiguous() or q.data_ptr() % 16:
@@ -65,7 +65,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         qs = _lib.row_counts(q_start, B, dev, "q_start")
         ql = ln if q_lengths is None and q_start is None and Tq == Tk else \
             _lib.row_counts(q_lengths, B, dev, "q_lengths")
-        pp = _lib.WindowParams(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], window, sink,
+        pp = _lib.window_params(B, Hq, Hkv, Tq, Tk, D, _lib.DTYPE_CODE[q.dtype], window, sink,
                                1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), *q.stride()[:3],
                                *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
         lib = _lib.load()

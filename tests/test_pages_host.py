@@ -105,13 +105,13 @@ def test_c_refusals():
     def append(**kw):
         f = dict(batch=1, n_heads=4, n_kv_heads=2, seq_len=1, head_dim=64, rotary_dim=64, dtype=0, pos_bits=64, n_pages=4,
                  max_pages=2, scale=1.0)
-        return lib.carekv_append_pages(_lib.AppendParams(**{**f, **kw}), *none12, None)
+        return lib.carekv_append_pages(C.byref(_lib.AppendParams(**{**f, **kw})), *none12, None)
     for kw in (dict(head_dim=96), dict(dtype=2), dict(batch=-1), dict(n_kv_heads=0), dict(rotary_dim=63), dict(rotary_dim=66),
                dict(seq_len=1 << 29), dict(max_pages=1 << 25), dict(n_pages=-1), {}):
         assert append(**kw) == -1 and "carekv_append_pages" in _last()
     assert append(batch=0) == 0 and append(seq_len=0) == 0
     assert lib.carekv_append_pages(None, *none12, None) == -1
-    p = _lib.AppendParams(1, 0, 2, 1, 64, 0, 0, 0, 64, 4, 2, 1.0, 0, 2, 0, 0, 0, 128, 64, 128, 128, 64, 128, 0, 0, 0)
+    p = _lib.append_params(1, 0, 2, 1, 64, 0, 0, 0, 64, 4, 2, 1.0, 0, 2, 0, 0, 0, 128, 64, 128, 128, 64, 128, 0, 0, 0)
     pool = 1 << 20  # (an address that nothing is read from: the calls are refused first)
     for k, v in ((pool + 4 * 2304 - 16, pool - 4096), (pool - 4096, pool), (pool - 240, pool - 4096), (pool - 4096, pool - 128)):
         assert lib.carekv_append_pages(p, None, k, v, None, None, pool, None, pool, pool, None, None, None, None) == -1
@@ -119,7 +119,7 @@ def test_c_refusals():
 
     def paged(**kw):
         f = dict(batch=1, n_heads=4, n_kv_heads=2, seq_len=1, head_dim=64, dtype=0, n_pages=4, max_pages=200, sm_scale=1.0)
-        p = _lib.PagedParams(**{**f, **kw})
+        p = C.byref(_lib.PagedParams(**{**f, **kw}))
         return lib.carekv_paged_attn(p, *none6, 0, None), lib.carekv_paged_attn_workspace_bytes(p)
     for kw in (dict(head_dim=32), dict(dtype=2), dict(batch=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(window=-1), dict(sink=-1),
                dict(max_pages=1 << 25), dict(seq_len=1 << 29), dict(batch=1 << 20, seq_len=1 << 20)):
@@ -128,7 +128,7 @@ def test_c_refusals():
     assert paged(batch=0)[0] == 0
     buf = torch.zeros(64, dtype=torch.int64)  # (never read: the calls are refused first)
     at = buf.data_ptr() + -buf.data_ptr() % 16
-    big = _lib.PagedParams(**dict(batch=1, n_heads=4, n_kv_heads=1, seq_len=1, head_dim=64, dtype=0, n_pages=4, max_pages=4000, sm_scale=1.0))
+    big = C.byref(_lib.PagedParams(batch=1, n_heads=4, n_kv_heads=1, seq_len=1, head_dim=64, dtype=0, n_pages=4, max_pages=4000, sm_scale=1.0))
     need = lib.carekv_paged_attn_workspace_bytes(big)
     assert need > 0
     assert lib.carekv_paged_attn(big, at, at, at, at, None, at, None, at, need - 1, None) == -3
@@ -136,7 +136,7 @@ def test_c_refusals():
 
     def window(**kw):
         f = dict(batch=1, n_heads=4, n_kv_heads=2, seq_len=1, n_keys=5, head_dim=64, dtype=0, sm_scale=1.0)
-        p = _lib.WindowParams(**{**f, **kw})
+        p = C.byref(_lib.WindowParams(**{**f, **kw}))
         return lib.carekv_window_attn(p, *([None] * 9), 0, None), lib.carekv_window_attn_workspace_bytes(p)
     for kw in (dict(head_dim=32), dict(dtype=2), dict(n_keys=-1), dict(n_heads=3), dict(window=-1), dict(n_keys=1 << 29),
                dict(k_st=1 << 22), dict(v_st=-1)):
@@ -144,7 +144,7 @@ def test_c_refusals():
     assert window()[0] == -1 and window(batch=0)[0] == 0
 
     def verify(**kw):
-        p = _lib.VerifyParams(**{**dict(batch=1, n_drafts=2, vocab=9, dtype=2), **kw})
+        p = C.byref(_lib.VerifyParams(**{**dict(batch=1, n_drafts=2, vocab=9, dtype=2), **kw}))
         return lib.carekv_verify_drafts(p, *([None] * 9), 0, None), lib.carekv_verify_drafts_workspace_bytes(p)
     for kw in (dict(dtype=3), dict(vocab=0), dict(batch=-1), dict(n_drafts=-1), dict(batch=1 << 16), dict(vocab=1 << 30)):
         assert verify(**kw) == (-1, -1)
@@ -156,3 +156,7 @@ def test_structs_match_the_header():
     assert C.sizeof(_lib.PagedParams) == 11 * 4 + 4 + 7 * 8
     assert C.sizeof(_lib.WindowParams) == 10 * 4 + 12 * 8
     assert C.sizeof(_lib.VerifyParams) == 4 * 4 + 6 * 8
+    for pack, cls in ((_lib.append_params, _lib.AppendParams), (_lib.paged_params, _lib.PagedParams),
+                      (_lib.window_params, _lib.WindowParams), (_lib.verify_params, _lib.VerifyParams)):
+        v = list(range(1, len(cls._fields_) + 1))
+        assert pack(*v) == bytes(cls(*v))
