@@ -121,11 +121,6 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedA
   const long page_bytes = (long)a.Hkv * P::kBytes;
   // (scalar loads: vector ones come back in order, behind the codes on their way)
   const cint32_t* table = (const cint32_t*)(a.table + b * a.table_sb);
-  auto page_of = [&](int tile, int i) {  // -1: not there
-    const int at = 2 * tile + i;
-    const int p = table[min(at, a.max_pages - 1)];
-    return at < a.max_pages && p >= 0 && p < a.n_pages ? p : -1;
-  };
   auto load = [&](Tile4<D>& x, int p0, int p1) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -254,16 +249,25 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedA
       }
     }
   };
-  // the next tile's codes are on their way while one is worked on, two tiles a turn: nothing is moved between them
+  // the next tile's codes are on their way while one is worked on, two tiles a turn: nothing is moved between them; the
+  // pages of the tile behind that are looked up (and checked when they are used: checked at once, they would be waited
+  // for at once)
   Tile4<D> x, y;
-  int x0 = -1, x1 = -1, y0 = -1, y1 = -1;
+  int x0 = -1, x1 = -1, y0 = -1, y1 = -1, at, n0, n1;
+  auto look = [&](int i) {
+    at = 2 * span.tile(max(min(i, i1 - 1), 0));
+    n0 = table[min(at, a.max_pages - 1)];
+    n1 = table[min(at + 1, a.max_pages - 1)];
+  };
+  auto checked = [&](int at, int p) { return at < a.max_pages && p >= 0 && p < a.n_pages ? p : -1; };  // -1: not there
   auto fetch = [&](Tile4<D>& t, int& p0, int& p1, int i) {
     if (i >= i1) return;
-    const int tile = span.tile(i);
-    p0 = page_of(tile, 0);
-    p1 = page_of(tile, 1);
+    p0 = checked(at, n0);
+    p1 = checked(at + 1, n1);
     load(t, p0, p1);
+    look(i + 4);
   };
+  if (i0 < i1) look(i0 + w);
   fetch(x, x0, x1, i0 + w);
   for (int i = i0 + w; i < i1; i += 8) {
     fetch(y, y0, y1, i + 4);
@@ -344,7 +348,7 @@ struct Pages4 {
   uint32_t kw[NW], vw[NW];
   half2_t vs[2 * NW];
   uint16_t ks;
-  int p0, p1;        // the next tile's pages
+  int at, p0, p1;    // the next tile's places in the table and what is there
   int loaded, held;  // which pages of the tile on its way, of the tile stored last, are there: bit i, page i
 
   __device__ __forceinline__ Pages4(const Args& a, int b, int hk, const SeqRows&, int hi_, int w, int lane_)
@@ -354,17 +358,19 @@ struct Pages4 {
   static __device__ __forceinline__ float load_q(V8* qf, const Args& a, int b, int hk, int r, int g) {
     return load_q4<E_, D>(qf, a, b, hk, r, g);
   }
-  __device__ __forceinline__ int page_of(int at) const {  // -1: not there
-    const int p = table[min(at, max_pages - 1)];
+  __device__ __forceinline__ int checked(int at, int p) const {  // -1: not there
     return at < max_pages && p >= 0 && p < n_pages ? p : -1;
   }
+  // (as they are read: checked here, they would be waited for here)
   __device__ __forceinline__ void look(int tile) {
-    p0 = page_of(2 * tile);
-    p1 = page_of(2 * tile + 1);
+    at = 2 * tile;
+    p0 = table[min(at, max_pages - 1)];
+    p1 = table[min(at + 1, max_pages - 1)];
   }
   __device__ __forceinline__ void load() {
-    loaded = (p0 >= 0) | (p1 >= 0) << 1;
-    const char* blk = pool + (long)max(pg ? p1 : p0, 0) * page_bytes;
+    const int q0 = checked(at, p0), q1 = checked(at + 1, p1);
+    loaded = (q0 >= 0) | (q1 >= 0) << 1;
+    const char* blk = pool + (long)max(pg ? q1 : q0, 0) * page_bytes;
     __builtin_memcpy(kw, __builtin_assume_aligned(blk + c16 * (D / 2) + (g * W + half * NW) * 4, 4 * NW), 4 * NW);
     __builtin_memcpy(vw, __builtin_assume_aligned(blk + P::kV + (lane * W + half * NW) * 4, 4 * NW), 4 * NW);
     __builtin_memcpy(vs, __builtin_assume_aligned(blk + P::kVS + (g * W + half * NW) * 8, 8 * NW), 8 * NW);
@@ -429,7 +435,7 @@ struct Pages4 {
   __device__ __forceinline__ void odd_values(const Args& a, float4_t (&o)[NQ][DT], const RowSight (&sight)[NQ], int tile) const {
 #pragma unroll 1
     for (int key = 0; key < kTile; ++key) {
-      const int p = page_of(2 * tile + key / kPage);
+      const int i = 2 * tile + key / kPage, p = checked(i, table[min(i, max_pages - 1)]);
       if (p < 0) continue;
       const uint16_t* src = reinterpret_cast<const uint16_t*>(pool + (long)p * page_bytes + P::kVS) + key % 16 / 4 * W * 4 + key % 4;
 #pragma unroll

@@ -3,17 +3,10 @@
 //   o = sum_j e^(s_j) v_j / sum_j e^(s_j), s_j = scale q . k_j,
 // over the keys that the row sees (rows_attn.h).
 //
-// A work-group has 128 rows of a kv head (4 waves of 32; all query heads of a
-// token side by side, so that their keys are the same) and walks over the tiles
-// of 32 keys that any of them sees: K and V in LDS (double buffered, one barrier
-// a tile), S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32, the softmax
-// over a query's column in 32 bits on base-2 logits.  The weights are rounded to
-// the element type for the second product (half a step, 2^-11 or 2^-8; their sum
-// is not); in fp16 against a reference 15 below the row's maximum, so that a
-// weight of 2^-29 of the largest is still normal.  Masks are applied where a
-// wave's tile has a key that some row of the wave does not see, tiles that none
-// sees are left out.  Up to 32 rows: the four waves split a tile of 128 keys.
-// Where work-groups are few the tiles are split over more of them and joined.
+// Many rows: bound by the products and, with them, the exponentials, at the clock
+// that the card's power allows; the main loop is tile_attn.h's, here are its tiles.
+// Few rows (single tokens, a few drafts): bound by reading K and V once, and in
+// short windows by the chain of latencies.
 #include <algorithm>
 #include <cmath>
 
@@ -173,16 +166,19 @@ struct Rows16 {
   }
 };
 
-template <typename ET, int D, int WQ, int WK>
-__global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_kernel(WindowArgs a) {
+// Up to 32 rows of a kv head: the four waves of a work-group have the same rows and
+// 32 keys each of a tile of 128, and are joined in LDS at the end.  One tile of LDS:
+// the next one's rows are on their way in registers.
+template <typename ET, int D>
+__global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
   using V8 = typename ET::V8;
   using E = typename ET::E;
-  constexpr int NT = 64 * WQ * WK, KT = 32 * WK, TT = 2, NQ = 2, QW = 16 * NQ, QB = WQ * QW;
+  constexpr int NT = 256, WK = 4, KT = 32 * WK, TT = 2, NQ = 2, QB = 16 * NQ;
   constexpr int KRS = 2 * D + 32, VRS = 2 * D + 32;  // padded LDS rows: every bank once per read pattern
   constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / NT;
-  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS, NBUF = WQ == 4 ? 2 : 1;
-  __shared__ __align__(16) char lds[NBUF * BUF];
-  __shared__ int s_odd[NBUF];  // the last tile in the buffer that held a V value that is not finite
+  constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS;
+  __shared__ __align__(16) char lds[BUF];
+  __shared__ int s_odd;  // the last tile that held a V value that is not finite
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
 
@@ -191,14 +187,12 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
   const int b = bh / a.by_hkv, hk = bh - b * a.Hkv;
   const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the wave, and its share of the keys
   const int g = lane >> 4, c16 = lane & 15;
-  const int wq = w % WQ, wk = w / WQ, r0 = qblk * QB + QW * wq;  // the wave's share of rows and keys, its first row
   const SeqRows seq(a, b);
-  const int b0 = qblk * QB, b1 = min(b0 + QB, a.M);
-  const Span<KT> span(a, seq, b0 / a.by_g, (b1 - 1) / a.by_g + 1);
-  const int w1 = min(r0 + QW, a.M);
-  const Span<32> mine(a, seq, r0 / a.by_g, w1 > r0 ? (w1 - 1) / a.by_g + 1 : 0);
+  const int r0 = qblk * QB, t0 = r0 / a.by_g, t1 = (min(r0 + QB, a.M) - 1) / a.by_g + 1;
+  const Span<KT> span(a, seq, t0, t1);
+  const Span<32> mine(a, seq, t0, t1);
   const int i0 = sp * a.tps, i1 = min(i0 + a.tps, span.n), nt = i1 - i0;
   if (a.nsplit > 1 && nt <= 0) return;  // (the join does not read it)
   const char* kbase = a.k + b * a.k_sb + hk * a.k_sh;
@@ -241,9 +235,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   // (a masked weight of 0 times a value that is not finite would be no number: such a value is 0 in the tile, its tile
   // noted and its rows' results set from the value itself)
   auto store_tile = [&](int i) {
-    const int buf = NBUF == 2 ? i & 1 : 0;
     if (__builtin_expect(not_finite<ET, 2 * NCH>(&stg[NCH / 2][0]), 0)) {
-      s_odd[buf] = i;
+      s_odd = i;
 #pragma unroll
       for (int k = NCH / 2; k < NCH; ++k)
 #pragma unroll
@@ -255,7 +248,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int row = srow + NT / CHR * (k % (NCH / 2));
-      char* dst = lds + buf * BUF + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + scol;
+      char* dst = lds + (k < NCH / 2 ? row * KRS : KBUF + row * VRS) + scol;
       *reinterpret_cast<uint4*>(dst) = make_uint4(stg[k][0], stg[k][1], stg[k][2], stg[k][3]);
     }
   };
@@ -270,7 +263,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   const float c = a.sm_log2;  // (not negative)
-  if (threadIdx.x < NBUF) s_odd[threadIdx.x] = -1;
+  if (threadIdx.x == 0) s_odd = -1;
   __syncthreads();
   if (nt > 0) {
     load_tile(0);
@@ -280,8 +273,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   if (nt > 1) load_tile(1);
   for (int i = 0; i < nt; ++i) {
     const int jw = span.tile(i0 + i) * KT + 32 * wk;  // the wave's first key of the tile
-    const char* kb = lds + (NBUF == 2 ? (i & 1) * BUF : 0) + 32 * wk * KRS;
-    const char* vb = lds + (NBUF == 2 ? (i & 1) * BUF : 0) + KBUF + 32 * wk * VRS;
+    const char* kb = lds + 32 * wk * KRS;
+    const char* vb = lds + KBUF + 32 * wk * VRS;
     if (mine.n > 0 && jw <= mine.hi && (jw + 31 > mine.first - a.window || jw < a.sink)) {
       // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
       __builtin_amdgcn_s_setprio(1);
@@ -299,15 +292,17 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      const bool whole = mine.whole(a, jw);
-      if (!whole) {
+      if (!mine.whole(a, jw)) {
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
+        for (int qb = 0; qb < NQ; ++qb) {
+          RowSight row = sight[qb];
+          row.stay_here();
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-            for (int qb = 0; qb < NQ; ++qb)
-              if (!sight[qb].sees(a, jw + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
+            for (int k = 0; k < 4; ++k)
+              if (!row.sees(a, jw + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
+        }
       }
       // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
       float mx[NQ];
@@ -357,7 +352,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
       }
-      if (__builtin_expect(s_odd[NBUF == 2 ? i & 1 : 0] == i, 0)) {
+      if (__builtin_expect(s_odd == i, 0)) {
         // values that are not finite, from where they came, into the rows that see them: with a weight over 0 they
         // are the result whatever it is
 #pragma unroll 1
@@ -381,7 +376,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
       }
     }
     __builtin_amdgcn_s_setprio(0);
-    if (NBUF == 1) __syncthreads();
+    __syncthreads();
     if (i + 1 < nt) store_tile(i + 1);
     if (i + 2 < nt) load_tile(i + 2);
     __syncthreads();
@@ -389,41 +384,38 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ == 4 ? 3 : 2) void window_attn_ker
   float lt[NQ];
 #pragma unroll
   for (int qb = 0; qb < NQ; ++qb) lt[qb] = col_sum(l_run[qb]);
-  if constexpr (WK > 1) {
-    // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum, 16 rows at a time
-    // in the tiles' LDS, added in wave order; a wave keeps the dims of tiles wk, wk + WK ..
-    __shared__ float s_ml[WK][QB][2];
-    float* so = reinterpret_cast<float*>(lds);  // [waves][DT][64 lanes][4]
-    static_assert(WQ * WK * DT * 1024 <= NBUF * BUF, "the waves' O fits the tiles' LDS");
-    const int rr = QW * wq + c16;
+  // the waves' parts of the same rows: (m, l) of every wave, then O scaled to the joint maximum, 16 rows at a time
+  // in the tiles' LDS, added in wave order; a wave keeps the dims of tiles wk, wk + WK ..
+  __shared__ float s_ml[WK][QB][2];
+  float* so = reinterpret_cast<float*>(lds);  // [waves][DT][64 lanes][4]
+  static_assert(WK * DT * 1024 <= BUF, "the waves' O fits the tiles' LDS");
 #pragma unroll
-    for (int qb = 0; qb < NQ; ++qb)
-      if (g == 0) { s_ml[wk][16 * qb + rr][0] = m_run[qb]; s_ml[wk][16 * qb + rr][1] = lt[qb]; }
+  for (int qb = 0; qb < NQ; ++qb)
+    if (g == 0) { s_ml[wk][16 * qb + c16][0] = m_run[qb]; s_ml[wk][16 * qb + c16][1] = lt[qb]; }
+  __syncthreads();
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    float m = kLowest, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + c16][0]);
+#pragma unroll
+    for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + c16][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + c16][0] - m);
+    const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((wk * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
+    m_run[qb] = m;
+    lt[qb] = l;
     __syncthreads();
 #pragma unroll
-    for (int qb = 0; qb < NQ; ++qb) {
-      float m = kLowest, l = 0.f;
+    for (int u = 0; u < (DT + WK - 1) / WK; ++u) {
+      const int dt = wk + WK * u;
+      if (dt >= DT) break;
+      float4_t v = *reinterpret_cast<const float4_t*>(so + (dt * 64 + lane) * 4);
 #pragma unroll
-      for (int i = 0; i < WK; ++i) m = fmaxf(m, s_ml[i][16 * qb + rr][0]);
-#pragma unroll
-      for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + rr][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + rr][0] - m);
-      const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((w * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
-      m_run[qb] = m;
-      lt[qb] = l;
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < (DT + WK - 1) / WK; ++u) {
-        const int dt = wk + WK * u;
-        if (dt >= DT) break;
-        float4_t v = *reinterpret_cast<const float4_t*>(so + ((wq * DT + dt) * 64 + lane) * 4);
-#pragma unroll
-        for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + (((i * WQ + wq) * DT + dt) * 64 + lane) * 4);
-        o[qb][u] = v;
-      }
-      __syncthreads();
+      for (int i = 1; i < WK; ++i) v += *reinterpret_cast<const float4_t*>(so + ((i * DT + dt) * 64 + lane) * 4);
+      o[qb][u] = v;
     }
+    __syncthreads();
   }
   // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..)
   constexpr int OT = (DT + WK - 1) / WK;
@@ -555,7 +547,7 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
     using ET = decltype(et);
     constexpr int D = decltype(d)::value;
     const dim3 grid((unsigned)wgs), block(256);
-    if (plan.wq == 1) hipLaunchKernelGGL((window_attn_kernel<ET, D, 1, 4>), grid, block, 0, s, a);
+    if (plan.wq == 1) hipLaunchKernelGGL((window_few_kernel<ET, D>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((tile_attn_kernel<Rows16<ET, D>>), grid, block, 0, s, a);
     CAREKV_CHECK_LAUNCH("window_attn");
     if (a.nsplit > 1) {
