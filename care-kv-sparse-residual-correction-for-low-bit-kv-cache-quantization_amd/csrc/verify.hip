@@ -7,10 +7,15 @@
 // between tokens by 2^-50 of the sum, in 32 bits by as much as a token holds.
 //
 // Bound by reading the one row of p and q that the next token is drawn from.  A
-// row is cut into segments of 1024 values, whose sums a wave takes each; from the
-// segments' sums one wave finds the segment and then the place in it.  Short rows
-// and large batches do both in one work-group a sequence, few long rows in two
-// launches, the first over the whole GPU.
+// row is cut into segments of 1024 values, whose sums a wave takes each (sixteen
+// values a lane, all in flight); from the segments' sums one wave finds the
+// segment and then the place in it.  Two launches, the first over the whole GPU;
+// short rows do both in one work-group a sequence, which saves a launch.
+// Measured in a graph (fp32, both p and q, 8 drafts): 128 x 131071, 134 MB in
+// 30.3 us (4.4 TB/s; one work-group a sequence 32.0), 1 x 131071 11.7 (25.9),
+// 16 x 65536 10.7 (16.1), 16 x 16384 10.4 (9.5), 1 x 2048 8.9 (7.0).  What is
+// left of a short row is the chain of dependent loads: the draft, its
+// probabilities, the row, the segment.
 #include <algorithm>
 
 #include "common.h"
@@ -27,38 +32,36 @@ struct VerifyArgs {
   const int32_t* counts; // or null
   int32_t* tokens;       // [B][T + 1]
   int32_t* accepted;     // [B]
-  double2* sums;         // [B][segs]: of max(p - q, 0), of p; null: kept in LDS
+  double2* sums;         // [B][segs]: of max(p - q, 0), of p; null with one launch
   long p_sb, p_st, q_sb, q_st, draft_sb, u_sb;  // elements
   int T, V, segs;
 };
 
 constexpr int kSeg = 1024;      // values of a segment
-constexpr int kSegsInLds = 512; // at most
+constexpr int kSegsInLds = 32; // at most: two for each wave of a work-group
 
 // How many of sequence b's tokens are accepted (every wave for itself).
 template <typename E>
 __device__ __forceinline__ int count_accepted(const VerifyArgs& a, int b, int count) {
-  {
-    int n = 0;
-    for (; n < count; n += 64) {
-      const int t = n + (threadIdx.x & 63);
-      bool ok = false;
-      if (t < count) {
-        const long x = a.draft[b * a.draft_sb + t];
-        if (x >= 0 && x < a.V) {  // (any other token is rejected)
-          const double px = (double)(float)reinterpret_cast<const E*>(a.p)[b * a.p_sb + t * a.p_st + x];
-          const double qx = a.q ? (double)(float)reinterpret_cast<const E*>(a.q)[b * a.q_sb + t * a.q_st + x] : 1.0;
-          ok = (double)a.u[b * a.u_sb + t] * qx < px;
-        }
-      }
-      const unsigned long long m = __ballot(ok);
-      if (m != ~0ull) {
-        n += __ffsll((long long)~m) - 1;
-        break;
+  int n = 0;
+  for (; n < count; n += 64) {
+    const int t = n + (threadIdx.x & 63);
+    bool ok = false;
+    if (t < count) {
+      const long x = a.draft[b * a.draft_sb + t];
+      if (x >= 0 && x < a.V) {  // (any other token is rejected)
+        const double px = (double)(float)reinterpret_cast<const E*>(a.p)[b * a.p_sb + t * a.p_st + x];
+        const double qx = a.q ? (double)(float)reinterpret_cast<const E*>(a.q)[b * a.q_sb + t * a.q_st + x] : 1.0;
+        ok = (double)a.u[b * a.u_sb + t] * qx < px;
       }
     }
-    return min(n, count);
+    const unsigned long long m = __ballot(ok);
+    if (m != ~0ull) {
+      n += __ffsll((long long)~m) - 1;
+      break;
+    }
   }
+  return min(n, count);
 }
 
 // The weights of row n: max(p - q, 0) and p, 0 where they are not over 0.
@@ -233,12 +236,11 @@ __global__ __launch_bounds__(1024) void verify_kernel(VerifyArgs a) {
 
 namespace {
 int verify_segs(const carekv_verify_params& p) { return (p.vocab + kSeg - 1) / kSeg; }
-// One work-group a sequence where its waves have at most four segments each, or where there are sequences for half of
-// the CUs; else two launches.
-bool verify_fused(const carekv_verify_params& p) {
-  const int segs = verify_segs(p);
-  return segs <= 64 || (p.batch >= 128 && segs <= kSegsInLds);
-}
+// One work-group a sequence where each of its waves has at most two segments and each CU at most one work-group; else two
+// launches.  In a graph (us, one launch against two): 128 x 16384 9.7 to 11.2, 1 x 32000 11.3 to 10.0, 1 x 65536 14.9 to
+// 9.3, 512 x 4096 15.1 to 11.2.  Called eagerly, the second launch and its workspace cost the host another 4 us (1 x 32000:
+// 11.5 to 15.8), so the border is where one launch loses less than that.
+bool verify_fused(const carekv_verify_params& p) { return verify_segs(p) <= kSegsInLds && p.batch <= 256; }
 int check_verify(const carekv_verify_params* pp) {
   CAREKV_REQUIRE(pp, "null argument");
   const carekv_verify_params& p = *pp;
@@ -281,8 +283,9 @@ extern "C" int carekv_verify_drafts(const carekv_verify_params* pp, const int64_
   }
   CAREKV_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
-  // work-groups of a sequence: each wave a segment, until 1024 are there
-  const int wgs = std::max(1, std::min((a.segs + 3) / 4, 1024 / p.batch));
+  // work-groups of a sequence: each wave a segment, until 2048 of them are there (256 x 131071: 41.1 us, with 1024 43.7,
+  // with 4096 40.8)
+  const int wgs = std::max(1, std::min((a.segs + 3) / 4, 2048 / p.batch));
   auto go = [&](auto e) {
     using E = decltype(e);
     if (fused) {
