@@ -77,7 +77,9 @@ __device__ __forceinline__ float load_q4(half8_t* qf, const RowsArgs& a, int b, 
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)ldexpf(x[s][i], -ex);
-    return ldexpf(a.sm_log2, ex);
+    // (never 0: times the -inf of a key that is not seen it would be no number)
+    const float c = ldexpf(a.sm_log2, ex);
+    return c < 1.17549435e-38f ? 1.17549435e-38f : c;
   }
 }
 

@@ -339,6 +339,18 @@ def test_scales_of_q():
     check(care_kv.paged_attention(x, pages, table, 300, return_lse=True), attend(x, K, V, see, weights=F16))
 
 
+@pytest.mark.parametrize("T", [3, 70])
+def test_the_smallest_values_of_q(T):
+    """bf16 rows of 2^-133 under a small scale: the factor of their logits is below what 32 bits hold, every weight 1."""
+    import care_kv
+    q, pages, table, K, V = _case(33, 2, 4, 2, 64, T, 150, BF16)
+    x = torch.where(q > 0, 2.0 ** -133, -2.0 ** -133).bfloat16()
+    lengths, rows = [150, 101], [T, T - 2]
+    see = sight(2, T, 150, 40, 3, lengths, rows, None)
+    check(care_kv.paged_attention(x, pages, table, lengths, q_lengths=rows, window=40, sink=3, sm_scale=1e-3, return_lse=True),
+          attend(x, K, V, see, 1e-3, F16))
+
+
 def test_strides_of_q():
     import care_kv
     q, pages, table, K, V = _case(32, 2, 6, 2, 128, 5, 90, BF16)
