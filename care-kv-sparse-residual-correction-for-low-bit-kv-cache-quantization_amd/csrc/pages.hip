@@ -53,26 +53,62 @@ __device__ __forceinline__ void load8(E* x, const char* p, bool wide = true) {
   }
 }
 
-// A lane's 8 fp16 values as codes: u[e] = c + 8, and the group's scale (its 4 lanes hold the other values)
+// x / s rounded to fp16, s and x fp16 values, r within 2 ulps of 1 / s: x r, and its exact rest times r.  What comes out is
+// the quotient within 2^-24 (1 + 2^-20) of itself, and the quotient itself where it has at most 24 bits; other quotients
+// of 11-bit numbers keep 2^-23 of themselves away from the borders of fp16's rounding, numbers of 12 bits.
+__device__ __forceinline__ _Float16 half_quotient(float x, float s, float r) {
+  const float q = x * r;
+  return (_Float16)fmaf(fmaf(-q, s, x), r, q);
+}
+
+// A lane's 8 fp16 values as codes: p[i], codes 2i and 2i + 1 as u = c + 8 in the low bits of the halves of fp16 1024 + u;
+// and the group's scale (its 4 lanes, neighbours, hold the other values).
 struct Coded {
-  uint32_t u[8];
+  uint32_t p[4];
   _Float16 s;
+  // the codes in 4 bits each, in a word's order
+  __device__ __forceinline__ uint32_t word() const {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (p[i] & 0x000f000fu) << (4 * i);
+    return w;
+  }
+  // what they stand for
+  __device__ __forceinline__ void values(half2_t* x) const {
+    const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f}, s2 = {s, s};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      half2_t h;
+      __builtin_memcpy(&h, &p[i], 4);
+      x[i] = (h + off) * s2;
+    }
+  }
 };
 __device__ __forceinline__ Coded code8(const _Float16* x) {
-  uint32_t m = 0;
+  typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+  ushort2_t m2 = {0, 0};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, (uint32_t)(half2bits(x[e]) & 0x7fff));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+  for (int i = 0; i < 4; ++i) {
+    ushort2_t b;
+    __builtin_memcpy(&b, x + 2 * i, 4);
+    m2 = __builtin_elementwise_max(m2, b & (uint16_t)0x7fff);
+  }
+  uint32_t m = max((uint32_t)m2.x, (uint32_t)m2.y);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
   Coded r;
   const bool bad = m >= 0x7c00;
-  r.s = bad ? bits2half(0x7e00) : (_Float16)(h2f((uint16_t)m) / 7.f);
-  const float s = (float)r.s;
+  r.s = half_quotient(h2f((uint16_t)m), 7.f, 1.f / 7.f);
+  const float s = (float)r.s, inv = s != 0.f ? __builtin_amdgcn_rcpf(s) : 0x1p60f;  // (s = 0: x 2^60, 0 or past every code)
+  const half2_t lo = {(_Float16)-8.f, (_Float16)-8.f}, hi = {(_Float16)7.f, (_Float16)7.f}, up = {(_Float16)1032.f, (_Float16)1032.f};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float c = rintf((float)(_Float16)((float)x[e] / s));  // (0 / 0: NaN, which fmaxf drops below)
-    r.u[e] = bad || c != c ? 8u : (uint32_t)((int)fminf(fmaxf(c, -8.f), 7.f) + 8);
+  for (int i = 0; i < 4; ++i) {
+    half2_t h = {half_quotient((float)x[2 * i], s, inv), half_quotient((float)x[2 * i + 1], s, inv)};
+    h = __builtin_elementwise_min(__builtin_elementwise_max(h, lo), hi) + up;  // (rounded to whole numbers, ties to even)
+    __builtin_memcpy(&r.p[i], &h, 4);
+    if (bad) r.p[i] = 0x64086408u;
   }
+  if (bad) r.s = bits2half(0x7e00);
   return r;
 }
 
@@ -81,7 +117,7 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendArgs a) {
   using P = Page4<D>;
   constexpr int CH = D / 8, TPW = 64 / CH;  // lanes of a token, tokens of a wave
   __shared__ double2 tab[256];              // [TPW][D / 2] cosine, sine
-  __shared__ __align__(8) uint8_t codes[4][TPW * D];
+  __shared__ __align__(16) uint32_t codes[4][64];  // a wave's words of V's codes, as K's: [token quads][CH][4 tokens]
   const int b = blockIdx.x / a.nu, unit = blockIdx.x - b * a.nu;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int start = min(max(a.start[b], -(1 << 29)), 1 << 29);
@@ -182,44 +218,40 @@ __global__ __launch_bounds__(256) void append_pages_kernel(AppendArgs a) {
     const Coded kc = code8(kx), vc = code8(vx);
     if (a.k_hat && in) {
       const long at = (((long)b * a.Hkv + w) * a.T + t) * D + 8 * c;
-      _Float16 kh[8], vh[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { kh[e] = dq((int)kc.u[e] - 8, kc.s); vh[e] = dq((int)vc.u[e] - 8, vc.s); }
+      half2_t h[4];
       uint4 u;
-      __builtin_memcpy(&u, kh, 16);
+      kc.values(h);
+      __builtin_memcpy(&u, h, 16);
       *reinterpret_cast<uint4*>(a.k_hat + at) = u;
-      __builtin_memcpy(&u, vh, 16);
+      vc.values(h);
+      __builtin_memcpy(&u, h, 16);
       *reinterpret_cast<uint4*>(a.v_hat + at) = u;
     }
     if (!there) continue;  // (the same for the whole wave)
     const int place = slot & (kPage - 1);
     if (fresh) {
-      uint32_t word = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) word |= kc.u[e] << nib4(e);
-      *reinterpret_cast<uint32_t*>(block + place * (D / 2) + 4 * c) = word;
+      *reinterpret_cast<uint32_t*>(block + place * (D / 2) + 4 * c) = kc.word();
       if ((c & 3) == 0) {
         *reinterpret_cast<uint16_t*>(block + P::kKS + ((c >> 2) * kPage + place) * 2) = half2bits(kc.s);
         *reinterpret_cast<uint16_t*>(block + P::kVS + (((place >> 2) * P::G + (c >> 2)) * 4 + (place & 3)) * 2) = half2bits(vc.s);
       }
     }
-    uint8_t* mine = codes[wave];
-    uint32_t lo = 0, hi = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { lo |= vc.u[e] << (8 * e); hi |= vc.u[e + 4] << (8 * e); }
-    lds_sync_wave();  // (the last head's bytes have been read)
-    *reinterpret_cast<uint2*>(mine + j * D + 8 * c) = make_uint2(lo, hi);
+    uint32_t* mine = codes[wave];
+    lds_sync_wave();  // (the last head's words have been read)
+    mine[((j / 4) * CH + c) * 4 + j % 4] = vc.word();
     lds_sync_wave();
-    // lane: word lane % (D / 2) of token quad lane / (D / 2)
+    // lane: word lane % (D / 2) of token quad lane / (D / 2), dims d and d + 16 of its four tokens
     constexpr int WQ = D / 2;  // words of a quad
-    const int quad = lane / WQ, l = lane % WQ, c16 = l / P::G, gr = l % P::G;
+    const int quad = lane / WQ, l = lane % WQ, d = 32 * (l % P::G) + l / P::G;
     const int s0 = slot0 + 4 * quad - start;  // the quad's first token
+    const uint4 w0 = *reinterpret_cast<const uint4*>(mine + (quad * CH + d / 8) * 4);
+    const uint4 w1 = *reinterpret_cast<const uint4*>(mine + (quad * CH + d / 8 + 2) * 4);
+    const uint32_t from[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     uint32_t word = 0, put = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int tok = e & 3;
-      word |= (uint32_t)mine[(4 * quad + tok) * D + 16 * (2 * gr + e / 4) + c16] << nib4(e);
-      if (s0 + tok >= 0 && s0 + tok < count) put |= 15u << nib4(e);
+      word |= (from[e] >> nib4(d % 8) & 15u) << nib4(e);
+      if (s0 + e % 4 >= 0 && s0 + e % 4 < count) put |= 15u << nib4(e);
     }
     if (put) {
       uint32_t* dst = reinterpret_cast<uint32_t*>(block + P::kV + (((slot0 + 4 * quad) & (kPage - 1)) / 4) * (WQ * 4)) + l;
