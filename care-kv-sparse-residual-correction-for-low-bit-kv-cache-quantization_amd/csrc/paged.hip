@@ -8,7 +8,13 @@
 // fourth tile; a wave loads a tile's codes and scales straight into the operands'
 // lanes, the next tile's while it works on this one, and turns them into fp16
 // there.  S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16, the softmax over a
-// query's column in 32 bits on base-2 logits, the waves joined in LDS.
+// query's column in 32 bits on base-2 logits, the waves joined in LDS.  Measured: 64
+// rows of 32 / 8 heads, D = 128, on 32768 keys (2.4 GB) 458 - 470 us, 5.2 TB/s, a copy's
+// rate (515 with the table read by vector loads and masks as literals); 16 x 5 rows
+// through a window of 4096 33 us: 20 rows fill 20 of 32 columns, a tile costs a SIMD
+// 2100 cycles (by count unpacking 830, softmax and products 510 each).  One row of 32 / 4 heads, D
+// = 64, on 2303 keys in a graph 8.7; with 16 waves a work-group and no splits, one
+// launch instead of two, 12.4.
 //
 // Products are fp16 whatever q's type: codes times scales are fp16 values by
 // definition, bf16 rows of q are scaled by a power of two to below 2^12, which
@@ -334,7 +340,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedA
 // Many rows: bound by the products, so that the codes are turned into fp16 once for
 // the 128 rows of tile_attn.h.  A wave takes half of one page's codes of a tile of 32
 // keys and writes them to LDS as the operands that all four read, 1 KB each in the
-// lanes' order.
+// lanes' order.  2 x 512 rows of 40 heads, D = 128, on 16896 keys: 526 us, 0.66 PFLOP/s.
 template <typename E_, int D_>
 struct Pages4 {
   using Args = PagedArgs;
@@ -378,6 +384,7 @@ struct Pages4 {
     __builtin_memcpy(vs, __builtin_assume_aligned(blk + P::kVS + (g * W + half * NW) * 8, 8 * NW), 8 * NW);
     ks = *reinterpret_cast<const uint16_t*>(blk + P::kKS + ((D == 128 ? g : g >> 1) * kPage + c16) * 2);
   }
+  template <bool CARE>
   __device__ __forceinline__ bool store(char* kb, char* vb, int tile) {
     held = loaded;
     const int j0 = tile * kTile;
@@ -388,17 +395,11 @@ struct Pages4 {
 #pragma unroll
           for (int x = 0; x < NW; ++x) vs[2 * x + k / 2][k & 1] = (_Float16)0.f;
     }
-    uint32_t odd = 0;
-#pragma unroll
-    for (int x = 0; x < 2 * NW; ++x) {
-      uint32_t bits;
-      __builtin_memcpy(&bits, &vs[x], 4);
-      odd |= ((bits & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-    }
-    if (__builtin_expect(odd != 0, 0)) {
+    bool odd = false;
+    if constexpr (CARE) {
 #pragma unroll
       for (int x = 0; x < 4 * NW; ++x)
-        if ((half2bits(vs[x / 2][x & 1]) & 0x7c00) == 0x7c00) vs[x / 2][x & 1] = (_Float16)0.f;
+        if ((half2bits(vs[x / 2][x & 1]) & 0x7c00) == 0x7c00) vs[x / 2][x & 1] = (_Float16)0.f, odd = true;
     }
     const Unpack4 dequant4;
     const _Float16 kf = bits2half(ks);
@@ -419,7 +420,7 @@ struct Pages4 {
         *reinterpret_cast<uint2*>(vb + (2 * (half * NW + x) + y) * 1024 + lane * 16 + 8 * pg) = t;
       }
     }
-    return odd != 0;
+    return odd;
   }
   __device__ __forceinline__ V8 k_op(const char* kb, int tt, int st) const {
     V8 r;

@@ -14,6 +14,12 @@
 // V's words hold four tokens of a dim: the places of a wave start at a multiple
 // of four, so that no other wave writes a word of it, and a word of which only
 // some tokens are new is read and joined.
+//
+// Measured in a graph, D = 128: 4 x 8192 tokens of 40 / 40 heads with the values
+// they stand for 434 us, 5.1 TB/s, a copy's rate; of 32 / 8 heads 169, 5.0 TB/s;
+// K and V alone (16 x 8192 tokens of 8 heads) 179 us at 3.9 TB/s of coding, and 223
+// with positions, a token's 64-bit angles over few heads.  Divisions, and V's codes
+// in bytes in LDS, took 467, 179, 222 and 268.  One token of 32 / 4 heads: 5 us.
 #include <algorithm>
 
 #include "common.h"

@@ -138,7 +138,8 @@ __device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, floa
 
 // The splits' partials of a row: 256 / D rows a work-group, four groups of D / 4
 // threads that take every fourth split, added up in LDS in group order.  Splits
-// behind the rows' last tile wrote nothing and are not read.
+// behind the rows' last tile wrote nothing and are not read.  4 - 5 us for the rows of
+// single tokens, 27 for 40960 rows of 4 splits (95 MB).
 template <typename E, int D, int KT>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
   constexpr int D4 = D / 4, JG = 4, RW = 256 / (D4 * JG);

@@ -9,6 +9,15 @@
 //
 // Masks are applied where a wave's tile has a key that some row of the wave does
 // not see, tiles that none sees are left out.
+//
+// Bound by products and exponentials, whose times add up more than they overlap: 4
+// x 8192 rows of 40 heads, D = 128, window 4096: 2386 us, 0.86 PFLOP/s, at the 1.7 -
+// 2.0 GHz that the card's power leaves.  Three work-groups a CU, their phases apart, did
+// better than 8 waves with 256 rows (3026 us, pages 725 against 570, with values looked at
+// as they are stored) and than two tiles on their way with two work-groups a CU (2735);
+// 32x32x16 products are slower by themselves (1735 against 1941 TFLOP/s from
+// registers).  Short windows add each work-group's start and end: q and the results of
+// its 128 rows are as many bytes as 4 tiles of K and V.
 #pragma once
 
 #include "rows_attn.h"
@@ -16,11 +25,15 @@
 namespace carekv {
 
 // Src: where K and V come from.  look says which tile is loaded next, load starts its loads into registers, store
-// writes them to LDS (and says whether the thread had a V value that is not finite: it writes 0 for it, so that a masked
-// weight of 0 times it is no NaN), k_op / v_op read operands, there() tells which halves of the tile stored last exist,
-// odd_values() brings the values that are not finite to the rows that see them.
+// writes them to LDS (and, where it is to take care, says whether the thread had a V value that is not finite: it writes
+// 0 for it, so that a masked weight of 0 times it is no NaN), k_op / v_op read operands, there() tells which halves of the
+// tile stored last exist, odd_values() brings the values that are not finite to the rows that see them.
+//
+// Values are looked at only where a sum came out not finite: the work-group then walks once more, with care.  (Looked at
+// as they are stored, they cost every walk: 2530 against 2386 us for 4 x 8192 rows of 40 heads, 138 against 127 for 8
+// ragged prompts of 2047.)
 template <class Src>
-__global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a) {
+__global__ __launch_bounds__(256, Src::D == 64 ? 4 : 3) void tile_attn_kernel(typename Src::Args a) {
   using ET = typename Src::ET;
   using V8 = typename ET::V8;
   using E = typename Src::Out;
@@ -28,6 +41,7 @@ __global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a)
   constexpr int BUF = Src::kK + Src::kV;
   __shared__ __align__(16) char lds[2 * BUF];
   __shared__ int s_odd[2];  // the last tile in the buffer that held a V value that is not finite
+  __shared__ int s_again;
   const int it = xcd_item(a);
   const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
   const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
@@ -41,6 +55,8 @@ __global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a)
   const int i0 = sp * a.tps, i1 = min(i0 + a.tps, span.n), nt = i1 - i0;
   if (a.nsplit > 1 && nt <= 0) return;  // (the join does not read it)
 
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = -1;
+  if (threadIdx.x == 0) s_again = 0;
   V8 qf[NQ][KS];
   float c[NQ];
   RowSight sight[NQ];
@@ -51,108 +67,121 @@ __global__ __launch_bounds__(256, 3) void tile_attn_kernel(typename Src::Args a)
   }
   float m_run[NQ], l_run[NQ];
   float4_t o[NQ][DT];
-#pragma unroll
-  for (int qb = 0; qb < NQ; ++qb) {
-    m_run[qb] = kLowest;
-    l_run[qb] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
   Src src(a, b, hk, seq, span.hi, w, lane);
   auto tile = [&](int i) { return span.tile(i0 + i); };
-  if (threadIdx.x < 2) s_odd[threadIdx.x] = -1;
-  __syncthreads();
-  if (nt > 0) {
-    src.look(tile(0));
-    src.load();
-    src.look(tile(min(1, nt - 1)));
-    if (src.store(lds, lds + Src::kK, tile(0))) s_odd[0] = 0;
-  }
-  __syncthreads();
-  if (nt > 1) src.load();
-  for (int i = 0; i < nt; ++i) {
-    const int j0 = tile(i) * KT, here = src.there();
-    src.look(tile(min(i + 2, nt - 1)));
-    const char* kb = lds + (i & 1) * BUF;
-    const char* vb = kb + Src::kK;
-    if (mine.n > 0 && j0 <= mine.hi && (j0 + KT - 1 > mine.first - a.window || j0 < a.sink)) {
-      // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
-      __builtin_amdgcn_s_setprio(1);
-      float4_t s[2][NQ];
+  auto walk = [&](auto with_care) {
+    constexpr bool care = decltype(with_care)::value;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
+    for (int qb = 0; qb < NQ; ++qb) {
+      m_run[qb] = kLowest;
+      l_run[qb] = 0.f;
 #pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    if (nt > 0) {
+      src.look(tile(0));
+      src.load();
+      src.look(tile(min(1, nt - 1)));
+      if (src.template store<care>(lds, lds + Src::kK, tile(0))) s_odd[0] = 0;
+    }
+    __syncthreads();
+    if (nt > 1) src.load();
+    for (int i = 0; i < nt; ++i) {
+      const int j0 = tile(i) * KT, here = src.there();
+      src.look(tile(min(i + 2, nt - 1)));
+      const char* kb = lds + (i & 1) * BUF;
+      const char* vb = kb + Src::kK;
+      if (mine.n > 0 && j0 <= mine.hi && (j0 + KT - 1 > mine.first - a.window || j0 < a.sink)) {
+        // (raised wave priority over the products: a wave with products to issue goes before others' softmax)
+        __builtin_amdgcn_s_setprio(1);
+        float4_t s[2][NQ];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const V8 ak = src.k_op(kb, tt, ks);
+        for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
-          for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = ET::mfma(ak, qf[qb][ks], s[tt][qb]);
+          for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const V8 ak = src.k_op(kb, tt, ks);
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb) s[tt][qb] = ET::mfma(ak, qf[qb][ks], s[tt][qb]);
+          }
         }
+        __builtin_amdgcn_s_setprio(0);
+        if (!mine.whole(a, j0) || here != 3) {
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) {
+            RowSight row = sight[qb];
+            row.stay_here();
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (!(here >> tt & 1) || !row.sees(a, j0 + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
+          }
+        }
+        // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
+        float mx[NQ];
+        bool any_over = false, over[NQ];
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          mx[qb] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
+          over[qb] = fmaf(mx[qb], c[qb], -ET::kUp) > m_run[qb];
+          any_over |= over[qb];
+        }
+        if (__any(any_over)) {
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) {
+            if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
+            const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c[qb], -ET::kUp));
+            const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+            m_run[qb] = m_new;
+            l_run[qb] *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
+          }
+        }
+        V8 bp[NQ];
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+          float ls = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[k / 4][qb][k % 4], c[qb], -m_run[qb]));
+            ls += p;
+            bp[qb][k] = (typename ET::E)p;
+          }
+          l_run[qb] += ls;
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const V8 av = src.v_op(vb, dt);
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
+        }
+        if (care && s_odd[i & 1] == i) src.odd_values(a, o, sight, tile(i));
       }
       __builtin_amdgcn_s_setprio(0);
-      if (!mine.whole(a, j0) || here != 3) {
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) {
-          RowSight row = sight[qb];
-          row.stay_here();
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (!(here >> tt & 1) || !row.sees(a, j0 + 16 * tt + 4 * g + k)) s[tt][qb][k] = -INFINITY;
-        }
-      }
-      // base-2 logits x = c s folded into the exponent: max x = c max s, e^.. = 2^fma(s, c, -reference)
-      float mx[NQ];
-      bool any_over = false, over[NQ];
-#pragma unroll
-      for (int qb = 0; qb < NQ; ++qb) {
-        mx[qb] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) mx[qb] = fmaxf(fmaxf(mx[qb], s[k / 4][qb][k % 4]), s[k / 4][qb][k % 4 + 1]);
-        over[qb] = fmaf(mx[qb], c[qb], -ET::kUp) > m_run[qb];
-        any_over |= over[qb];
-      }
-      if (__any(any_over)) {
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) {
-          if (!__any(over[qb])) continue;  // columns that keep their reference get a factor of exactly 1
-          const float m_new = fmaxf(m_run[qb], fmaf(col_max(mx[qb]), c[qb], -ET::kUp));
-          const float f = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
-          m_run[qb] = m_new;
-          l_run[qb] *= f;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
-        }
-      }
-      V8 bp[NQ];
-#pragma unroll
-      for (int qb = 0; qb < NQ; ++qb) {
-        float ls = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[k / 4][qb][k % 4], c[qb], -m_run[qb]));
-          ls += p;
-          bp[qb][k] = (typename ET::E)p;
-        }
-        l_run[qb] += ls;
-      }
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const V8 av = src.v_op(vb, dt);
-#pragma unroll
-        for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
-      }
-      if (__builtin_expect(s_odd[i & 1] == i, 0)) src.odd_values(a, o, sight, tile(i));
+      if (i + 1 < nt && src.template store<care>(lds + (i + 1 & 1) * BUF, lds + (i + 1 & 1) * BUF + Src::kK, tile(i + 1)))
+        s_odd[(i + 1) & 1] = i + 1;
+      if (i + 2 < nt) src.load();
+      __syncthreads();
     }
-    __builtin_amdgcn_s_setprio(0);
-    if (i + 1 < nt && src.store(lds + (i + 1 & 1) * BUF, lds + (i + 1 & 1) * BUF + Src::kK, tile(i + 1)))
-      s_odd[(i + 1) & 1] = i + 1;
-    if (i + 2 < nt) src.load();
-    __syncthreads();
+  };
+  walk(std::false_type{});
+#pragma unroll
+  for (int qb = 0; qb < NQ; ++qb) {
+    float sum = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum = fmaf(o[qb][dt][x], 0.f, sum);
+    if (!(sum == 0.f) && sight[qb].top >= 0) s_again = 1;
   }
+  __syncthreads();
+  if (__builtin_expect(s_again, 0)) walk(std::true_type{});
 
   // the rows' results, or the split's partial (lane: row r0 + 16qb + c16, dims 16dt + 4g ..).  Results go through the
   // wave's part of LDS, 16-byte pieces exchanged against bank conflicts, so that whole rows are written.

@@ -104,14 +104,16 @@ struct Rows16 {
     load(k, kbase, k_st, k_off, 32 * next, len);
     load(v, vbase, v_st, v_off, 32 * next, len);
   }
+  template <bool CARE>
   __device__ __forceinline__ bool store(char* kb, char* vb, int) {
-    const bool odd = not_finite<ET, 4 * NCH>(&v[0][0]);
-    if (__builtin_expect(odd, 0)) {
+    bool odd = false;
+    if constexpr (CARE) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t u = not_finite2<ET>(v[i][x]);
+          odd |= u != 0;
           v[i][x] &= (u & 0x8000u ? 0u : 0xffffu) | (u >> 31 ? 0u : 0xffff0000u);
         }
     }
@@ -168,7 +170,9 @@ struct Rows16 {
 
 // Up to 32 rows of a kv head: the four waves of a work-group have the same rows and
 // 32 keys each of a tile of 128, and are joined in LDS at the end.  One tile of LDS:
-// the next one's rows are on their way in registers.
+// the next one's rows are on their way in registers.  16 rows of 32 / 8 heads, D = 128,
+// on 4097 keys (268 MB): 47 us, 5.7 TB/s; one row of 32 / 4 heads, D = 64, through a
+// window of 1024 in a graph 8.5 us, two launches.
 template <typename ET, int D>
 __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
   using V8 = typename ET::V8;
