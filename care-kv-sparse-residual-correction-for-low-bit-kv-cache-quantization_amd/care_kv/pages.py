@@ -195,9 +195,9 @@ def paged_attention(q: torch.Tensor, pages: Int4Pages, table: torch.Tensor, leng
 
     Returns o like q and, with ``return_lse``, the natural log-sum-exp of each
     row's scaled scores, fp32 (B, Hq, T).  Rows of padding and rows that see
-    nothing are 0 with lse -inf.  What places that a row does not see hold (NaN
-    included) is never used.  ``out`` may be q itself.  The results carry no
-    autograd history."""
+    nothing are 0 with lse -inf; a score of -inf counts as not seen.  What places
+    that a row does not see hold (NaN included) is never used.  ``out`` may be q
+    itself.  The results carry no autograd history."""
     one = q.dim() == 3
     if one:
         q = q.unsqueeze(2)
