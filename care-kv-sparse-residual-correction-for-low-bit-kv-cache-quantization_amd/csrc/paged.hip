@@ -565,9 +565,7 @@ extern "C" int carekv_paged_attn(const carekv_paged_params* pp, const void* q, c
     else hipLaunchKernelGGL((tile_attn_kernel<Pages4<E, D>>), grid, block, 0, s, a);
     CAREKV_CHECK_LAUNCH("paged_rows");
     if (a.nsplit > 1) {
-      constexpr int RW = 256 / D;
-      hipLaunchKernelGGL((rows_join_kernel<E, D, kTile>), dim3((unsigned)((rows + RW - 1) / RW)), dim3(256), 0, s,
-                         (RowsArgs)a);
+      launch_join<E, D, kTile>(a, s);
       CAREKV_CHECK_LAUNCH("rows_join");
     }
     return CAREKV_OK;

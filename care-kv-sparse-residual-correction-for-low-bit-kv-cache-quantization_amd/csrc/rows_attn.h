@@ -142,11 +142,9 @@ __device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, floa
 // threads that take every fourth split, added up in LDS in group order.  Splits
 // behind the rows' last tile wrote nothing and are not read.  4 - 5 us for the rows of
 // single tokens, 27 for 40960 rows of 4 splits (95 MB).
-template <typename E, int D, int KT>
+template <typename E, int D, int KT, int JG>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
-  constexpr int D4 = D / 4, JG = 4, RW = 256 / (D4 * JG);
-  __shared__ float4_t s_o[256];
-  __shared__ float2 s_ml[RW][JG];
+  constexpr int D4 = D / 4, RW = 256 / (D4 * JG);
   const int d4 = threadIdx.x % D4, grp = threadIdx.x / D4 % JG, rw = threadIdx.x / (D4 * JG);
   const long pr = (long)blockIdx.x * RW + rw;
   const bool in = pr < a.rows;
@@ -183,23 +181,38 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
       }
     }
   }
-  s_o[threadIdx.x] = o;
-  if (d4 == 0) s_ml[rw][grp] = make_float2(m, L);
-  __syncthreads();
-  if (!in || grp != 0) return;
-  float mm = kLowest, LL = 0.f;
-  float4_t O = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (JG > 1) {
+    __shared__ float4_t s_o[256];
+    __shared__ float2 s_ml[RW][JG];
+    s_o[threadIdx.x] = o;
+    if (d4 == 0) s_ml[rw][grp] = make_float2(m, L);
+    __syncthreads();
+    m = kLowest;
+    L = 0.f;
+    o = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < JG; ++i) mm = fmaxf(mm, s_ml[rw][i].x);
+    for (int i = 0; i < JG; ++i) m = fmaxf(m, s_ml[rw][i].x);
 #pragma unroll
-  for (int i = 0; i < JG; ++i) {
-    const float f = __builtin_amdgcn_exp2f(s_ml[rw][i].x - mm);
-    LL += s_ml[rw][i].y * f;
-    O += s_o[(rw * JG + i) * D4 + d4] * f;
+    for (int i = 0; i < JG; ++i) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[rw][i].x - m);
+      L += s_ml[rw][i].y * f;
+      o += s_o[(rw * JG + i) * D4 + d4] * f;
+    }
   }
-  if (pad) { LL = 0.f; O = float4_t{0.f, 0.f, 0.f, 0.f}; }  // (what a row of padding holds is not used)
-  write4<E>(a, out_row(a, b, hk, r), 4 * d4, O, LL);
-  if (a.lse && d4 == 0) write_lse(a, b, hk, r, mm, LL);
+  if (!in || grp != 0) return;
+  if (pad) { L = 0.f; o = float4_t{0.f, 0.f, 0.f, 0.f}; }  // (what a row of padding holds is not used)
+  write4<E>(a, out_row(a, b, hk, r), 4 * d4, o, L);
+  if (a.lse && d4 == 0) write_lse(a, b, hk, r, m, L);
+}
+
+template <typename E, int D, int KT>
+inline void launch_join(const RowsArgs& a, hipStream_t s) {
+  auto go = [&](auto jg) {
+    constexpr int JG = decltype(jg)::value, RW = 1024 / (D * JG);
+    hipLaunchKernelGGL((rows_join_kernel<E, D, KT, JG>), dim3((unsigned)((a.rows + RW - 1) / RW)), dim3(256), 0, s, a);
+  };
+  if (a.nsplit <= 8) go(std::integral_constant<int, 1>{});
+  else go(std::integral_constant<int, 4>{});
 }
 
 // Whether rows of out lie on 8 and on 16 bytes.

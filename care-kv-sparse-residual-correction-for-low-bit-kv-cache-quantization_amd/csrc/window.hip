@@ -555,10 +555,8 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
     else hipLaunchKernelGGL((tile_attn_kernel<Rows16<ET, D>>), grid, block, 0, s, a);
     CAREKV_CHECK_LAUNCH("window_attn");
     if (a.nsplit > 1) {
-      constexpr int RW = 256 / D;
-      const dim3 jg((unsigned)((rows + RW - 1) / RW));
-      if (plan.wk == 4) hipLaunchKernelGGL((rows_join_kernel<typename ET::E, D, 128>), jg, dim3(256), 0, s, (RowsArgs)a);
-      else hipLaunchKernelGGL((rows_join_kernel<typename ET::E, D, 32>), jg, dim3(256), 0, s, (RowsArgs)a);
+      if (plan.wk == 4) launch_join<typename ET::E, D, 128>(a, s);
+      else launch_join<typename ET::E, D, 32>(a, s);
       CAREKV_CHECK_LAUNCH("rows_join");
     }
     return CAREKV_OK;
