@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedA
 // Many rows: bound by the products, so that the codes are turned into fp16 once for
 // the 128 rows of tile_attn.h.  A wave takes half of one page's codes of a tile of 32
 // keys and writes them to LDS as the operands that all four read, 1 KB each in the
-// lanes' order.  2 x 512 rows of 40 heads, D = 128, on 16896 keys: 526 us, 0.66 PFLOP/s.
+// lanes' order.  2 x 512 rows of 40 heads, D = 128, on 16896 keys: 507 us, 0.69 PFLOP/s.
 template <typename E_, int D_>
 struct Pages4 {
   using Args = PagedArgs;
@@ -457,14 +457,13 @@ struct Pages4 {
 };
 
 namespace {
-// How a call is cut: 16 rows of a kv head at once or 32, more in blocks of 128.  Key
-// splits of at least 8 tiles (two a wave), at most 32: the join reads every split's
-// partials.  us a call, by splits: one row of 32 / 4 heads, D = 64, on 2303 keys 1 / 4
-// / 8 / 16 / 32: 17.2 / 10.3 / 9.1 / 8.7 / 9.2, on 8000 8 / 16 / 32 / 64: 12.4 / 10.0 /
-// 9.9 / 12.3; 32 / 8 heads, D = 128, on 16000 16 / 32 / 64: 16.7 / 14.1 / 16.6; 16 x 5 rows
-// on 8191 through a window of 4096 2 / 4 / 6 / 8: 39 / 34 / 39 / 39; 64 rows on 32768 2 / 4
-// / 6 / 8: 479 / 461 / 460 / 463.  512 rows of 40 heads on 16896 1 / 2 / 3 / 4 / 6: 877 / 568 /
-// 608 / 533 / 548.
+// How a call is cut: 16 rows of a kv head at once or 32, more in blocks of 128, whose
+// splits best_splits gives.  Key splits of few rows: of at least 8 tiles (two a wave),
+// at most 32: the join reads every split's partials.  us a call, by splits: one row of
+// 32 / 4 heads, D = 64, on 2303 keys 1 / 4 / 8 / 16 / 32: 17.2 / 10.3 / 9.1 / 8.7 / 9.2, on
+// 8000 8 / 16 / 32 / 64: 12.4 / 10.0 / 9.9 / 12.3; 32 / 8 heads, D = 128, on 16000 16 / 32 /
+// 64: 16.7 / 14.1 / 16.6; 16 x 5 rows on 8191 through a window of 4096 2 / 4 / 6 / 8: 39 / 34
+// / 39 / 39; 64 rows on 32768 2 / 4 / 6 / 8: 479 / 461 / 460 / 463.
 // Up to 1024 keys (D = 128: 512) of few rows one split: the join's launch costs the
 // host 4 us, its splits save less (one row on 500 keys split 7.9 / 9.3 us on the GPU,
 // whole 6.9 / 9.1, with the host 16.8 and 12.6; on 1000 keys 7.9 / 9.3 and 9.9 / 13.1).
@@ -482,9 +481,9 @@ PagedPlan paged_plan(const carekv_paged_params& p) {
     keys = std::min(keys, sees);
   }
   const long tiles = std::max(1L, (keys + kTile - 1) / kTile), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
-  const long at = r.nq == 8 ? 1280 : wgs * tiles < 512 * 64 ? 512 : 2048;  // work-groups
-  const bool whole = r.nq < 8 && tiles * p.head_dim <= 32 * 64;
-  const long ns = whole ? 1 : std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
+  const long at = wgs * tiles < 512 * 64 ? 512 : 2048;  // work-groups
+  const long ns = r.nq == 8 ? best_splits(tiles, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
+                  : tiles * p.head_dim <= 32 * 64 ? 1 : std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
   return r;

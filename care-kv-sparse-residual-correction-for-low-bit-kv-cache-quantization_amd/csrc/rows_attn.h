@@ -138,10 +138,10 @@ __device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, floa
     for (int i = 0; i < 4; ++i) dst[i] = w[i];
 }
 
-// The splits' partials of a row: 256 / D rows a work-group, four groups of D / 4
-// threads that take every fourth split, added up in LDS in group order.  Splits
+// The splits' partials of a row: D / 4 threads a row for up to 8 splits, else JG = 4
+// groups of them that take every fourth split, added up in LDS in group order.  Splits
 // behind the rows' last tile wrote nothing and are not read.  4 - 5 us for the rows of
-// single tokens, 27 for 40960 rows of 4 splits (95 MB).
+// single tokens; 40960 rows of 4 splits (95 MB) 18, with the groups 27.
 template <typename E, int D, int KT, int JG>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
   constexpr int D4 = D / 4, RW = 256 / (D4 * JG);
@@ -213,6 +213,25 @@ inline void launch_join(const RowsArgs& a, hipStream_t s) {
   };
   if (a.nsplit <= 8) go(std::integral_constant<int, 1>{});
   else go(std::integral_constant<int, 4>{});
+}
+
+// Key splits of a call of many rows (`tiles` tiles of 32 keys for each of `wgs` work-groups): of 1 to 32 the number with
+// the smallest estimate of its time: rounds of the work-groups' places (4 a CU at D = 64, 3 at 128) by a work-group's
+// tiles, and what the join of two and more costs.  Over 16 shapes it takes 2 % more on average than the best number
+// (until 768 or 1280 work-groups are there: 7 %), at most 7 % (23).  us by splits: 2 x 512 rows of 40 heads on 16896 keys 1
+// / 2 / 4 / 7 / 8: 837 / 533 / 517 / 514 / 534; 8 x 16 rows of 32 / 8 heads on 4000 4 / 8 / 12 / 16: 59 / 43 / 38 / 47;
+// prompts of 512 tokens, 40 heads, 1 / 2 / 4: 25 / 31 / 30.
+inline long best_splits(long tiles, long wgs, long rows, int d) {
+  const long places = d == 64 ? 1024 : 768;
+  const double tile = d == 64 ? 0.8 : 1.3, start = 6.0, join = 12.0, split = rows * (d + 2) * 4 / 3.5e6;  // us
+  long best = 1;
+  double least = 0.0;
+  for (long ns = 1; ns <= std::min(tiles, 32L); ++ns) {
+    const long tps = (tiles + ns - 1) / ns, rounds = (wgs * ns + places - 1) / places;
+    const double cost = rounds * (tps * tile + start) + (ns > 1 ? join + ns * split : 0.0);
+    if (ns == 1 || cost < least) least = cost, best = ns;
+  }
+  return best;
 }
 
 // Whether rows of out lie on 8 and on 16 bytes.

@@ -457,9 +457,8 @@ namespace {
 // each, at most 32 for the join's sake, and none up to 512 keys (D = 128: 256), where
 // the join's launch costs the host more than they save; us a call, by splits: 32 / 4 heads, D = 64,
 // on 1000 keys 1 / 4 / 8: 12.9 / 8.9 / 8.1, on 4097 4 / 8 / 16 / 32: 16.6 / 12.5 / 10.7 /
-// 10.3; 16 x 32 / 8 heads, D = 128, on 4097 2 / 4 / 8 / 16: 47.9 / 46.9 / 48.4 / 50.9.  Many: of
-// at least 4 tiles until 768 (3 a CU) are there: 300 rows of 32 / 8 heads on 4097 3 / 6 /
-// 8 / 12 / 16: 67.6 / 51.5 / 54.7 / 58.7 / 60.5.
+// 10.3; 16 x 32 / 8 heads, D = 128, on 4097 2 / 4 / 8 / 16: 47.9 / 46.9 / 48.4 / 50.9.  Many:
+// best_splits.
 struct WindowPlan {
   int wq, wk, nqb, nsplit, tps;
 };
@@ -473,8 +472,8 @@ WindowPlan window_plan(const carekv_window_params& p) {
   long keys = p.n_keys;  // that a block of rows may see
   if (p.window > 0) keys = std::min(keys, (long)p.window + std::min<long>(p.seq_len, 32L * r.wq) + p.sink + 2 * kt);
   const long tiles = std::max(1L, (keys + kt - 1) / kt), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
-  const long ns = r.wq == 1 ? (tiles * p.head_dim <= 4 * 64 ? 1 : std::max(1L, std::min(std::min(32L, 512 / wgs), tiles)))
-                            : tiles <= 8 ? 1 : std::max(1L, std::min(768 / wgs, (tiles + 3) / 4));
+  const long ns = r.wq == 4 ? best_splits(tiles, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
+                  : tiles * p.head_dim <= 4 * 64 ? 1 : std::max(1L, std::min(std::min(32L, 512 / wgs), tiles));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);
   return r;
