@@ -457,8 +457,11 @@ struct Pages4 {
 };
 
 namespace {
-// How a call is cut: 16 rows of a kv head at once or 32, more in blocks of 128, whose
-// splits best_splits gives.  Key splits of few rows: of at least 8 tiles (two a wave),
+// How a call is cut: 16 rows of a kv head at once or 32 (up to 64: twice), more in
+// blocks of 128, whose splits best_splits gives.  (us, 40 rows of 4 heads as two blocks
+// of few and as one of many, D = 64: 64 sequences of 2000 keys 28 / 39, one of 8000 12 /
+// 18; of 8 heads, D = 128, on 8000 keys: 64 sequences 288 / 338, 16 89 / 87; 96 rows there
+// 129 / 106.)  Key splits of few rows: of at least 8 tiles (two a wave),
 // at most 32: the join reads every split's partials.  us a call, by splits: one row of
 // 32 / 4 heads, D = 64, on 2303 keys 1 / 4 / 8 / 16 / 32: 17.2 / 10.3 / 9.1 / 8.7 / 9.2, on
 // 8000 8 / 16 / 32 / 64: 12.4 / 10.0 / 9.9 / 12.3; 32 / 8 heads, D = 128, on 16000 16 / 32 /
@@ -473,7 +476,7 @@ struct PagedPlan {
 PagedPlan paged_plan(const carekv_paged_params& p) {
   PagedPlan r{};
   const long M = (long)p.seq_len * (p.n_heads / p.n_kv_heads);
-  r.nq = M <= 16 ? 1 : M <= 32 ? 2 : 8;
+  r.nq = M <= 16 ? 1 : M <= 64 ? 2 : 8;
   r.nqb = (int)((M + 16 * r.nq - 1) / (16 * r.nq));
   long keys = (long)p.max_pages * kPage;  // that a block of rows may see
   if (p.window > 0) {

@@ -263,7 +263,7 @@ def test_paged(dtype, window, sink, B, Hq, Hkv, D, T, N):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("window,sink", [(None, 0), (50, 4)])
-@pytest.mark.parametrize("Hq,Hkv,D,T", [(8, 2, 64, 1), (4, 4, 128, 6), (6, 1, 128, 30)])
+@pytest.mark.parametrize("Hq,Hkv,D,T", [(8, 2, 64, 1), (4, 4, 128, 6), (8, 2, 64, 12), (9, 3, 128, 21), (6, 1, 128, 30)])
 def test_ragged(dtype, window, sink, Hq, Hkv, D, T):
     """Lengths of zero and one, before a page's end, past the table; rows of padding; pages that are not there."""
     import care_kv
@@ -293,7 +293,7 @@ def test_ragged(dtype, window, sink, Hq, Hkv, D, T):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("T,G", [(1, 4), (12, 1), (40, 3)])
+@pytest.mark.parametrize("T,G", [(1, 4), (12, 1), (16, 3), (40, 3)])
 def test_not_a_number_where_a_row_does_not_look(D, T, G):
     """Values that are not finite at single tokens: the rows that see them are NaN there, the others untouched."""
     import care_kv
