@@ -219,7 +219,7 @@ inline void launch_join(const RowsArgs& a, hipStream_t s) {
 // the smallest estimate of its time: rounds of the work-groups' places (4 a CU at D = 64, 3 at 128) by a work-group's
 // tiles, and what the join of two and more costs.  Over 16 shapes it takes 2 % more on average than the best number
 // (until 768 or 1280 work-groups are there: 7 %), at most 7 % (23).  us by splits: 2 x 512 rows of 40 heads on 16896 keys 1
-// / 2 / 4 / 7 / 8: 837 / 533 / 517 / 514 / 534; 8 x 16 rows of 32 / 8 heads on 4000 4 / 8 / 12 / 16: 59 / 43 / 38 / 47;
+// / 2 / 4 / 7 / 8: 837 / 533 / 517 / 514 / 534; 4 x 64 rows of 32 / 8 heads on 8000 5 / 8 / 12 / 16: 103 / 76 / 72 / 92;
 // prompts of 512 tokens, 40 heads, 1 / 2 / 4: 25 / 31 / 30.
 inline long best_splits(long tiles, long wgs, long rows, int d) {
   const long places = d == 64 ? 1024 : 768;

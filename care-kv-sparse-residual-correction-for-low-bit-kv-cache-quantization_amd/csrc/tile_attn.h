@@ -42,9 +42,10 @@ __global__ __launch_bounds__(256, Src::D == 64 ? 4 : 3) void tile_attn_kernel(ty
   __shared__ __align__(16) char lds[2 * BUF];
   __shared__ int s_odd[2];  // the last tile in the buffer that held a V value that is not finite
   __shared__ int s_again;
-  const int it = xcd_item(a);
-  const int sp_blk = it / a.by_nsplit, sp = it - sp_blk * a.nsplit;
-  const int bh = sp_blk / a.by_nqb, qblk = a.nqb - 1 - (sp_blk - bh * a.nqb);  // (blocks with more keys first)
+  // the items of a kv head (by_group): a split's blocks side by side, those with more keys first (a block's splits side by
+  // side, of which a prompt's short blocks have one or two, load the CUs unevenly: 2 x 1744 rows of 8 heads 38 us, so 33)
+  const int it = xcd_item(a), bh = it / a.by_group, in = it - bh * a.by_group.d;
+  const int sp = in / a.by_nqb, qblk = a.nqb - 1 - (in - sp * a.nqb);
   const int b = bh / a.by_hkv, hk = bh - b * a.Hkv;
   const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
