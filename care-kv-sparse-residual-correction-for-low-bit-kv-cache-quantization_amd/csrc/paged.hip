@@ -548,7 +548,8 @@ extern "C" int carekv_paged_attn(const carekv_paged_params* pp, const void* q, c
   a.sink = p.sink;
   a.nqb = plan.nqb; a.nsplit = plan.nsplit; a.tps = plan.tps; a.qb_rows = 16 * plan.nq;
   a.by_g = FastDiv(a.G); a.by_nqb = FastDiv(a.nqb); a.by_hkv = FastDiv(a.Hkv); a.by_nsplit = FastDiv(a.nsplit); a.by_m = FastDiv(a.M);
-  a.by_group = FastDiv((long)a.nqb * (plan.nq == 8 ? a.nsplit : a.Hkv));
+  if (plan.nq == 8) set_groups(a, (long)a.nqb * a.nsplit, (long)p.batch * a.Hkv);
+  else set_groups(a, (long)a.nqb * a.Hkv, (long)p.batch * a.nsplit);
   a.po = (float*)workspace;
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);

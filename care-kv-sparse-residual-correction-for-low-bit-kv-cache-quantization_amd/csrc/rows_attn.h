@@ -31,7 +31,7 @@ struct RowsArgs {
   int Hq, Hkv, G, T, M, max_keys, window, sink, nqb, nsplit, qb_rows;
   int tps;                   // tiles of a split
   FastDiv by_g, by_nqb, by_hkv, by_nsplit, by_m;
-  FastDiv by_group;          // items of a group (see xcd_item)
+  FastDiv by_group, by_left; // items of a group, groups that eight does not divide (see xcd_item)
   FastDiv by_period;         // tiles of a window and a block's tokens (see Span)
   float sm_log2;             // |scale| log2(e), 1 where that is 0
   uint32_t q_sign, q_keep;   // sign bits of two elements where the scale is negative; 0 where it is 0
@@ -42,7 +42,9 @@ struct RowsArgs {
 // memory; work-groups go round the 8 XCDs, and an XCD takes one group of every
 // eight, each time another one of them, so that the items of a group meet in its
 // L2 and each XCD has some of every (ragged) sequence (8 ragged prompts of 2047 tokens
-// 159 us, in plain order 208); of the groups that are left over each XCD takes a share.
+// 159 us, in plain order 208).  The up to seven groups that are left over go side by
+// side, longest items first, over all XCDs (8192 rows of 4 kv heads, D = 64: 339 us, one
+// after the other 405, a part of them to each XCD 449).
 // Blocks of 2 to 8 heads in turn, longest first: full 8192 rows 2 % better, through a
 // window the same, ragged batches up to a fifth worse.
 __device__ __forceinline__ int xcd_item(const RowsArgs& a) {
@@ -52,8 +54,8 @@ __device__ __forceinline__ int xcd_item(const RowsArgs& a) {
     const int j = (idx >> 3) / a.by_group;
     return (8 * j + (x + j & 7)) * per + (idx >> 3) - j * per;
   }
-  const int left = n - whole;
-  return whole + left / 8 * x + min(x, left & 7) + ((idx - whole) >> 3);
+  const int j = idx - whole, at = j / a.by_left;
+  return whole + (j - at * a.by_left.d) * per + at;
 }
 
 // Sequence b's counts, kept where sums of them stay in 32 bits.
@@ -239,6 +241,12 @@ inline void set_alignment(RowsArgs& a, int batch) {
   const uintptr_t bits = operand_bits(a.out, {{batch, a.o_sb}, {a.Hq, a.o_sh}, {a.T, a.o_st}});
   a.al8 = (bits & 7) == 0;
   a.al16 = (bits & 15) == 0;
+}
+
+// The groups of a launch, of `per` items each.
+inline void set_groups(RowsArgs& a, long per, long groups) {
+  a.by_group = FastDiv(per);
+  a.by_left = FastDiv(std::max(1L, groups % 8));
 }
 
 // The period of blocks of `tokens` tokens and tiles of kt keys.

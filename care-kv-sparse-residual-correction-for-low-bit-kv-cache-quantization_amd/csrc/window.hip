@@ -537,7 +537,7 @@ extern "C" int carekv_window_attn(const carekv_window_params* pp, const void* q,
   a.sink = p.sink;
   a.nqb = plan.nqb; a.nsplit = plan.nsplit; a.tps = plan.tps; a.qb_rows = 32 * plan.wq;
   a.by_g = FastDiv(a.G); a.by_nqb = FastDiv(a.nqb); a.by_hkv = FastDiv(a.Hkv); a.by_nsplit = FastDiv(a.nsplit); a.by_m = FastDiv(a.M);
-  a.by_group = FastDiv((long)a.nqb * a.nsplit);
+  set_groups(a, (long)a.nqb * a.nsplit, (long)p.batch * a.Hkv);
   a.po = (float*)workspace;
   a.pml = a.po + plan.nsplit * rows * p.head_dim;
   set_scale(a, p.sm_scale);
