@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void paged_rows_kernel(PagedA
 // Many rows: bound by the products, so that the codes are turned into fp16 once for
 // the 128 rows of tile_attn.h.  A wave takes half of one page's codes of a tile of 32
 // keys and writes them to LDS as the operands that all four read, 1 KB each in the
-// lanes' order.  2 x 512 rows of 40 heads, D = 128, on 16896 keys: 507 us, 0.69 PFLOP/s.
+// lanes' order.  2 x 512 rows of 40 heads, D = 128, on 16896 keys: 511 - 518 us, 0.68 PFLOP/s.
 template <typename E_, int D_>
 struct Pages4 {
   using Args = PagedArgs;
