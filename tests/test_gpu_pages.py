@@ -427,3 +427,33 @@ def test_streams_and_graphs():
             assert torch.equal(out[0], eager[i][0]) and torch.equal(out[1], eager[i][1]), f"replay {i}"
     torch.cuda.synchronize()
     assert all(torch.equal(pg.data, pages.data) for *_, pg in graphs)
+
+
+def test_two_streams_with_splits():
+    """Many rows in a few key splits, groups that stand for NaN in some of them, two streams at once."""
+    import care_kv
+    g, r = _gen(60)
+    B, H, D, T, N = 2, 24, 64, 150, 3000
+    table, n = _table(B, -(-N // 16), g)
+    K, V = r(B, H, N, D).half(), r(B, H, N, D).half()
+    V[0, 3, 2990, 5], V[1, 2, 600, 9] = math.inf, math.nan
+    pages = _fill(care_kv, K, V, table, n)
+    q = r(B, H, T, D).half()
+    lengths, rows = [N, 1203], [T, T - 1]
+    dev = torch.tensor([lengths, rows], dtype=torch.int32, device="cuda")
+    call = lambda x: care_kv.paged_attention(x, pages, table, dev[0], q_lengths=dev[1], window=2500, sink=3,  # noqa: E731
+                                             return_lse=True)
+    see = sight(B, T, N, 2500, 3, lengths, rows, None)
+    check(call(q), attend(q, round4(K)[2], round4(V)[2], see, weights=F16))
+    xs = [q * (1 + 0.1 * i) for i in range(6)]
+    want = [call(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * 6
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, x in enumerate(xs):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = call(x)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(torch.nan_to_num(a[0]), torch.nan_to_num(b[0])) and torch.equal(a[1], b[1])

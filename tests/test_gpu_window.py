@@ -200,3 +200,27 @@ def test_a_captured_call():
         want = call()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_two_streams_with_splits():
+    """Many rows in a few key splits, values that are not finite in some of them, two streams at once: each call's own."""
+    import care_kv
+    q, k, v = _inputs(15, 2, 24, 24, 64, 300, 2000, F16)
+    v[0, 3, 1990, 5], v[1, 2, 600, 9] = math.inf, math.nan
+    lengths, rows = [2000, 1203], [300, 299]
+    dev = torch.tensor([lengths, rows], dtype=torch.int32, device="cuda")
+    call = lambda x: care_kv.window_attention(x, k, v, window=1500, sink=3, lengths=dev[0], q_lengths=dev[1],  # noqa: E731
+                                              return_lse=True)
+    check(call(q), attend(q, k, v, sight(2, 300, 2000, 1500, 3, lengths, rows, None)))
+    xs = [q * (1 + 0.1 * i) for i in range(6)]
+    want = [call(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * 6
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, x in enumerate(xs):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = call(x)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(torch.nan_to_num(a[0]), torch.nan_to_num(b[0])) and torch.equal(a[1], b[1])
