@@ -384,7 +384,8 @@ class CAREKVLayer(nn.Module):
         ``append_pages`` takes them or None for places in the sequence.  ``fresh``: a
         prompt of sequences that hold nothing yet (lengths are not looked at),
         whose attention runs over its rows as they are (``window_attention``, the
-        ``fp`` mode of ``prefill``).  Nothing waits for the device, and with tensors
+        ``fp`` mode of ``prefill``); its pages are those of the same tokens written
+        as a chunk.  Nothing waits for the device, and with tensors
         for lengths and counts the call can be captured."""
         plan, pos = (None, None) if position_embeddings is None else position_embeddings
         if plan is not None and not isinstance(plan, RotaryPlan):
@@ -397,10 +398,10 @@ class CAREKVLayer(nn.Module):
             Q, K, V = Q.to(F16), K.to(F16), V.to(F16)
         n = _lib.row_counts(counts, B, Q.device, "counts")
         if fresh:
-            if plan is not None:
-                Q, K = rotate_heads(Q, K, torch.arange(T, device=Q.device) if pos is None else pos, plan)
-            append_pages(pages, table, 0, K, V, counts=n)
-            O = window_attention(Q, K, V, window=window, sink=sink, lengths=n, q_lengths=n)
+            # the pages take the keys before their turn, so that they round them to fp16 once, as those of a chunk
+            q, k = (Q, K) if plan is None else rotate_heads(Q, K, torch.arange(T, device=Q.device) if pos is None else pos, plan)
+            append_pages(pages, table, 0, K, V, plan=plan, positions=pos, counts=n)
+            O = window_attention(q, k, V, window=window, sink=sink, lengths=n, q_lengths=n)
         else:
             if lengths is None:
                 raise ValueError("paged_step needs lengths, the tokens that the sequences hold")

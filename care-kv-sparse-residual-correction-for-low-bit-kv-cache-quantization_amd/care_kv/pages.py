@@ -111,8 +111,8 @@ def append_pages(pages: Int4Pages, table: torch.Tensor, start, k: torch.Tensor, 
     start, counts: a device tensor of B integers, one int for all, or (not in
     captured code) a host sequence.  ``plan``: turned as by ``rotate_heads`` at
     ``positions`` (int32 or int64 (B, T), (1, T) or (T,); default start + t), in 64
-    bits, rounded to 32 and then to the type; without a plan k and q are taken as
-    they are.  k_hat, v_hat: fp16 (B, Hkv, T, D), the values that the new rows
+    bits, rounded to 32 and then, q to the type, k to fp16; without a plan k and q
+    are taken as they are.  k_hat, v_hat: fp16 (B, Hkv, T, D), the values that the new rows
     stand for, zeros behind the counts.
 
     Tokens before place 0, behind the table or on pages that are not there are

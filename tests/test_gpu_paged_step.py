@@ -154,3 +154,24 @@ def test_serving_with_drafts():
         step(begin(), draft[i], q[i], u[i], un[i])  # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(out.tokens, eager[i][0]) and torch.equal(out.accepted, eager[i][1]), f"replay {i}"
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,D,R,layout", [(8, 2, 64, 64, "half"), (4, 4, 128, 64, "interleaved")])
+def test_a_fresh_prompt_is_a_chunk(dtype, Hq, Hkv, D, R, layout):
+    """A prompt leaves the same bytes whether it is written fresh or as a chunk of sequences that hold nothing: keys are
+    turned and rounded to fp16 once."""
+    import care_kv
+    B, T, model, P = 3, 90, 64, 6
+    layer, r = _layer(care_kv, Hq, Hkv, D, model, dtype, seed=5)
+    plan = care_kv.rotary_plan(R, layout=layout)
+    table = torch.randperm(B * P, device="cuda").view(B, P).int()
+    h = r(B, T, model)
+    for pos in (None, torch.arange(T, device="cuda") + 70000, torch.randint(0, 9000, (B, T), device="cuda")):
+        for pe in ((plan, pos), None):
+            left = []
+            for fresh in (True, False):
+                pages = care_kv.int4_pages(B * P, Hkv, D)
+                layer.paged_step(pages, h, table, 0, pe, counts=[T, 33, 0], fresh=fresh)
+                left.append(pages.data)
+            assert torch.equal(*left), (pos is None, pe is None)
