@@ -375,10 +375,11 @@ class CAREKVLayer(nn.Module):
         K and V go behind the ``lengths[b]`` tokens that the sequence holds in
         ``pages`` (``append_pages``), their queries attend to all of them, with
         ``window`` to the last ``window`` and the first ``sink``
-        (``paged_attention``).  Of a ragged batch the first ``counts[b]`` tokens
-        count; what the others' rows of the result hold means nothing.  The caller
-        adds the tokens that stay to lengths: one of a decode step, the accepted
-        ones of drafts and the one behind them, all of a prompt's chunk.
+        (``paged_attention``).  Of a ragged batch the first ``counts[b]`` tokens (0
+        to T, what is outside counts as the nearer one) count; what the others' rows
+        of the result hold means nothing.  The caller adds the tokens that stay to
+        lengths: one of a decode step, the accepted ones of drafts and the one behind
+        them, all of a prompt's chunk.
 
         position_embeddings: (RotaryPlan, positions), positions as
         ``append_pages`` takes them or None for places in the sequence.  ``fresh``: a
@@ -397,6 +398,7 @@ class CAREKVLayer(nn.Module):
         if Q.dtype not in (F16, torch.bfloat16):
             Q, K, V = Q.to(F16), K.to(F16), V.to(F16)
         n = _lib.row_counts(counts, B, Q.device, "counts")
+        n = None if n is None else n.clamp(0, T)  # (also where the lengths are made of it)
         if fresh:
             # the pages take the keys before their turn, so that they round them to fp16 once, as those of a chunk
             q, k = (Q, K) if plan is None else rotate_heads(Q, K, torch.arange(T, device=Q.device) if pos is None else pos, plan)

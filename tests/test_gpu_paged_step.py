@@ -175,3 +175,25 @@ def test_a_fresh_prompt_is_a_chunk(dtype, Hq, Hkv, D, R, layout):
                 layer.paged_step(pages, h, table, 0, pe, counts=[T, 33, 0], fresh=fresh)
                 left.append(pages.data)
             assert torch.equal(*left), (pos is None, pe is None)
+
+
+def test_counts_past_the_step():
+    """Counts above T are T and counts below 0 are 0, as the operators take them, also for where the rows stand."""
+    import care_kv
+    B, T, model, Hq, Hkv, D, P = 4, 5, 64, 8, 2, 64, 4
+    layer, r = _layer(care_kv, Hq, Hkv, D, model, F16, seed=6)
+    plan = care_kv.rotary_plan(D)
+    table = torch.arange(B * P, device="cuda").view(B, P).int()
+    before, h = r(B, 30, model), r(B, T, model)
+    held, counts, cut = [30, 4, 17, 9], [T + 4, -3, 2, 2 ** 31 - 1], [T, 0, 2, T]
+    forms = (cut, counts, torch.tensor(counts, device="cuda"), torch.tensor(counts, device="cuda", dtype=torch.int32))
+    want = None
+    for fresh in (False, True):
+        for i, n in enumerate(forms):
+            pages = care_kv.int4_pages(B * P, Hkv, D)
+            layer.paged_step(pages, before, table, 0, (plan, None))  # (what is behind held: tokens that did not stay)
+            got = layer.paged_step(pages, h, table, held, (plan, None), counts=n, window=20, sink=2, fresh=fresh)
+            want = (got, pages.data) if i == 0 else want
+            assert torch.equal(pages.data, want[1])
+            for b in range(B):
+                assert torch.equal(got[b, :cut[b]], want[0][b, :cut[b]]), (fresh, i, b)
