@@ -389,7 +389,7 @@ class CAREKVLayer(nn.Module):
         as a chunk.  Nothing waits for the device, and with tensors
         for lengths and counts the call can be captured."""
         plan, pos = (None, None) if position_embeddings is None else position_embeddings
-        if plan is not None and not isinstance(plan, RotaryPlan):
+        if not isinstance(plan, RotaryPlan) and (plan is not None or pos is not None):
             raise ValueError("paged_step: position_embeddings must be (RotaryPlan, positions or None)")
         if hidden.dim() != 3:
             raise ValueError(f"paged_step: hidden must be (B, T, model_dim); got {tuple(hidden.shape)}")

@@ -197,3 +197,15 @@ def test_counts_past_the_step():
             assert torch.equal(pages.data, want[1])
             for b in range(B):
                 assert torch.equal(got[b, :cut[b]], want[0][b, :cut[b]]), (fresh, i, b)
+
+
+@pytest.mark.parametrize("fresh", [False, True])
+def test_positions_need_a_plan(fresh):
+    import care_kv
+    layer, r = _layer(care_kv, 4, 2, 64, 32, F16)
+    pages, table = care_kv.int4_pages(4, 2, 64), torch.arange(4, device="cuda").view(2, 2).int()
+    with pytest.raises(ValueError):
+        layer.paged_step(pages, r(2, 3, 32), table, 0, (None, torch.arange(3, device="cuda")), fresh=fresh)
+    assert not pages.data.any()
+    got = layer.paged_step(pages, r(2, 3, 32), table, 0, (None, None), fresh=fresh)
+    assert got.shape == (2, 3, 32) and pages.data.any()
