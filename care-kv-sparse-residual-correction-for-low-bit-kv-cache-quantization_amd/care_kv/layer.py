@@ -39,7 +39,7 @@ from .attention import (debug_stats_enabled, decode_attention, decode_read_mode,
                         get_imp_per_layer, importance_probe, prefill_correction, reset_debug_stats)
 from .cache import CAREKVCache
 from .eviction import attention_mass, evict_rows
-from .pages import Int4Pages, append_pages, paged_attention
+from .pages import Int4Pages, append_pages, check_window, paged_attention
 from .prefix import check_prefix, prefix_attention
 from .window import window_attention
 from .rotary import RotaryPlan, rotate_heads
@@ -386,13 +386,15 @@ class CAREKVLayer(nn.Module):
         prompt of sequences that hold nothing yet (lengths are not looked at),
         whose attention runs over its rows as they are (``window_attention``, the
         ``fp`` mode of ``prefill``); its pages are those of the same tokens written
-        as a chunk.  Nothing waits for the device, and with tensors
-        for lengths and counts the call can be captured."""
+        as a chunk.  Nothing waits for the device, and with tensors for lengths and
+        counts the call can be captured.  A call that is refused has written
+        nothing."""
         plan, pos = (None, None) if position_embeddings is None else position_embeddings
         if not isinstance(plan, RotaryPlan) and (plan is not None or pos is not None):
             raise ValueError("paged_step: position_embeddings must be (RotaryPlan, positions or None)")
         if hidden.dim() != 3:
             raise ValueError(f"paged_step: hidden must be (B, T, model_dim); got {tuple(hidden.shape)}")
+        check_window(window, sink)  # (what is refused is refused before the pages are written to)
         B, T, _ = hidden.shape
         Q, K, V = self._project(hidden)
         if Q.dtype not in (F16, torch.bfloat16):

@@ -209,3 +209,19 @@ def test_positions_need_a_plan(fresh):
     assert not pages.data.any()
     got = layer.paged_step(pages, r(2, 3, 32), table, 0, (None, None), fresh=fresh)
     assert got.shape == (2, 3, 32) and pages.data.any()
+
+
+def test_a_refused_step_writes_nothing():
+    import care_kv
+    B, T, P = 2, 3, 2
+    layer, r = _layer(care_kv, 4, 2, 64, 32, F16)
+    pages, table, h = care_kv.int4_pages(B * P, 2, 64), torch.arange(B * P, device="cuda").view(B, P).int(), r(B, T, 32)
+    plan = care_kv.rotary_plan(64)
+    for fresh in (False, True):
+        for bad in (dict(window=0), dict(window=-4), dict(sink=-1), dict(counts=[1]), dict(table=table[:1]),
+                    dict(position_embeddings=(care_kv.rotary_plan(128), None)),
+                    dict(position_embeddings=(plan, torch.zeros(T + 1, dtype=torch.int64, device="cuda")))):
+            kw = {**dict(pages=pages, hidden=h, table=table, lengths=0, position_embeddings=(plan, None)), **bad}
+            with pytest.raises(ValueError):
+                layer.paged_step(**kw, fresh=fresh)
+            assert not pages.data.any(), (fresh, bad)
