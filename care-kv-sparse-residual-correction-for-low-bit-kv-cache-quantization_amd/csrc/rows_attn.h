@@ -126,6 +126,16 @@ __device__ __forceinline__ void write_lse(const RowsArgs& a, int b, int hk, int 
   const int t = r / a.by_g, h = hk * a.G + r - t * a.G;
   a.lse[((long)b * a.Hq + h) * a.T + t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
+// A row's sums under a new reference.  What is not finite stays as it is: an infinity that a row sees is its result however
+// small its weight, and 0 times it, where f is that small, would be no number.
+__device__ __forceinline__ float4_t rescaled(float4_t o, float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = fabsf(o[i]) < INFINITY ? o[i] * f : o[i];
+  return o;
+}
+__device__ __forceinline__ bool all_finite(float4_t o) {
+  return fmaf(o[0], 0.f, fmaf(o[1], 0.f, fmaf(o[2], 0.f, o[3] * 0.f))) == 0.f;
+}
 // four neighbouring dims of a row, o / l (0 for a row that sees nothing)
 template <typename E>
 __device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, float4_t o, float l) {
@@ -142,8 +152,10 @@ __device__ __forceinline__ void write4(const RowsArgs& a, char* row, int d, floa
 
 // The splits' partials of a row: D / 4 threads a row for up to 8 splits, else JG = 4
 // groups of them that take every fourth split, added up in LDS in group order.  Splits
-// behind the rows' last tile wrote nothing and are not read.  4 - 5 us for the rows of
-// single tokens; 40960 rows of 4 splits (95 MB) 18, with the groups 27.
+// behind the rows' last tile wrote nothing and are not read.  Sums that come out not
+// finite are added up once more, by what rescaled does (in every sum it cost one row on
+// 2303 keys 0.7 us, so 0.1).  4 - 5 us for the rows of single tokens; 40960 rows of 4
+// splits (95 MB) 18, with the groups 27.
 template <typename E, int D, int KT, int JG>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
   constexpr int D4 = D / 4, RW = 256 / (D4 * JG);
@@ -164,24 +176,31 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
     const Span<KT> span(a, s, r0 / a.by_g, (r1 - 1) / a.by_g + 1);
     const int ns = (span.n + a.tps - 1) / a.tps;
     pad = r / a.by_g >= s.qlen;
-    for (int s0 = grp; s0 < ns; s0 += 4 * JG) {  // four splits' loads in flight
-      float2 ml[4];
-      float4_t v[4];
+    auto add_up = [&](auto with_care) {
+      m = kLowest;
+      L = 0.f;
+      o = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int s0 = grp; s0 < ns; s0 += 4 * JG) {  // four splits' loads in flight
+        float2 ml[4];
+        float4_t v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const long at = min(s0 + u * JG, ns - 1) * a.rows + pr;
-        ml[u] = *reinterpret_cast<const float2*>(a.pml + 2 * at);
-        v[u] = *reinterpret_cast<const float4_t*>(a.po + at * D + 4 * d4);
-      }
+        for (int u = 0; u < 4; ++u) {
+          const long at = min(s0 + u * JG, ns - 1) * a.rows + pr;
+          ml[u] = *reinterpret_cast<const float2*>(a.pml + 2 * at);
+          v[u] = *reinterpret_cast<const float4_t*>(a.po + at * D + 4 * d4);
+        }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (s0 + u * JG >= ns) break;
-        const float mn = fmaxf(m, ml[u].x), f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[u].x - mn);
-        o = o * f + v[u] * e;
-        L = L * f + ml[u].y * e;
-        m = mn;
+        for (int u = 0; u < 4; ++u) {
+          if (s0 + u * JG >= ns) break;
+          const float mn = fmaxf(m, ml[u].x), f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[u].x - mn);
+          o = decltype(with_care)::value ? rescaled(o, f) + rescaled(v[u], e) : o * f + v[u] * e;
+          L = L * f + ml[u].y * e;
+          m = mn;
+        }
       }
-    }
+    };
+    add_up(std::false_type{});
+    if (__builtin_expect(!all_finite(o), 0)) add_up(std::true_type{});
   }
   if constexpr (JG > 1) {
     __shared__ float4_t s_o[256];
@@ -199,6 +218,10 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a) {
       const float f = __builtin_amdgcn_exp2f(s_ml[rw][i].x - m);
       L += s_ml[rw][i].y * f;
       o += s_o[(rw * JG + i) * D4 + d4] * f;
+    }
+    if (__builtin_expect(!all_finite(o), 0)) {
+      o = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < JG; ++i) o += rescaled(s_o[(rw * JG + i) * D4 + d4], __builtin_amdgcn_exp2f(s_ml[rw][i].x - m));
     }
   }
   if (!in || grp != 0) return;

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256, Src::D == 64 ? 4 : 3) void tile_attn_kernel(ty
             m_run[qb] = m_new;
             l_run[qb] *= f;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= f;
+            for (int dt = 0; dt < DT; ++dt) o[qb][dt] = care ? rescaled(o[qb][dt], f) : o[qb][dt] * f;
           }
         }
         V8 bp[NQ];

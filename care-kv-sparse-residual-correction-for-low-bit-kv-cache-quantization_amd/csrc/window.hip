@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
   constexpr int KS = D / 32, DT = D / 16, CHR = D / 8, NCH = 2 * KT * CHR / NT;
   constexpr int KBUF = KT * KRS, BUF = KBUF + KT * VRS;
   __shared__ __align__(16) char lds[BUF];
-  __shared__ int s_odd;  // the last tile that held a V value that is not finite
+  __shared__ int s_odd;  // whether a tile held a V value that is not finite
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t lds_short4;
 
@@ -236,11 +236,11 @@ __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
       stg[k][0] = v[0]; stg[k][1] = v[1]; stg[k][2] = v[2]; stg[k][3] = v[3];
     }
   };
-  // (a masked weight of 0 times a value that is not finite would be no number: such a value is 0 in the tile, its tile
-  // noted and its rows' results set from the value itself)
-  auto store_tile = [&](int i) {
+  // (a weight of 0 times a value that is not finite would be no number: such a value is 0 in the tile, and added at the
+  // end to the rows that see it)
+  auto store_tile = [&] {
     if (__builtin_expect(not_finite<ET, 2 * NCH>(&stg[NCH / 2][0]), 0)) {
-      s_odd = i;
+      s_odd = 1;
 #pragma unroll
       for (int k = NCH / 2; k < NCH; ++k)
 #pragma unroll
@@ -267,11 +267,11 @@ __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   const float c = a.sm_log2;  // (not negative)
-  if (threadIdx.x == 0) s_odd = -1;
+  if (threadIdx.x == 0) s_odd = 0;
   __syncthreads();
   if (nt > 0) {
     load_tile(0);
-    store_tile(0);
+    store_tile();
   }
   __syncthreads();
   if (nt > 1) load_tile(1);
@@ -356,34 +356,46 @@ __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) o[qb][dt] = ET::mfma(av, bp[qb], o[qb][dt]);
       }
-      if (__builtin_expect(s_odd == i, 0)) {
-        // values that are not finite, from where they came, into the rows that see them: with a weight over 0 they
-        // are the result whatever it is
-#pragma unroll 1
-        for (int key = 0; key < min(32, seq.len - jw); ++key) {
-          const char* src = vbase + (long)(jw + key) * a.v_st + 8 * g;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
-            uint32_t x[2];
-            __builtin_memcpy(x, __builtin_assume_aligned(src + 32 * dt, 8), 8);
-            if (!(not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]))) continue;
-            E v[4];
-            __builtin_memcpy(v, x, 8);
-#pragma unroll
-            for (int qb = 0; qb < NQ; ++qb)
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                if (sight[qb].sees(a, jw + key) && !(fabsf((float)v[y]) < INFINITY)) o[qb][dt][y] += (float)v[y];
-          }
-        }
-      }
     }
     __builtin_amdgcn_s_setprio(0);
     __syncthreads();
-    if (i + 1 < nt) store_tile(i + 1);
+    if (i + 1 < nt) store_tile();
     if (i + 2 < nt) load_tile(i + 2);
     __syncthreads();
+  }
+  // Values that are not finite, from where they came, into the rows that see them: with a weight over 0 they are the
+  // result whatever it is, so that they are added when no sum is rescaled any more.
+  const bool odd = s_odd;
+  if (__builtin_expect(odd, 0)) {
+#pragma unroll 1
+    for (int i = 0; i < nt; ++i) {
+      const int jw = span.tile(i0 + i) * KT + 32 * wk, keys = min(32, seq.len - jw);
+      bool some = false;
+      for (int x = lane; x < keys * CHR; x += 64) {
+        uint32_t u[4];
+        __builtin_memcpy(u, __builtin_assume_aligned(vbase + (long)(jw + x / CHR) * a.v_st + x % CHR * 16, 16), 16);
+        some |= not_finite<ET, 4>(u);
+      }
+      if (!__any(some)) continue;
+#pragma unroll 1
+      for (int key = 0; key < keys; ++key) {
+        const char* src = vbase + (long)(jw + key) * a.v_st + 8 * g;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          asm volatile("" ::: "memory");  // (one at a time: in flight together they would cost the loop its registers)
+          uint32_t x[2];
+          __builtin_memcpy(x, __builtin_assume_aligned(src + 32 * dt, 8), 8);
+          if (!(not_finite2<ET>(x[0]) | not_finite2<ET>(x[1]))) continue;
+          E v[4];
+          __builtin_memcpy(v, x, 8);
+#pragma unroll
+          for (int qb = 0; qb < NQ; ++qb)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (sight[qb].sees(a, jw + key) && !(fabsf((float)v[y]) < INFINITY)) o[qb][dt][y] += (float)v[y];
+        }
+      }
+    }
   }
   float lt[NQ];
 #pragma unroll
@@ -406,7 +418,8 @@ __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
     for (int i = 0; i < WK; ++i) l += s_ml[i][16 * qb + c16][1] * __builtin_amdgcn_exp2f(s_ml[i][16 * qb + c16][0] - m);
     const float f = __builtin_amdgcn_exp2f(m_run[qb] - m);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(so + ((wk * DT + dt) * 64 + lane) * 4) = o[qb][dt] * f;
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<float4_t*>(so + ((wk * DT + dt) * 64 + lane) * 4) = odd ? rescaled(o[qb][dt], f) : o[qb][dt] * f;
     m_run[qb] = m;
     lt[qb] = l;
     __syncthreads();

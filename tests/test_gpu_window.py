@@ -224,3 +224,36 @@ def test_two_streams_with_splits():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(torch.nan_to_num(a[0]), torch.nan_to_num(b[0])) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,Tq,Tk", [(1, 4, 2, 64, 1, 300), (2, 4, 2, 64, 3, 5000), (1, 2, 2, 128, 5, 2000),
+                                              (1, 4, 2, 64, 130, 130), (1, 2, 2, 128, 40, 700), (2, 4, 1, 64, 60, 3000),
+                                              (1, 8, 1, 128, 30, 9000)])
+def test_infinite_values_of_small_weight(dtype, B, Hq, Hkv, D, Tq, Tk):
+    """An infinity that a row sees is its result however small its weight: before the key that outweighs it by 2^250 or
+    behind it, in its tile, in another wave's keys, in another split."""
+    import care_kv
+    q, k, v = _inputs(21, B, Hq, Hkv, D, Tq, Tk, dtype)
+    u = torch.ones(D, device="cuda")
+    u[::3] = -1
+    q = (0.5 * q + 2 * u).to(dtype)
+    # the strong keys' logits: 2 |u|^2 a / sqrt(D) = 180 with a deviation of 0.5 |u| a / sqrt(D)
+    a = 90 / D ** 0.5
+    see = sight(B, Tq, Tk, None, 0, [Tk] * B, [Tq] * B, None)
+    first = Tk - Tq
+    for odd, strong in ((2, 5), (5, 2), (3, 40), (40, 3), (10, 75), (75, 10), (20, Tk // 2), (Tk // 2, 20), (first + 1, 1),
+                        (1, first + Tq // 2)):
+        if odd == strong or max(odd, strong) >= Tk:
+            continue
+        kk, vv = k.clone(), v.clone()
+        kk[:, :, strong] = (a * u).to(dtype)
+        vv[:, :, odd, 7], vv[0, 0, odd, 20], vv[:, :, odd, D - 1] = math.inf, -math.inf, math.nan
+        ref = attend(q, kk, vv, see)
+        assert float(ref[1].max()) > 150
+        print(f"{dtype} {B} {Hq}/{Hkv} D={D} {Tq} on {Tk}: infinite {odd}, strong {strong}", flush=True)
+        check(care_kv.window_attention(q, kk, vv, return_lse=True), ref)
+    vv = v.clone()  # infinities of both signs: no number
+    kk[:, :, Tk // 2] = (a * u).to(dtype)
+    vv[:, :, 1, 3], vv[:, :, Tk // 3, 3], vv[:, :, Tk // 3, 4] = math.inf, -math.inf, -math.inf
+    check(care_kv.window_attention(q, kk, vv, return_lse=True), attend(q, kk, vv, see))
