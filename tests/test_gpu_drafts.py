@@ -175,3 +175,54 @@ def test_a_captured_call():
         want = call()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,V", [(1, 2, 65537), (3, 3, 70001), (2, 1, 131071), (1, 1, 262145)])
+def test_more_segments_than_lanes(dtype, B, T, V):
+    """Vocabularies of more than 64 segments of 1024."""
+    import care_kv
+    print(f"verify {dtype} B={B} T={T} V={V}", flush=True)
+    draft, p, u, un, q = _inputs(V + T, B, T, V, dtype)
+    for kw in (dict(draft_probs=q), dict()):
+        for next_at in (un, torch.full_like(un, 0.999), torch.full_like(un, 0.0), torch.full_like(un, 1.0)):
+            ref = _ref(draft, p, u, next_at, kw.get("draft_probs"))
+            assert ref[2] > 2.0 ** -45  # sums in another order agree on every token
+            _check(care_kv.verify_drafts(draft, p, u, next_at, **kw), ref)
+
+
+def test_borders_of_segments():
+    """Weights that are exact, at the first and last places of segments, of lanes' runs and of lanes."""
+    import care_kv
+    V = 200000
+    at = torch.tensor([0, 1023, 1024, 4095, 4096, 65535, 65536, 131071, V - 1], device="cuda")
+    p = torch.zeros(1, 1, V, device="cuda")
+    p[0, 0, at] = 0.125
+    p[0, 0, 1] = math.nan
+    p[0, 0, 130000] = -1.0
+    none = torch.zeros(1, 0, device="cuda")
+    for i, x in enumerate(at.tolist()):
+        for share in (i / 9, (i + 0.5) / 9):
+            un = torch.tensor([share], device="cuda")
+            want = min(8, math.floor(float(un.double()) * 9))
+            got = care_kv.verify_drafts(none.long(), p, none, un)
+            assert got.tokens.tolist() == [[int(at[want])]], (i, share)
+
+
+def test_a_captured_call_of_two_launches():
+    import care_kv
+    draft, p, u, un, q = _inputs(6, 3, 4, 70001, F32)
+    call = lambda: care_kv.verify_drafts(draft, p, u, un, draft_probs=q)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        new = _inputs(80 + i, 3, 4, 70001, F32)
+        for x, y in zip((draft, p, u, un, q), new):
+            x.copy_(y)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        _check(out, _ref(draft, p, u, un, q))

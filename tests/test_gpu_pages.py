@@ -457,3 +457,34 @@ def test_two_streams_with_splits():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(torch.nan_to_num(a[0]), torch.nan_to_num(b[0])) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Hq,Hkv,D,T", [(4, 2, 64, 1), (8, 2, 128, 5), (8, 1, 64, 5), (2, 2, 128, 80)])
+def test_captured_attention_with_splits(dtype, Hq, Hkv, D, T):
+    """Tables much wider than the text, splits, workspace and join in a graph: lengths that move between replays, eager
+    calls among them, two graphs at once."""
+    import care_kv
+    B, N = 2, 1500
+    q, pages, short, K, V = _case(71, B, Hq, Hkv, D, T, N, dtype)
+    table = torch.full((B, 700), -1, dtype=torch.int32, device="cuda")
+    table[:, :short.shape[1]] = short
+    lengths = torch.tensor([N, 100], dtype=torch.int32, device="cuda")
+    call = lambda x: care_kv.paged_attention(x, pages, table, lengths, window=1200, sink=4, return_lse=True)  # noqa: E731
+    call(q)
+    graphs = []
+    for i in range(2):
+        x = q.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(x)
+        graphs.append((graph, x, out))
+    for n in (N, T, 777, 0, 1030):
+        lengths[1] = n
+        for graph, x, out in graphs:
+            x.copy_(torch.randn(x.shape, device="cuda"))
+            graph.replay()
+        for graph, x, out in graphs:
+            want = call(x)
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+            check(out, attend(x, K, V, sight(B, T, N, 1200, 4, [N, n], [T] * B, None), weights=F16))

@@ -257,3 +257,24 @@ def test_infinite_values_of_small_weight(dtype, B, Hq, Hkv, D, Tq, Tk):
     kk[:, :, Tk // 2] = (a * u).to(dtype)
     vv[:, :, 1, 3], vv[:, :, Tk // 3, 3], vv[:, :, Tk // 3, 4] = math.inf, -math.inf, -math.inf
     check(care_kv.window_attention(q, kk, vv, return_lse=True), attend(q, kk, vv, see))
+
+
+@pytest.mark.parametrize("Tq", [2, 40])
+def test_a_captured_call_with_splits(Tq):
+    """Two launches and a workspace in a graph: lengths that move between replays, eager calls among them."""
+    import care_kv
+    q, k, v = _inputs(16, 2, 4, 2, 64, Tq, 6000, F16)
+    lengths = torch.tensor([6000, 100], dtype=torch.int32, device="cuda")
+    call = lambda: care_kv.window_attention(q, k, v, window=5000, sink=4, lengths=lengths, return_lse=True)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for n in (6000, 60, 3001, 0, 133):
+        lengths[1] = n
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        check(out, attend(q, k, v, sight(2, Tq, 6000, 5000, 4, [6000, n], [Tq] * 2, None)))
