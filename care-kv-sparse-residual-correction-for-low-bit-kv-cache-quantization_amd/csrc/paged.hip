@@ -484,8 +484,9 @@ PagedPlan paged_plan(const carekv_paged_params& p) {
     keys = std::min(keys, sees);
   }
   const long tiles = std::max(1L, (keys + kTile - 1) / kTile), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
+  const double mean = std::min((double)tiles, mean_keys((long)p.max_pages * kPage, p.seq_len, keys) / kTile + 1);
   const long at = wgs * tiles < 512 * 64 ? 512 : 2048;  // work-groups
-  const long ns = r.nq == 8 ? best_splits(tiles, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
+  const long ns = r.nq == 8 ? best_splits(tiles, mean, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
                   : tiles * p.head_dim <= 32 * 64 ? 1 : std::max(1L, std::min(std::min(32L, at / wgs), (tiles + 7) / 8));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);

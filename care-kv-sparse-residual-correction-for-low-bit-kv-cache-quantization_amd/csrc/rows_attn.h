@@ -240,21 +240,35 @@ inline void launch_join(const RowsArgs& a, hipStream_t s) {
   else go(std::integral_constant<int, 4>{});
 }
 
-// Key splits of a call of many rows (`tiles` tiles of 32 keys for each of `wgs` work-groups): of 1 to 32 the number with
-// the smallest estimate of its time: rounds of the work-groups' places (4 a CU at D = 64, 3 at 128) by a work-group's
-// tiles, and what the join of two and more costs.  Over 16 shapes it takes 2 % more on average than the best number
-// (until 768 or 1280 work-groups are there: 7 %), at most 7 % (23).  us by splits: 2 x 512 rows of 40 heads on 16896 keys 1
-// / 2 / 4 / 7 / 8: 837 / 533 / 517 / 514 / 534; 4 x 64 rows of 32 / 8 heads on 8000 5 / 8 / 12 / 16: 103 / 76 / 72 / 92;
-// prompts of 512 tokens, 40 heads, 1 / 2 / 4: 25 / 31 / 30.
-inline long best_splits(long tiles, long wgs, long rows, int d) {
-  const long places = d == 64 ? 1024 : 768;
+// Keys that a row sees on average: the last `rows` positions of `keys`, each those up to itself, at most `most`.
+inline double mean_keys(long keys, long rows, long most) {
+  const double m = (double)most;
+  auto area = [&](double x) { return x <= m ? x * x / 2 : m * m / 2 + m * (x - m); };
+  return (area((double)keys) - area((double)std::max(0L, keys - rows))) / (double)std::max(1L, rows);
+}
+
+// Key splits of a call of many rows (at most `tiles` tiles of 32 keys for each of `wgs` work-groups, `mean` on average): of
+// 1 to 32 the number with the smallest estimate of its time.  Work-groups, longest first, fill the places (4 a CU at D = 64,
+// 3 at 128): the longest of them, or their sum over the places, and where they are alike what the last round leaves empty.
+// Two and more splits cost the join and the partials, and have to be a tenth better than one.  Over 29 shapes it takes 0.9 %
+// more on average than the best number, at most 9.5 % (with whole rounds of work-groups that all have `tiles` 3.4 and 23: a
+// prompt's have half of them).  us by splits: 2 x 512 rows of 40 heads on 16896 keys 1 / 2 / 4 / 7 / 8: 837 / 530 / 516 /
+// 516 / 532; 4 x 64 rows of 32 / 8 heads on 8000 5 / 8 / 12 / 16: 104 / 76 / 73 / 93; prompts, 1 / 2 / 3: 512 tokens of 40
+// heads 26 / 31 / 30, 4096 of 32 / 8 173 / 210 / 212 (3: 195 MB of partials), 8192 of 40 812 / 850 / 884 (2: 325 MB).
+inline long best_splits(long tiles, double mean, long wgs, long rows, int d) {
+  const double places = d == 64 ? 1024 : 768;
   const double tile = d == 64 ? 0.8 : 1.3, start = 6.0, join = 12.0, split = rows * (d + 2) * 4 / 3.5e6;  // us
   long best = 1;
   double least = 0.0;
   for (long ns = 1; ns <= std::min(tiles, 32L); ++ns) {
-    const long tps = (tiles + ns - 1) / ns, rounds = (wgs * ns + places - 1) / places;
-    const double cost = rounds * (tps * tile + start) + (ns > 1 ? join + ns * split : 0.0);
-    if (ns == 1 || cost < least) least = cost, best = ns;
+    const long tps = (tiles + ns - 1) / ns;
+    const double used = std::min((double)ns, std::max(1.0, mean / tps + 0.5)), items = wgs * used;  // splits that have tiles
+    const double longest = tps * tile + start, sum = wgs * mean * tile + items * start;
+    const double alike = std::max(0.0, 2 * sum / (items * longest) - 1);  // 0 for a prompt's, 1 where all are as long
+    const double fill = sum / places + alike * longest * (std::ceil(items / places) - items / places);
+    const double cost = std::max(longest, fill) + (ns > 1 ? join + used * split : 0.0);
+    if (ns == 1) least = 0.9 * cost;
+    else if (cost < least) least = cost, best = ns;
   }
   return best;
 }

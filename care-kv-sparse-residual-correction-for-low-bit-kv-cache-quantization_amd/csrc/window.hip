@@ -485,7 +485,8 @@ WindowPlan window_plan(const carekv_window_params& p) {
   long keys = p.n_keys;  // that a block of rows may see
   if (p.window > 0) keys = std::min(keys, (long)p.window + std::min<long>(p.seq_len, 32L * r.wq) + p.sink + 2 * kt);
   const long tiles = std::max(1L, (keys + kt - 1) / kt), wgs = std::max(1L, (long)p.batch * p.n_kv_heads * r.nqb);
-  const long ns = r.wq == 4 ? best_splits(tiles, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
+  const double mean = std::min((double)tiles, mean_keys(p.n_keys, p.seq_len, keys) / kt + 1);
+  const long ns = r.wq == 4 ? best_splits(tiles, mean, wgs, (long)p.batch * p.seq_len * p.n_heads, p.head_dim)
                   : tiles * p.head_dim <= 4 * 64 ? 1 : std::max(1L, std::min(std::min(32L, 512 / wgs), tiles));
   r.tps = (int)((tiles + ns - 1) / ns);
   r.nsplit = (int)((tiles + r.tps - 1) / r.tps);

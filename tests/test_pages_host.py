@@ -160,3 +160,19 @@ def test_structs_match_the_header():
                       (_lib.window_params, _lib.WindowParams), (_lib.verify_params, _lib.VerifyParams)):
         v = list(range(1, len(cls._fields_) + 1))
         assert pack(*v) == bytes(cls(*v))
+
+
+def test_splits_of_prompts():
+    """Prompts that fill the GPU by themselves have no workspace; few long rows and short tables of work-groups do."""
+    lib = _lib.load()
+
+    def ws(B, T, N, Hq, Hkv, D, window=0):
+        p = C.byref(_lib.WindowParams(batch=B, n_heads=Hq, n_kv_heads=Hkv, seq_len=T, n_keys=N, head_dim=D, dtype=0, window=window,
+                                      sm_scale=1.0))
+        return lib.carekv_window_attn_workspace_bytes(p)
+    for B, T, N, Hq, Hkv, D in ((1, 4096, 4096, 32, 8, 128), (1, 8192, 8192, 40, 40, 128), (1, 16384, 16384, 32, 8, 128),
+                                (1, 32768, 131072, 32, 8, 128), (4, 8192, 8192, 40, 40, 128), (1, 131072, 131072, 32, 4, 64)):
+        assert ws(B, T, N, Hq, Hkv, D) == 0
+    row = 4 * (128 + 2)
+    assert ws(1, 2048, 16384, 8, 8, 128) >= 4 * 2048 * 8 * row
+    assert ws(1, 512, 8192, 32, 8, 128) >= 4 * 512 * 32 * row
