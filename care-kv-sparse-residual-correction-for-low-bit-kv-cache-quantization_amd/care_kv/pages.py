@@ -195,9 +195,14 @@ def paged_attention(q: torch.Tensor, pages: Int4Pages, table: torch.Tensor, leng
 
     Returns o like q and, with ``return_lse``, the natural log-sum-exp of each
     row's scaled scores, fp32 (B, Hq, T).  Rows of padding and rows that see
-    nothing are 0 with lse -inf; a score of -inf counts as not seen.  What places
-    that a row does not see hold (NaN included) is never used.  ``out`` may be q
-    itself.  The results carry no autograd history."""
+    nothing are 0 with lse -inf; a score of -inf has no weight.  What places that a
+    row does not see hold (NaN included) is never used; a group that stands for NaN
+    is NaN in the rows that see it.  ``out`` may be q itself.  The results carry no
+    autograd history.
+
+    Scores, the softmax's sums and the output's are 32 bits; the weights are
+    rounded to fp16 (half a step, 2^-11 of each) before their product with V, and
+    bf16 rows of q are scaled by a power of two into fp16."""
     one = q.dim() == 3
     if one:
         q = q.unsqueeze(2)

@@ -31,9 +31,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     Returns o like q and, with ``return_lse``, the natural log-sum-exp of each
     row's scaled scores, fp32 (B, Hq, Tq), as ``attention_mass`` and
     ``prefix_attention`` take it.  Rows that see nothing are 0 with lse -inf; a
-    score of -inf counts as not seen.  What keys that a row does not see hold (NaN
-    included) is never used.  ``out`` may be q itself.  The results carry no
-    autograd history."""
+    score of -inf has no weight.  What keys that a row does not see hold (NaN
+    included) is never used; an infinite value that it sees is its result whatever
+    the weight.  ``out`` may be q itself.  The results carry no autograd
+    history.
+
+    Scores, the softmax's sums and the output's are 32 bits; the weights are
+    rounded to the operands' type (half a step of each, 2^-11 in fp16, 2^-8 in
+    bf16) before their product with v."""
     squeeze = q.dim() == 3
     if squeeze:
         q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)

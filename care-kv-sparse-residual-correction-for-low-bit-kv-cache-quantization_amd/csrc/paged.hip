@@ -11,10 +11,12 @@
 // query's column in 32 bits on base-2 logits, the waves joined in LDS.  Measured: 64
 // rows of 32 / 8 heads, D = 128, on 32768 keys (2.4 GB) 458 - 470 us, 5.2 TB/s, a copy's
 // rate (515 with the table read by vector loads and masks as literals); 16 x 5 rows
-// through a window of 4096 33 us: 20 rows fill 20 of 32 columns, a tile costs a SIMD
-// 2100 cycles (by count unpacking 830, softmax and products 510 each).  One row of 32 / 4 heads, D
-// = 64, on 2303 keys in a graph 8.7; with 16 waves a work-group and no splits, one
-// launch instead of two, 12.4.
+// through a window of 4096 33 us, 30 of them this kernel: 20 rows fill 20 of 32 columns,
+// and of the 50000 cycles that a wave lives (at some 2 GHz) its SIMD issues vector
+// instructions in 33700, 2070 for each of 16.25 tiles (by count unpacking 830, softmax
+// and products 510 each), while a wave waits in 18600 of them (all from counters).  One
+// row of 32 / 4 heads, D = 64, on 2303 keys in a graph 8.7; with 16 waves a work-group
+// and no splits, one launch instead of two, 12.4.
 //
 // Products are fp16 whatever q's type: codes times scales are fp16 values by
 // definition, bf16 rows of q are scaled by a power of two to below 2^12, which
@@ -466,7 +468,12 @@ namespace {
 // 32 / 4 heads, D = 64, on 2303 keys 1 / 4 / 8 / 16 / 32: 17.2 / 10.3 / 9.1 / 8.7 / 9.2, on
 // 8000 8 / 16 / 32 / 64: 12.4 / 10.0 / 9.9 / 12.3; 32 / 8 heads, D = 128, on 16000 16 / 32 /
 // 64: 16.7 / 14.1 / 16.6; 16 x 5 rows on 8191 through a window of 4096 2 / 4 / 6 / 8: 39 / 34
-// / 39 / 39; 64 rows on 32768 2 / 4 / 6 / 8: 479 / 461 / 460 / 463.
+// / 39 / 39; 64 rows on 32768 1 / 2 / 4 / 6 / 8: 489 / 479 / 461 / 460 / 463.
+// Work-groups in all: 512 up to 512 x 64 tiles, then 2048.  us with 512 / 2048, in a graph, below that: 16 x 8 heads, D =
+// 128, on 4000 keys 24.5 / 26.8, on 8000 37.8 / 38.6, 5 tokens of each on 7900 46.7 / 59.3, 64 x 4 heads, D = 64, on 3900
+// 26.9 / 26.7; above: 64 x 8 heads on 8000 125.9 / 131.1, on 16000 244 / 240, on 32768 489 / 465 (ragged 417 / 342), 64 x 4
+// heads, D = 64, on 8000 43.9 / 40.6, on 32000 165 / 144.  For 17 rows and more, two work-groups a CU, the border lies too
+// low: 16 x 5 tokens on 8600 49 / 63, on 16000 84 / 101, 64 x 5 on 8000 158 / 176.
 // Up to 1024 keys (D = 128: 512) of few rows one split: the join's launch costs the
 // host 4 us, its splits save less (one row on 500 keys split 7.9 / 9.3 us on the GPU,
 // whole 6.9 / 9.1, with the host 16.8 and 12.6; on 1000 keys 7.9 / 9.3 and 9.9 / 13.1).

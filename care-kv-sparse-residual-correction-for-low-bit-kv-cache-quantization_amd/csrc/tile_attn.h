@@ -11,7 +11,7 @@
 // not see, tiles that none sees are left out.
 //
 // Bound by products and exponentials, whose times add up more than they overlap: 4
-// x 8192 rows of 40 heads, D = 128, window 4096: 2290 - 2400 us, 0.86 - 0.90 PFLOP/s,
+// x 8192 rows of 40 heads, D = 128, window 4096: 2250 - 2410 us, 0.86 - 0.92 PFLOP/s,
 // at the 1.7 - 2.0 GHz that the card's power leaves.  Three work-groups a CU, their phases apart, did
 // better than 8 waves with 256 rows (3026 us, pages 725 against 570, with values looked at
 // as they are stored) and than two tiles on their way with two work-groups a CU (2735);

@@ -171,8 +171,8 @@ struct Rows16 {
 // Up to 32 rows of a kv head: the four waves of a work-group have the same rows and
 // 32 keys each of a tile of 128, and are joined in LDS at the end.  One tile of LDS:
 // the next one's rows are on their way in registers.  16 rows of 32 / 8 heads, D = 128,
-// on 4097 keys (268 MB): 47 us, 5.7 TB/s; one row of 32 / 4 heads, D = 64, through a
-// window of 1024 in a graph 8.5 us, two launches.
+// on 4097 keys (268 MB): 48 us, 5.6 TB/s; one row of 32 / 4 heads, D = 64, through a
+// window of 1024 in a graph 8.6 us, two launches.
 template <typename ET, int D>
 __global__ __launch_bounds__(256, 2) void window_few_kernel(WindowArgs a) {
   using V8 = typename ET::V8;

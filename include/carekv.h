@@ -697,7 +697,9 @@ int carekv_append_pages(const carekv_append_params* params, const void* q, const
  * sees the tokens j <= p with j > p - window (0: no bound) or j < sink.  Rows of
  * padding and rows that see nothing are 0, their log-sum-exp (lse, optional:
  * fp32 [batch][n_heads][seq_len]) -inf; what places that a row does not see
- * hold is not used.  Strides in elements, rows of q 16-byte aligned. */
+ * hold is not used.  The softmax's weights are rounded to fp16 before their
+ * product with V, sums are 32 bits.  Strides in elements, rows of q 16-byte
+ * aligned. */
 typedef struct carekv_paged_params {
   int32_t batch, n_heads, n_kv_heads, seq_len, head_dim;
   int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
@@ -713,8 +715,9 @@ int carekv_paged_attn(const carekv_paged_params* params, const void* q, const vo
 int64_t carekv_paged_attn_workspace_bytes(const carekv_paged_params* params);
 
 /* The same over 16-bit rows k, v [batch][n_kv_heads][n_keys][head_dim] of q's
- * type: lengths NULL: n_keys; row t stands at q_start[b] + t (NULL: the rows are
- * the sequence's last).  Rows of q, k and v 16-byte aligned. */
+ * type, to which the weights are rounded: lengths NULL: n_keys; row t stands at
+ * q_start[b] + t (NULL: the rows are the sequence's last).  Rows of q, k and v
+ * 16-byte aligned. */
 typedef struct carekv_window_params {
   int32_t batch, n_heads, n_kv_heads, seq_len, n_keys, head_dim;
   int32_t dtype;           /* CAREKV_F16 or CAREKV_BF16                        */
