@@ -163,7 +163,7 @@ def test_structs_match_the_header():
 
 
 def test_splits_of_prompts():
-    """Prompts that fill the GPU by themselves have no workspace; few long rows and short tables of work-groups do."""
+    """Prompts whose blocks fill the GPU by themselves have no workspace; few blocks of rows on many keys do."""
     lib = _lib.load()
 
     def ws(B, T, N, Hq, Hkv, D, window=0):
